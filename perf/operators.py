@@ -106,8 +106,8 @@ def draw(rng):
     causal = rng.random() < 0.75
     lse = rng.random() < 0.3
     if kind == "plan":
-        return _case(kind, _log_int(rng, 1, 512), new, ctx, lengths, page=page)
-    if kind == "write":
+        case = _case(kind, _log_int(rng, 1, 512), new, ctx, lengths, page=page)
+    elif kind == "write":
         case = _case(kind, _log_int(rng, 1, 256), new, (ctx[0], min(ctx[1], 5000)), lengths,
                      page=page, kv_heads=kv_heads, dim=dim, dtype=dtype)
     elif kind == "paged":

@@ -168,6 +168,41 @@ SIGNATURES = {
         _c_int, _c_int, _c_int, _c_ptr, _c_i64,    # rows, dim, rows_per_group, out, out_stride
         _c_ptr,                                    # stream
     )),
+    "dsa_paged_plan": (_c_int, (
+        _c_ptr, _c_ptr, _c_int,                    # cached, fresh, requests
+        _c_ptr, _c_i64, _c_int,                    # table, table_stride, table_width
+        _c_ptr, _c_int, _c_int, _c_int,            # free_pages, free_count, page_size, tokens
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,    # q_start, kv_lens, slots, status, stream
+    )),
+    "dsa_paged_write": (_c_int, (
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr,            # k, v, k_cache, v_cache
+        ctypes.POINTER(_c_i64),                    # strides[10], bytes
+        _c_int, _c_int, _c_int, _c_int, _c_int,    # tokens, heads, row_bytes, pages, page_size
+        _c_ptr, _c_ptr,                            # slots, stream
+    )),
+    "dsa_packed_attention": (_c_int, (
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,  # q, k, v, o, dtype
+        ctypes.POINTER(_c_i64),                    # strides[8]
+        _c_int, _c_int, _c_int,                    # q_rows, k_rows, requests
+        _c_int, _c_int, _c_int,                    # heads, kv_heads, head_dim
+        _c_ptr, _c_ptr, _c_float,                  # q_start, k_start, scale
+        _c_int, _c_int, _c_ptr,                    # causal, fill, lse
+        _c_ptr, _c_size, _c_ptr,                   # workspace, workspace_bytes, stream
+    )),
+    "dsa_paged_attention": (_c_int, (
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,  # q, k_cache, v_cache, o, dtype
+        ctypes.POINTER(_c_i64),                    # strides[10]
+        _c_int, _c_int,                            # q_rows, requests
+        _c_int, _c_int, _c_int,                    # heads, kv_heads, head_dim
+        _c_int, _c_int,                            # pages, page_size
+        _c_ptr, _c_i64, _c_int,                    # table, table_stride, table_width
+        _c_ptr, _c_ptr, _c_float,                  # kv_lens, q_start, scale
+        _c_int, _c_int, _c_ptr,                    # causal, fill, lse
+        _c_ptr, _c_size, _c_ptr,                   # workspace, workspace_bytes, stream
+    )),
+    "dsa_seq_attention_workspace_bytes": (_c_size, (
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,  # q_rows, requests, heads, kv_heads, head_dim, max_keys
+    )),
 }
 
 _lock = threading.Lock()

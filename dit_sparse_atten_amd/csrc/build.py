@@ -35,6 +35,9 @@ SOURCES = (
     "tile_route.hip",
     "permute.hip",
     "dit_ops.hip",
+    "paged_cache.hip",
+    "seq_attn.hip",
+    "seq_attn_f16.hip",
 )
 
 # Packed FP32 VALU forms are disabled: the device code relies on scalar and

@@ -1,0 +1,860 @@
+// Attention of packed sequences of different lengths with shared key/value
+// heads (gfx950), bf16 or fp16 in and out, fp32 softmax: whole prompts whose
+// keys lie side by side in one tensor, and new tokens over a paged cache.  The
+// kernel templates shared by seq_attn.hip (bf16 instances and the C-ABI entry
+// points) and seq_attn_f16.hip (fp16 instances).
+//
+// For sequence r with n query rows and m keys, query head h and key/value head
+// h / G (G = heads / kv_heads):
+//   O[t,h,:] = sum_j p_j V[j,h/G,:],  p = softmax_j(scale <Q[t,h,:], K[j,h/G,:]>),
+// over j < m or, causal, over j <= t + (m - n): the last query row sees every
+// key.  A row that sees none gives O = 0 and LSE = -inf.
+//
+// Layout of the work.  The G query heads of a key head and the sequence's query
+// tokens form one list of n G rows (row = token G + head in group), cut into
+// tiles: every key staged for a tile serves all heads of the group.  A tile's
+// keys may be cut into parts, whose fp32 partials seq_merge_kernel joins.
+// Lengths live on the device, so seq_schedule_kernel lists the (tile, part)
+// items there, near-equal in length, longest first; the grids are the host's
+// upper bounds and workgroups past the list end at once.
+//
+//  * seq_wide_kernel: 128 rows, four waves of 32, the 64-key staged walk of
+//    bsa_fwd_kernel (S^T = K Q^T, O^T = V^T P^T on 32x32x16 products).
+//  * seq_narrow_kernel: 16 rows, for calls of few rows per sequence (decoding
+//    steps): four waves walk different keys of the tile, each through its own
+//    LDS stages without workgroup barriers, and join at the end.
+#pragma once
+
+#include "bsa_tiles.h"
+
+namespace seq {
+
+using dsa::lds_load16;
+using dsa::make_rsrc;
+
+// One (tile, key part) of one sequence, for every key/value head.
+struct Item {
+  int32_t request, q0, n, k0, m;  // sequence: first query row and count, first key and count
+  int32_t tile;                   // rows tile * tile_rows ..
+  int32_t s0, s1;                 // key steps
+  int32_t slot;                   // partial slot, -1: the whole tile, written to O
+  int32_t parts;                  // of the tile
+  int32_t pad[6];
+};
+static_assert(sizeof(Item) == 64, "items are read as one 64-byte line");
+
+struct Params {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;                  // [heads, q_rows] or null
+  int64_t q_st, q_sh, o_st, o_sh;
+  int64_t k_sp, k_st, k_sh;    // page (paged calls), token and head strides, in elements
+  int64_t v_sp, v_st, v_sh;
+  const int32_t* q_start;      // [requests + 1]
+  const int32_t* k_start;      // [requests + 1] (packed calls)
+  const int32_t* kv_lens;      // [requests] (paged calls)
+  const int32_t* table;        // [requests, table_width] pages (paged calls)
+  int64_t table_stride;
+  int32_t table_width, pages, page_shift;
+  int32_t requests, q_rows, k_rows;
+  int32_t heads, kv_heads, group, head_dim;
+  int32_t causal;
+  int32_t fill;                // rows of o outside every sequence become 0
+  float scale_log2;            // scale * log2(e)
+  // Schedule.
+  int32_t tile_rows, step_keys, min_chunk;
+  int32_t target;              // (tile, part, key head) items to cut the work into
+  int32_t max_items, max_splits, max_slots;  // room in the lists, per key head
+  int32_t* counts;             // items, split tiles
+  int32_t* tile_base;          // [requests + 1] tiles before each sequence
+  Item* items;
+  Item* splits;                // split tiles: slot = the first of `parts` slots
+  float* part;                 // partial slots, kv_heads each
+};
+
+// One partial: O [tile_rows][kD] relative to the row's reference max, then m
+// (log2 units of the scaled scores) and l per row, in fp32.
+__host__ __device__ constexpr int part_floats(int tile_rows, int dim) {
+  return tile_rows * (dim + 2);
+}
+
+constexpr float kRescaleLog2 = 8.0f;  // move the reference max once a p could exceed 2^8
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kWideRows = 128, kWideKeys = 64;
+constexpr int kNarrowRows = 16, kNarrowKeys = 128;  // 32 keys for each of four waves
+
+// ds_read_b64_tr_b16: in each 16-lane group lane j receives element j % 4 of
+// the 8 bytes that lane 4 r + j / 4 addresses, r = 0..3.
+template <typename T>
+__device__ __forceinline__ typename dsa::Elem<T>::x4 read_tr(const unsigned char* lds) {
+  const dsa_i16x4 raw = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) dsa_i16x4*)(lds));
+  return __builtin_bit_cast(typename dsa::Elem<T>::x4, raw);
+}
+
+// s_waitcnt with only vmcnt(n) set.
+constexpr int vmcnt(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+
+// Position of 16-byte chunk c in row r of a K stage, distinct banks for the 16
+// rows that one chunk of a fragment read touches: rows of 256 bytes (kD 128) by
+// their low four bits, rows of 128 bytes, two to a bank round, by bits 1..3.
+template <int kD>
+__device__ __forceinline__ int k_swz(int r, int c) {
+  return kD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+}
+
+// The item's page table row, and the page of a key in it; an entry outside the
+// cache is -1: its keys are not read and take no part.
+__device__ __forceinline__ int page_at(const Params& p, int request, int key) {
+  const int id = p.table[(int64_t)request * p.table_stride + (key >> p.page_shift)];
+  return (unsigned)id < (unsigned)p.pages ? id : -1;
+}
+
+// Resource of `rows` (<= 16) staged rows from key `key` of key head h: none
+// when they lie past the last key or in a bad page.
+template <bool kPaged>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int64_t sp,
+                                                            int64_t st, int64_t sh, int h, int key,
+                                                            int k0, int page, int rows,
+                                                            const Params& p) {
+  if (kPaged && page < 0) rows = 0;
+  const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * st * 2 + p.head_dim * 2) : 0u;
+  const int64_t at = kPaged ? (int64_t)page * sp + (int64_t)(key & ((1 << p.page_shift) - 1)) * st
+                            : (int64_t)(k0 + key) * st;
+  return make_rsrc(static_cast<const unsigned char*>(base) + (rows > 0 ? (at + h * sh) * 2 : 0),
+                   bytes);
+}
+
+__device__ __forceinline__ Item load_item(const Item* at) {
+  Item it;
+  const dsa::const_i32 s = (dsa::const_i32)(const int32_t*)at;
+  it.request = s[0]; it.q0 = s[1]; it.n = s[2]; it.k0 = s[3]; it.m = s[4];
+  it.tile = s[5]; it.s0 = s[6]; it.s1 = s[7]; it.slot = s[8]; it.parts = s[9];
+  return it;
+}
+
+// One row's sum of p_j V_j over the keys it sees of `blocks` key blocks (`width`
+// <= 64 keys from key_lo, key_lo + stride, ..; below key_hi), element by element:
+// lane l ends with the dims l kD / 64 ...  In the matrix products a hidden key's
+// p is 0, and 0 times a value that is not finite is NaN, so a wave whose O is not
+// finite, and whose rows see different keys, takes this way instead.
+template <typename T, int kD, bool kPaged>
+__device__ __forceinline__ void exact_row(const Params& p, const Item& it, int h, int64_t q_at,
+                                          int key_lo, int blocks, int stride, int width,
+                                          int key_hi, float m_use, float acc[kD / 64]) {
+  const int lane = threadIdx.x & 63;
+  const int d0 = lane * (kD / 64);
+  const T* const q = static_cast<const T*>(p.q) + q_at;
+#pragma unroll
+  for (int e = 0; e < kD / 64; ++e) acc[e] = 0.f;
+#pragma unroll 1
+  for (int b = 0; b < blocks; ++b) {
+    const int key0 = key_lo + b * stride;
+    if (key0 >= key_hi) break;
+    const int key = key0 + lane;
+    int page = -1;
+    if (lane < width && key < key_hi) page = kPaged ? page_at(p, it.request, key) : 0;
+    const int in_page = kPaged ? key & ((1 << p.page_shift) - 1) : it.k0 + key;
+    float prob = 0.f;
+    if (page >= 0) {
+      const T* k = static_cast<const T*>(p.k) + page * p.k_sp + in_page * p.k_st + h * p.k_sh;
+      float s = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < p.head_dim; ++d) s = fmaf((float)q[d], (float)k[d], s);
+      prob = __builtin_amdgcn_exp2f(fmaf(s, p.scale_log2, -m_use));
+    }
+#pragma unroll 1
+    for (int j = 0; j < width; ++j) {
+      const int page_j = __shfl(page, j);
+      if (page_j < 0) continue;
+      const float prob_j = __shfl(prob, j);
+      const T* v = static_cast<const T*>(p.v) + page_j * p.v_sp +
+                   (int64_t)__shfl(in_page, j) * p.v_st + h * p.v_sh;
+#pragma unroll
+      for (int e = 0; e < kD / 64; ++e)
+        if (d0 + e < p.head_dim) acc[e] = fmaf(prob_j, (float)v[d0 + e], acc[e]);
+    }
+  }
+}
+
+// 128 rows x the item's keys.  Each wave owns 32 rows; keys stream as 64-key
+// half-tiles of K and V, double-buffered in LDS by direct loads issued one
+// half-tile ahead; lane (g, qi) = (lane / 32, lane % 32) holds row qi's scores
+// of the keys 32 kt + 8 (r / 4) + 4 g + r % 4 and, of O, the dims 32 dt +
+// 8 (r / 4) + 4 g + r % 4.
+template <typename T, int kD, bool kPaged>
+__global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
+  typedef dsa::Elem<T> E;
+  typedef typename E::x8 x8;
+  constexpr int kRow = kD * 2;               // bytes of a staged row
+  constexpr int kStage = kWideKeys * kRow;
+  constexpr int kChunks = kD / 8;            // 16-byte chunks per row
+  constexpr int kSlices = kD / 32;           // 1 KB loads per wave, K or V
+  constexpr int kRowsPer = 64 / kChunks;     // rows of one load
+  constexpr int kDt = kD / 32;               // 32-dim output tiles
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v1[kStage];
+
+  const int count = ((dsa::const_i32)p.counts)[0];
+  const int wg = (int)blockIdx.x;
+  if (wg >= count * p.kv_heads) return;
+  const int h = wg / count;
+  const Item it = load_item(p.items + (wg - h * count));
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 5, qi = lane & 31;
+  const int rows = it.n * p.group;
+  const int local = wave * 32 + qi;
+  const int row = it.tile * kWideRows + local;
+  const bool row_ok = row < rows;
+  const int row_c = min(row, rows - 1);
+  const int token = row_c / p.group;
+  const int head = h * p.group + row_c - token * p.group;
+  // Keys [0, lim) are visible to the lane's row.
+  const int lim = p.causal ? max(0, min(it.m, it.m - it.n + token + 1)) : it.m;
+  const bool wave_active = it.tile * kWideRows + wave * 32 < rows;
+  const int lim_first = __builtin_amdgcn_readlane(lim, 0);
+  const int lim_last = __builtin_amdgcn_readlane(lim, 31);
+  // Keys the tile's last row sees: rows past it stage as zeros.
+  const int last_row = min(it.tile * kWideRows + kWideRows, rows) - 1;
+  const int kend =
+      p.causal ? max(0, min(it.m, it.m - it.n + last_row / p.group + 1)) : it.m;
+
+  x8 qf[kD / 16];
+  {
+    const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
+                    head * p.q_sh;
+#pragma unroll
+    for (int dc = 0; dc < kD / 16; ++dc) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[dc][e] = (T)0.0f;
+      if (dc * 16 + g * 8 < p.head_dim)
+        qf[dc] = *reinterpret_cast<const x8*>(qrow + dc * 16 + g * 8);
+    }
+  }
+
+  // Wave w stages rows 16 w .. 16 w + 15: one page, one resource.  Lane offsets
+  // from the first of them (a chunk past head_dim loads zeros).
+  uint32_t koff[kSlices], voff[kSlices];
+#pragma unroll
+  for (int j = 0; j < kSlices; ++j) {
+    const int r = j * kRowsPer + lane / kChunks;  // row in the wave's 16
+    const int c = lane % kChunks;
+    const int kc = k_swz<kD>(wave * 16 + r, c);
+    const int vc = kD == 128 ? c ^ ((0xCA60 >> (4 * (r & 3))) & 15) : c ^ (4 * ((r >> 1) & 1));
+    koff[j] = (uint32_t)((r * (int)p.k_st + kc * 8) * 2) | dsa::dead_bits(kc, p.head_dim);
+    voff[j] = (uint32_t)((r * (int)p.v_st + vc * 8) * 2) | dsa::dead_bits(vc, p.head_dim);
+  }
+  int vfrag[kDt];
+  {
+    const int lam = lane & 15, r = lam >> 2, c = lam & 3;
+    const int vrow = 4 * g + r;
+    const int sub = 2 * ((lane >> 4) & 1) + (c >> 1);
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt) {
+      const int chunk = 4 * dt + sub;
+      const int pos = kD == 128 ? chunk ^ ((0xCA60 >> (4 * (vrow & 3))) & 15)
+                                : chunk ^ (4 * ((vrow >> 1) & 1));
+      vfrag[dt] = vrow * kRow + pos * 16 + (c & 1) * 8;
+    }
+  }
+
+  // Pages of a 1,024-key window, one 16-key granule per lane; the next window's
+  // are loaded a window ahead.
+  auto window_ids = [&](int window) -> int {
+    const int key = window * 1024 + lane * 16;
+    return key < kend ? page_at(p, it.request, key) : -1;
+  };
+  int ids = -1, ids_next = -1, window = it.s0 >> 4;
+  if constexpr (kPaged) {
+    ids = window_ids(window);
+    ids_next = window_ids(window + 1);
+  }
+  // Stages step s; returns the keys' granules (bits 0..3) that lie in a bad page.
+  auto issue = [&](int s, unsigned char* kdst, unsigned char* vdst)
+      __attribute__((always_inline)) -> int {
+    const int key = s * kWideKeys + wave * 16;
+    int page = 0, bad = 0;
+    if constexpr (kPaged) {
+      if ((s >> 4) != window) {
+        window = s >> 4;
+        ids = ids_next;
+        ids_next = window_ids(window + 1);
+      }
+      page = __builtin_amdgcn_readlane(ids, (s & 15) * 4 + wave);
+      bad = (int)(__ballot(ids < 0) >> ((s & 15) * 4)) & 15;
+    }
+    const int left = min(16, kend - key);
+    const __amdgpu_buffer_rsrc_t kr =
+        rows_rsrc<kPaged>(p.k, p.k_sp, p.k_st, p.k_sh, h, key, it.k0, page, left, p);
+    const __amdgpu_buffer_rsrc_t vr =
+        rows_rsrc<kPaged>(p.v, p.v_sp, p.v_st, p.v_sh, h, key, it.k0, page, left, p);
+#pragma unroll
+    for (int j = 0; j < kSlices; ++j)
+      lds_load16(kr, kdst + (wave * kSlices + j) * 1024, koff[j], 0);
+#pragma unroll
+    for (int j = 0; j < kSlices; ++j)
+      lds_load16(vr, vdst + (wave * kSlices + j) * 1024, voff[j], 0);
+    return bad;
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  dsa_f32x16 oacc[kDt];
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
+
+  auto compute = [&](const unsigned char* k_lds, const unsigned char* v_lds, int key0, int bad)
+      __attribute__((always_inline)) {
+    dsa_f32x16 sacc[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sacc[kt][r] = 0.f;
+#pragma unroll
+    for (int dc = 0; dc < kD / 16; ++dc)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int krow = kt * 32 + qi;
+        const x8 a = *reinterpret_cast<const x8*>(k_lds + krow * kRow +
+                                                  k_swz<kD>(krow, dc * 2 + g) * 16);
+        sacc[kt] = E::mfma32(a, qf[dc], sacc[kt]);
+      }
+    // Four K reads in flight ahead of the products.
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < kD / 8 - 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    if (key0 + kWideKeys > lim_first) {
+      const int bound = lim - key0 - 4 * g;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kt * 32 + 8 * (r >> 2) + (r & 3) >= bound) sacc[kt][r] = -INFINITY;
+    }
+    if (kPaged && bad != 0) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (bad & (1 << (2 * kt + (r >> 3)))) sacc[kt][r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kt][r]);
+    const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
+    const bool up = mx2 > m_run + kRescaleLog2;
+    if (__any(up)) {
+      const float m_new = up ? mx2 : m_run;
+      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    x8 pf[4];
+    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(
+            fmaf(sacc[j >> 1][(j & 1) * 8 + t], p.scale_log2, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(
+            fmaf(sacc[j >> 1][(j & 1) * 8 + t + 1], p.scale_log2, -m_use));
+        const dsa_f32x2 two = {p0, p1};
+        const typename E::x2 pb = __builtin_convertvector(two, typename E::x2);
+        sum0 += p0;
+        sum1 += p1;
+        pf[j][t] = pb[0];
+        pf[j][t + 1] = pb[1];
+      }
+    l_run += sum0 + sum1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) {
+        // Key rows 16 j + 4 g + r (slots 0..3) and 16 j + 8 + 4 g + r (4..7).
+        const unsigned char* at = v_lds + vfrag[dt] + j * 16 * kRow;
+        const typename E::x4 lo = read_tr<T>(at);
+        const typename E::x4 hi = read_tr<T>(at + 8 * kRow);
+        const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        oacc[dt] = E::mfma32(a, pf[j], oacc[dt]);
+      }
+  };
+  int bad_cur = 0, bad_next = 0;
+  auto step = [&](int s, const unsigned char* kc, const unsigned char* vc, unsigned char* kn,
+                  unsigned char* vn) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(vmcnt(0));
+    __syncthreads();
+    if (s + 1 < it.s1) bad_next = issue(s + 1, kn, vn);
+    // (a wave whose rows see none of the step's keys only stages)
+    if (wave_active && s * kWideKeys < lim_last) compute(kc, vc, s * kWideKeys, bad_cur);
+    bad_cur = bad_next;
+  };
+  if (it.s0 < it.s1) {
+    bad_cur = issue(it.s0, lds_k0, lds_v0);
+    for (int s = it.s0; s < it.s1; s += 2) {
+      step(s, lds_k0, lds_v0, lds_k1, lds_v1);
+      if (s + 1 >= it.s1) break;
+      step(s + 1, lds_k1, lds_v1, lds_k0, lds_v0);
+    }
+  }
+
+  const float l_tot = dsa::pair32_sum(l_run);
+  float unfinite = 0.f;  // NaN once an element of O is not finite
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) unfinite = fmaf(oacc[dt][r], 0.f, unfinite);
+  // (a row whose scores are not finite stays as it is)
+  const bool redo = lim_first < kend && __any(unfinite != 0.f && l_tot * 0.f == 0.f);
+  if (redo) {
+#pragma unroll 1
+    for (int r = 0; r < 32; ++r) {
+      const int row_r = it.tile * kWideRows + wave * 32 + r;
+      if (row_r >= rows) break;
+      const int token_r = __builtin_amdgcn_readlane(token, r);
+      const int head_r = __builtin_amdgcn_readlane(head, r);
+      const float m_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), r));
+      const float l_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_tot), r));
+      const int lim_r = __builtin_amdgcn_readlane(lim, r);
+      float acc[kD / 64];
+      exact_row<T, kD, kPaged>(p, it, h, (it.q0 + token_r) * p.q_st + head_r * p.q_sh,
+                               it.s0 * kWideKeys, it.s1 - it.s0, kWideKeys, kWideKeys,
+                               min(lim_r, it.s1 * kWideKeys), m_r == -INFINITY ? 0.f : m_r, acc);
+      const float inv = l_r > 0.f ? 1.f / l_r : (l_r == 0.f ? 0.f : l_r);
+#pragma unroll
+      for (int e = 0; e < kD / 64; ++e) {
+        const int d = lane * (kD / 64) + e;
+        if (it.slot >= 0)
+          p.part[((int64_t)it.slot * p.kv_heads + h) * part_floats(kWideRows, kD) +
+                 (wave * 32 + r) * kD + d] = acc[e];
+        else if (d < p.head_dim)
+          static_cast<T*>(p.o)[(it.q0 + token_r) * p.o_st + head_r * p.o_sh + d] =
+              (T)(acc[e] * inv);
+      }
+    }
+  }
+  if (!row_ok) return;
+  if (it.slot >= 0) {
+    float* po = p.part + ((int64_t)it.slot * p.kv_heads + h) * part_floats(kWideRows, kD);
+    float* prow = po + local * kD;
+    if (!redo)
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) {
+        const dsa_f32x4 v4 = {oacc[dt][rr * 4 + 0], oacc[dt][rr * 4 + 1], oacc[dt][rr * 4 + 2],
+                              oacc[dt][rr * 4 + 3]};
+        *reinterpret_cast<dsa_f32x4*>(prow + dt * 32 + rr * 8 + g * 4) = v4;
+      }
+    if (g == 0) {
+      po[kWideRows * kD + local] = m_run;
+      po[kWideRows * (kD + 1) + local] = l_tot;
+    }
+    return;
+  }
+  const float inv = l_tot > 0.f ? 1.f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
+  T* orow = static_cast<T*>(p.o) + (int64_t)(it.q0 + token) * p.o_st + head * p.o_sh;
+  if (!redo)
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      typename E::x4 v4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v4[e] = (T)(oacc[dt][rr * 4 + e] * inv);
+      if (dt * 32 + rr * 8 + g * 4 < p.head_dim)
+        *reinterpret_cast<typename E::x4*>(orow + dt * 32 + rr * 8 + g * 4) = v4;
+    }
+  if (p.lse && g == 0)
+    p.lse[(int64_t)head * p.q_rows + it.q0 + token] =
+        l_tot == 0.f ? -INFINITY : m_run * kLn2 + logf(l_tot);
+}
+
+// 16 rows x the item's keys, on 16x16x32 products.  Wave w takes keys 128 s +
+// 32 w .. + 31 of every step s through its own two LDS stage pairs; lane (q4,
+// c16) = (lane / 16, lane % 16) holds row c16's scores of the keys 16 kg + 4 q4
+// + r and, of O, the dims 16 dt + 4 q4 + r.
+template <typename T, int kD, bool kPaged>
+__global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
+  typedef dsa::Elem<T> E;
+  typedef typename E::x8 x8;
+  constexpr int kRow = kD * 2;
+  constexpr int kStage = 32 * kRow;         // K or V of one wave's 32 keys
+  constexpr int kChunks = kD / 8;
+  constexpr int kRowsPer = 64 / kChunks;    // rows of one 1 KB load
+  constexpr int kLoads = 16 / kRowsPer;     // loads per 16-key granule
+  constexpr int kDt = kD / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[4 * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[4 * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[4 * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v1[4 * kStage];
+
+  const int count = ((dsa::const_i32)p.counts)[0];
+  const int wg = (int)blockIdx.x;
+  if (wg >= count * p.kv_heads) return;
+  const int i_item = wg / p.kv_heads;
+  const int h = wg - i_item * p.kv_heads;
+  const Item it = load_item(p.items + i_item);
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q4 = lane >> 4, c16 = lane & 15;
+  const int rows = it.n * p.group;
+  const int row_c = min(it.tile * kNarrowRows + c16, rows - 1);
+  const int token = row_c / p.group;
+  const int head = h * p.group + row_c - token * p.group;
+  const int lim = p.causal ? max(0, min(it.m, it.m - it.n + token + 1)) : it.m;
+  const int lim_first = __builtin_amdgcn_readlane(lim, 0);
+  const int kend = __builtin_amdgcn_readlane(lim, 15);
+
+  x8 qf[kD / 32];
+  {
+    const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
+                    head * p.q_sh;
+#pragma unroll
+    for (int dc = 0; dc < kD / 32; ++dc) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[dc][e] = (T)0.0f;
+      if (dc * 32 + q4 * 8 < p.head_dim)
+        qf[dc] = *reinterpret_cast<const x8*>(qrow + dc * 32 + q4 * 8);
+    }
+  }
+  // V chunk c of row r sits at c ^ 2 (r & 7) (256-byte rows) or c ^ 2 ((r / 2) & 3).
+  auto v_swz = [](int r, int c) { return kD == 128 ? c ^ (2 * (r & 7)) : c ^ (2 * ((r >> 1) & 3)); };
+  uint32_t koff[kLoads], voff[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const int r = j * kRowsPer + lane / kChunks;  // row in its 16-key granule
+    const int c = lane % kChunks;
+    const int kc = k_swz<kD>(r, c), vc = v_swz(r, c);
+    koff[j] = (uint32_t)((r * (int)p.k_st + kc * 8) * 2) | dsa::dead_bits(kc, p.head_dim);
+    voff[j] = (uint32_t)((r * (int)p.v_st + vc * 8) * 2) | dsa::dead_bits(vc, p.head_dim);
+  }
+
+  // Pages of a window of 32 steps: lane l holds granule l & 1 of step l / 2.
+  auto window_ids = [&](int window) -> int {
+    const int key = (window * 32 + (lane >> 1)) * kNarrowKeys + wave * 32 + (lane & 1) * 16;
+    return key < kend ? page_at(p, it.request, key) : -1;
+  };
+  int ids = -1, ids_next = -1, window = it.s0 >> 5;
+  if constexpr (kPaged) {
+    ids = window_ids(window);
+    ids_next = window_ids(window + 1);
+  }
+  auto issue = [&](int s, unsigned char* kdst, unsigned char* vdst)
+      __attribute__((always_inline)) -> int {
+    const int key = s * kNarrowKeys + wave * 32;
+    int bad = 0;
+    if constexpr (kPaged) {
+      if ((s >> 5) != window) {
+        window = s >> 5;
+        ids = ids_next;
+        ids_next = window_ids(window + 1);
+      }
+      bad = (int)(__ballot(ids < 0) >> ((s & 31) * 2)) & 3;
+    }
+#pragma unroll
+    for (int kg = 0; kg < 2; ++kg) {
+      const int page = kPaged ? __builtin_amdgcn_readlane(ids, (s & 31) * 2 + kg) : 0;
+      const int left = min(16, kend - key - 16 * kg);
+      const __amdgpu_buffer_rsrc_t kr =
+          rows_rsrc<kPaged>(p.k, p.k_sp, p.k_st, p.k_sh, h, key + 16 * kg, it.k0, page, left, p);
+      const __amdgpu_buffer_rsrc_t vr =
+          rows_rsrc<kPaged>(p.v, p.v_sp, p.v_st, p.v_sh, h, key + 16 * kg, it.k0, page, left, p);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        lds_load16(kr, kdst + wave * kStage + (kg * kLoads + j) * 1024, koff[j], 0);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        lds_load16(vr, vdst + wave * kStage + (kg * kLoads + j) * 1024, voff[j], 0);
+    }
+    return bad;
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  dsa_f32x4 oacc[kDt];
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt) oacc[dt] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
+  const int vr_row = 4 * q4 + (c16 >> 2);
+
+  auto compute = [&](const unsigned char* k_lds, const unsigned char* v_lds, int key0, int bad)
+      __attribute__((always_inline)) {
+    dsa_f32x4 s[2];
+#pragma unroll
+    for (int kg = 0; kg < 2; ++kg) s[kg] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dc = 0; dc < kD / 32; ++dc)
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+        const x8 a = *reinterpret_cast<const x8*>(
+            k_lds + wave * kStage + (16 * kg + c16) * kRow + k_swz<kD>(c16, dc * 4 + q4) * 16);
+        s[kg] = E::mfma16(a, qf[dc], s[kg]);
+      }
+    if (key0 + 32 > lim_first) {
+      const int bound = lim - key0 - 4 * q4;
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * kg + r >= bound) s[kg][r] = -INFINITY;
+    }
+    if (kPaged && bad != 0) {
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (bad & (1 << kg)) s[kg][r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[kg][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
+    const bool up = mx2 > m_run + kRescaleLog2;
+    if (__any(up)) {
+      const float m_new = up ? mx2 : m_run;
+      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) oacc[dt] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    x8 pf;
+    float sum = 0.f;
+#pragma unroll
+    for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kg][r], p.scale_log2, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kg][r + 1], p.scale_log2, -m_use));
+        const dsa_f32x2 two = {p0, p1};
+        const typename E::x2 pb = __builtin_convertvector(two, typename E::x2);
+        sum += p0 + p1;
+        pf[4 * kg + r] = pb[0];
+        pf[4 * kg + r + 1] = pb[1];
+      }
+    l_run += sum;
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt) {
+      const int pos = v_swz(vr_row, 2 * dt + ((c16 & 3) >> 1));
+      const unsigned char* at =
+          v_lds + wave * kStage + vr_row * kRow + pos * 16 + (c16 & 1) * 8;
+      const typename E::x4 lo = read_tr<T>(at);
+      const typename E::x4 hi = read_tr<T>(at + 16 * kRow);
+      const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      oacc[dt] = E::mfma16(a, pf, oacc[dt]);
+    }
+  };
+  // A wave's stages are its own: it waits for its loads alone.
+  int bad_cur = 0, bad_next = 0;
+  auto step = [&](int s, const unsigned char* kc, const unsigned char* vc, unsigned char* kn,
+                  unsigned char* vn) __attribute__((always_inline)) {
+    if (s + 1 < it.s1) {
+      bad_next = issue(s + 1, kn, vn);
+      __builtin_amdgcn_s_waitcnt(vmcnt(4 * kLoads));
+    } else {
+      __builtin_amdgcn_s_waitcnt(vmcnt(0));
+    }
+    const int key0 = s * kNarrowKeys + wave * 32;
+    if (key0 < kend) compute(kc, vc, key0, bad_cur);
+    bad_cur = bad_next;
+  };
+  if (it.s0 < it.s1) {
+    bad_cur = issue(it.s0, lds_k0, lds_v0);
+    for (int s = it.s0; s < it.s1; s += 2) {
+      step(s, lds_k0, lds_v0, lds_k1, lds_v1);
+      if (s + 1 >= it.s1) break;
+      step(s + 1, lds_k1, lds_v1, lds_k0, lds_v0);
+    }
+  }
+
+  // Join the waves: their O, m and l through the K stages (row-major fp32).
+  l_run += __shfl_xor(l_run, 16);
+  const float l_wave = dsa::pair32_sum(l_run);
+  constexpr int kWaveFloats = part_floats(kNarrowRows, kD);
+  static_assert(4 * kWaveFloats * 4 <= 4 * kStage + 4 * 16 * 8, "joins through lds_k0 and join_ml");
+  __shared__ float join_ml[2][4][16];
+  float unfinite = 0.f;  // NaN once an element of O is not finite
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) unfinite = fmaf(oacc[dt][r], 0.f, unfinite);
+  dsa::lds_barrier<true>();
+  float* const mine = reinterpret_cast<float*>(lds_k0) + wave * kNarrowRows * kD;
+  // (a row whose scores are not finite stays as it is)
+  if (lim_first < kend && __any(unfinite != 0.f && l_wave * 0.f == 0.f)) {
+#pragma unroll 1
+    for (int r = 0; r < kNarrowRows; ++r) {
+      if (it.tile * kNarrowRows + r >= rows) break;
+      const int token_r = __builtin_amdgcn_readlane(token, r);
+      const int head_r = __builtin_amdgcn_readlane(head, r);
+      const float m_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), r));
+      float acc[kD / 64];
+      exact_row<T, kD, kPaged>(p, it, h, (it.q0 + token_r) * p.q_st + head_r * p.q_sh,
+                               it.s0 * kNarrowKeys + wave * 32, it.s1 - it.s0, kNarrowKeys, 32,
+                               __builtin_amdgcn_readlane(lim, r), m_r == -INFINITY ? 0.f : m_r,
+                               acc);
+#pragma unroll
+      for (int e = 0; e < kD / 64; ++e) mine[r * kD + lane * (kD / 64) + e] = acc[e];
+    }
+  } else {
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+      *reinterpret_cast<dsa_f32x4*>(mine + c16 * kD + 16 * dt + 4 * q4) = oacc[dt];
+  }
+  if (q4 == 0) {
+    join_ml[0][wave][c16] = m_run;
+    join_ml[1][wave][c16] = l_wave;
+  }
+  dsa::lds_barrier();
+  // Thread (r, c): row r, dims 8 c .. 8 c + 7.
+  const int r = tid / kChunks, d0 = (tid % kChunks) * 8;
+  const int out_row = it.tile * kNarrowRows + r;
+  if (r >= kNarrowRows || out_row >= rows) return;
+  float m_all = -INFINITY, l_all = 0.f, w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float mi = join_ml[0][i][r];
+    // (no finite score: l is 0, or NaN from NaN scores)
+    w[i] = mi == -INFINITY ? join_ml[1][i][r] : __builtin_amdgcn_exp2f(mi - m_all);
+    l_all = fmaf(w[i], join_ml[1][i][r], l_all);
+  }
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (w[i] == 0.f) continue;
+    const float* src = reinterpret_cast<const float*>(lds_k0) + (i * kNarrowRows + r) * kD + d0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = fmaf(w[i], src[e], acc[e]);
+  }
+  if (it.slot >= 0) {
+    float* po = p.part + ((int64_t)it.slot * p.kv_heads + h) * part_floats(kNarrowRows, kD);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      *reinterpret_cast<dsa_f32x4*>(po + r * kD + d0 + 4 * c) =
+          dsa_f32x4{acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]};
+    if (d0 == 0) {
+      po[kNarrowRows * kD + r] = m_all;
+      po[kNarrowRows * (kD + 1) + r] = l_all;
+    }
+    return;
+  }
+  const int out_token = it.q0 + out_row / p.group;
+  const int out_head = h * p.group + out_row % p.group;
+  const float inv = l_all > 0.f ? 1.f / l_all : (l_all == 0.f ? 0.f : l_all);
+  if (d0 < p.head_dim) {
+    x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv);
+    *reinterpret_cast<x8*>(static_cast<T*>(p.o) + (int64_t)out_token * p.o_st +
+                           out_head * p.o_sh + d0) = y;
+  }
+  if (p.lse && d0 == 0)
+    p.lse[(int64_t)out_head * p.q_rows + out_token] =
+        l_all == 0.f ? -INFINITY : m_all * kLn2 + logf(l_all);
+}
+
+// Joins the parts of a split tile: with M the largest reference, O = sum_i O_i
+// 2^(m_i - M) / sum_i l_i 2^(m_i - M).  One workgroup per (row, split tile, key
+// head): 16 groups of 16 threads take every 16th part, 8 dims to a thread, and
+// join through LDS, so that the many parts of a long single-row walk load at
+// once.
+template <typename T, int kD, int kRows>
+__global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
+  __shared__ float acc_lds[16][kD];
+  __shared__ float ml[2][16];
+  const int splits = ((dsa::const_i32)p.counts)[1];
+  const int h = blockIdx.y;
+  const int tid = threadIdx.x, grp = tid >> 4, d0 = (tid & 15) * 8;
+  for (int work = blockIdx.x; work < splits * kRows; work += gridDim.x) {
+    const Item it = load_item(p.splits + work / kRows);
+    const int r = work % kRows;
+    const int row = it.tile * kRows + r;
+    if (row >= it.n * p.group) continue;  // uniform
+    const int64_t stride = (int64_t)p.kv_heads * part_floats(kRows, kD);
+    const float* base = p.part + ((int64_t)it.slot * p.kv_heads + h) * part_floats(kRows, kD);
+    float m = -INFINITY, l = 0.f, acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int i = grp; i < it.parts; i += 16) {
+      const float* part = base + i * stride;
+      const float mi = part[kRows * kD + r], li = part[kRows * (kD + 1) + r];
+      dsa_f32x4 x[2] = {};
+      if (d0 < kD) {
+        x[0] = *reinterpret_cast<const dsa_f32x4*>(part + r * kD + d0);
+        x[1] = *reinterpret_cast<const dsa_f32x4*>(part + r * kD + d0 + 4);
+      }
+      if (li == 0.f) continue;  // no key of the part is visible
+      const float m_new = fmaxf(m, mi);
+      // (no finite score: l is NaN)
+      const float a = m == m_new ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      const float b = mi == -INFINITY ? li : __builtin_amdgcn_exp2f(mi - m_new);
+      l = fmaf(l, a, b * li);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], a, b * x[e >> 2][e & 3]);
+      m = m_new;
+    }
+    if (d0 < kD) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc_lds[grp][d0 + e] = acc[e];
+    }
+    if (d0 == 0) {
+      ml[0][grp] = m;
+      ml[1][grp] = l;
+    }
+    dsa::lds_barrier();
+    if (tid < kD) {
+      float m_all = -INFINITY, l_all = 0.f, o = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m_all = fmaxf(m_all, ml[0][i]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float w =
+            ml[0][i] == -INFINITY ? ml[1][i] : __builtin_amdgcn_exp2f(ml[0][i] - m_all);
+        if (w == 0.f) continue;
+        l_all = fmaf(w, ml[1][i], l_all);
+        o = fmaf(w, acc_lds[i][tid], o);
+      }
+      const int token = it.q0 + row / p.group, head = h * p.group + row % p.group;
+      const float inv = l_all > 0.f ? 1.f / l_all : (l_all == 0.f ? 0.f : l_all);
+      if (tid < p.head_dim)
+        static_cast<T*>(p.o)[(int64_t)token * p.o_st + head * p.o_sh + tid] = (T)(o * inv);
+      if (p.lse && tid == 0)
+        p.lse[(int64_t)head * p.q_rows + token] =
+            l_all == 0.f ? -INFINITY : m_all * kLn2 + logf(l_all);
+    }
+    dsa::lds_barrier();
+  }
+}
+
+}  // namespace seq
+
+// fp16 instances (seq_attn_f16.hip).
+int seq_launch_f16(const seq::Params& p, bool paged, bool narrow, int max_groups, bool merge,
+                   hipStream_t stream, const char* who);

@@ -1,0 +1,40 @@
+// Launches of the sequence attention kernels of one element type.
+#pragma once
+
+#include <algorithm>
+
+#include "seq_attn.h"
+
+namespace seq {
+
+template <typename T, int kD>
+int launch_dim(const Params& p, bool paged, bool narrow, int max_groups, bool merge,
+               hipStream_t stream, const char* who) {
+  const dim3 grid((unsigned)max_groups), block(256);
+  if (narrow) {
+    if (paged) hipLaunchKernelGGL((seq_narrow_kernel<T, kD, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((seq_narrow_kernel<T, kD, false>), grid, block, 0, stream, p);
+  } else {
+    if (paged) hipLaunchKernelGGL((seq_wide_kernel<T, kD, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((seq_wide_kernel<T, kD, false>), grid, block, 0, stream, p);
+  }
+  if (merge) {
+    const int rows = narrow ? kNarrowRows : kWideRows;
+    const dim3 groups((unsigned)std::min<int64_t>((int64_t)p.max_splits * rows,
+                                                  std::max(1, 4096 / p.kv_heads)),
+                      (unsigned)p.kv_heads);
+    if (narrow) hipLaunchKernelGGL((seq_merge_kernel<T, kD, kNarrowRows>), groups, block, 0, stream, p);
+    else hipLaunchKernelGGL((seq_merge_kernel<T, kD, kWideRows>), groups, block, 0, stream, p);
+  }
+  return dsa::check_launch(who);
+}
+
+template <typename T>
+int launch_typed(const Params& p, bool paged, bool narrow, int max_groups, bool merge,
+                 hipStream_t stream, const char* who) {
+  return p.head_dim <= 64
+             ? launch_dim<T, 64>(p, paged, narrow, max_groups, merge, stream, who)
+             : launch_dim<T, 128>(p, paged, narrow, max_groups, merge, stream, who);
+}
+
+}  // namespace seq

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import functools
 import math
+import typing
 
 import torch
 
@@ -965,3 +966,300 @@ def gated_residual(x, y, gate=None, out=None):
             rows_out.data_ptr(), rows_out.stride(0), _stream_handle(x.device))
     _lib.check(status, "dsa_gated_residual")
     return out if out is not None else rows_out.view(x.shape)
+
+
+# ---------------------------------------------------------------------------
+# Sequences of different lengths: a paged key/value cache and the attentions
+# around it
+# ---------------------------------------------------------------------------
+
+class PagedPlan(typing.NamedTuple):
+    """Where a step's new tokens go (``paged_plan``); all on the device."""
+
+    q_start: torch.Tensor  # int32 [requests + 1]: new tokens before each request
+    kv_lens: torch.Tensor  # int32 [requests]: cached and new tokens
+    slots: torch.Tensor    # int64 [tokens]: page * page_size + row, -1: no place
+    status: torch.Tensor   # int32 [2]: pages needed, new tokens without a slot
+
+
+def _index_vector(name, t, device, size=None):
+    _require_cuda(name, t)
+    if t.dtype != torch.int32 or t.ndim != 1:
+        raise ValueError(f"{name} must be a one-dimensional int32 tensor")
+    if t.device != device:
+        raise ValueError(f"{name} must live on {device}")
+    if size is not None and t.shape[0] != size:
+        raise ValueError(f"{name} must hold {size} values, got {t.shape[0]}")
+    return t.contiguous()
+
+
+def _block_table(t, device, requests):
+    _require_cuda("block_table", t)
+    if t.dtype != torch.int32 or t.ndim != 2:
+        raise ValueError("block_table must be an int32 tensor [requests, pages per request]")
+    if t.device != device or t.shape[0] != requests:
+        raise ValueError(f"block_table must have {requests} rows on {device}")
+    if t.shape[1] and (t.stride(1) != 1 or (requests > 1 and t.stride(0) < t.shape[1])):
+        raise ValueError("block_table rows must be contiguous and apart")
+    return t
+
+
+def _page_size(value):
+    if value < 16 or value & (value - 1):
+        raise ValueError(f"page_size {value} unsupported (a power of two from 16)")
+    return int(value)
+
+
+def _aligned_view(t):
+    """Whether the kernels can address the tensor in place: rows of 16-byte
+    chunks, contiguous along the last axis."""
+    chunk = 16 // t.element_size()
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(stride % chunk == 0 for stride in _strides(t)))
+
+
+def _strides(t):
+    """Strides but the last; 0 for axes of one entry, whose stride says nothing."""
+    return [stride if size > 1 else 0 for stride, size in zip(t.stride()[:-1], t.shape)]
+
+
+def _cache_view(name, t, dtype):
+    """A [pages, page_size, kv_heads, head_dim] cache, used in place."""
+    _require_cuda(name, t)
+    if t.ndim != 4:
+        raise ValueError(f"{name} must have shape [pages, page_size, kv_heads, head_dim]")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.numel() and not _aligned_view(t):
+        raise ValueError(f"{name} must have a contiguous, 16-byte aligned head dimension")
+    return t
+
+
+def _sequence_rows(name, t, dtype=None):
+    """A [rows, heads, head_dim] tensor the kernels can read (copied if needed)."""
+    _require_cuda(name, t)
+    if t.ndim != 3:
+        raise ValueError(f"{name} must have shape [rows, heads, head_dim]")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} like q, got {t.dtype}")
+    return t if _aligned_view(t) else t.contiguous()
+
+
+def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
+    """Places for a step's new tokens in a paged key/value cache.
+
+    ``cached`` and ``new`` (int32 [requests], on the device): tokens of every
+    request in the cache, and new ones.  Request r's pages are listed in
+    ``block_table[r]`` (int32); the first ceil(cached / page_size) entries are
+    its own already, and the pages its new tokens need beyond them are taken
+    from ``free_pages`` (int32, in request order) and entered in its row, in
+    place.  ``tokens`` is the length of the slot map: at least the sum of
+    ``new``, which the host need not know exactly.  Nothing is read back; at
+    most 8,192 requests.
+
+    Returns a ``PagedPlan``: ``q_start``, ``kv_lens`` for ``paged_attention``,
+    ``slots`` for ``paged_write`` (-1 behind the last request's tokens, and for
+    tokens without a page because ``free_pages`` or the table's row is too
+    short), and ``status`` = (pages needed, tokens without a slot): the caller's
+    free list starts behind the first ``status[0]`` pages next time.
+    """
+    lib = _lib.load()
+    _require_cuda("cached", cached)
+    device = cached.device
+    cached = _index_vector("cached", cached, device)
+    requests = cached.shape[0]
+    new = _index_vector("new", new, device, requests)
+    block_table = _block_table(block_table, device, requests)
+    free_pages = _index_vector("free_pages", free_pages, device)
+    page_size = _page_size(page_size)
+    if tokens < 0:
+        raise ValueError("tokens must not be negative")
+    ints = torch.empty(2 * requests + 3, dtype=torch.int32, device=device)
+    slots = torch.empty(tokens, dtype=torch.int64, device=device)
+    base = ints.data_ptr()
+    with torch.cuda.device(device):
+        status = lib.dsa_paged_plan(
+            cached.data_ptr(), new.data_ptr(), requests, block_table.data_ptr(),
+            max(block_table.stride(0), block_table.shape[1]), block_table.shape[1],
+            free_pages.data_ptr(), free_pages.shape[0], page_size, tokens, base,
+            base + 4 * (requests + 1), slots.data_ptr(), base + 4 * (2 * requests + 1),
+            _stream_handle(device))
+    _lib.check(status, "dsa_paged_plan")
+    q_start, kv_lens, state = ints.split((requests + 1, requests, 2))
+    return PagedPlan(q_start, kv_lens, slots, state)
+
+
+def paged_write(k, v, k_cache, v_cache, slots):
+    """Writes keys and values [tokens, kv_heads, head_dim] into the caches
+    [pages, page_size, kv_heads, head_dim], row t at slot ``slots[t]`` (int64 on
+    the device; page * page_size + row).  Rows whose slot lies outside the cache
+    (-1) are skipped.  A call's slots are distinct, as ``paged_plan`` gives
+    them: of rows that share one, parts of either may be kept.  Any element type
+    of 2 or 4 bytes."""
+    lib = _lib.load()
+    k = _sequence_rows("k", k)
+    v = _sequence_rows("v", v, k.dtype)
+    if k.dtype.itemsize not in (2, 4):
+        raise ValueError(f"paged_write moves elements of 2 or 4 bytes, not {k.dtype}")
+    k_cache = _cache_view("k_cache", k_cache, k.dtype)
+    v_cache = _cache_view("v_cache", v_cache, k.dtype)
+    tokens, heads, head_dim = k.shape
+    pages, page_size = k_cache.shape[:2]
+    if v.shape != k.shape or v_cache.shape != k_cache.shape:
+        raise ValueError("k and v, and their caches, must have the same shape")
+    if k_cache.shape[2:] != k.shape[1:]:
+        raise ValueError("the caches and k must agree on heads and head dimension")
+    _page_size(page_size)
+    _require_cuda("slots", slots)
+    if slots.dtype != torch.int64 or slots.shape != (tokens,):
+        raise ValueError(f"slots must be an int64 tensor of {tokens} values")
+    device = k_cache.device
+    if any(t.device != device for t in (k, v, v_cache, slots)):
+        raise ValueError("k, v, the caches and slots must be on the same device")
+    size = k.element_size()
+    if head_dim * size % 16:
+        raise ValueError("rows must be a multiple of 16 bytes")
+    if tokens == 0 or pages == 0 or heads == 0:
+        return
+    slots = slots.contiguous()
+    strides = _lib.int64_array([s * size for s in (
+        *_strides(k), *_strides(v), *_strides(k_cache), *_strides(v_cache))])
+    with torch.cuda.device(device):
+        status = lib.dsa_paged_write(
+            k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides, tokens,
+            heads, head_dim * size, pages, page_size, slots.data_ptr(), _stream_handle(device))
+    _lib.check(status, "dsa_paged_write")
+
+
+@functools.lru_cache(maxsize=256)
+def _sequence_workspace_bytes(q_rows, requests, heads, kv_heads, head_dim, max_keys):
+    return _lib.load().dsa_seq_attention_workspace_bytes(q_rows, requests, heads, kv_heads,
+                                                         head_dim, max_keys)
+
+
+def _sequence_call(q, kv_heads, q_start, scale, out, return_lse, max_keys, others):
+    """What both sequence attentions check and allocate:
+    (q, q_start, scale, out, fill, lse, workspace)."""
+    q = _sequence_rows("q", q)
+    dtype_code(q.dtype)
+    rows, heads, head_dim = q.shape
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key/value heads")
+    if head_dim % 8 or not 8 <= head_dim <= HEAD_DIM:
+        raise ValueError(f"head_dim {head_dim} unsupported (a multiple of 8 up to {HEAD_DIM})")
+    if any(t.device != q.device for t in others):
+        raise ValueError("every operand must be on q's device")
+    q_start = _index_vector("q_start", q_start, q.device)
+    if q_start.shape[0] == 0:
+        raise ValueError("q_start must hold one value more than there are sequences")
+    if scale is None:
+        scale = head_dim ** -0.5
+    scale = float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    fill = out is None
+    if fill:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _require_cuda("out", out)
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError("out must have q's shape, type and device")
+        if out.numel() and not _aligned_view(out):
+            raise ValueError("out must have a contiguous, 16-byte aligned head dimension")
+    lse = (torch.empty((heads, rows), dtype=torch.float32, device=q.device) if return_lse
+           else None)
+    workspace = torch.empty(
+        _sequence_workspace_bytes(rows, q_start.shape[0] - 1, heads, kv_heads, head_dim, max_keys),
+        dtype=torch.uint8, device=q.device)
+    return q, q_start, scale, out, fill, lse, workspace
+
+
+def packed_attention(q, k, v, q_start, k_start=None, causal=True, scale=None, out=None,
+                     return_lse=False):
+    """Attention over sequences of different lengths packed side by side.
+
+    q: [rows, heads, head_dim], k/v: [keys, kv_heads, head_dim], bf16 or fp16,
+    head_dim a multiple of 8 up to 128, heads a multiple of kv_heads (query head
+    h reads key/value head h // (heads / kv_heads)), any strides with a
+    contiguous head dim.  Sequence r has the rows ``q_start[r]`` ..
+    ``q_start[r + 1]`` of q and the same of k and v, or those of ``k_start``
+    (int32 on the device, ascending).  ``causal``: of n rows and m keys row t
+    attends to keys j <= t + m - n, so that the last row sees every key.  Lengths
+    are read on the device only; a call of fewer sequences passes equal starts.
+
+    Returns O [rows, heads, head_dim] (0 for rows that see no key) and, with
+    ``return_lse``, the natural-log LSE [heads, rows] fp32 (-inf for those).  Rows
+    outside every sequence are 0, or left as they were in a given ``out``.
+    Forward only, as every attention here.
+    """
+    lib = _lib.load()
+    k = _sequence_rows("k", k, q.dtype)
+    v = _sequence_rows("v", v, q.dtype)
+    if k.shape != v.shape or k.shape[2] != q.shape[-1]:
+        raise ValueError("k and v must share their shape, and q's head dimension")
+    k_rows, kv_heads = k.shape[:2]
+    q, q_start, scale, out, fill, lse, workspace = _sequence_call(
+        q, kv_heads, q_start, scale, out, return_lse, k_rows, (k, v))
+    rows, heads, head_dim = q.shape
+    requests = q_start.shape[0] - 1
+    if k_start is not None:
+        k_start = _index_vector("k_start", k_start, q.device, requests + 1)
+    if rows == 0:
+        return (out, lse) if return_lse else out
+    strides = _lib.int64_array([*_strides(q), *_strides(k), *_strides(v), *_strides(out)])
+    with torch.cuda.device(q.device):
+        status = lib.dsa_packed_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dtype_code(q.dtype),
+            strides, rows, k_rows, requests, heads, kv_heads, head_dim, q_start.data_ptr(),
+            k_start.data_ptr() if k_start is not None else None, scale, int(bool(causal)),
+            int(fill), lse.data_ptr() if lse is not None else None, workspace.data_ptr(),
+            workspace.numel(), _stream_handle(q.device))
+    _lib.check(status, "dsa_packed_attention")
+    return (out, lse) if return_lse else out
+
+
+def paged_attention(q, k_cache, v_cache, block_table, kv_lens, q_start, causal=True, scale=None,
+                    out=None, return_lse=False):
+    """Attention of new tokens over a paged key/value cache.
+
+    q: [rows, heads, head_dim] as in ``packed_attention``; request r has the
+    rows ``q_start[r]`` .. ``q_start[r + 1]`` and attends to the first
+    ``kv_lens[r]`` tokens (its new ones, already written, included) of the pages
+    in ``block_table[r]``.  One row per request is a decoding step, more are a
+    chunk of a prompt or of a video's next frames; ``causal=False`` lets every
+    row see every key.  k_cache, v_cache: [pages, page_size, kv_heads, head_dim],
+    page_size a power of two from 16, read in place.  A table entry outside the
+    cache takes no part: its keys are left out.  Returns as ``packed_attention``.
+    """
+    lib = _lib.load()
+    _require_cuda("q", q)
+    k_cache = _cache_view("k_cache", k_cache, q.dtype)
+    v_cache = _cache_view("v_cache", v_cache, q.dtype)
+    if k_cache.shape != v_cache.shape or q.ndim != 3 or k_cache.shape[3] != q.shape[2]:
+        raise ValueError("the caches must share their shape, and q [rows, heads, head_dim] "
+                         "their head dimension")
+    pages, page_size, kv_heads = k_cache.shape[:3]
+    _page_size(page_size)
+    _require_cuda("kv_lens", kv_lens)
+    kv_lens = _index_vector("kv_lens", kv_lens, q.device)
+    requests = kv_lens.shape[0]
+    block_table = _block_table(block_table, q.device, requests)
+    q_start = _index_vector("q_start", q_start, q.device, requests + 1)
+    width = block_table.shape[1]
+    q, q_start, scale, out, fill, lse, workspace = _sequence_call(
+        q, kv_heads, q_start, scale, out, return_lse, width * page_size, (k_cache, v_cache))
+    rows, heads, head_dim = q.shape
+    if rows == 0:
+        return (out, lse) if return_lse else out
+    strides = _lib.int64_array([*_strides(q), *_strides(k_cache), *_strides(v_cache),
+                                *_strides(out)])
+    with torch.cuda.device(q.device):
+        status = lib.dsa_paged_attention(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+            dtype_code(q.dtype), strides, rows, requests, heads, kv_heads, head_dim, pages,
+            page_size, block_table.data_ptr(), max(block_table.stride(0), width), width,
+            kv_lens.data_ptr(), q_start.data_ptr(), scale, int(bool(causal)), int(fill),
+            lse.data_ptr() if lse is not None else None, workspace.data_ptr(),
+            workspace.numel(), _stream_handle(q.device))
+    _lib.check(status, "dsa_paged_attention")
+    return (out, lse) if return_lse else out

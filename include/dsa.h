@@ -486,6 +486,77 @@ int dsa_gated_residual(const void* x, int64_t x_stride, const void* y, int64_t y
                        const float* gate, int32_t rows, int32_t dim, int32_t rows_per_group,
                        void* out, int64_t out_stride, hipStream_t stream);
 
+/*
+ * A paged key/value cache for sequences that grow: k_cache and v_cache are
+ * [pages, page_size, kv_heads, head_dim] tensors (page_size a power of two from
+ * 16), and token i of request r lies in row i % page_size of page
+ * table[r][i / page_size].  Slot = page * page_size + row.  The reference has no
+ * counterpart: its calls attend to whole tensors of one length.
+ *
+ * dsa_paged_plan: where a step's new tokens go.  cached[r] tokens of request r
+ * are in the cache, fresh[r] are new; the pages they need beyond the
+ * ceil(cached / page_size) already listed in its table row are taken from
+ * free_pages, in request order, and entered in the row.
+ *   q_start[requests + 1]: new tokens before each request; kv_lens[r] = cached
+ *   + fresh; slots[tokens]: the slot of every new token in request order, -1
+ *   for a token without a page (the free list or the row is too short; its
+ *   table entry becomes -1) and behind the last request's; status[2]: pages the
+ *   step needs (more than free_count: the first free_count were given out), and
+ *   new tokens without a slot.  Negative lengths count as 0.  Up to 8,192
+ *   requests.  Nothing but the new table entries changes, so a repeated call
+ *   gives the same plan.
+ *
+ * dsa_paged_write: row t of k and v [tokens, heads, row_bytes] into slot
+ * slots[t] of the caches; a slot outside them is skipped.  strides[10] in BYTES,
+ * multiples of 16: k (token, head), v (token, head), k_cache (page, token,
+ * head), v_cache (page, token, head).  Any element type; of tokens that share a
+ * slot one or parts of several are kept.
+ */
+int dsa_paged_plan(const int32_t* cached, const int32_t* fresh, int32_t requests, int32_t* table,
+                   int64_t table_stride, int32_t table_width, const int32_t* free_pages,
+                   int32_t free_count, int32_t page_size, int32_t tokens, int32_t* q_start,
+                   int32_t* kv_lens, int64_t* slots, int32_t* status, hipStream_t stream);
+int dsa_paged_write(const void* k, const void* v, void* k_cache, void* v_cache,
+                    const int64_t* strides, int32_t tokens, int32_t heads, int32_t row_bytes,
+                    int32_t pages, int32_t page_size, const int64_t* slots, hipStream_t stream);
+
+/*
+ * Attention of sequences of different lengths, bf16 or fp16, with heads /
+ * kv_heads query heads to a key/value head (dense.py:14-48 attends to one length
+ * with as many key heads as query heads).  Sequence r has the n = q_start[r + 1]
+ * - q_start[r] query rows from q_start[r] of q [q_rows, heads, head_dim], and m
+ * keys; row t attends to keys j < m or, causal, to j <= t + m - n (the last row
+ * sees every key).  A row that sees none gives 0 and an LSE of -inf.
+ *   dsa_packed_attention: the keys k_start[r] .. k_start[r + 1] of k and v
+ *     [k_rows, kv_heads, head_dim] (k_start NULL: q_start); strides[8], in
+ *     elements: q, k, v, o (token, head).
+ *   dsa_paged_attention: the first kv_lens[r] tokens of request r in the paged
+ *     cache; strides[10]: q (token, head), k_cache, v_cache (page, token, head),
+ *     o (token, head).  Keys of a table entry outside [0, pages) take no part.
+ *   Strides multiples of 8, pointers 16-byte aligned, head_dim a multiple of 8 up
+ *   to 128, scale > 0.  lse: [heads, q_rows] natural log or NULL.  fill = 1: rows
+ *   of o outside every sequence become 0; 0: they are left as they were (lse
+ *   has -inf there).  Starts and lengths are device arrays, never read on the host;
+ *   ones that leave the tensors are cut to them.  workspace: at least
+ *   dsa_seq_attention_workspace_bytes() with max_keys = k_rows, or table_width *
+ *   page_size; calls that overlap in time need one each.
+ */
+int dsa_packed_attention(const void* q, const void* k, const void* v, void* o, int32_t dtype,
+                         const int64_t* strides, int32_t q_rows, int32_t k_rows, int32_t requests,
+                         int32_t heads, int32_t kv_heads, int32_t head_dim,
+                         const int32_t* q_start, const int32_t* k_start, float scale,
+                         int32_t causal, int32_t fill, float* lse, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+int dsa_paged_attention(const void* q, const void* k_cache, const void* v_cache, void* o,
+                        int32_t dtype, const int64_t* strides, int32_t q_rows, int32_t requests,
+                        int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                        int32_t page_size, const int32_t* table, int64_t table_stride,
+                        int32_t table_width, const int32_t* kv_lens, const int32_t* q_start,
+                        float scale, int32_t causal, int32_t fill, float* lse, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32_t heads,
+                                         int32_t kv_heads, int32_t head_dim, int64_t max_keys);
+
 #ifdef __cplusplus
 }
 #endif

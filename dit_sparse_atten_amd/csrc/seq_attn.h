@@ -15,7 +15,7 @@
 // tiles: every key staged for a tile serves all heads of the group.  A tile's
 // keys may be cut into parts, whose fp32 partials seq_merge_kernel joins.
 // Lengths live on the device, so seq_schedule_kernel lists the (tile, part)
-// items there, near-equal in length, longest first; the grids are the host's
+// items there, longest first; the grids are the host's
 // upper bounds and workgroups past the list end at once.
 //
 //  * seq_wide_kernel: 128 rows, four waves of 32, the 64-key staged walk of
@@ -65,9 +65,10 @@ struct Params {
   float scale_log2;            // scale * log2(e)
   // Schedule.
   int32_t tile_rows, step_keys, min_chunk;
-  int32_t target;              // (tile, part, key head) items to cut the work into
-  int32_t max_items, max_splits, max_slots;  // room in the lists, per key head
-  int32_t* counts;             // items, split tiles
+  int32_t slots;               // workgroups that run at a time
+  int32_t max_tiles, max_items, max_splits, max_slots;  // room in the lists, per key head
+  float item_cost, part_cost, merge_cost;    // of an item and a partial, in key steps
+  int32_t* counts;             // items, split tiles, items that run by head groups
   int32_t* tile_base;          // [requests + 1] tiles before each sequence
   Item* items;
   Item* splits;                // split tiles: slot = the first of `parts` slots
@@ -82,6 +83,7 @@ __host__ __device__ constexpr int part_floats(int tile_rows, int dim) {
 
 constexpr float kRescaleLog2 = 8.0f;  // move the reference max once a p could exceed 2^8
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kHeadGroup = 8;  // key heads that run together: one per XCD
 constexpr int kWideRows = 128, kWideKeys = 64;
 constexpr int kNarrowRows = 16, kNarrowKeys = 128;  // 32 keys for each of four waves
 
@@ -105,26 +107,43 @@ __device__ __forceinline__ int k_swz(int r, int c) {
   return kD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
 }
 
-// The item's page table row, and the page of a key in it; an entry outside the
-// cache is -1: its keys are not read and take no part.
+// The page of a request's key in its block table row, as it stands there: an
+// entry outside [0, pages) is a bad page, whose keys are not read and take no part.
 __device__ __forceinline__ int page_at(const Params& p, int request, int key) {
-  const int id = p.table[(int64_t)request * p.table_stride + (key >> p.page_shift)];
-  return (unsigned)id < (unsigned)p.pages ? id : -1;
+  return p.table[(int64_t)request * p.table_stride + (key >> p.page_shift)];
 }
 
-// Resource of `rows` (<= 16) staged rows from key `key` of key head h: none
-// when they lie past the last key or in a bad page.
+// K or V of one key head: a row's bytes start at base + 16 (page page16 + row
+// row16), rows counted within the page (paged) or the sequence (packed).
+struct Source {
+  const unsigned char* base;
+  uint32_t page16, row16;
+};
 template <bool kPaged>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int64_t sp,
-                                                            int64_t st, int64_t sh, int h, int key,
-                                                            int k0, int page, int rows,
-                                                            const Params& p) {
-  if (kPaged && page < 0) rows = 0;
-  const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * st * 2 + p.head_dim * 2) : 0u;
-  const int64_t at = kPaged ? (int64_t)page * sp + (int64_t)(key & ((1 << p.page_shift) - 1)) * st
-                            : (int64_t)(k0 + key) * st;
-  return make_rsrc(static_cast<const unsigned char*>(base) + (rows > 0 ? (at + h * sh) * 2 : 0),
-                   bytes);
+__device__ __forceinline__ Source source_of(const void* tensor, int64_t sp, int64_t st, int64_t sh,
+                                            int h, int k0) {
+  return {static_cast<const unsigned char*>(tensor) + (h * sh + (kPaged ? 0 : k0 * st)) * 2,
+          (uint32_t)(sp >> 3), (uint32_t)(st >> 3)};
+}
+
+// Resource of the `rows` (at most 16) staged rows from row `row` of `page`: no
+// records, and so zeros, when there are none (the base is then never used).
+template <bool kPaged>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const Source& s, uint32_t page, int row,
+                                                            int rows, int head_dim) {
+  uint64_t at = (uint64_t)(uint32_t)row * s.row16;
+  if (kPaged) at += (uint64_t)page * s.page16;
+  const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * s.row16 * 16 + head_dim * 2 : 0u;
+  return make_rsrc(s.base + (at << 4), bytes);
+}
+
+// The kernel's arguments read again from memory: what only the end of a kernel
+// uses does not hold registers through its loop.
+typedef const __attribute__((address_space(4))) Params* LateParams;
+__device__ __forceinline__ LateParams late_params() {
+  auto at = (LateParams)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return at;
 }
 
 __device__ __forceinline__ Item load_item(const Item* at) {
@@ -141,12 +160,12 @@ __device__ __forceinline__ Item load_item(const Item* at) {
 // p is 0, and 0 times a value that is not finite is NaN, so a wave whose O is not
 // finite, and whose rows see different keys, takes this way instead.
 template <typename T, int kD, bool kPaged>
-__device__ __forceinline__ void exact_row(const Params& p, const Item& it, int h, int64_t q_at,
+__device__ __forceinline__ void exact_row(LateParams p, const Item& it, int h, int64_t q_at,
                                           int key_lo, int blocks, int stride, int width,
                                           int key_hi, float m_use, float acc[kD / 64]) {
   const int lane = threadIdx.x & 63;
   const int d0 = lane * (kD / 64);
-  const T* const q = static_cast<const T*>(p.q) + q_at;
+  const T* const q = static_cast<const T*>(p->q) + q_at;
 #pragma unroll
   for (int e = 0; e < kD / 64; ++e) acc[e] = 0.f;
 #pragma unroll 1
@@ -155,26 +174,29 @@ __device__ __forceinline__ void exact_row(const Params& p, const Item& it, int h
     if (key0 >= key_hi) break;
     const int key = key0 + lane;
     int page = -1;
-    if (lane < width && key < key_hi) page = kPaged ? page_at(p, it.request, key) : 0;
-    const int in_page = kPaged ? key & ((1 << p.page_shift) - 1) : it.k0 + key;
+    if (lane < width && key < key_hi) {
+      page = kPaged ? p->table[(int64_t)it.request * p->table_stride + (key >> p->page_shift)] : 0;
+      if (kPaged && (unsigned)page >= (unsigned)p->pages) page = -1;
+    }
+    const int in_page = kPaged ? key & ((1 << p->page_shift) - 1) : it.k0 + key;
     float prob = 0.f;
     if (page >= 0) {
-      const T* k = static_cast<const T*>(p.k) + page * p.k_sp + in_page * p.k_st + h * p.k_sh;
+      const T* k = static_cast<const T*>(p->k) + page * p->k_sp + in_page * p->k_st + h * p->k_sh;
       float s = 0.f;
 #pragma unroll 1
-      for (int d = 0; d < p.head_dim; ++d) s = fmaf((float)q[d], (float)k[d], s);
-      prob = __builtin_amdgcn_exp2f(fmaf(s, p.scale_log2, -m_use));
+      for (int d = 0; d < p->head_dim; ++d) s = fmaf((float)q[d], (float)k[d], s);
+      prob = __builtin_amdgcn_exp2f(fmaf(s, p->scale_log2, -m_use));
     }
 #pragma unroll 1
     for (int j = 0; j < width; ++j) {
       const int page_j = __shfl(page, j);
       if (page_j < 0) continue;
       const float prob_j = __shfl(prob, j);
-      const T* v = static_cast<const T*>(p.v) + page_j * p.v_sp +
-                   (int64_t)__shfl(in_page, j) * p.v_st + h * p.v_sh;
+      const T* v = static_cast<const T*>(p->v) + page_j * p->v_sp +
+                   (int64_t)__shfl(in_page, j) * p->v_st + h * p->v_sh;
 #pragma unroll
       for (int e = 0; e < kD / 64; ++e)
-        if (d0 + e < p.head_dim) acc[e] = fmaf(prob_j, (float)v[d0 + e], acc[e]);
+        if (d0 + e < p->head_dim) acc[e] = fmaf(prob_j, (float)v[d0 + e], acc[e]);
     }
   }
 }
@@ -194,6 +216,10 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   constexpr int kSlices = kD / 32;           // 1 KB loads per wave, K or V
   constexpr int kRowsPer = 64 / kChunks;     // rows of one load
   constexpr int kDt = kD / 32;               // 32-dim output tiles
+#ifndef KPRIO
+#define KPRIO 1
+#endif
+  constexpr bool kPrio = KPRIO;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[kStage];
@@ -202,8 +228,22 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   const int count = ((dsa::const_i32)p.counts)[0];
   const int wg = (int)blockIdx.x;
   if (wg >= count * p.kv_heads) return;
-  const int h = wg / count;
-  const Item it = load_item(p.items + (wg - h * count));
+  // The list's first `grouped` items run eight key heads at a time, so that each
+  // XCD streams the keys of one head through its L2; the others, which even out
+  // the end of the call, run all heads of one item before the next.  (40 heads of
+  // one query head, 16,384 x 16,384: 5.45 ms all heads at a time, 4.82 ms eight.)
+  const int grouped = ((dsa::const_i32)p.counts)[2];
+  int item, h;
+  if (wg < grouped * p.kv_heads) {
+    const int first = wg / (grouped * kHeadGroup) * kHeadGroup;
+    const int rest = wg - first * grouped, heads = min(kHeadGroup, p.kv_heads - first);
+    item = rest / heads;
+    h = first + rest - item * heads;
+  } else {
+    item = wg / p.kv_heads;
+    h = wg - item * p.kv_heads;
+  }
+  const Item it = load_item(p.items + item);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -270,37 +310,45 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
     const int key = window * 1024 + lane * 16;
     return key < kend ? page_at(p, it.request, key) : -1;
   };
-  int ids = -1, ids_next = -1, window = it.s0 >> 4;
+  int ids = -1, ids_next = -1;
+  uint64_t bad_ids = 0;  // the window's granules in bad pages
   if constexpr (kPaged) {
-    ids = window_ids(window);
-    ids_next = window_ids(window + 1);
+    ids = window_ids(it.s0 >> 4);
+    ids_next = window_ids((it.s0 >> 4) + 1);
+    bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
   }
-  // Stages step s; returns the keys' granules (bits 0..3) that lie in a bad page.
-  auto issue = [&](int s, unsigned char* kdst, unsigned char* vdst)
-      __attribute__((always_inline)) -> int {
-    const int key = s * kWideKeys + wave * 16;
-    int page = 0, bad = 0;
+  const Source ks = source_of<kPaged>(p.k, p.k_sp, p.k_st, p.k_sh, h, it.k0);
+  const Source vs = source_of<kPaged>(p.v, p.v_sp, p.v_st, p.v_sh, h, it.k0);
+  // Where step s of this wave's rows lies, worked out a step before its loads go
+  // out; bad: the granules (bits 0..3) of the step whose page is outside the cache.
+  __amdgpu_buffer_rsrc_t kr, vr;
+  int bad_next = 0;
+  auto locate = [&](int s) __attribute__((always_inline)) {
+    int row = s * kWideKeys + wave * 16;
+    int left = min(16, kend - row);
+    uint32_t page = 0;
     if constexpr (kPaged) {
-      if ((s >> 4) != window) {
-        window = s >> 4;
+      if ((s & 15) == 0) {  // the next window (step s0's is there already)
         ids = ids_next;
-        ids_next = window_ids(window + 1);
+        bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
+        ids_next = window_ids((s >> 4) + 1);
       }
-      page = __builtin_amdgcn_readlane(ids, (s & 15) * 4 + wave);
-      bad = (int)(__ballot(ids < 0) >> ((s & 15) * 4)) & 15;
+      page = (uint32_t)__builtin_amdgcn_readlane(ids, (s & 15) * 4 + wave);
+      bad_next = (int)(bad_ids >> ((s & 15) * 4)) & 15;
+      if (page >= (uint32_t)p.pages) left = 0;
+      row &= (1 << p.page_shift) - 1;
     }
-    const int left = min(16, kend - key);
-    const __amdgpu_buffer_rsrc_t kr =
-        rows_rsrc<kPaged>(p.k, p.k_sp, p.k_st, p.k_sh, h, key, it.k0, page, left, p);
-    const __amdgpu_buffer_rsrc_t vr =
-        rows_rsrc<kPaged>(p.v, p.v_sp, p.v_st, p.v_sh, h, key, it.k0, page, left, p);
+    kr = rows_rsrc<kPaged>(ks, page, row, left, p.head_dim);
+    vr = rows_rsrc<kPaged>(vs, page, row, left, p.head_dim);
+  };
+  // (the empty asm keeps the stage addresses from being held for every load)
+  auto issue = [&](unsigned char* kdst, unsigned char* vdst) __attribute__((always_inline)) {
+    int at = wave * kSlices * 1024;
+    asm volatile("" : "+s"(at));
 #pragma unroll
-    for (int j = 0; j < kSlices; ++j)
-      lds_load16(kr, kdst + (wave * kSlices + j) * 1024, koff[j], 0);
+    for (int j = 0; j < kSlices; ++j) lds_load16(kr, kdst + at + j * 1024, koff[j], 0);
 #pragma unroll
-    for (int j = 0; j < kSlices; ++j)
-      lds_load16(vr, vdst + (wave * kSlices + j) * 1024, voff[j], 0);
-    return bad;
+    for (int j = 0; j < kSlices; ++j) lds_load16(vr, vdst + at + j * 1024, voff[j], 0);
   };
 
   float m_run = -INFINITY, l_run = 0.f;
@@ -385,6 +433,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
         pf[j][t + 1] = pb[1];
       }
     l_run += sum0 + sum1;
+    if (kPrio) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -396,19 +445,30 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
         const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         oacc[dt] = E::mfma32(a, pf[j], oacc[dt]);
       }
+    if (kPrio) __builtin_amdgcn_s_setprio(0);
   };
-  int bad_cur = 0, bad_next = 0;
+  int bad_cur = 0, bad_ahead = 0;  // of the staged step and of the one on its way
   auto step = [&](int s, const unsigned char* kc, const unsigned char* vc, unsigned char* kn,
                   unsigned char* vn) __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(vmcnt(0));
     __syncthreads();
-    if (s + 1 < it.s1) bad_next = issue(s + 1, kn, vn);
+    if (s + 1 < it.s1) {
+      issue(kn, vn);
+      bad_ahead = bad_next;
+      locate(s + 2);  // (past the last key: no rows)
+    }
     // (a wave whose rows see none of the step's keys only stages)
     if (wave_active && s * kWideKeys < lim_last) compute(kc, vc, s * kWideKeys, bad_cur);
-    bad_cur = bad_next;
+    bad_cur = bad_ahead;
   };
   if (it.s0 < it.s1) {
-    bad_cur = issue(it.s0, lds_k0, lds_v0);
+    if constexpr (kPaged) {
+      if ((it.s0 & 15) == 0) ids_next = ids;  // locate() takes it up
+    }
+    locate(it.s0);
+    issue(lds_k0, lds_v0);
+    bad_cur = bad_next;
+    locate(it.s0 + 1);
     for (int s = it.s0; s < it.s1; s += 2) {
       step(s, lds_k0, lds_v0, lds_k1, lds_v1);
       if (s + 1 >= it.s1) break;
@@ -416,6 +476,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
     }
   }
 
+  const LateParams late = late_params();
   const float l_tot = dsa::pair32_sum(l_run);
   float unfinite = 0.f;  // NaN once an element of O is not finite
 #pragma unroll
@@ -435,7 +496,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
       const float l_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_tot), r));
       const int lim_r = __builtin_amdgcn_readlane(lim, r);
       float acc[kD / 64];
-      exact_row<T, kD, kPaged>(p, it, h, (it.q0 + token_r) * p.q_st + head_r * p.q_sh,
+      exact_row<T, kD, kPaged>(late, it, h, (it.q0 + token_r) * late->q_st + head_r * late->q_sh,
                                it.s0 * kWideKeys, it.s1 - it.s0, kWideKeys, kWideKeys,
                                min(lim_r, it.s1 * kWideKeys), m_r == -INFINITY ? 0.f : m_r, acc);
       const float inv = l_r > 0.f ? 1.f / l_r : (l_r == 0.f ? 0.f : l_r);
@@ -443,17 +504,17 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
       for (int e = 0; e < kD / 64; ++e) {
         const int d = lane * (kD / 64) + e;
         if (it.slot >= 0)
-          p.part[((int64_t)it.slot * p.kv_heads + h) * part_floats(kWideRows, kD) +
+          late->part[((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD) +
                  (wave * 32 + r) * kD + d] = acc[e];
-        else if (d < p.head_dim)
-          static_cast<T*>(p.o)[(it.q0 + token_r) * p.o_st + head_r * p.o_sh + d] =
+        else if (d < late->head_dim)
+          static_cast<T*>(late->o)[(it.q0 + token_r) * late->o_st + head_r * late->o_sh + d] =
               (T)(acc[e] * inv);
       }
     }
   }
   if (!row_ok) return;
   if (it.slot >= 0) {
-    float* po = p.part + ((int64_t)it.slot * p.kv_heads + h) * part_floats(kWideRows, kD);
+    float* po = late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD);
     float* prow = po + local * kD;
     if (!redo)
 #pragma unroll
@@ -471,7 +532,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
     return;
   }
   const float inv = l_tot > 0.f ? 1.f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
-  T* orow = static_cast<T*>(p.o) + (int64_t)(it.q0 + token) * p.o_st + head * p.o_sh;
+  T* orow = static_cast<T*>(late->o) + (int64_t)(it.q0 + token) * late->o_st + head * late->o_sh;
   if (!redo)
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt)
@@ -480,11 +541,11 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
       typename E::x4 v4;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v4[e] = (T)(oacc[dt][rr * 4 + e] * inv);
-      if (dt * 32 + rr * 8 + g * 4 < p.head_dim)
+      if (dt * 32 + rr * 8 + g * 4 < late->head_dim)
         *reinterpret_cast<typename E::x4*>(orow + dt * 32 + rr * 8 + g * 4) = v4;
     }
-  if (p.lse && g == 0)
-    p.lse[(int64_t)head * p.q_rows + it.q0 + token] =
+  if (late->lse && g == 0)
+    late->lse[(int64_t)head * late->q_rows + it.q0 + token] =
         l_tot == 0.f ? -INFINITY : m_run * kLn2 + logf(l_tot);
 }
 
@@ -555,39 +616,47 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
     const int key = (window * 32 + (lane >> 1)) * kNarrowKeys + wave * 32 + (lane & 1) * 16;
     return key < kend ? page_at(p, it.request, key) : -1;
   };
-  int ids = -1, ids_next = -1, window = it.s0 >> 5;
+  int ids = -1, ids_next = -1, bad_next = 0;
+  uint64_t bad_ids = 0;  // the window's granules in bad pages
   if constexpr (kPaged) {
-    ids = window_ids(window);
-    ids_next = window_ids(window + 1);
+    ids = window_ids(it.s0 >> 5);
+    ids_next = (it.s0 & 31) == 0 ? ids : window_ids((it.s0 >> 5) + 1);
+    bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
   }
+  const Source ks = source_of<kPaged>(p.k, p.k_sp, p.k_st, p.k_sh, h, it.k0);
+  const Source vs = source_of<kPaged>(p.v, p.v_sp, p.v_st, p.v_sh, h, it.k0);
   auto issue = [&](int s, unsigned char* kdst, unsigned char* vdst)
-      __attribute__((always_inline)) -> int {
+      __attribute__((always_inline)) {
     const int key = s * kNarrowKeys + wave * 32;
-    int bad = 0;
+    int at = wave * kStage;
+    asm volatile("" : "+s"(at));
     if constexpr (kPaged) {
-      if ((s >> 5) != window) {
-        window = s >> 5;
+      if ((s & 31) == 0) {  // the next window (the first step's is there already)
         ids = ids_next;
-        ids_next = window_ids(window + 1);
+        bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
+        ids_next = window_ids((s >> 5) + 1);
       }
-      bad = (int)(__ballot(ids < 0) >> ((s & 31) * 2)) & 3;
+      bad_next = (int)(bad_ids >> ((s & 31) * 2)) & 3;
     }
 #pragma unroll
     for (int kg = 0; kg < 2; ++kg) {
-      const int page = kPaged ? __builtin_amdgcn_readlane(ids, (s & 31) * 2 + kg) : 0;
-      const int left = min(16, kend - key - 16 * kg);
-      const __amdgpu_buffer_rsrc_t kr =
-          rows_rsrc<kPaged>(p.k, p.k_sp, p.k_st, p.k_sh, h, key + 16 * kg, it.k0, page, left, p);
-      const __amdgpu_buffer_rsrc_t vr =
-          rows_rsrc<kPaged>(p.v, p.v_sp, p.v_st, p.v_sh, h, key + 16 * kg, it.k0, page, left, p);
+      int row = key + 16 * kg;
+      int left = min(16, kend - row);
+      uint32_t page = 0;
+      if constexpr (kPaged) {
+        page = (uint32_t)__builtin_amdgcn_readlane(ids, (s & 31) * 2 + kg);
+        if (page >= (uint32_t)p.pages) left = 0;
+        row &= (1 << p.page_shift) - 1;
+      }
+      const __amdgpu_buffer_rsrc_t kr = rows_rsrc<kPaged>(ks, page, row, left, p.head_dim);
+      const __amdgpu_buffer_rsrc_t vr = rows_rsrc<kPaged>(vs, page, row, left, p.head_dim);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j)
-        lds_load16(kr, kdst + wave * kStage + (kg * kLoads + j) * 1024, koff[j], 0);
+        lds_load16(kr, kdst + at + (kg * kLoads + j) * 1024, koff[j], 0);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j)
-        lds_load16(vr, vdst + wave * kStage + (kg * kLoads + j) * 1024, voff[j], 0);
+        lds_load16(vr, vdst + at + (kg * kLoads + j) * 1024, voff[j], 0);
     }
-    return bad;
   };
 
   float m_run = -INFINITY, l_run = 0.f;
@@ -668,11 +737,11 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
     }
   };
   // A wave's stages are its own: it waits for its loads alone.
-  int bad_cur = 0, bad_next = 0;
+  int bad_cur = 0;
   auto step = [&](int s, const unsigned char* kc, const unsigned char* vc, unsigned char* kn,
                   unsigned char* vn) __attribute__((always_inline)) {
     if (s + 1 < it.s1) {
-      bad_next = issue(s + 1, kn, vn);
+      issue(s + 1, kn, vn);
       __builtin_amdgcn_s_waitcnt(vmcnt(4 * kLoads));
     } else {
       __builtin_amdgcn_s_waitcnt(vmcnt(0));
@@ -682,7 +751,8 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
     bad_cur = bad_next;
   };
   if (it.s0 < it.s1) {
-    bad_cur = issue(it.s0, lds_k0, lds_v0);
+    issue(it.s0, lds_k0, lds_v0);
+    bad_cur = bad_next;
     for (int s = it.s0; s < it.s1; s += 2) {
       step(s, lds_k0, lds_v0, lds_k1, lds_v1);
       if (s + 1 >= it.s1) break;
@@ -690,6 +760,7 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
     }
   }
 
+  const LateParams late = late_params();
   // Join the waves: their O, m and l through the K stages (row-major fp32).
   l_run += __shfl_xor(l_run, 16);
   const float l_wave = dsa::pair32_sum(l_run);
@@ -712,12 +783,12 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
       const int head_r = __builtin_amdgcn_readlane(head, r);
       const float m_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), r));
       float acc[kD / 64];
-      exact_row<T, kD, kPaged>(p, it, h, (it.q0 + token_r) * p.q_st + head_r * p.q_sh,
+      exact_row<T, kD, kPaged>(late, it, h, (it.q0 + token_r) * late->q_st + head_r * late->q_sh,
                                it.s0 * kNarrowKeys + wave * 32, it.s1 - it.s0, kNarrowKeys, 32,
                                __builtin_amdgcn_readlane(lim, r), m_r == -INFINITY ? 0.f : m_r,
                                acc);
 #pragma unroll
-      for (int e = 0; e < kD / 64; ++e) mine[r * kD + lane * (kD / 64) + e] = acc[e];
+      for (int x = 0; x < kD / 64; ++x) mine[r * kD + lane * (kD / 64) + x] = acc[x];
     }
   } else {
 #pragma unroll
@@ -745,16 +816,16 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
   }
   float acc[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  for (int x = 0; x < 8; ++x) acc[x] = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (w[i] == 0.f) continue;
     const float* src = reinterpret_cast<const float*>(lds_k0) + (i * kNarrowRows + r) * kD + d0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(w[i], src[e], acc[e]);
+    for (int x = 0; x < 8; ++x) acc[x] = fmaf(w[i], src[x], acc[x]);
   }
   if (it.slot >= 0) {
-    float* po = p.part + ((int64_t)it.slot * p.kv_heads + h) * part_floats(kNarrowRows, kD);
+    float* po = late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kNarrowRows, kD);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
       *reinterpret_cast<dsa_f32x4*>(po + r * kD + d0 + 4 * c) =
@@ -765,18 +836,18 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
     }
     return;
   }
-  const int out_token = it.q0 + out_row / p.group;
-  const int out_head = h * p.group + out_row % p.group;
+  const int out_token = it.q0 + out_row / late->group;
+  const int out_head = h * late->group + out_row % late->group;
   const float inv = l_all > 0.f ? 1.f / l_all : (l_all == 0.f ? 0.f : l_all);
-  if (d0 < p.head_dim) {
+  if (d0 < late->head_dim) {
     x8 y;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (T)(acc[e] * inv);
-    *reinterpret_cast<x8*>(static_cast<T*>(p.o) + (int64_t)out_token * p.o_st +
-                           out_head * p.o_sh + d0) = y;
+    for (int x = 0; x < 8; ++x) y[x] = (T)(acc[x] * inv);
+    *reinterpret_cast<x8*>(static_cast<T*>(late->o) + (int64_t)out_token * late->o_st +
+                           out_head * late->o_sh + d0) = y;
   }
-  if (p.lse && d0 == 0)
-    p.lse[(int64_t)out_head * p.q_rows + out_token] =
+  if (late->lse && d0 == 0)
+    late->lse[(int64_t)out_head * late->q_rows + out_token] =
         l_all == 0.f ? -INFINITY : m_all * kLn2 + logf(l_all);
 }
 

@@ -5,26 +5,41 @@
 
 namespace seq {
 
-constexpr int kScheduleThreads = 1024;
-constexpr int kLdsRequests = 4096;  // sequences whose tile counts the schedule keeps in LDS
+constexpr int kLdsRequests = 1024;  // sequences the schedule keeps in LDS
+constexpr int kLdsTiles = 2048;     // tiles whose lengths it keeps there
 constexpr int kBuckets = 256;       // item lengths are ordered to 1/256 of the longest
+constexpr int kManyParts = 8;       // tiles of more parts are listed by the whole workgroup
+// Parts that the longest tile may be cut into, tried on calls of few tiles.
+__constant__ const short kTryParts[32] = {1,  2,  3,  4,  5,  6,  7,  8,   9,   10,  11,  12,  14, 16,
+                                          18, 20, 24, 28, 32, 40, 48, 56,  64,  80,  96,  112, 128,
+                                          160, 192, 256, 384, 512};
 
-// Inclusive sum over the workgroup, `total` for every thread.  `lds` holds 16.
-__device__ __forceinline__ uint64_t group_scan(uint64_t v, uint64_t* lds, uint64_t* total) {
+// Inclusive sum over the 64 lanes (row shifts by 1, 2, 4, 8, then the row sums
+// broadcast into the rows behind).  Every lane of the wave must be active.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
+// Inclusive sum over the workgroup, `total` for every thread.
+template <int kThreads>
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t other = (uint64_t)__shfl_up((unsigned long long)v, d);
-    if (lane >= d) v += other;
-  }
+  v = wave_scan(v);
   dsa::lds_barrier();  // the last scan's reads are done
   if (lane == 63) lds[wave] = v;
   dsa::lds_barrier();
-  uint64_t before = 0, all = 0;
+  uint32_t before = 0, all = 0;
 #pragma unroll
-  for (int i = 0; i < kScheduleThreads / 64; ++i) {
-    if (i < wave) before += lds[i];
-    all += lds[i];
+  for (int i = 0; i < kThreads / 64; ++i) {
+    const uint32_t x = lds[i];
+    if (i < wave) before += x;
+    all += x;
   }
   *total = all;
   return before + v;
@@ -65,12 +80,23 @@ __device__ __forceinline__ int steps_of(const Params& p, const Sequence& s, int 
 }
 
 // Workgroup 0 lists the call's items and split tiles; the others give the rows
-// that belong to no sequence their values (O 0 with p.fill, LSE -inf).  Parts: a tile longer than `chunk` steps
-// is cut into near-equal parts of at most that, with chunk = the whole work /
-// p.target, so that `target` workgroups share it evenly.  A call of more items
-// than that is ordered longest first, by a counting sort of the lengths (the
-// order inside a bucket is that of the atomics; no result depends on it).
-__global__ void __launch_bounds__(kScheduleThreads) seq_schedule_kernel(Params p, int esize) {
+// that belong to no sequence their values (O 0 with p.fill, LSE -inf).
+//
+// The workgroups of the chip (p.slots at a time) take items in list order, all
+// key heads of one before the next, longest first.  Which tiles are cut, in units
+// of one tile's key steps, with `work` the steps of all tiles and heads:
+//  * up to one round of tiles: every tile longer than `chunk` in near-equal
+//    parts of at most that.  Each candidate (the longest tile in 1, 2, 3, ..
+//    512 parts) costs rounds x (mean length + p.item_cost), or its share of the
+//    work plus half the longest part if that is more; the cheapest is taken.
+//  * more: whole tiles, longest first, even out by themselves but for the last
+//    round.  Tiles longer than a slot's share of the work are cut to it; if there
+//    are none, the shortest tiles, as many as the last round is short of full,
+//    are cut into as many parts as pay.
+// Parts cost their partials (p.part_cost).  No choice depends on the order of
+// the atomics that place items of nearly equal length.
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     const int first = min(max(p.q_start[0], 0), p.q_rows);
@@ -80,38 +106,56 @@ __global__ void __launch_bounds__(kScheduleThreads) seq_schedule_kernel(Params p
     const dsa_u32x4 zero = {0u, 0u, 0u, 0u};
     for (int i = blockIdx.x - 1; i < empty; i += gridDim.x - 1) {
       const int row = i < first ? i : last + i - first;
-      for (int c = tid; p.fill && c < chunks; c += kScheduleThreads) {
+      for (int c = tid; p.fill && c < chunks; c += kThreads) {
         const int head = c / (p.head_dim / 8), d = c % (p.head_dim / 8) * 8;
-        *reinterpret_cast<dsa_u32x4*>(static_cast<unsigned char*>(p.o) +
-                                      ((int64_t)row * p.o_st + head * p.o_sh + d) * esize) = zero;
+        *reinterpret_cast<dsa_u32x4*>(static_cast<uint16_t*>(p.o) + (int64_t)row * p.o_st +
+                                      head * p.o_sh + d) = zero;
       }
       if (p.lse)
-        for (int head = tid; head < p.heads; head += kScheduleThreads)
+        for (int head = tid; head < p.heads; head += kThreads)
           p.lse[(int64_t)head * p.q_rows + row] = -INFINITY;
     }
     return;
   }
-  __shared__ uint64_t scan_lds[kScheduleThreads / 64];
+  __shared__ uint32_t scan_lds[kThreads / 64];
+  __shared__ Sequence seq_lds[kLdsRequests];
   __shared__ int base_lds[kLdsRequests + 1];
+  __shared__ int tile_steps[kLdsTiles];
   __shared__ int hist[kBuckets];
+  __shared__ uint32_t tried[32];
+  __shared__ int many[3][kLdsTiles / kManyParts];  // tile, place, slot of the tiles of many parts
   __shared__ unsigned long long work_lds;
-  __shared__ int longest_lds;
-  int* const base = p.requests <= kLdsRequests ? base_lds : p.tile_base;
+  __shared__ int longest_lds, many_count, grouped_lds, chunk_lds, tail_parts, cut_bucket, cut_left;
+  const bool in_lds = p.requests <= kLdsRequests;
+  int* const base = in_lds ? base_lds : p.tile_base;
+  auto seq_of = [&](int r) -> Sequence { return in_lds ? seq_lds[r] : sequence(p, r); };
   if (tid == 0) {
     work_lds = 0;
     longest_lds = 0;
+    many_count = 0;
+    grouped_lds = 0;
+    tail_parts = 1;
+    cut_bucket = kBuckets;
+    cut_left = 0;
   }
+  if (tid < 32) tried[tid] = 0;
   // Tiles before each sequence.
-  uint64_t total = 0, before = 0;
-  for (int r0 = 0; r0 < p.requests; r0 += kScheduleThreads) {
+  uint32_t total = 0;
+  uint64_t before = 0;
+  for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
     const int r = r0 + tid;
-    const int tiles = r < p.requests ? tiles_of(p, sequence(p, r)) : 0;
-    const uint64_t upto = group_scan((uint64_t)tiles, scan_lds, &total);
-    if (r < p.requests) base[r] = (int)(before + upto - tiles);
+    int count = 0;
+    if (r < p.requests) {
+      const Sequence s = sequence(p, r);
+      if (in_lds) seq_lds[r] = s;
+      count = tiles_of(p, s);
+    }
+    const uint32_t upto = group_scan<kThreads>((uint32_t)count, scan_lds, &total);
+    if (r < p.requests) base[r] = (int)min(before + upto - count, (uint64_t)p.max_tiles);
     before += total;
   }
   // (starts that overlap list more tiles than the lists have room for)
-  const int tiles = (int)min(before, (uint64_t)p.max_items);
+  const int tiles = (int)min(before, (uint64_t)p.max_tiles);
   if (tid == 0) base[p.requests] = tiles;
   __syncthreads();
   auto find = [&](int i) -> int {  // the last sequence with base <= i
@@ -123,84 +167,226 @@ __global__ void __launch_bounds__(kScheduleThreads) seq_schedule_kernel(Params p
     }
     return lo;
   };
-  // The work, in key steps of one key head, and the longest tile.
-  uint64_t mine = 0;
-  int longest = 0;
-  for (int i = tid; i < tiles; i += kScheduleThreads) {
+  auto length = [&](int i) -> int {
     const int r = find(i);
-    const int steps = steps_of(p, sequence(p, r), i - base[r]);
-    mine += steps;
-    longest = max(longest, steps);
+    return steps_of(p, seq_of(r), i - base[r]);
+  };
+  auto steps_at = [&](int i) -> int { return i < kLdsTiles ? tile_steps[i] : length(i); };
+  // The work, in key steps of one key head, and the longest tile.
+  {
+    unsigned long long mine = 0;
+    int longest = 0;
+    for (int i = tid; i < tiles; i += kThreads) {
+      const int steps = length(i);
+      if (i < kLdsTiles) tile_steps[i] = steps;
+      mine += steps;
+      longest = max(longest, steps);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      mine += __shfl_xor(mine, d);
+      longest = max(longest, __shfl_xor(longest, d));
+    }
+    if ((tid & 63) == 0) {
+      atomicAdd(&work_lds, mine);
+      atomicMax(&longest_lds, longest);
+    }
   }
-  atomicAdd(&work_lds, (unsigned long long)mine);
-  atomicMax(&longest_lds, longest);
   __syncthreads();
-  const uint64_t work = work_lds * (uint64_t)p.kv_heads;
-  const int chunk =
-      (int)max((work + p.target - 1) / (uint64_t)p.target, (uint64_t)p.min_chunk);
-  const int longest_part = min(longest_lds, chunk);
-  auto parts_of = [&](int steps) { return max(1, (steps + chunk - 1) / chunk); };
-  // Calls of more than one round of workgroups list the longest first.
-  const bool sorted = (int64_t)tiles * p.kv_heads > p.target;
-  auto bucket = [&](int length) {
-    return longest_part > 0 ? (kBuckets - 1) - (int)((int64_t)length * (kBuckets - 1) / longest_part)
-                            : 0;
+  const int longest = longest_lds;
+  const int64_t work = (int64_t)work_lds * p.kv_heads, count = (int64_t)tiles * p.kv_heads;
+  const int slots = p.slots;
+  const int whole = max(longest, 1);  // a chunk that cuts nothing
+  auto bucket = [&](int steps) {      // of whole tiles, longest first
+    return (kBuckets - 1) - (int)((int64_t)steps * (kBuckets - 1) / whole);
+  };
+  if (p.max_slots == 0 || longest < 2 * p.min_chunk || tiles == 0) {
+    if (tid == 0) chunk_lds = whole;
+  } else if (count <= slots) {
+    // Up to a round of tiles: at most `slots` <= kLdsTiles of them.
+    const int which = tid & 31;
+    const int chunk = max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which]);
+    uint32_t items = 0;
+    for (int i = tid >> 5; i < tiles; i += kThreads / 32)
+      items += max(1, (tile_steps[i] + chunk - 1) / chunk);
+    atomicAdd(&tried[which], items);
+    __syncthreads();
+    if (tid < 64) {
+      const int64_t n = (int64_t)tried[which] * p.kv_heads;
+      const float cost = p.item_cost + (which > 0 ? p.part_cost : 0.f);
+      const float mean = (float)work / (float)n + cost;
+      const float rounds = (float)((n + slots - 1) / slots);
+      const float even = ((float)work + cost * (float)n) / (float)slots;
+      float price = n <= slots ? (float)chunk + cost
+                               : fmaxf(rounds * mean, even + 0.5f * ((float)chunk + cost));
+      if (which > 0) price += p.merge_cost * (float)n;
+      if (which > 0 && tried[which] > (uint32_t)p.max_slots) price = INFINITY;
+      int best = which;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const float other = __shfl_xor(price, d);
+        const int its = __shfl_xor(best, d);
+        if (other < price || (other == price && its < best)) {
+          price = other;
+          best = its;
+        }
+      }
+      if (tid == 0)
+        chunk_lds = max(p.min_chunk, (longest + kTryParts[best] - 1) / kTryParts[best]);
+    }
+  } else {
+    const int share = (int)max((work + slots - 1) / slots, (int64_t)p.min_chunk);
+    if (longest > share) {
+      if (tid == 0) chunk_lds = share;
+    } else {
+      // The K shortest tiles fill the last round: found by their bucket, and in
+      // the bucket that K ends in by their order.
+      const int k = (int)((count % slots + p.kv_heads - 1) / p.kv_heads);
+      if (tid < kBuckets) hist[tid] = 0;
+      __syncthreads();
+      for (int i = tid; i < tiles; i += kThreads) atomicAdd(&hist[bucket(steps_at(i))], 1);
+      __syncthreads();
+      const uint32_t own = tid < kBuckets ? hist[tid] : 0;
+      const uint32_t upto = group_scan<kThreads>(own, scan_lds, &total);
+      // (bucket tid holds the ranks upto - own .. upto - 1, longest first)
+      const int from = tiles - k;  // first rank of the tail
+      if (k > 0 && tid < kBuckets && (int)upto > from && (int)(upto - own) <= from) {
+        const float steps = (float)(kBuckets - tid) * (float)whole / (float)(kBuckets - 1);
+        float best = steps + p.item_cost;
+        int parts = 1;
+        for (int q = 2; q <= 8; ++q) {
+          const int64_t n = (int64_t)k * q * p.kv_heads;
+          if ((int64_t)k * q > p.max_slots || steps < (float)(q * p.min_chunk)) break;
+          const float price =
+              (float)((n + slots - 1) / slots) * (steps / (float)q + p.item_cost + p.part_cost) +
+              p.merge_cost * (float)n;
+          if (price < best) {
+            best = price;
+            parts = q;
+          }
+        }
+        tail_parts = parts;
+        cut_bucket = tid;
+        cut_left = (int)upto - from;  // of this bucket, its first tiles in order
+      }
+      if (tid == 0) chunk_lds = whole;
+    }
+  }
+  __syncthreads();
+  const int chunk = chunk_lds, tail = tail_parts, cut_at = cut_bucket;
+  // Parts of tile i; `seen`: tiles of the cut bucket before it.
+  auto parts_of = [&](int steps, uint32_t seen) -> int {
+    if (tail > 1) {
+      const int at = bucket(steps);
+      return at > cut_at || (at == cut_at && (int)seen < cut_left) ? tail : 1;
+    }
+    return max(1, (steps + chunk - 1) / chunk);
+  };
+  // Two sweeps over the tiles in order: the lengths' histogram, then the lists
+  // (calls that fit one round need no order).
+  const bool sorted = count > slots || chunk < whole;
+  const int longest_part = max(1, min(whole, chunk));
+  // (a tail's parts come last of all)
+  auto place_bucket = [&](int steps, int parts) {
+    const int len = min((steps + parts - 1) / parts, longest_part);
+    const int at = (kBuckets - 1) - (int)((int64_t)len * (kBuckets - 1) / longest_part);
+    return tail > 1 ? (parts > 1 ? kBuckets - 1 : min(at, kBuckets - 2)) : at;
   };
   if (sorted) {
     if (tid < kBuckets) hist[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < tiles; i += kScheduleThreads) {
-      const int r = find(i);
-      const int steps = steps_of(p, sequence(p, r), i - base[r]);
-      const int parts = parts_of(steps);
-      atomicAdd(&hist[bucket((steps + parts - 1) / parts)], parts);
-    }
-    __syncthreads();
-    const int count = tid < kBuckets ? hist[tid] : 0;
-    const uint64_t upto = group_scan((uint64_t)count, scan_lds, &total);
-    __syncthreads();
-    if (tid < kBuckets) hist[tid] = (int)upto - count;
-    __syncthreads();
   }
-  // Items, split tiles and partial slots, in tile order: 21 bits each.
-  uint64_t sums = 0;
-  for (int i0 = 0; i0 < tiles; i0 += kScheduleThreads) {
-    const int i = i0 + tid;
-    Item it = {};
-    int steps = 0, parts = 0;
-    if (i < tiles) {
+  uint32_t items = 0, split_sums = 0;
+  for (int sweep = sorted ? 0 : 1; sweep < 2; ++sweep) {
+    uint32_t seen = 0;
+    for (int i0 = 0; i0 < tiles; i0 += kThreads) {
+      const int i = i0 + tid;
+      const int steps = i < tiles ? steps_at(i) : 0;
+      uint32_t cut_before = 0;
+      if (tail > 1) {
+        const uint32_t flag = i < tiles && bucket(steps) == cut_at;
+        cut_before = seen + group_scan<kThreads>(flag, scan_lds, &total) - flag;
+        seen += total;
+      }
+      const int parts = i < tiles ? parts_of(steps, cut_before) : 0;
+      if (sweep == 0) {
+        if (parts > 0) atomicAdd(&hist[place_bucket(steps, parts)], parts);
+        continue;
+      }
+      const bool split = parts > 1;
+      int place = 0;
+      if (sorted) {
+        if (parts > 0) place = atomicAdd(&hist[place_bucket(steps, parts)], parts);
+      } else {
+        place = (int)(items + group_scan<kThreads>((uint32_t)parts, scan_lds, &total)) - parts;
+        items += total;
+      }
+      // Slots and split tiles in tile order: 16 bits each.
+      uint32_t at = 0;
+      if (p.max_slots > 0) {
+        const uint32_t own = split ? (uint32_t)parts << 16 | 1u : 0u;
+        at = split_sums + group_scan<kThreads>(own, scan_lds, &total) - own;
+        split_sums += total;
+      }
+      if (parts == 0) continue;
+      Item it = {};
       it.request = find(i);
-      const Sequence s = sequence(p, it.request);
+      const Sequence s = seq_of(it.request);
       it.q0 = s.q0; it.n = s.n; it.k0 = s.k0; it.m = s.m;
       it.tile = i - base[it.request];
-      steps = steps_of(p, s, it.tile);
-      parts = parts_of(steps);
+      it.parts = parts;
+      const int slot0 = (int)(at >> 16), split0 = (int)(at & 0xffff);
+      if (split && split0 < p.max_splits) {
+        it.slot = slot0;
+        p.splits[split0] = it;
+      }
+      if (parts > kManyParts && i < kLdsTiles) {
+        const int n = atomicAdd(&many_count, 1);
+        many[0][n] = i; many[1][n] = place; many[2][n] = slot0;
+        tile_steps[i] = steps;
+        continue;
+      }
+      for (int j = 0; j < parts; ++j) {
+        it.s0 = (int)((int64_t)steps * j / parts);
+        it.s1 = (int)((int64_t)steps * (j + 1) / parts);
+        it.slot = split ? slot0 + j : -1;
+        if (place + j < p.max_items) p.items[place + j] = it;
+      }
     }
-    const bool split = parts > 1;
-    const uint64_t own = (uint64_t)parts | (uint64_t)(split ? parts : 0) << 21 |
-                         (uint64_t)(split ? 1 : 0) << 42;
-    const uint64_t at = sums + group_scan(own, scan_lds, &total) - own;
-    sums += total;
-    const int item0 = (int)(at & 0x1fffff), slot0 = (int)(at >> 21 & 0x1fffff),
-              split0 = (int)(at >> 42);
-    it.parts = parts;
-    if (split && split0 < p.max_splits) {
-      it.slot = slot0;
-      p.splits[split0] = it;
-    }
-    const int place = sorted && parts > 0
-                          ? atomicAdd(&hist[bucket((steps + parts - 1) / parts)], parts)
-                          : item0;
-    for (int j = 0; j < parts; ++j) {
-      it.s0 = (int)((int64_t)steps * j / parts);
-      it.s1 = (int)((int64_t)steps * (j + 1) / parts);
-      it.slot = split ? slot0 + j : -1;
-      if (place + j < p.max_items) p.items[place + j] = it;
+    if (sweep == 0) {
+      __syncthreads();
+      const uint32_t own = tid < kBuckets ? hist[tid] : 0;
+      const uint32_t upto = group_scan<kThreads>(own, scan_lds, &total);
+      items = total;
+      if (tid < kBuckets) hist[tid] = (int)(upto - own);
+      // By head groups: whole tiles before a tail, else those of more than half
+      // the longest's length; a call that cuts more evens out as one list.
+      const int edge = tail > 1 ? kBuckets - 2 : kBuckets / 2;
+      if (tid == edge) grouped_lds = chunk < whole || count <= slots ? 0 : (int)upto;
+      __syncthreads();
     }
   }
   if (tid == 0) {
-    p.counts[0] = (int)min(sums & 0x1fffff, (uint64_t)p.max_items);
-    p.counts[1] = (int)min(sums >> 42, (uint64_t)p.max_splits);
+    p.counts[0] = (int)min(items, (uint32_t)p.max_items);
+    p.counts[1] = (int)min(split_sums & 0xffff, (uint32_t)p.max_splits);
+    p.counts[2] = min(grouped_lds, p.counts[0]);
+  }
+  __syncthreads();
+  for (int n = 0; n < many_count; ++n) {
+    const int i = many[0][n], steps = tile_steps[i];
+    const int parts = parts_of(steps, 0);  // (tails have at most kManyParts)
+    Item it = {};
+    it.request = find(i);
+    const Sequence s = seq_of(it.request);
+    it.q0 = s.q0; it.n = s.n; it.k0 = s.k0; it.m = s.m;
+    it.tile = i - base[it.request];
+    it.parts = parts;
+    for (int j = tid; j < parts; j += kThreads) {
+      it.s0 = (int)((int64_t)steps * j / parts);
+      it.s1 = (int)((int64_t)steps * (j + 1) / parts);
+      it.slot = many[2][n] + j;
+      if (many[1][n] + j < p.max_items) p.items[many[1][n] + j] = it;
+    }
   }
 }
 
@@ -211,8 +397,8 @@ size_t round256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 // Shape of a call's schedule, from what the host knows of it.
 struct Plan {
   bool narrow, merge;
-  int tile_rows, step_keys, min_chunk, target;
-  int64_t max_items, max_splits, max_slots;
+  int tile_rows, step_keys, min_chunk, slots;
+  int64_t max_tiles, max_items, max_splits, max_slots;
   size_t counts, base, items, splits, parts, bytes;
 };
 
@@ -223,16 +409,16 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   s.narrow = q_rows * group <= 16 * requests;
   s.tile_rows = s.narrow ? kNarrowRows : kWideRows;
   s.step_keys = s.narrow ? kNarrowKeys : kWideKeys;
-  s.target = s.narrow ? 256 : 512;
-  s.min_chunk = s.narrow ? 2 : 4;
-  const int64_t tiles = q_rows * group / s.tile_rows + requests;
-  // Every part but a tile's last is a whole chunk, of which the work of all key
-  // heads holds at most `target`; a split tile has at least one whole chunk.
-  const int64_t chunks = s.target / kv_heads;
-  s.merge = max_keys > (int64_t)s.min_chunk * s.step_keys && chunks > 0;
-  s.max_items = std::max<int64_t>(1, tiles + (s.merge ? chunks : 0));
-  s.max_splits = s.merge ? std::min(tiles, chunks) : 0;
-  s.max_slots = s.merge ? 2 * s.target / kv_heads : 0;
+  s.slots = s.narrow ? 256 : 512;
+  s.min_chunk = s.narrow ? 1 : 2;
+  s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);
+  // Of one key head: no more than 2 `slots` partials over all of them.  Tiles cut
+  // at a slot's share of the work keep to that by themselves: each has more than
+  // one whole chunk, of which the work of all heads holds `slots`.
+  s.merge = max_keys >= 2 * (int64_t)s.min_chunk * s.step_keys && s.slots >= kv_heads;
+  s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
+  s.max_splits = std::min(s.max_tiles, s.max_slots / 2);
+  s.max_items = s.max_tiles + s.max_slots;
   const int dim = head_dim <= 64 ? 64 : 128;
   s.counts = 0;
   s.base = 256;
@@ -291,19 +477,30 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   p.scale_log2 = scale * 1.4426950408889634f;
   p.tile_rows = s.tile_rows;
   p.step_keys = s.step_keys;
-  p.min_chunk = s.merge ? s.min_chunk : 0x7fffffff;
-  p.target = s.target;
+  p.min_chunk = s.min_chunk;
+  p.slots = s.slots;
+  p.max_tiles = (int32_t)s.max_tiles;
   p.max_items = (int32_t)s.max_items;
   p.max_splits = (int32_t)s.max_splits;
   p.max_slots = (int32_t)s.max_slots;
+  // In key steps: what an item costs beside its keys, what a partial adds, and
+  // its share of the join.
+  p.item_cost = s.narrow ? 1.0f : 2.0f;
+  p.part_cost = s.narrow ? 0.25f : 2.5f;
+  p.merge_cost = s.narrow ? 0.0005f : 0.011f;
   p.counts = reinterpret_cast<int32_t*>(ws + s.counts);
   p.tile_base = reinterpret_cast<int32_t*>(ws + s.base);
   p.items = reinterpret_cast<Item*>(ws + s.items);
   p.splits = reinterpret_cast<Item*>(ws + s.splits);
   p.part = reinterpret_cast<float*>(ws + s.parts);
   dsa::clear_error();
-  hipLaunchKernelGGL(seq_schedule_kernel, dim3(p.fill || p.lse ? 65 : 1), dim3(kScheduleThreads), 0, stream,
-                     p, 2);
+  // Workgroups for the rows outside every sequence, beside the one that lists.
+  const unsigned lists =
+      1 + (p.fill || p.lse ? (unsigned)std::min<int64_t>(64, (p.q_rows + 3) / 4) : 0u);
+  if (s.max_tiles <= 512 && p.requests <= 512)
+    hipLaunchKernelGGL(seq_schedule_kernel<256>, dim3(lists), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL(seq_schedule_kernel<1024>, dim3(lists), dim3(1024), 0, stream, p);
   const int groups = (int)(s.max_items * p.kv_heads);
   return dtype == DSA_BF16
              ? launch_typed<__bf16>(p, paged, s.narrow, groups, s.merge, stream, who)

@@ -15,8 +15,9 @@
 // tiles: every key staged for a tile serves all heads of the group.  A tile's
 // keys may be cut into parts, whose fp32 partials seq_merge_kernel joins.
 // Lengths live on the device, so seq_schedule_kernel lists the (tile, part)
-// items there, longest first; the grids are the host's
-// upper bounds and workgroups past the list end at once.
+// items there, longest first; the grids are the host's upper bounds and
+// workgroups past the list end at once.  In a call of few tiles every workgroup
+// works its item out by itself (own_item) and that kernel is left out.
 //
 //  * seq_wide_kernel: 128 rows, four waves of 32, the 64-key staged walk of
 //    bsa_fwd_kernel (S^T = K Q^T, O^T = V^T P^T on 32x32x16 products).
@@ -64,6 +65,7 @@ struct Params {
   int32_t fill;                // rows of o outside every sequence become 0
   float scale_log2;            // scale * log2(e)
   // Schedule.
+  int32_t unlisted;            // no schedule kernel: workgroups work their items out (own_item)
   int32_t tile_rows, step_keys, min_chunk;
   int32_t slots;               // workgroups that run at a time
   int32_t max_tiles, max_items, max_splits, max_slots;  // room in the lists, per key head
@@ -154,6 +156,198 @@ __device__ __forceinline__ Item load_item(const Item* at) {
   return it;
 }
 
+// Inclusive sum over the 64 lanes (row shifts by 1, 2, 4, 8, then the row sums
+// broadcast into the rows behind).  Every lane of the wave must be active.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
+struct Sequence {
+  int32_t q0, n, k0, m;
+};
+
+// Sequence r, whatever the arrays hold: rows and keys within the tensors.
+__device__ __forceinline__ Sequence sequence(const Params& p, int r) {
+  Sequence s;
+  s.q0 = min(max(p.q_start[r], 0), p.q_rows);
+  s.n = min(max(p.q_start[r + 1], s.q0), p.q_rows) - s.q0;
+  if (p.kv_lens) {
+    s.k0 = 0;
+    const int64_t room = (int64_t)p.table_width << p.page_shift;
+    s.m = (int32_t)min((int64_t)max(p.kv_lens[r], 0), room);
+  } else {
+    s.k0 = min(max(p.k_start[r], 0), p.k_rows);
+    s.m = min(max(p.k_start[r + 1], s.k0), p.k_rows) - s.k0;
+  }
+  return s;
+}
+
+__device__ __forceinline__ int tiles_of(const Params& p, const Sequence& s) {
+  return (s.n * p.group + p.tile_rows - 1) / p.tile_rows;
+}
+
+// Key steps of a tile: up to the last key its last row sees.
+__device__ __forceinline__ int steps_of(const Params& p, const Sequence& s, int tile) {
+  int end = s.m;
+  if (p.causal) {
+    const int last = min((tile + 1) * p.tile_rows, s.n * p.group) - 1;
+    end = max(0, min(s.m, s.m - s.n + last / p.group + 1));
+  }
+  return (end + p.step_keys - 1) / p.step_keys;
+}
+
+// Rows that belong to no sequence, the `share`-th of `shares` workgroups' part of
+// them: O 0 with p.fill, LSE -inf.
+__device__ __forceinline__ void clear_outside(const Params& p, int share, int shares) {
+  if (!p.fill && !p.lse) return;
+  const int first = min(max(p.q_start[0], 0), p.q_rows);
+  const int last = min(max(p.q_start[p.requests], first), p.q_rows);
+  const int chunks = p.head_dim / 8 * p.heads;  // 16-byte chunks of a row
+  const int empty = first + p.q_rows - last;
+  const dsa_u32x4 zero = {0u, 0u, 0u, 0u};
+  for (int i = share; i < empty; i += shares) {
+    const int row = i < first ? i : last + i - first;
+    for (int c = threadIdx.x; p.fill && c < chunks; c += blockDim.x) {
+      const int head = c / (p.head_dim / 8), d = c % (p.head_dim / 8) * 8;
+      *reinterpret_cast<dsa_u32x4*>(static_cast<uint16_t*>(p.o) + (int64_t)row * p.o_st +
+                                    head * p.o_sh + d) = zero;
+    }
+    if (p.lse)
+      for (int head = threadIdx.x; head < p.heads; head += blockDim.x)
+        p.lse[(int64_t)head * p.q_rows + row] = -INFINITY;
+  }
+}
+
+// The item and key head of workgroup `wg` in a call without a schedule kernel:
+// at most 64 sequences and 64 tiles, all of them (times the key heads) at once on
+// the chip.  Every wave works it out for itself, a lane per sequence, then per
+// tile, then per candidate: the longest tile in 1, 2, 3, .. parts, priced by its
+// part and the join, as long as the parts of all tiles still run at once.  The
+// first workgroup leaves the split tiles for the merge.  False: no item is left,
+// and the workgroup clears its part of the rows outside the sequences.
+__device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int* head) {
+  const int lane = threadIdx.x & 63;
+  Sequence s = {0, 0, 0, 0};
+  if (lane < p.requests) s = sequence(p, lane);
+  const int tiles = tiles_of(p, s);
+  const int base = (int)wave_scan((uint32_t)tiles) - tiles;
+  // (starts that overlap list more tiles than fit)
+  const int count = min(__builtin_amdgcn_readlane(base + tiles, 63), p.max_tiles);
+  // Lane i: tile i of sequence r, the last that starts at or before it.
+  // (at most 64 sequences: six bisection steps)
+  int r = 0;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const int at = __shfl(base, r + d);
+    if (r + d < p.requests && at <= lane) r += d;
+  }
+  Sequence t;
+  t.q0 = __shfl(s.q0, r); t.n = __shfl(s.n, r); t.k0 = __shfl(s.k0, r); t.m = __shfl(s.m, r);
+  const int tile = lane - __shfl(base, r);
+  const int steps = lane < count ? steps_of(p, t, tile) : 0;
+  int longest = steps;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) longest = max(longest, __shfl_xor(longest, d));
+  int chunk = max(longest, 1);
+  if (p.max_slots > 0 && longest >= 2 * p.min_chunk) {
+    const int parts = lane < 32 ? lane + 1 : 32 + (lane - 31) * 8;
+    const int mine = max(p.min_chunk, (longest + parts - 1) / parts);
+    const float per = 1.f / (float)mine;
+    int items = 0;
+    for (int i = 0; i < count; ++i) {
+      const int len = __builtin_amdgcn_readlane(steps, i);
+      // (rounded up generously; what is taken is counted below)
+      items += max(1, (int)((float)(len + mine - 1) * per + 0.01f));
+    }
+    float price = (float)mine + (lane > 0 ? p.part_cost + p.merge_cost * (float)(items * p.kv_heads)
+                                          : 0.f);
+    if (lane > 0 && (items * p.kv_heads > p.slots || items > p.max_slots)) price = INFINITY;
+    int best = lane;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const float other = __shfl_xor(price, d);
+      const int its = __shfl_xor(best, d);
+      if (other < price || (other == price && its < best)) {
+        price = other;
+        best = its;
+      }
+    }
+    chunk = __shfl(mine, best);
+  }
+  int parts = lane < count ? max(1, (steps + chunk - 1) / chunk) : 0;
+  uint32_t split = parts > 1 ? (uint32_t)parts << 16 | 1u : 0u;
+  uint32_t splits = wave_scan(split);
+  if ((__builtin_amdgcn_readlane((int)splits, 63) >> 16) > p.max_slots) {  // (never by the price)
+    parts = min(parts, 1);
+    split = splits = 0;
+  }
+  const int first = (int)wave_scan((uint32_t)parts) - parts;
+  const int items = __builtin_amdgcn_readlane(first + parts, 63);
+  Item it = {};
+  it.request = r;
+  it.q0 = t.q0; it.n = t.n; it.k0 = t.k0; it.m = t.m;
+  it.tile = tile;
+  it.parts = parts;
+  it.slot = parts > 1 ? (int)((splits - split) >> 16) : -1;
+  if (wg == 0 && threadIdx.x < 64) {
+    if (parts > 1) p.splits[(splits - split) & 0xffff] = it;
+    if (lane == 63) p.counts[1] = (int)(splits & 0xffff);
+  }
+  const int item = wg / p.kv_heads;
+  if (item >= items) {
+    clear_outside(p, wg - items * p.kv_heads, (int)gridDim.x - items * p.kv_heads);
+    return false;
+  }
+  const int i = (int)__popcll(__ballot(lane < count && first <= item)) - 1;
+  const int part = item - __builtin_amdgcn_readlane(first, i);
+  const int len = __builtin_amdgcn_readlane(steps, i);
+  out->request = __builtin_amdgcn_readlane(it.request, i);
+  out->q0 = __builtin_amdgcn_readlane(it.q0, i);
+  out->n = __builtin_amdgcn_readlane(it.n, i);
+  out->k0 = __builtin_amdgcn_readlane(it.k0, i);
+  out->m = __builtin_amdgcn_readlane(it.m, i);
+  out->tile = __builtin_amdgcn_readlane(it.tile, i);
+  out->parts = __builtin_amdgcn_readlane(it.parts, i);
+  out->s0 = (int)((int64_t)len * part / out->parts);
+  out->s1 = (int)((int64_t)len * (part + 1) / out->parts);
+  const int slot = __builtin_amdgcn_readlane(it.slot, i);
+  out->slot = slot >= 0 ? slot + part : -1;
+  *head = wg - item * p.kv_heads;
+  return true;
+}
+
+// The item and key head of this workgroup; false: none.  kGrouped: the list's
+// first counts[2] items run eight key heads at a time, so that each XCD streams
+// the keys of one head through its L2; the others, which even out the end of the
+// call, run all heads of one item before the next.  (40 heads of one query head,
+// 16,384 x 16,384: 5.45 ms all heads at a time, 4.82 ms eight.)
+template <bool kGrouped>
+__device__ __forceinline__ bool take_item(const Params& p, Item* it, int* h) {
+  const int wg = (int)blockIdx.x;
+  if (p.unlisted) return own_item(p, wg, it, h);
+  const int count = ((dsa::const_i32)p.counts)[0];
+  if (wg >= count * p.kv_heads) return false;
+  const int grouped = kGrouped ? ((dsa::const_i32)p.counts)[2] : 0;
+  int item;
+  if (wg < grouped * p.kv_heads) {
+    const int first = wg / (grouped * kHeadGroup) * kHeadGroup;
+    const int rest = wg - first * grouped, heads = min(kHeadGroup, p.kv_heads - first);
+    item = rest / heads;
+    *h = first + rest - item * heads;
+  } else {
+    item = wg / p.kv_heads;
+    *h = wg - item * p.kv_heads;
+  }
+  *it = load_item(p.items + item);
+  return true;
+}
+
 // One row's sum of p_j V_j over the keys it sees of `blocks` key blocks (`width`
 // <= 64 keys from key_lo, key_lo + stride, ..; below key_hi), element by element:
 // lane l ends with the dims l kD / 64 ...  In the matrix products a hidden key's
@@ -225,25 +419,9 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v1[kStage];
 
-  const int count = ((dsa::const_i32)p.counts)[0];
-  const int wg = (int)blockIdx.x;
-  if (wg >= count * p.kv_heads) return;
-  // The list's first `grouped` items run eight key heads at a time, so that each
-  // XCD streams the keys of one head through its L2; the others, which even out
-  // the end of the call, run all heads of one item before the next.  (40 heads of
-  // one query head, 16,384 x 16,384: 5.45 ms all heads at a time, 4.82 ms eight.)
-  const int grouped = ((dsa::const_i32)p.counts)[2];
-  int item, h;
-  if (wg < grouped * p.kv_heads) {
-    const int first = wg / (grouped * kHeadGroup) * kHeadGroup;
-    const int rest = wg - first * grouped, heads = min(kHeadGroup, p.kv_heads - first);
-    item = rest / heads;
-    h = first + rest - item * heads;
-  } else {
-    item = wg / p.kv_heads;
-    h = wg - item * p.kv_heads;
-  }
-  const Item it = load_item(p.items + item);
+  Item it;
+  int h;
+  if (!take_item<true>(p, &it, &h)) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -568,12 +746,9 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[4 * kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v1[4 * kStage];
 
-  const int count = ((dsa::const_i32)p.counts)[0];
-  const int wg = (int)blockIdx.x;
-  if (wg >= count * p.kv_heads) return;
-  const int i_item = wg / p.kv_heads;
-  const int h = wg - i_item * p.kv_heads;
-  const Item it = load_item(p.items + i_item);
+  Item it;
+  int h;
+  if (!take_item<false>(p, &it, &h)) return;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;

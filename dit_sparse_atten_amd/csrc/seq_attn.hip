@@ -14,18 +14,6 @@ __constant__ const short kTryParts[32] = {1,  2,  3,  4,  5,  6,  7,  8,   9,   
                                           18, 20, 24, 28, 32, 40, 48, 56,  64,  80,  96,  112, 128,
                                           160, 192, 256, 384, 512};
 
-// Inclusive sum over the 64 lanes (row shifts by 1, 2, 4, 8, then the row sums
-// broadcast into the rows behind).  Every lane of the wave must be active.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
-  return v;
-}
-
 // Inclusive sum over the workgroup, `total` for every thread.
 template <int kThreads>
 __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
@@ -43,40 +31,6 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* lds, uint32
   }
   *total = all;
   return before + v;
-}
-
-struct Sequence {
-  int32_t q0, n, k0, m;
-};
-
-// Sequence r, whatever the arrays hold: rows and keys within the tensors.
-__device__ __forceinline__ Sequence sequence(const Params& p, int r) {
-  Sequence s;
-  s.q0 = min(max(p.q_start[r], 0), p.q_rows);
-  s.n = min(max(p.q_start[r + 1], s.q0), p.q_rows) - s.q0;
-  if (p.kv_lens) {
-    s.k0 = 0;
-    const int64_t room = (int64_t)p.table_width << p.page_shift;
-    s.m = (int32_t)min((int64_t)max(p.kv_lens[r], 0), room);
-  } else {
-    s.k0 = min(max(p.k_start[r], 0), p.k_rows);
-    s.m = min(max(p.k_start[r + 1], s.k0), p.k_rows) - s.k0;
-  }
-  return s;
-}
-
-__device__ __forceinline__ int tiles_of(const Params& p, const Sequence& s) {
-  return (s.n * p.group + p.tile_rows - 1) / p.tile_rows;
-}
-
-// Key steps of a tile: up to the last key its last row sees.
-__device__ __forceinline__ int steps_of(const Params& p, const Sequence& s, int tile) {
-  int end = s.m;
-  if (p.causal) {
-    const int last = min((tile + 1) * p.tile_rows, s.n * p.group) - 1;
-    end = max(0, min(s.m, s.m - s.n + last / p.group + 1));
-  }
-  return (end + p.step_keys - 1) / p.step_keys;
 }
 
 // Workgroup 0 lists the call's items and split tiles; the others give the rows
@@ -99,22 +53,7 @@ template <int kThreads>
 __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
-    const int first = min(max(p.q_start[0], 0), p.q_rows);
-    const int last = min(max(p.q_start[p.requests], first), p.q_rows);
-    const int chunks = p.head_dim / 8 * p.heads;  // 16-byte chunks of a row
-    const int empty = first + p.q_rows - last;
-    const dsa_u32x4 zero = {0u, 0u, 0u, 0u};
-    for (int i = blockIdx.x - 1; i < empty; i += gridDim.x - 1) {
-      const int row = i < first ? i : last + i - first;
-      for (int c = tid; p.fill && c < chunks; c += kThreads) {
-        const int head = c / (p.head_dim / 8), d = c % (p.head_dim / 8) * 8;
-        *reinterpret_cast<dsa_u32x4*>(static_cast<uint16_t*>(p.o) + (int64_t)row * p.o_st +
-                                      head * p.o_sh + d) = zero;
-      }
-      if (p.lse)
-        for (int head = tid; head < p.heads; head += kThreads)
-          p.lse[(int64_t)head * p.q_rows + row] = -INFINITY;
-    }
+    clear_outside(p, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   __shared__ uint32_t scan_lds[kThreads / 64];
@@ -396,7 +335,7 @@ size_t round256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 // Shape of a call's schedule, from what the host knows of it.
 struct Plan {
-  bool narrow, merge;
+  bool narrow, merge, unlisted;
   int tile_rows, step_keys, min_chunk, slots;
   int64_t max_tiles, max_items, max_splits, max_slots;
   size_t counts, base, items, splits, parts, bytes;
@@ -419,6 +358,8 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
   s.max_splits = std::min(s.max_tiles, s.max_slots / 2);
   s.max_items = s.max_tiles + s.max_slots;
+  // A call whose tiles all run at once, few enough for the lanes of a wave.
+  s.unlisted = requests <= 64 && s.max_tiles <= 64 && s.max_tiles * kv_heads <= s.slots;
   const int dim = head_dim <= 64 ? 64 : 128;
   s.counts = 0;
   s.base = 256;
@@ -494,14 +435,18 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   p.splits = reinterpret_cast<Item*>(ws + s.splits);
   p.part = reinterpret_cast<float*>(ws + s.parts);
   dsa::clear_error();
-  // Workgroups for the rows outside every sequence, beside the one that lists.
-  const unsigned lists =
-      1 + (p.fill || p.lse ? (unsigned)std::min<int64_t>(64, (p.q_rows + 3) / 4) : 0u);
-  if (s.max_tiles <= 512 && p.requests <= 512)
-    hipLaunchKernelGGL(seq_schedule_kernel<256>, dim3(lists), dim3(256), 0, stream, p);
-  else
-    hipLaunchKernelGGL(seq_schedule_kernel<1024>, dim3(lists), dim3(1024), 0, stream, p);
-  const int groups = (int)(s.max_items * p.kv_heads);
+  p.unlisted = s.unlisted;
+  // Workgroups for the rows outside every sequence, beside those with items.
+  const int outside =
+      p.fill || p.lse ? (int)std::min<int64_t>(64, (p.q_rows + 3) / 4) : 0;
+  int groups = (int)(s.max_items * p.kv_heads);
+  if (s.unlisted) {
+    groups = (s.merge ? s.slots : (int)s.max_tiles * p.kv_heads) + outside;
+  } else if (s.max_tiles <= 512 && p.requests <= 512) {
+    hipLaunchKernelGGL(seq_schedule_kernel<256>, dim3(1 + outside), dim3(256), 0, stream, p);
+  } else {
+    hipLaunchKernelGGL(seq_schedule_kernel<1024>, dim3(1 + outside), dim3(1024), 0, stream, p);
+  }
   return dtype == DSA_BF16
              ? launch_typed<__bf16>(p, paged, s.narrow, groups, s.merge, stream, who)
              : seq_launch_f16(p, paged, s.narrow, groups, s.merge, stream, who);

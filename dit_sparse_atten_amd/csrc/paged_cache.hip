@@ -191,12 +191,12 @@ __global__ void __launch_bounds__(256) paged_write_kernel(WriteParams p) {
     const int d = (c - head * p.chunks) * 16;
     to[u] = p.dst[which] + page * p.dst_sp[which] + in_page * p.dst_st[which] +
             head * p.dst_sh[which] + d;
-    x[u] = *reinterpret_cast<const dsa_u32x4*>(p.src[which] + t * p.src_st[which] +
-                                               head * p.src_sh[which] + d);
+    x[u] = __builtin_nontemporal_load(reinterpret_cast<const dsa_u32x4*>(
+        p.src[which] + t * p.src_st[which] + head * p.src_sh[which] + d));
   }
 #pragma unroll
   for (int u = 0; u < kWriteUnroll; ++u)
-    if (to[u]) *reinterpret_cast<dsa_u32x4*>(to[u]) = x[u];
+    if (to[u]) __builtin_nontemporal_store(x[u], reinterpret_cast<dsa_u32x4*>(to[u]));
 }
 
 bool bad_page_size(int32_t size) { return size < 16 || (size & (size - 1)) != 0; }

@@ -39,11 +39,13 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* lds, uint32
 // The workgroups of the chip (p.slots at a time) take items in list order, all
 // key heads of one before the next, longest first.  Which tiles are cut, in units
 // of one tile's key steps, with `work` the steps of all tiles and heads:
-//  * up to one round of tiles: every tile longer than `chunk` in near-equal
-//    parts of at most that.  Each candidate (the longest tile in 1, 2, 3, ..
-//    512 parts) costs rounds x (mean length + p.item_cost), or its share of the
-//    work plus half the longest part if that is more; the cheapest is taken.
-//  * more: whole tiles, longest first, even out by themselves but for the last
+//  * up to one round of tiles, and wherever partials are small (16-row tiles):
+//    every tile longer than `chunk` in near-equal parts of at most that.  Each
+//    candidate (the longest tile in 1, 2, 3, .. 512 parts; of more than a round, a
+//    slot's share of the work times 2 / 3, 2 / 4, ..) costs rounds x (mean length
+//    + p.item_cost), or the share plus half the longest part if that is more; the
+//    cheapest is taken.
+//  * else whole tiles, longest first, even out by themselves but for the last
 //    round.  Tiles longer than a slot's share of the work are cut to it; if there
 //    are none, the shortest tiles, as many as the last round is short of full,
 //    are cut into as many parts as pay.
@@ -139,12 +141,16 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   auto bucket = [&](int steps) {      // of whole tiles, longest first
     return (kBuckets - 1) - (int)((int64_t)steps * (kBuckets - 1) / whole);
   };
+  const int share = (int)max((work + slots - 1) / slots, (int64_t)p.min_chunk);
   if (p.max_slots == 0 || longest < 2 * p.min_chunk || tiles == 0) {
     if (tid == 0) chunk_lds = whole;
-  } else if (count <= slots) {
-    // Up to a round of tiles: at most `slots` <= kLdsTiles of them.
+  } else if (count <= slots || (p.cheap_parts && tiles <= kLdsTiles)) {
+    // Candidate 0 leaves every tile whole, unless one alone is too long.
     const int which = tid & 31;
-    const int chunk = max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which]);
+    const int chunk =
+        count <= slots ? max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which])
+        : which == 0   ? min(whole, share)
+                       : max(p.min_chunk, 2 * share / (which + 2));
     uint32_t items = 0;
     for (int i = tid >> 5; i < tiles; i += kThreads / 32)
       items += max(1, (tile_steps[i] + chunk - 1) / chunk);
@@ -152,14 +158,15 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     __syncthreads();
     if (tid < 64) {
       const int64_t n = (int64_t)tried[which] * p.kv_heads;
-      const float cost = p.item_cost + (which > 0 ? p.part_cost : 0.f);
+      const bool cuts = chunk < whole;
+      const float cost = p.item_cost + (cuts ? p.part_cost : 0.f);
       const float mean = (float)work / (float)n + cost;
       const float rounds = (float)((n + slots - 1) / slots);
       const float even = ((float)work + cost * (float)n) / (float)slots;
       float price = n <= slots ? (float)chunk + cost
                                : fmaxf(rounds * mean, even + 0.5f * ((float)chunk + cost));
-      if (which > 0) price += p.merge_cost * (float)n;
-      if (which > 0 && tried[which] > (uint32_t)p.max_slots) price = INFINITY;
+      if (cuts) price += p.merge_cost * (float)n;
+      if (which > 0 && cuts && tried[which] > (uint32_t)p.max_slots) price = INFINITY;
       int best = which;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -170,11 +177,10 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
           best = its;
         }
       }
-      if (tid == 0)
-        chunk_lds = max(p.min_chunk, (longest + kTryParts[best] - 1) / kTryParts[best]);
+      const int taken = __shfl(chunk, best);
+      if (tid == 0) chunk_lds = taken;
     }
   } else {
-    const int share = (int)max((work + slots - 1) / slots, (int64_t)p.min_chunk);
     if (longest > share) {
       if (tid == 0) chunk_lds = share;
     } else {
@@ -351,11 +357,12 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   s.slots = s.narrow ? 256 : 512;
   s.min_chunk = s.narrow ? 1 : 2;
   s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);
-  // Of one key head: no more than 2 `slots` partials over all of them.  Tiles cut
+  // Of one key head: no more than 2 `slots` partials over all of them (16-row
+  // tiles, with a sixteenth of the floats each: 8).  Tiles cut
   // at a slot's share of the work keep to that by themselves: each has more than
   // one whole chunk, of which the work of all heads holds `slots`.
   s.merge = max_keys >= 2 * (int64_t)s.min_chunk * s.step_keys && s.slots >= kv_heads;
-  s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
+  s.max_slots = s.merge ? (s.narrow ? 8 : 2) * s.slots / kv_heads : 0;
   s.max_splits = std::min(s.max_tiles, s.max_slots / 2);
   s.max_items = s.max_tiles + s.max_slots;
   // A call whose tiles all run at once, few enough for the lanes of a wave.
@@ -427,6 +434,7 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   // In key steps: what an item costs beside its keys, what a partial adds, and
   // its share of the join.
   p.item_cost = s.narrow ? 1.0f : 2.0f;
+  p.cheap_parts = s.narrow;
   p.part_cost = s.narrow ? 0.25f : 2.5f;
   p.merge_cost = s.narrow ? 0.0005f : 0.011f;
   p.counts = reinterpret_cast<int32_t*>(ws + s.counts);

@@ -19,10 +19,12 @@ int launch_dim(const Params& p, bool paged, bool narrow, int max_groups, bool me
     else hipLaunchKernelGGL((seq_wide_kernel<T, kD, false>), grid, block, 0, stream, p);
   }
   if (merge) {
-    const int rows = narrow ? kNarrowRows : kWideRows;
-    const dim3 groups((unsigned)std::min<int64_t>((int64_t)p.max_splits * rows,
-                                                  std::max(1, 4096 / p.kv_heads)),
-                      (unsigned)p.kv_heads);
+    const int units = (narrow ? kNarrowRows : kWideRows) / 16;
+    // Tiles have many parts only where there are few of them.
+    const bool few_tiles = (int64_t)p.max_tiles * kFewParts <= p.max_slots;
+    const dim3 groups((unsigned)std::min<int64_t>((int64_t)p.max_splits * units,
+                                                  std::max(1, 8192 / p.kv_heads)),
+                      (unsigned)p.kv_heads, few_tiles ? 16u : 1u);
     if (narrow) hipLaunchKernelGGL((seq_merge_kernel<T, kD, kNarrowRows>), groups, block, 0, stream, p);
     else hipLaunchKernelGGL((seq_merge_kernel<T, kD, kWideRows>), groups, block, 0, stream, p);
   }

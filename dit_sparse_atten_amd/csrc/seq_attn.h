@@ -80,10 +80,18 @@ struct Params {
   float* part;                 // partial slots, kv_heads each
 };
 
-// One partial: O [tile_rows][kD] relative to the row's reference max, then m
-// (log2 units of the scaled scores) and l per row, in fp32.
+// One partial: O [tile_rows][kD] relative to the row's reference max (in the order
+// of part_at), then m (log2 units of the scaled scores) and l per row, in fp32.
 __host__ __device__ constexpr int part_floats(int tile_rows, int dim) {
   return tile_rows * (dim + 2);
+}
+
+// Where dim d of row r lies in a partial: 16-row tiles row by row, 128-row tiles as
+// the waves hold them, quads of dims of 32 rows side by side.
+template <int kD, int kRows>
+__device__ __forceinline__ int part_at(int r, int d) {
+  return kRows == 16 ? r * kD + d
+                     : (r >> 5) * (32 * kD) + ((d >> 2) * 32 + (r & 31)) * 4 + (d & 3);
 }
 
 constexpr float kRescaleLog2 = 8.0f;  // move the reference max once a p could exceed 2^8
@@ -693,35 +701,45 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
         const int d = lane * (kD / 64) + e;
         if (it.slot >= 0)
           late->part[((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD) +
-                 (wave * 32 + r) * kD + d] = acc[e];
+                     part_at<kD, kWideRows>(wave * 32 + r, d)] = acc[e];
         else if (d < late->head_dim)
           static_cast<T*>(late->o)[(it.q0 + token_r) * late->o_st + head_r * late->o_sh + d] =
               (T)(acc[e] * inv);
       }
     }
   }
-  if (!row_ok) return;
   if (it.slot >= 0) {
-    float* po = late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD);
-    float* prow = po + local * kD;
-    if (!redo)
+    // A partial keeps the accumulators' own order (part_at): whole lines per store.
+    float* const po =
+        late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD);
+    if (!redo) {
 #pragma unroll
-    for (int dt = 0; dt < kDt; ++dt)
+      for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
-      for (int rr = 0; rr < 4; ++rr) {
-        const dsa_f32x4 v4 = {oacc[dt][rr * 4 + 0], oacc[dt][rr * 4 + 1], oacc[dt][rr * 4 + 2],
-                              oacc[dt][rr * 4 + 3]};
-        *reinterpret_cast<dsa_f32x4*>(prow + dt * 32 + rr * 8 + g * 4) = v4;
-      }
+        for (int rr = 0; rr < 4; ++rr) {
+          const dsa_f32x4 v4 = {oacc[dt][rr * 4 + 0], oacc[dt][rr * 4 + 1],
+                                oacc[dt][rr * 4 + 2], oacc[dt][rr * 4 + 3]};
+          *reinterpret_cast<dsa_f32x4*>(po +
+                                        part_at<kD, kWideRows>(local, dt * 32 + rr * 8 + g * 4)) = v4;
+        }
+    }
     if (g == 0) {
       po[kWideRows * kD + local] = m_run;
       po[kWideRows * (kD + 1) + local] = l_tot;
     }
     return;
   }
+  if (late->lse && g == 0 && row_ok)
+    late->lse[(int64_t)head * late->q_rows + it.q0 + token] =
+        l_tot == 0.f ? -INFINITY : m_run * kLn2 + logf(l_tot);
+  if (redo) return;
+  // O goes out through the wave's quarter of the stages that the last step left
+  // alone (every wave is past its reads of them, and no load is on its way there):
+  // written row by row as 16-byte chunks, whole rows to a store.
   const float inv = l_tot > 0.f ? 1.f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
-  T* orow = static_cast<T*>(late->o) + (int64_t)(it.q0 + token) * late->o_st + head * late->o_sh;
-  if (!redo)
+  const bool odd = (it.s1 - it.s0) & 1;
+  unsigned char* const mine = (wave < 2 ? (odd ? lds_k1 : lds_k0) : (odd ? lds_v1 : lds_v0)) +
+                              (wave & 1) * (kStage / 2);
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
@@ -729,12 +747,20 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
       typename E::x4 v4;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v4[e] = (T)(oacc[dt][rr * 4 + e] * inv);
-      if (dt * 32 + rr * 8 + g * 4 < late->head_dim)
-        *reinterpret_cast<typename E::x4*>(orow + dt * 32 + rr * 8 + g * 4) = v4;
+      *reinterpret_cast<typename E::x4*>(mine + qi * kRow + k_swz<kD>(qi, dt * 4 + rr) * 16 +
+                                         g * 8) = v4;
     }
-  if (late->lse && g == 0)
-    late->lse[(int64_t)head * late->q_rows + it.q0 + token] =
-        l_tot == 0.f ? -INFINITY : m_run * kLn2 + logf(l_tot);
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_wave_barrier();
+  const int64_t o_at = row_ok ? (int64_t)(it.q0 + token) * late->o_st + head * late->o_sh : -1;
+#pragma unroll
+  for (int i = 0; i < kD / 16; ++i) {
+    const int r = i * kRowsPer + lane / kChunks, c = lane % kChunks;
+    const x8 y = *reinterpret_cast<const x8*>(mine + r * kRow + k_swz<kD>(r, c) * 16);
+    const int64_t at = __shfl(o_at, r);
+    if (at >= 0 && c * 8 < late->head_dim)
+      *reinterpret_cast<x8*>(static_cast<T*>(late->o) + at + c * 8) = y;
+  }
 }
 
 // 16 rows x the item's keys, on 16x16x32 products.  Wave w takes keys 128 s +
@@ -1057,7 +1083,7 @@ __global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
   __shared__ float ml[2][16];
   const int splits = ((dsa::const_i32)p.counts)[1];
   const int h = blockIdx.y;
-  const int tid = threadIdx.x, grp = tid >> 4, d0 = (tid & 15) * 8;
+  const int tid = threadIdx.x;
   // Units of 16 rows along x; z counts the rows of one where each takes a
   // workgroup.
   constexpr int kUnits = kRows / 16;
@@ -1066,6 +1092,9 @@ __global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
     const Item it = load_item(p.splits + work / kUnits);
     const bool few = it.parts <= kFewParts;
     if (few && z > 0) break;
+    // (rows side by side where a partial has them so)
+    const bool across = kRows != 16 && few;
+    const int grp = across ? tid & 15 : tid >> 4, d0 = (across ? tid >> 4 : tid & 15) * 8;
     const int r0 = work % kUnits * 16 + z;
     const int r = few ? r0 + grp : r0;
     const int row = it.tile * kRows + r;
@@ -1087,8 +1116,8 @@ __global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
         mi[u] = part[kRows * kD + r];
         li[u] = part[kRows * (kD + 1) + r];
         if (d0 < kD) {
-          x[u][0] = *reinterpret_cast<const dsa_f32x4*>(part + r * kD + d0);
-          x[u][1] = *reinterpret_cast<const dsa_f32x4*>(part + r * kD + d0 + 4);
+          x[u][0] = *reinterpret_cast<const dsa_f32x4*>(part + part_at<kD, kRows>(r, d0));
+          x[u][1] = *reinterpret_cast<const dsa_f32x4*>(part + part_at<kD, kRows>(r, d0 + 4));
         }
       }
 #pragma unroll

@@ -68,7 +68,7 @@ struct Params {
   float scale_log2;            // scale * log2(e)
   // Schedule.
   int32_t unlisted;            // no schedule kernel: workgroups work their items out (own_item)
-  int32_t tile_rows, step_keys, min_chunk;
+  int32_t tile_shift, step_shift, min_chunk;  // log2 of a tile's rows, of a step's keys
   int32_t slots;               // workgroups that run at a time
   int32_t max_tiles, max_items, max_splits, max_slots;  // room in the lists, per key head
   int32_t cheap_parts;         // tiles are cut freely, whatever their number
@@ -209,18 +209,27 @@ __device__ __forceinline__ Sequence sequence(const Params& p, int r) {
 }
 
 __device__ __forceinline__ int tiles_of(const Params& p, const Sequence& s) {
-  return (s.n * p.group + p.tile_rows - 1) / p.tile_rows;
+  return (int)(((int64_t)s.n * p.group + (1 << p.tile_shift) - 1) >> p.tile_shift);
 }
 
 // Key steps of a tile: up to the last key its last row sees.
 __device__ __forceinline__ int steps_of(const Params& p, const Sequence& s, int tile) {
   int end = s.m;
   if (p.causal) {
-    const int last = min((tile + 1) * p.tile_rows, s.n * p.group) - 1;
-    end = max(0, min(s.m, s.m - s.n + last / p.group + 1));
+    const uint32_t last =
+        min((uint32_t)(tile + 1) << p.tile_shift, (uint32_t)s.n * (uint32_t)p.group) - 1;
+    end = max(0, min(s.m, s.m - s.n + (int)(last / (uint32_t)p.group) + 1));
   }
-  return (end + p.step_keys - 1) / p.step_keys;
+  return (int)(((int64_t)end + (1 << p.step_shift) - 1) >> p.step_shift);
 }
+
+// Near-equal parts of a tile's steps: part j is [from(j), from(j + 1)).
+struct Cut {
+  int each, more;  // the first `more` parts hold one step more
+  __device__ __forceinline__ Cut(int steps, int parts)
+      : each((int)((uint32_t)steps / (uint32_t)parts)), more(steps - each * parts) {}
+  __device__ __forceinline__ int from(int j) const { return j * each + min(j, more); }
+};
 
 // Rows that belong to no sequence, the `share`-th of `shares` workgroups' part of
 // them: O 0 with p.fill, LSE -inf.
@@ -334,8 +343,9 @@ __device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int
   out->m = __builtin_amdgcn_readlane(it.m, i);
   out->tile = __builtin_amdgcn_readlane(it.tile, i);
   out->parts = __builtin_amdgcn_readlane(it.parts, i);
-  out->s0 = (int)((int64_t)len * part / out->parts);
-  out->s1 = (int)((int64_t)len * (part + 1) / out->parts);
+  const Cut cut(len, out->parts);
+  out->s0 = cut.from(part);
+  out->s1 = cut.from(part + 1);
   const int slot = __builtin_amdgcn_readlane(it.slot, i);
   out->slot = slot >= 0 ? slot + part : -1;
   *head = wg - item * p.kv_heads;

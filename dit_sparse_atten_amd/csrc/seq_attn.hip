@@ -138,9 +138,13 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   const int64_t work = (int64_t)work_lds * p.kv_heads, count = (int64_t)tiles * p.kv_heads;
   const int slots = p.slots;
   const int whole = max(longest, 1);  // a chunk that cuts nothing
-  auto bucket = [&](int steps) {      // of whole tiles, longest first
-    return (kBuckets - 1) - (int)((int64_t)steps * (kBuckets - 1) / whole);
+  // Bucket of a length, the longest first (by a multiplication: any monotone map
+  // serves).
+  auto bucket_of = [](int steps, float per) {
+    return (kBuckets - 1) - min(kBuckets - 1, (int)((float)steps * per));
   };
+  const float per_whole = (float)(kBuckets - 1) / (float)whole;
+  auto bucket = [&](int steps) { return bucket_of(steps, per_whole); };  // of whole tiles
   const int share = (int)max((work + slots - 1) / slots, (int64_t)p.min_chunk);
   if (p.max_slots == 0 || longest < 2 * p.min_chunk || tiles == 0) {
     if (tid == 0) chunk_lds = whole;
@@ -153,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
                        : max(p.min_chunk, 2 * share / (which + 2));
     uint32_t items = 0;
     for (int i = tid >> 5; i < tiles; i += kThreads / 32)
-      items += max(1, (tile_steps[i] + chunk - 1) / chunk);
+      items += max(1u, (uint32_t)(tile_steps[i] + chunk - 1) / (uint32_t)chunk);
     atomicAdd(&tried[which], items);
     __syncthreads();
     if (tid < 64) {
@@ -225,16 +229,16 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
       const int at = bucket(steps);
       return at > cut_at || (at == cut_at && (int)seen < cut_left) ? tail : 1;
     }
-    return max(1, (steps + chunk - 1) / chunk);
+    return max(1, (int)((uint32_t)(steps + chunk - 1) / (uint32_t)chunk));
   };
   // Two sweeps over the tiles in order: the lengths' histogram, then the lists
   // (calls that fit one round need no order).
   const bool sorted = count > slots || chunk < whole;
-  const int longest_part = max(1, min(whole, chunk));
+  const float per_part = (float)(kBuckets - 1) / (float)max(1, min(whole, chunk));
   // (a tail's parts come last of all)
   auto place_bucket = [&](int steps, int parts) {
-    const int len = min((steps + parts - 1) / parts, longest_part);
-    const int at = (kBuckets - 1) - (int)((int64_t)len * (kBuckets - 1) / longest_part);
+    const int len = parts == 1 ? steps : (int)((float)(steps + parts - 1) / (float)parts);
+    const int at = bucket_of(len, per_part);
     return tail > 1 ? (parts > 1 ? kBuckets - 1 : min(at, kBuckets - 2)) : at;
   };
   if (sorted) {
@@ -291,9 +295,10 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
         tile_steps[i] = steps;
         continue;
       }
+      const Cut cut(steps, parts);
       for (int j = 0; j < parts; ++j) {
-        it.s0 = (int)((int64_t)steps * j / parts);
-        it.s1 = (int)((int64_t)steps * (j + 1) / parts);
+        it.s0 = cut.from(j);
+        it.s1 = cut.from(j + 1);
         it.slot = split ? slot0 + j : -1;
         if (place + j < p.max_items) p.items[place + j] = it;
       }
@@ -326,9 +331,10 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     it.q0 = s.q0; it.n = s.n; it.k0 = s.k0; it.m = s.m;
     it.tile = i - base[it.request];
     it.parts = parts;
+    const Cut cut(steps, parts);
     for (int j = tid; j < parts; j += kThreads) {
-      it.s0 = (int)((int64_t)steps * j / parts);
-      it.s1 = (int)((int64_t)steps * (j + 1) / parts);
+      it.s0 = cut.from(j);
+      it.s1 = cut.from(j + 1);
       it.slot = many[2][n] + j;
       if (many[1][n] + j < p.max_items) p.items[many[1][n] + j] = it;
     }
@@ -423,8 +429,8 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
                           workspace ? workspace_bytes : (size_t)0, s.bytes);
   unsigned char* const ws = static_cast<unsigned char*>(workspace);
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.tile_rows = s.tile_rows;
-  p.step_keys = s.step_keys;
+  p.tile_shift = __builtin_ctz(s.tile_rows);
+  p.step_shift = __builtin_ctz(s.step_keys);
   p.min_chunk = s.min_chunk;
   p.slots = s.slots;
   p.max_tiles = (int32_t)s.max_tiles;

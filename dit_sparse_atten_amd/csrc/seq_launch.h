@@ -23,7 +23,7 @@ int launch_dim(const Params& p, bool paged, bool narrow, int max_groups, bool me
     // Tiles have many parts only where there are few of them.
     const bool few_tiles = (int64_t)p.max_tiles * kFewParts <= p.max_slots;
     const dim3 groups((unsigned)std::min<int64_t>((int64_t)p.max_splits * units,
-                                                  std::max(1, 8192 / p.kv_heads)),
+                                                  std::max(1, 2048 / p.kv_heads)),
                       (unsigned)p.kv_heads, few_tiles ? 16u : 1u);
     if (narrow) hipLaunchKernelGGL((seq_merge_kernel<T, kD, kNarrowRows>), groups, block, 0, stream, p);
     else hipLaunchKernelGGL((seq_merge_kernel<T, kD, kWideRows>), groups, block, 0, stream, p);

@@ -42,7 +42,8 @@ struct Item {
   int32_t s0, s1;                 // key steps
   int32_t slot;                   // partial slot, -1: the whole tile, written to O
   int32_t parts;                  // of the tile
-  int32_t pad[6];
+  int32_t chain;                  // 16-row tiles: the workgroup, of its key head's
+  int32_t pad[5];
 };
 static_assert(sizeof(Item) == 64, "items are read as one 64-byte line");
 
@@ -71,9 +72,9 @@ struct Params {
   int32_t tile_shift, step_shift, min_chunk;  // log2 of a tile's rows, of a step's keys
   int32_t slots;               // workgroups that run at a time
   int32_t max_tiles, max_items, max_splits, max_slots;  // room in the lists, per key head
-  int32_t cheap_parts;         // tiles are cut freely, whatever their number
   float item_cost, part_cost, merge_cost;    // of an item and a partial, in key steps
   int32_t* counts;             // items, split tiles, items that run by head groups
+  int32_t* chain_start;        // [kMaxChains] first item of each chain (16-row tiles)
   int32_t* tile_base;          // [requests + 1] tiles before each sequence
   Item* items;
   Item* splits;                // split tiles: slot = the first of `parts` slots
@@ -98,7 +99,9 @@ constexpr float kRescaleLog2 = 8.0f;  // move the reference max once a p could e
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kHeadGroup = 8;  // key heads that run together: one per XCD
 constexpr int kWideRows = 128, kWideKeys = 64;
-constexpr int kNarrowRows = 16, kNarrowKeys = 128;  // 32 keys for each of four waves
+constexpr int kMaxChains = 256;
+constexpr int kNarrowWaves = 4;
+constexpr int kNarrowRows = 16, kNarrowKeys = 32 * kNarrowWaves;  // 32 keys for each wave
 
 // ds_read_b64_tr_b16: in each 16-lane group lane j receives element j % 4 of
 // the 8 bytes that lane 4 r + j / 4 addresses, r = 0..3.
@@ -173,6 +176,7 @@ __device__ __forceinline__ Item load_item(const Item* at) {
   const dsa::const_i32 s = (dsa::const_i32)(const int32_t*)at;
   it.request = s[0]; it.q0 = s[1]; it.n = s[2]; it.k0 = s[3]; it.m = s[4];
   it.tile = s[5]; it.s0 = s[6]; it.s1 = s[7]; it.slot = s[8]; it.parts = s[9];
+  it.chain = s[10];
   return it;
 }
 
@@ -352,21 +356,19 @@ __device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int
   return true;
 }
 
-// The item and key head of this workgroup; false: none.  kGrouped: the list's
-// first counts[2] items run eight key heads at a time, so that each XCD streams
-// the keys of one head through its L2; the others, which even out the end of the
-// call, run all heads of one item before the next.  (40 heads of one query head,
-// 16,384 x 16,384: 5.45 ms all heads at a time, 4.82 ms eight.)
-template <bool kGrouped>
+// The item and key head of this workgroup; false: none.  The list's first
+// counts[2] items run eight key heads at a time, so that each XCD streams the
+// keys of one head through its L2; the others, which even out the end of the call,
+// run all heads of one item before the next.  (40 heads of one query head, 16,384
+// x 16,384: 5.45 ms all heads at a time, 4.82 ms eight.)
 __device__ __forceinline__ bool take_item(const Params& p, Item* it, int* h) {
   const int wg = (int)blockIdx.x;
   if (p.unlisted) return own_item(p, wg, it, h);
-  const int count = ((dsa::const_i32)p.counts)[0];
+  const int count = ((dsa::const_i32)p.counts)[0], grouped = ((dsa::const_i32)p.counts)[2];
   if (wg >= count * p.kv_heads) return false;
-  int item = wg / p.kv_heads, grouped = 0;
+  int item = wg / p.kv_heads;
   *h = wg - item * p.kv_heads;
-  if constexpr (kGrouped) grouped = ((dsa::const_i32)p.counts)[2];
-  if (kGrouped && wg < grouped * p.kv_heads) {
+  if (wg < grouped * p.kv_heads) {
     const int first = wg / max(1, grouped * kHeadGroup) * kHeadGroup;
     const int rest = wg - first * grouped, heads = min(kHeadGroup, p.kv_heads - first);
     item = rest / heads;
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
 
   Item it;
   int h;
-  if (!take_item<true>(p, &it, &h)) return;
+  if (!take_item(p, &it, &h)) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
 // c16) = (lane / 16, lane % 16) holds row c16's scores of the keys 16 kg + 4 q4
 // + r and, of O, the dims 16 dt + 4 q4 + r.
 template <typename T, int kD, bool kPaged>
-__global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
+__global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params p) {
   typedef dsa::Elem<T> E;
   typedef typename E::x8 x8;
   constexpr int kRow = kD * 2;
@@ -787,19 +789,17 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
   constexpr int kRowsPer = 64 / kChunks;    // rows of one 1 KB load
   constexpr int kLoads = 16 / kRowsPer;     // loads per 16-key granule
   constexpr int kDt = kD / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[4 * kStage];
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[4 * kStage];
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[4 * kStage];
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_v1[4 * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[kNarrowWaves * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[kNarrowWaves * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[kNarrowWaves * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v1[kNarrowWaves * kStage];
 
-  Item it;
-  int h;
-  if (!take_item<false>(p, &it, &h)) return;
-
+  __shared__ float join_ml[2][kNarrowWaves][16];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q4 = lane >> 4, c16 = lane & 15;
+  auto run = [&](const Item& it, const int h) __attribute__((always_inline)) {
   const int rows = it.n * p.group;
   const int row_c = min(it.tile * kNarrowRows + c16, rows - 1);
   const int token = row_c / p.group;
@@ -993,9 +993,7 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
   // Join the waves: their O, m and l through the K stages (row-major fp32).
   l_run += __shfl_xor(l_run, 16);
   const float l_wave = dsa::pair32_sum(l_run);
-  constexpr int kWaveFloats = part_floats(kNarrowRows, kD);
-  static_assert(4 * kWaveFloats * 4 <= 4 * kStage + 4 * 16 * 8, "joins through lds_k0 and join_ml");
-  __shared__ float join_ml[2][4][16];
+  static_assert(kNarrowRows * kD * 4 <= kStage, "a wave joins through its own K stage");
   float unfinite = 0.f;  // NaN once an element of O is not finite
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt)
@@ -1030,14 +1028,15 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
   }
   dsa::lds_barrier();
   // Thread (r, c): row r, dims 8 c .. 8 c + 7.
-  const int r = tid / kChunks, d0 = (tid % kChunks) * 8;
+  for (int r = tid / kChunks; r < kNarrowRows; r += kNarrowWaves * kRowsPer) {
+  const int d0 = (tid % kChunks) * 8;
   const int out_row = it.tile * kNarrowRows + r;
-  if (r >= kNarrowRows || out_row >= rows) return;
-  float m_all = -INFINITY, l_all = 0.f, w[4];
+  if (out_row >= rows) break;
+  float m_all = -INFINITY, l_all = 0.f, w[kNarrowWaves];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
+  for (int i = 0; i < kNarrowWaves; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kNarrowWaves; ++i) {
     const float mi = join_ml[0][i][r];
     // (no finite score: l is 0, or NaN from NaN scores)
     w[i] = mi == -INFINITY ? join_ml[1][i][r] : __builtin_amdgcn_exp2f(mi - m_all);
@@ -1047,7 +1046,7 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
 #pragma unroll
   for (int x = 0; x < 8; ++x) acc[x] = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kNarrowWaves; ++i) {
     if (w[i] == 0.f) continue;
     const float* src = reinterpret_cast<const float*>(lds_k0) + (i * kNarrowRows + r) * kD + d0;
 #pragma unroll
@@ -1063,7 +1062,7 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
       po[kNarrowRows * kD + r] = m_all;
       po[kNarrowRows * (kD + 1) + r] = l_all;
     }
-    return;
+    continue;
   }
   const int out_token = it.q0 + out_row / late->group;
   const int out_head = h * late->group + out_row % late->group;
@@ -1078,6 +1077,29 @@ __global__ void __launch_bounds__(256, 1) seq_narrow_kernel(Params p) {
   if (late->lse && d0 == 0)
     late->lse[(int64_t)out_head * late->q_rows + out_token] =
         l_all == 0.f ? -INFINITY : m_all * kLn2 + logf(l_all);
+  }  };
+
+  // An unlisted call gives the workgroup one item, a listed one its chain.
+  Item it;
+  int h;
+  if (p.unlisted) {
+    if (own_item(p, (int)blockIdx.x, &it, &h)) run(it, h);
+    return;
+  }
+  const int chain = (int)blockIdx.x / p.kv_heads;
+  h = (int)blockIdx.x - chain * p.kv_heads;
+  const int count = ((dsa::const_i32)p.counts)[0];
+  int i = ((dsa::const_i32)p.chain_start)[chain];
+  if (i >= count) return;
+  it = load_item(p.items + i);
+#pragma unroll 1
+  for (;;) {
+    run(it, h);
+    if (++i >= count) break;
+    it = load_item(p.items + i);
+    if (it.chain != chain) break;
+    dsa::lds_barrier();  // the join's reads are done
+  }
 }
 
 // Joins the parts of split tiles: with M the largest reference, O = sum_i O_i

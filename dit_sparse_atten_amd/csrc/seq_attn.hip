@@ -36,22 +36,27 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* lds, uint32
 // Workgroup 0 lists the call's items and split tiles; the others give the rows
 // that belong to no sequence their values (O 0 with p.fill, LSE -inf).
 //
-// The workgroups of the chip (p.slots at a time) take items in list order, all
-// key heads of one before the next, longest first.  Which tiles are cut, in units
-// of one tile's key steps, with `work` the steps of all tiles and heads:
-//  * up to one round of tiles, and wherever partials are small (16-row tiles):
-//    every tile longer than `chunk` in near-equal parts of at most that.  Each
-//    candidate (the longest tile in 1, 2, 3, .. 512 parts; of more than a round, a
-//    slot's share of the work times 2 / 3, 2 / 4, ..) costs rounds x (mean length
-//    + p.item_cost), or the share plus half the longest part if that is more; the
-//    cheapest is taken.
-//  * else whole tiles, longest first, even out by themselves but for the last
+// kChains (16-row tiles, bound by the reads of their keys): the tiles of a key
+// head in a row, each counted as its key steps and a set-up of p.item_cost steps,
+// are cut into as many equal ranges as the head has workgroups, and a workgroup
+// walks the tiles and parts of one range, its chain.  (A decoding step of 64
+// requests of 1,000 to 16,000 tokens: 582 us with parts listed longest first,
+// 554 us with chains.)
+//
+// Else (128-row tiles, bound by their products) the workgroups of the chip (p.slots
+// at a time) take items in list order, longest first.  Which tiles are cut, in
+// key steps, with `work` the steps of all tiles and heads:
+//  * up to one round of tiles: every tile longer than `chunk` in near-equal parts
+//    of at most that.  Each candidate (the longest tile in 1, 2, 3, .. 512 parts)
+//    costs rounds x (mean length + p.item_cost), or its share of the work plus
+//    half the longest part if that is more; the cheapest is taken.
+//  * more: whole tiles, longest first, even out by themselves but for the last
 //    round.  Tiles longer than a slot's share of the work are cut to it; if there
 //    are none, the shortest tiles, as many as the last round is short of full,
 //    are cut into as many parts as pay.
 // Parts cost their partials (p.part_cost).  No choice depends on the order of
 // the atomics that place items of nearly equal length.
-template <int kThreads>
+template <int kThreads, bool kChains>
 __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
@@ -65,6 +70,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   __shared__ int hist[kBuckets];
   __shared__ uint32_t tried[32];
   __shared__ int many[3][kLdsTiles / kManyParts];  // tile, place, slot of the tiles of many parts
+  __shared__ int starts[kMaxChains];
   __shared__ unsigned long long work_lds;
   __shared__ int longest_lds, many_count, grouped_lds, chunk_lds, tail_parts, cut_bucket, cut_left;
   const bool in_lds = p.requests <= kLdsRequests;
@@ -134,6 +140,63 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     }
   }
   __syncthreads();
+  if constexpr (kChains) {
+    // Units of a tile: its set-up, then its steps; chain c holds the units from c
+    // quota on.  A tile starts in the chain of its first step.
+    const int setup = (int)p.item_cost;
+    const int chains = max(1, p.slots / p.kv_heads);
+    const uint64_t units = work_lds + (uint64_t)tiles * setup;
+    const uint32_t quota =
+        (uint32_t)max((units + chains - 1) / (uint64_t)chains, (uint64_t)(setup + p.min_chunk));
+    const int last_chain = (int)((units + quota - 1) / quota) - 1;
+    for (int c = tid; c < kMaxChains; c += kThreads) starts[c] = 0x7fffffff;
+    uint32_t items = 0, split_sums = 0, unit_sum = 0;
+    for (int i0 = 0; i0 < tiles; i0 += kThreads) {
+      const int i = i0 + tid;
+      const int steps = i < tiles ? steps_at(i) : 0;
+      const uint32_t own = i < tiles ? (uint32_t)(steps + setup) : 0u;
+      const uint32_t from = unit_sum + group_scan<kThreads>(own, scan_lds, &total) - own + setup;
+      unit_sum += total;
+      const int first = min((int)(from / quota), last_chain);
+      int parts = i < tiles ? 1 : 0;
+      if (steps > 0 && p.max_slots > 0)
+        parts += min((int)((from + steps - 1) / quota), last_chain) - first;
+      const int place = (int)(items + group_scan<kThreads>((uint32_t)parts, scan_lds, &total)) - parts;
+      items += total;
+      const uint32_t cuts = parts > 1 ? (uint32_t)parts << 16 | 1u : 0u;
+      const uint32_t at = split_sums + group_scan<kThreads>(cuts, scan_lds, &total) - cuts;
+      split_sums += total;
+      if (parts == 0) continue;
+      Item it = {};
+      it.request = find(i);
+      const Sequence s = seq_of(it.request);
+      it.q0 = s.q0; it.n = s.n; it.k0 = s.k0; it.m = s.m;
+      it.tile = i - base[it.request];
+      it.parts = parts;
+      const int slot0 = (int)(at >> 16), split0 = (int)(at & 0xffff);
+      if (parts > 1 && split0 < p.max_splits) {
+        it.slot = slot0;
+        p.splits[split0] = it;
+      }
+      for (int j = 0; j < parts; ++j) {
+        it.chain = first + j;
+        it.s0 = j == 0 ? 0 : (int)(it.chain * quota - from);
+        it.s1 = j + 1 == parts ? steps : (int)((it.chain + 1) * quota - from);
+        it.slot = parts > 1 ? slot0 + j : -1;
+        if (place + j < p.max_items) {
+          p.items[place + j] = it;
+          atomicMin(&starts[it.chain], place + j);
+        }
+      }
+    }
+    __syncthreads();
+    for (int c = tid; c < kMaxChains; c += kThreads) p.chain_start[c] = starts[c];
+    if (tid == 0) {
+      p.counts[0] = (int)min(items, (uint32_t)p.max_items);
+      p.counts[1] = (int)min(split_sums & 0xffff, (uint32_t)p.max_splits);
+    }
+    return;
+  }
   const int longest = longest_lds;
   const int64_t work = (int64_t)work_lds * p.kv_heads, count = (int64_t)tiles * p.kv_heads;
   const int slots = p.slots;
@@ -148,13 +211,10 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   const int share = (int)max((work + slots - 1) / slots, (int64_t)p.min_chunk);
   if (p.max_slots == 0 || longest < 2 * p.min_chunk || tiles == 0) {
     if (tid == 0) chunk_lds = whole;
-  } else if (count <= slots || (p.cheap_parts && tiles <= kLdsTiles)) {
-    // Candidate 0 leaves every tile whole, unless one alone is too long.
+  } else if (count <= slots) {
+    // Up to a round of tiles: at most `slots` <= kLdsTiles of them.
     const int which = tid & 31;
-    const int chunk =
-        count <= slots ? max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which])
-        : which == 0   ? min(whole, share)
-                       : max(p.min_chunk, 2 * share / (which + 2));
+    const int chunk = max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which]);
     uint32_t items = 0;
     for (int i = tid >> 5; i < tiles; i += kThreads / 32)
       items += max(1u, (uint32_t)(tile_steps[i] + chunk - 1) / (uint32_t)chunk);
@@ -170,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
       float price = n <= slots ? (float)chunk + cost
                                : fmaxf(rounds * mean, even + 0.5f * ((float)chunk + cost));
       if (cuts) price += p.merge_cost * (float)n;
-      if (which > 0 && cuts && tried[which] > (uint32_t)p.max_slots) price = INFINITY;
+      if (cuts && tried[which] > (uint32_t)p.max_slots) price = INFINITY;
       int best = which;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -350,7 +410,7 @@ struct Plan {
   bool narrow, merge, unlisted;
   int tile_rows, step_keys, min_chunk, slots;
   int64_t max_tiles, max_items, max_splits, max_slots;
-  size_t counts, base, items, splits, parts, bytes;
+  size_t counts, chains, base, items, splits, parts, bytes;
 };
 
 // Few rows per sequence (decoding steps) run 16-row tiles.
@@ -363,19 +423,19 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   s.slots = s.narrow ? 256 : 512;
   s.min_chunk = s.narrow ? 1 : 2;
   s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);
-  // Of one key head: no more than 2 `slots` partials over all of them (16-row
-  // tiles, with a sixteenth of the floats each: 8).  Tiles cut
+  // Of one key head: no more than 2 `slots` partials over all of them.  Tiles cut
   // at a slot's share of the work keep to that by themselves: each has more than
   // one whole chunk, of which the work of all heads holds `slots`.
   s.merge = max_keys >= 2 * (int64_t)s.min_chunk * s.step_keys && s.slots >= kv_heads;
-  s.max_slots = s.merge ? (s.narrow ? 8 : 2) * s.slots / kv_heads : 0;
+  s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
   s.max_splits = std::min(s.max_tiles, s.max_slots / 2);
   s.max_items = s.max_tiles + s.max_slots;
   // A call whose tiles all run at once, few enough for the lanes of a wave.
   s.unlisted = requests <= 64 && s.max_tiles <= 64 && s.max_tiles * kv_heads <= s.slots;
   const int dim = head_dim <= 64 ? 64 : 128;
   s.counts = 0;
-  s.base = 256;
+  s.chains = 256;
+  s.base = s.chains + kMaxChains * sizeof(int32_t);
   s.items = s.base + round256((size_t)(requests + 1) * sizeof(int32_t));
   s.splits = s.items + (size_t)s.max_items * sizeof(Item);
   s.parts = s.splits + round256((size_t)s.max_splits * sizeof(Item));
@@ -439,11 +499,11 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   p.max_slots = (int32_t)s.max_slots;
   // In key steps: what an item costs beside its keys, what a partial adds, and
   // its share of the join.
-  p.item_cost = s.narrow ? 1.0f : 2.0f;
-  p.cheap_parts = s.narrow;
+  p.item_cost = 2.0f;
   p.part_cost = s.narrow ? 0.25f : 2.5f;
   p.merge_cost = s.narrow ? 0.0005f : 0.011f;
   p.counts = reinterpret_cast<int32_t*>(ws + s.counts);
+  p.chain_start = reinterpret_cast<int32_t*>(ws + s.chains);
   p.tile_base = reinterpret_cast<int32_t*>(ws + s.base);
   p.items = reinterpret_cast<Item*>(ws + s.items);
   p.splits = reinterpret_cast<Item*>(ws + s.splits);
@@ -456,10 +516,16 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   int groups = (int)(s.max_items * p.kv_heads);
   if (s.unlisted) {
     groups = (s.merge ? s.slots : (int)s.max_tiles * p.kv_heads) + outside;
-  } else if (s.max_tiles <= 512 && p.requests <= 512) {
-    hipLaunchKernelGGL(seq_schedule_kernel<256>, dim3(1 + outside), dim3(256), 0, stream, p);
   } else {
-    hipLaunchKernelGGL(seq_schedule_kernel<1024>, dim3(1 + outside), dim3(1024), 0, stream, p);
+    const bool small = s.max_tiles <= 512 && p.requests <= 512;
+    const dim3 lists((unsigned)(1 + outside)), threads(small ? 256 : 1024);
+    auto schedule = [&](auto kernel) { hipLaunchKernelGGL(kernel, lists, threads, 0, stream, p); };
+    if (s.narrow) {
+      groups = std::max(1, s.slots / p.kv_heads) * p.kv_heads;
+      small ? schedule(seq_schedule_kernel<256, true>) : schedule(seq_schedule_kernel<1024, true>);
+    } else {
+      small ? schedule(seq_schedule_kernel<256, false>) : schedule(seq_schedule_kernel<1024, false>);
+    }
   }
   return dtype == DSA_BF16
              ? launch_typed<__bf16>(p, paged, s.narrow, groups, s.merge, stream, who)

@@ -10,10 +10,10 @@ namespace seq {
 template <typename T, int kD>
 int launch_dim(const Params& p, bool paged, bool narrow, int max_groups, bool merge,
                hipStream_t stream, const char* who) {
-  const dim3 grid((unsigned)max_groups), block(256);
+  const dim3 grid((unsigned)max_groups), block(256), narrow_block(kNarrowWaves * 64);
   if (narrow) {
-    if (paged) hipLaunchKernelGGL((seq_narrow_kernel<T, kD, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((seq_narrow_kernel<T, kD, false>), grid, block, 0, stream, p);
+    if (paged) hipLaunchKernelGGL((seq_narrow_kernel<T, kD, true>), grid, narrow_block, 0, stream, p);
+    else hipLaunchKernelGGL((seq_narrow_kernel<T, kD, false>), grid, narrow_block, 0, stream, p);
   } else {
     if (paged) hipLaunchKernelGGL((seq_wide_kernel<T, kD, true>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((seq_wide_kernel<T, kD, false>), grid, block, 0, stream, p);

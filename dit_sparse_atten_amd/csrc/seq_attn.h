@@ -440,10 +440,6 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   constexpr int kSlices = kD / 32;           // 1 KB loads per wave, K or V
   constexpr int kRowsPer = 64 / kChunks;     // rows of one load
   constexpr int kDt = kD / 32;               // 32-dim output tiles
-#ifndef KPRIO
-#define KPRIO 1
-#endif
-  constexpr bool kPrio = KPRIO;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[kStage];
@@ -641,7 +637,8 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
         pf[j][t + 1] = pb[1];
       }
     l_run += sum0 + sum1;
-    if (kPrio) __builtin_amdgcn_s_setprio(1);
+    // The two waves of a SIMD fall into opposite phases (2 to 4% on every long case).
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -653,7 +650,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
         const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         oacc[dt] = E::mfma32(a, pf[j], oacc[dt]);
       }
-    if (kPrio) __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_s_setprio(0);
   };
   int bad_cur = 0, bad_ahead = 0;  // of the staged step and of the one on its way
   auto step = [&](int s, const unsigned char* kc, const unsigned char* vc, unsigned char* kn,
@@ -833,7 +830,10 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
   }
 
   // Keys that no other tile of the request reads stream past the caches (64
-  // requests of 1,000 to 16,000 tokens, 8 key heads: 661 -> 601 us).
+  // requests of 1,000 to 16,000 tokens, 8 key heads: 661 -> 601 us).  Keys that
+  // still lie in the 256 MB cache from an earlier call take some 12% longer so,
+  // but a model's layers each have their own.  (The same in seq_wide_kernel gained
+  // 14% on cold single tiles and cost the long calls 2 to 3%.)
   const bool only_tile = rows <= kNarrowRows;
 
   // Pages of a window of 32 steps: lane l holds granule l & 1 of step l / 2.

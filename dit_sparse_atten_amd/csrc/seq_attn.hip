@@ -413,7 +413,10 @@ struct Plan {
   size_t counts, chains, base, items, splits, parts, bytes;
 };
 
-// Few rows per sequence (decoding steps) run 16-row tiles.
+// Calls of at most 16 rows (tokens x heads of a group) per sequence on average,
+// decoding steps, run 16-row tiles.  32 requests of 8,000 tokens, 8 key heads: 8
+// and 16 rows 172 us on 16-row tiles and 212 on 128-row ones, 24 and 32 rows (two
+// 16-row tiles) 365 and 212 us, 64 rows 716 and 213.
 Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int head_dim,
                int64_t max_keys) {
   Plan s;

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   __shared__ int many[3][kLdsTiles / kManyParts];  // tile, place, slot of the tiles of many parts
   __shared__ int starts[kMaxChains];
   __shared__ unsigned long long work_lds;
-  __shared__ int longest_lds, many_count, grouped_lds, chunk_lds, tail_parts, cut_bucket, cut_left;
+  __shared__ int longest_lds, many_count, grouped_lds, ranked, chunk_lds, tail_parts, cut_bucket, cut_left;
   const bool in_lds = p.requests <= kLdsRequests;
   int* const base = in_lds ? base_lds : p.tile_base;
   auto seq_of = [&](int r) -> Sequence { return in_lds ? seq_lds[r] : sequence(p, r); };
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     longest_lds = 0;
     many_count = 0;
     grouped_lds = 0;
+    ranked = 0;
     tail_parts = 1;
     cut_bucket = kBuckets;
     cut_left = 0;
@@ -257,7 +258,11 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
       __syncthreads();
       const uint32_t own = tid < kBuckets ? hist[tid] : 0;
       const uint32_t upto = group_scan<kThreads>(own, scan_lds, &total);
-      // (bucket tid holds the ranks upto - own .. upto - 1, longest first)
+      // (bucket tid holds the ranks upto - own .. upto - 1, longest first: where
+      // nothing is cut, the places of its items)
+      if (tid < kBuckets) hist[tid] = (int)(upto - own);
+      if (tid == kBuckets / 2) grouped_lds = (int)upto;
+      if (tid == 0) ranked = 1;
       const int from = tiles - k;  // first rank of the tail
       if (k > 0 && tid < kBuckets && (int)upto > from && (int)(upto - own) <= from) {
         const float steps = (float)(kBuckets - tid) * (float)whole / (float)(kBuckets - 1);
@@ -301,12 +306,14 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     const int at = bucket_of(len, per_part);
     return tail > 1 ? (parts > 1 ? kBuckets - 1 : min(at, kBuckets - 2)) : at;
   };
-  if (sorted) {
+  const bool cuts = tail > 1 || chunk < whole;
+  const bool placed = ranked != 0 && !cuts;  // the histogram is there already
+  if (sorted && !placed) {
     if (tid < kBuckets) hist[tid] = 0;
     __syncthreads();
   }
-  uint32_t items = 0, split_sums = 0;
-  for (int sweep = sorted ? 0 : 1; sweep < 2; ++sweep) {
+  uint32_t items = placed ? tiles : 0, split_sums = 0;
+  for (int sweep = sorted && !placed ? 0 : 1; sweep < 2; ++sweep) {
     uint32_t seen = 0;
     for (int i0 = 0; i0 < tiles; i0 += kThreads) {
       const int i = i0 + tid;
@@ -332,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
       }
       // Slots and split tiles in tile order: 16 bits each.
       uint32_t at = 0;
-      if (p.max_slots > 0) {
+      if (cuts) {
         const uint32_t own = split ? (uint32_t)parts << 16 | 1u : 0u;
         at = split_sums + group_scan<kThreads>(own, scan_lds, &total) - own;
         split_sums += total;

@@ -196,6 +196,10 @@ struct Sequence {
   int32_t q0, n, k0, m;
 };
 
+// Keys of a sequence at most, so that no key index of a step or a page window past
+// the last one leaves 32 bits.
+constexpr int kMaxKeys = 1 << 30;
+
 // Sequence r, whatever the arrays hold: rows and keys within the tensors.
 __device__ __forceinline__ Sequence sequence(const Params& p, int r) {
   Sequence s;
@@ -204,10 +208,10 @@ __device__ __forceinline__ Sequence sequence(const Params& p, int r) {
   if (p.kv_lens) {
     s.k0 = 0;
     const int64_t room = (int64_t)p.table_width << p.page_shift;
-    s.m = (int32_t)min((int64_t)max(p.kv_lens[r], 0), room);
+    s.m = (int32_t)min((int64_t)min(max(p.kv_lens[r], 0), kMaxKeys), room);
   } else {
     s.k0 = min(max(p.k_start[r], 0), p.k_rows);
-    s.m = min(max(p.k_start[r + 1], s.k0), p.k_rows) - s.k0;
+    s.m = min(min(max(p.k_start[r + 1], s.k0), p.k_rows) - s.k0, kMaxKeys);
   }
   return s;
 }

@@ -983,7 +983,7 @@ class PagedPlan(typing.NamedTuple):
     q_start: torch.Tensor  # int32 [requests + 1]: new tokens before each request
     kv_lens: torch.Tensor  # int32 [requests]: cached and new tokens
     slots: torch.Tensor    # int64 [tokens]: page * page_size + row, -1: no place
-    status: torch.Tensor   # int32 [2]: pages needed, new tokens without a slot
+    status: torch.Tensor   # int32 [2]: pages needed, new tokens past their last page
 
 
 # Short calls (a plan, a step's write, a decoding step of a few requests) are bound
@@ -1030,7 +1030,7 @@ def _block_table(t, device, requests):
 
 
 def _page_size(value):
-    if value < 16 or value & (value - 1):
+    if not 16 <= value <= 1 << 30 or value & (value - 1):
         raise ValueError(f"page_size {value} unsupported (a power of two from 16)")
 
 
@@ -1066,6 +1066,12 @@ def _cache_strides(name, t, dtype):
     return strides
 
 
+def _apart(name, t):
+    """Refuses a tensor to write into whose rows share memory (an expanded one)."""
+    if any(stride == 0 and size > 1 for stride, size in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} is written in place and must not be an expanded view")
+
+
 def _sequence_rows(name, t, dtype=None):
     """(tensor, strides) of a [rows, heads, head_dim] operand, copied if the
     kernels cannot read it in place."""
@@ -1074,6 +1080,8 @@ def _sequence_rows(name, t, dtype=None):
         raise ValueError(f"{name} must have shape [rows, heads, head_dim]")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype} like q, got {t.dtype}")
+    if t.shape[0] >= 1 << 31:
+        raise ValueError(f"{name} must have fewer than 2^31 rows")
     strides = _row_strides(t)
     if strides is None:
         t = t.clone(memory_format=torch.contiguous_format)
@@ -1096,8 +1104,9 @@ def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
     Returns a ``PagedPlan``: ``q_start``, ``kv_lens`` for ``paged_attention``,
     ``slots`` for ``paged_write`` (-1 behind the last request's tokens, and for
     tokens without a page because ``free_pages`` or the table's row is too
-    short), and ``status`` = (pages needed, tokens without a slot): the caller's
-    free list starts behind the first ``status[0]`` pages next time.
+    short), and ``status`` = (pages needed, new tokens past their request's last
+    page or behind ``tokens``): the caller's free list starts behind the first
+    ``status[0]`` pages next time.
     """
     lib = _lib.load()
     _require_cuda("cached", cached)
@@ -1108,8 +1117,8 @@ def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
     table, table_stride, width = _block_table(block_table, device, requests)
     free_pages = _index_vector("free_pages", free_pages, device)
     _page_size(page_size)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+    if not 0 <= tokens < 1 << 31:
+        raise ValueError(f"tokens must be in [0, 2^31), got {tokens}")
     ints = torch.empty(2 * requests + 3, dtype=torch.int32, device=device)
     slots = torch.empty(tokens, dtype=torch.int64, device=device)
     base = ints.data_ptr()
@@ -1151,6 +1160,8 @@ def paged_write(k, v, k_cache, v_cache, slots):
         raise ValueError("k, v, the caches and slots must be on the same device")
     if head_dim * size % 16:
         raise ValueError("rows must be a multiple of 16 bytes")
+    _apart("k_cache", k_cache)
+    _apart("v_cache", v_cache)
     if tokens == 0 or pages == 0 or heads == 0 or head_dim == 0:
         return
     if not slots.is_contiguous():
@@ -1185,12 +1196,13 @@ def _sequence_call(q, kv_heads, q_start, requests, scale, out, return_lse, max_k
         raise ValueError(f"scale must be positive and finite, got {scale}")
     fill = out is None
     if fill:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         o_strides = [heads * head_dim, head_dim]
     else:
         _require_cuda("out", out)
         if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
             raise ValueError("out must have q's shape, type and device")
+        _apart("out", out)
         o_strides = _row_strides(out)
         if o_strides is None:
             if rows:

@@ -502,7 +502,7 @@ int dsa_gated_residual(const void* x, int64_t x_stride, const void* y, int64_t y
  *   for a token without a page (the free list or the row is too short; its
  *   table entry becomes -1) and behind the last request's; status[2]: pages the
  *   step needs (more than free_count: the first free_count were given out), and
- *   new tokens without a slot.  Negative lengths count as 0.  Up to 8,192
+ *   new tokens past their request's last page or behind `tokens`.  Negative lengths count as 0.  Up to 8,192
  *   requests.  Nothing but the new table entries changes, so a repeated call
  *   gives the same plan.
  *
@@ -537,7 +537,7 @@ int dsa_paged_write(const void* k, const void* v, void* k_cache, void* v_cache,
  *   to 128, scale > 0.  lse: [heads, q_rows] natural log or NULL.  fill = 1: rows
  *   of o outside every sequence become 0; 0: they are left as they were (lse
  *   has -inf there).  Starts and lengths are device arrays, never read on the host;
- *   ones that leave the tensors are cut to them.  workspace: at least
+ *   ones that leave the tensors (or 2^30 keys) are cut to them.  workspace: at least
  *   dsa_seq_attention_workspace_bytes() with max_keys = k_rows, or table_width *
  *   page_size; calls that overlap in time need one each.
  */

@@ -600,3 +600,173 @@ def test_calls_on_two_streams(cuda_device):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(r, expected[i]) for r in results[i])
+
+
+def test_two_captured_graphs_replayed_in_turn(cuda_device):
+    """Two graphs of calls that split their keys, replayed alternately with eager
+    calls between: neither disturbs the other's results."""
+    kv_lens = [6000, 300]
+    k_cache, v_cache, table = _cache(kv_lens, 16, 2, 128, torch.bfloat16, 90, cuda_device)
+    at = (k_cache, v_cache, _ints(table, cuda_device), _ints(kv_lens, cuda_device))
+    q = [_rows((n, 8, 128), torch.bfloat16, 91 + n, cuda_device) for n in (2, 90)]
+    starts = [_starts([1, 1], cuda_device), _starts([60, 30], cuda_device)]
+    expected = [ops.paged_attention(x, *at, s) for x, s in zip(q, starts)]
+    graphs, outs = [], []
+    for x, s in zip(q, starts):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            ops.paged_attention(x, *at, s)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.paged_attention(x, *at, s))
+        graphs.append(graph)
+    for i in range(6):
+        graphs[i % 2].replay()
+        ops.paged_attention(q[1], *at, starts[1])
+        graphs[1 - i % 2].replay()
+        torch.cuda.synchronize()
+        for out, want in zip(outs, expected):
+            assert torch.equal(out, want), i
+
+
+@pytest.mark.parametrize("requests", [65, 1025, 3000])
+def test_many_requests(cuda_device, requests):
+    """More requests than one wave, one workgroup or the list's LDS holds; some
+    bring nothing, some have no keys."""
+    g = torch.Generator().manual_seed(requests)
+    kv_lens = torch.randint(0, 60, (requests,), generator=g).tolist()
+    q_lens = [int(i % 7 != 3) for i in range(requests)]
+    k_cache, v_cache, table = _cache(kv_lens, 16, 1, 64, torch.bfloat16, 92, cuda_device)
+    q = _rows((sum(q_lens), 4, 64), torch.bfloat16, 93, cuda_device)
+    out, lse = ops.paged_attention(q, k_cache, v_cache, _ints(table, cuda_device),
+                                   _ints(kv_lens, cuda_device), _starts(q_lens, cuda_device),
+                                   return_lse=True)
+    _check(out, lse, oracle.paged(q, k_cache, v_cache, table, kv_lens, q_lens), 64, 60,
+           v_cache[~v_cache.isnan()].abs().max().item())
+    # Their prompts, packed: 128-row tiles, several requests of none.
+    lens = [n * (1 + i % 3) for i, n in enumerate(q_lens)]
+    total = sum(lens)
+    q, k, v = (_rows((total, h, 64), torch.bfloat16, 94 + h, cuda_device) for h in (20, 1, 1))
+    out = ops.packed_attention(q, k, v, _starts(lens, cuda_device))
+    _check(out, None, oracle.packed(q, k, v, lens), 64, 3, v.abs().max().item())
+
+
+def test_tail_and_long_tiles_are_cut(cuda_device):
+    """Calls of more than one round of 128-row tiles: equal tiles whose last round
+    is cut, one tile far longer than its share, ragged ones that stay whole."""
+    g = torch.Generator().manual_seed(95)
+    for q_lens, k_lens, heads in (
+            ([128] * 50, [512] * 50, 12),        # 600 equal tiles: 88 of them are cut
+            ([128] * 129, [130] * 128 + [6000], 4),  # one long
+            (torch.randint(1, 400, (60,), generator=g).tolist(), None, 8)):
+        k_lens = k_lens or q_lens
+        q = _rows((sum(q_lens), heads, 64), torch.bfloat16, 96, cuda_device)
+        k = _rows((sum(k_lens), heads, 64), torch.bfloat16, 97, cuda_device)
+        v = _rows((sum(k_lens), heads, 64), torch.bfloat16, 98, cuda_device)
+        out, lse = ops.packed_attention(q, k, v, _starts(q_lens, cuda_device),
+                                        _starts(k_lens, cuda_device), causal=False,
+                                        return_lse=True)
+        _check(out, lse, oracle.packed(q, k, v, q_lens, k_lens, causal=False), 64, max(k_lens),
+               v.abs().max().item())
+
+
+def test_shared_pages_and_output_over_q(cuda_device):
+    """Requests that share a prefix's pages, and an output that takes q's place."""
+    k_cache, v_cache, table = _cache([64, 40], 16, 2, 64, torch.bfloat16, 99, cuda_device)
+    table[1][:2] = table[0][:2]
+    q = _rows((30, 4, 64), torch.bfloat16, 100, cuda_device)
+    args = (k_cache, v_cache, _ints(table, cuda_device), _ints([64, 40], cuda_device),
+            _ints([0, 10, 30], cuda_device))
+    out = ops.paged_attention(q, *args)
+    _check(out, None, oracle.paged(q, k_cache, v_cache, table, [64, 40], [10, 20]), 64, 64,
+           v_cache[~v_cache.isnan()].abs().max().item())
+    assert ops.paged_attention(q, *args, out=q) is q
+    assert torch.equal(q, out)
+
+
+def test_refusals(cuda_device):
+    def rows(n, h, d=64, t=torch.bfloat16):
+        return torch.zeros((n, h, d), dtype=t, device=cuda_device)
+
+    starts = _ints([0, 4], cuda_device)
+    q, k = rows(4, 4), rows(4, 2)
+    with pytest.raises(ValueError, match="float32"):
+        ops.packed_attention(rows(4, 4, t=torch.float32), rows(4, 2, t=torch.float32),
+                             rows(4, 2, t=torch.float32), starts)
+    with pytest.raises(ValueError, match="like q"):
+        ops.packed_attention(q, k.half(), k, starts)
+    with pytest.raises(ValueError, match="share"):
+        ops.packed_attention(rows(4, 5), k, k, starts)
+    with pytest.raises(ValueError, match="head dimension"):
+        ops.packed_attention(q, rows(4, 2, 72), rows(4, 2, 72), starts)
+    with pytest.raises(ValueError, match="head_dim"):
+        ops.packed_attention(rows(4, 4, 136), rows(4, 2, 136), rows(4, 2, 136), starts)
+    with pytest.raises(ValueError, match="head_dim"):
+        ops.packed_attention(rows(4, 4, 60), rows(4, 2, 60), rows(4, 2, 60), starts)
+    with pytest.raises(ValueError, match="int32"):
+        ops.packed_attention(q, k, k, starts.long())
+    with pytest.raises(ValueError, match="one value more"):
+        ops.packed_attention(q, k, k, starts[:0])
+    with pytest.raises(ValueError, match="k_start"):
+        ops.packed_attention(q, k, k, starts, _ints([0, 1, 2], cuda_device))
+    with pytest.raises(ValueError, match="scale"):
+        ops.packed_attention(q, k, k, starts, scale=-0.5)
+    with pytest.raises(ValueError, match="out"):
+        ops.packed_attention(q, k, k, starts, out=torch.zeros_like(k))
+    with pytest.raises(ValueError, match="expanded"):
+        ops.packed_attention(q, k, k, starts, out=q[:1].expand(4, -1, -1))
+    with pytest.raises(ValueError, match="aligned"):
+        ops.packed_attention(q, k, k, starts, out=rows(4, 4, 66)[..., :64])
+    with pytest.raises(ValueError, match="rows, heads, head_dim"):
+        ops.packed_attention(q[0], k, k, starts)
+    cache = torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+    table, lens = torch.zeros((1, 2), dtype=torch.int32, device=cuda_device), starts[1:]
+    odd = torch.zeros((3, 24, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+    with pytest.raises(ValueError, match="page_size"):
+        ops.paged_attention(q, odd, odd, table, lens, starts)
+    with pytest.raises(ValueError, match="block_table"):
+        ops.paged_attention(q, cache, cache, table.expand(2, -1), lens, starts)
+    with pytest.raises(ValueError, match="block_table"):
+        ops.paged_attention(q, cache, cache, table.long(), lens, starts)
+    with pytest.raises(ValueError, match="kv_lens"):
+        ops.paged_attention(q, cache, cache, table, lens.long(), starts)
+    with pytest.raises(ValueError, match="q_start"):
+        ops.paged_attention(q, cache, cache, table, lens, starts[:1])
+    with pytest.raises(ValueError, match="k_cache"):
+        ops.paged_attention(q, cache[..., ::2], cache[..., ::2], table, lens, starts)
+    with pytest.raises(ValueError, match="k_cache"):
+        ops.paged_attention(q, cache.half(), cache, table, lens, starts)
+    with pytest.raises(ValueError, match="shape"):
+        ops.paged_attention(q, cache, cache[:2], table, lens, starts)
+    slots = torch.zeros(4, dtype=torch.int64, device=cuda_device)
+    with pytest.raises(ValueError, match="slots"):
+        ops.paged_write(k, k, cache, cache.clone(), slots.int())
+    with pytest.raises(ValueError, match="expanded"):
+        ops.paged_write(k, k, cache[:1].expand(3, -1, -1, -1), cache, slots)
+    with pytest.raises(ValueError, match="agree"):
+        ops.paged_write(rows(4, 3), rows(4, 3), cache, cache.clone(), slots)
+    with pytest.raises(ValueError, match="2 or 4 bytes"):
+        ops.paged_write(k.double(), k.double(), cache.double(), cache.double(), slots)
+    with pytest.raises(ValueError, match="16-byte"):
+        ops.paged_write(rows(4, 2, 12), rows(4, 2, 12), cache[..., :12].contiguous(),
+                        cache[..., :12].contiguous(), slots)
+    with pytest.raises(ValueError, match="new"):
+        ops.paged_plan(lens, starts, table, starts, 16, 4)
+    with pytest.raises(ValueError, match="tokens"):
+        ops.paged_plan(lens, lens, table, starts, 16, -1)
+    with pytest.raises(ValueError, match="page_size"):
+        ops.paged_plan(lens, lens, table, starts, 20, 4)
+
+
+def test_axes_of_one_entry(cuda_device):
+    """An axis of one entry may have any stride."""
+    base = _rows((7, 3, 64), torch.bfloat16, 101, cuda_device)
+    one = torch.as_strided(base, (1, 2, 64), (13, 64, 1))
+    out = ops.packed_attention(one, one, one, _ints([0, 1], cuda_device))
+    assert torch.equal(out, one)
+    single = torch.as_strided(base, (7, 1, 64), (192, 5, 1))
+    expected = oracle.packed(single, single, single, [7])
+    out = ops.packed_attention(single, single, single, _ints([0, 7], cuda_device))
+    _check(out, None, expected, 64, 7, single.abs().max().item())

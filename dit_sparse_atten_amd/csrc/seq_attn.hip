@@ -436,12 +436,22 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // Of one key head: no more than 2 `slots` partials over all of them.  Tiles cut
   // at a slot's share of the work keep to that by themselves: each has more than
   // one whole chunk, of which the work of all heads holds `slots`.
-  s.merge = max_keys >= 2 * (int64_t)s.min_chunk * s.step_keys && s.slots >= kv_heads;
+  // Few keys are not cut: the join's launch costs what it saves.  Cut against whole,
+  // 8 key heads: 16-row tiles of 4 requests, 1,024 keys 15.9 / 13.1 us (the host's
+  // time), 1,536 keys 16.0 / 18.2; 128-row tiles of 2 requests, 512 keys 17.5 / 16.9,
+  // 768 keys 19.3 / 21.7, 1,536 keys 22.7 / 36.1.
+  s.merge = max_keys > (s.narrow ? 1024 : 640) && s.slots >= kv_heads;
   s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
   s.max_splits = std::min(s.max_tiles, s.max_slots / 2);
   s.max_items = s.max_tiles + s.max_slots;
-  // A call whose tiles all run at once, few enough for the lanes of a wave.
-  s.unlisted = requests <= 64 && s.max_tiles <= 64 && s.max_tiles * kv_heads <= s.slots;
+  // A call whose tiles all run at once, few enough for the lanes of a wave, works
+  // its items out by itself; 128-row tiles of long walks are better listed, for the
+  // list may cut them into more than one round of parts.
+  // (16 tiles x 8 key heads, listed against not: 4,096 keys 59 / 54 us, 16,384 keys
+  // 146 / 143, 32,768 keys 272 / 294.)
+  const int64_t walk = s.max_tiles * kv_heads * (max_keys / s.step_keys) / s.slots;
+  s.unlisted = requests <= 64 && s.max_tiles <= 64 && s.max_tiles * kv_heads <= s.slots &&
+               (s.narrow || walk <= 80);
   const int dim = head_dim <= 64 ? 64 : 128;
   s.counts = 0;
   s.chains = 256;

@@ -239,15 +239,15 @@ def test_nothing_to_write_is_no_call(lib):
 def test_workspace_sizes(lib):
     """Lists and partials by the host's bounds: q_rows G / tile rows + requests
     tiles, twice the chip's workgroups (512 of 128 rows, 256 of 16) of partials
-    over all key heads where the keys can be cut, none where they cannot."""
+    over all key heads where the keys may be cut, none where they are too few."""
     size = lib.dsa_seq_attention_workspace_bytes
 
     def expected(rows, requests, heads, kv, dim, keys):
         group = heads // kv
         narrow = rows * group <= 16 * requests
-        tile, step, slots, least = (16, 128, 256, 1) if narrow else (128, 64, 512, 2)
+        tile, slots, uncut = (16, 256, 1024) if narrow else (128, 512, 640)
         tiles = max(1, rows * group // tile + requests)
-        cut = keys >= 2 * least * step and slots >= kv
+        cut = keys > uncut and slots >= kv
         partials = 2 * slots // kv if cut else 0
         splits = min(tiles, partials // 2)
         at = 256 + 1024 + ((requests + 1) * 4 + 255) // 256 * 256 + (tiles + partials) * 64
@@ -255,8 +255,8 @@ def test_workspace_sizes(lib):
         return at + partials * kv * tile * ((64 if dim <= 64 else 128) + 2) * 4
 
     for case in ((8, 2, 4, 2, 64, 100), (4, 4, 32, 8, 128, 1536), (64, 64, 64, 8, 128, 16384),
-                 (2500, 8, 32, 8, 128, 30000), (32760, 1, 40, 8, 128, 32760), (3, 1, 3, 3, 40, 255),
-                 (3, 1, 3, 3, 40, 256), (300, 2, 600, 600, 64, 10 ** 6), (5, 0, 1, 1, 8, 0)):
+                 (2500, 8, 32, 8, 128, 30000), (32760, 1, 40, 8, 128, 32760), (3, 1, 3, 3, 40, 1024),
+                 (3, 1, 3, 3, 40, 1025), (30, 1, 3, 3, 40, 640), (30, 1, 3, 3, 40, 641), (300, 2, 600, 600, 64, 10 ** 6), (5, 0, 1, 1, 8, 0)):
         assert size(*case) == expected(*case), case
     assert size(0, 3, 4, 2, 64, 100) == 0
     assert size(4, 3, 5, 2, 64, 100) == 0

@@ -15,9 +15,10 @@
 // tiles: every key staged for a tile serves all heads of the group.  A tile's
 // keys may be cut into parts, whose fp32 partials seq_merge_kernel joins.
 // Lengths live on the device, so seq_schedule_kernel lists the (tile, part)
-// items there, longest first; the grids are the host's upper bounds and
-// workgroups past the list end at once.  In a call of few tiles every workgroup
-// works its item out by itself (own_item) and that kernel is left out.
+// items there: 128-row tiles longest first, 16-row tiles as one chain of items for
+// each workgroup.  The grids are the host's upper bounds, and workgroups past the
+// list end at once.  In a call of few tiles every workgroup works its item out by
+// itself (own_item) and that kernel is left out.
 //
 //  * seq_wide_kernel: 128 rows, four waves of 32, the 64-key staged walk of
 //    bsa_fwd_kernel (S^T = K Q^T, O^T = V^T P^T on 32x32x16 products).

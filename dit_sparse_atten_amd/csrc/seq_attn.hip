@@ -146,21 +146,25 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     // quota on.  A tile starts in the chain of its first step.
     const int setup = (int)p.item_cost;
     const int chains = max(1, p.slots / p.kv_heads);
-    const uint64_t units = work_lds + (uint64_t)tiles * setup;
+    const uint64_t all_units = work_lds + (uint64_t)tiles * setup;
+    // More than 32 bits count (5e11 keys): whole tiles, as many to each chain.
+    const bool vast = all_units >> 31 != 0;
+    const uint64_t units = vast ? (uint64_t)tiles : all_units;
     const uint32_t quota =
-        (uint32_t)max((units + chains - 1) / (uint64_t)chains, (uint64_t)(setup + p.min_chunk));
+        (uint32_t)max((units + chains - 1) / (uint64_t)chains, (uint64_t)(vast ? 1 : setup + p.min_chunk));
     const int last_chain = (int)((units + quota - 1) / quota) - 1;
     for (int c = tid; c < kMaxChains; c += kThreads) starts[c] = 0x7fffffff;
     uint32_t items = 0, split_sums = 0, unit_sum = 0;
     for (int i0 = 0; i0 < tiles; i0 += kThreads) {
       const int i = i0 + tid;
       const int steps = i < tiles ? steps_at(i) : 0;
-      const uint32_t own = i < tiles ? (uint32_t)(steps + setup) : 0u;
-      const uint32_t from = unit_sum + group_scan<kThreads>(own, scan_lds, &total) - own + setup;
+      const uint32_t own = i < tiles ? (vast ? 1u : (uint32_t)(steps + setup)) : 0u;
+      const uint32_t from =
+          unit_sum + group_scan<kThreads>(own, scan_lds, &total) - own + (vast ? 0 : setup);
       unit_sum += total;
       const int first = min((int)(from / quota), last_chain);
       int parts = i < tiles ? 1 : 0;
-      if (steps > 0 && p.max_slots > 0)
+      if (steps > 0 && p.max_slots > 0 && !vast)
         parts += min((int)((from + steps - 1) / quota), last_chain) - first;
       const int place = (int)(items + group_scan<kThreads>((uint32_t)parts, scan_lds, &total)) - parts;
       items += total;
@@ -209,7 +213,8 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   };
   const float per_whole = (float)(kBuckets - 1) / (float)whole;
   auto bucket = [&](int steps) { return bucket_of(steps, per_whole); };  // of whole tiles
-  const int share = (int)max((work + slots - 1) / slots, (int64_t)p.min_chunk);
+  const int share =
+      (int)min(max((work + slots - 1) / slots, (int64_t)p.min_chunk), (int64_t)0x7fffffff);
   if (p.max_slots == 0 || longest < 2 * p.min_chunk || tiles == 0) {
     if (tid == 0) chunk_lds = whole;
   } else if (count <= slots) {
@@ -446,12 +451,12 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   s.max_items = s.max_tiles + s.max_slots;
   // A call whose tiles all run at once, few enough for the lanes of a wave, works
   // its items out by itself; 128-row tiles of long walks are better listed, for the
-  // list may cut them into more than one round of parts.
-  // (16 tiles x 8 key heads, listed against not: 4,096 keys 59 / 54 us, 16,384 keys
-  // 146 / 143, 32,768 keys 272 / 294.)
-  const int64_t walk = s.max_tiles * kv_heads * (max_keys / s.step_keys) / s.slots;
+  // list may cut them into more than one round of parts.  (16 tiles x 8 key heads,
+  // listed against not: 4,096 keys 59 / 54 us, 16,384 keys 146 / 143, 32,768 keys
+  // 272 / 294.)
   s.unlisted = requests <= 64 && s.max_tiles <= 64 && s.max_tiles * kv_heads <= s.slots &&
-               (s.narrow || walk <= 80);
+               (s.narrow || s.max_tiles * kv_heads * std::min<int64_t>(max_keys, kMaxKeys) <=
+                                80 * (int64_t)s.slots * s.step_keys);
   const int dim = head_dim <= 64 ? 64 : 128;
   s.counts = 0;
   s.chains = 256;
@@ -489,9 +494,11 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
                              p.v_sp, p.v_st, p.v_sh};
   for (int64_t s : strides)
     if (s % 8 != 0 || s < 0) return dsa::set_error(DSA_EINVAL, "%s: strides must be multiples of 8", who);
-  // 16 staged rows are addressed by 32-bit byte offsets.
+  // 16 staged rows are addressed by 32-bit byte offsets, pages by 32 bits of 16 bytes.
   if (std::max(p.k_st, p.v_st) > (int64_t)1 << 25)
     return dsa::set_error(DSA_EUNSUPPORTED, "%s: token stride above 2^25 elements", who);
+  if (p.pages > 1 && std::max(p.k_sp, p.v_sp) >= (int64_t)1 << 35)
+    return dsa::set_error(DSA_EUNSUPPORTED, "%s: page stride of 2^35 elements or more", who);
   const void* const pointers[] = {p.q, p.k, p.v, p.o, workspace};
   for (const void* ptr : pointers)
     if (reinterpret_cast<uintptr_t>(ptr) & 15)
@@ -501,7 +508,8 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
     return dsa::set_error(DSA_EUNSUPPORTED, "%s: more than 2^31 query rows per key head", who);
   if (p.q_rows == 0) return DSA_OK;
   const Plan s = make_plan(p.q_rows, p.requests, p.group, p.kv_heads, p.head_dim, max_keys);
-  if (s.max_items > kMaxItems || s.max_items * p.kv_heads > 0x7fffffff)
+  // (a launch counts its threads, 256 for each item and key head, in 32 bits)
+  if (s.max_items > kMaxItems || (!s.narrow && s.max_items * p.kv_heads >= 1 << 24))
     return dsa::set_error(DSA_EUNSUPPORTED, "%s: too many query tiles (%lld)", who,
                           (long long)s.max_items);
   if (!workspace || workspace_bytes < s.bytes)
@@ -602,7 +610,7 @@ extern "C" int dsa_paged_attention(const void* q, const void* k_cache, const voi
                           page_size);
   if (pages < 0 || table_width < 0 || table_stride < table_width)
     return dsa::set_error(DSA_EINVAL, "%s: bad table or page count", who);
-  if (!kv_lens || (!table && table_width > 0))
+  if (requests > 0 && (!kv_lens || (!table && table_width > 0)))
     return dsa::set_error(DSA_EINVAL, "%s: null block table or lengths", who);
   const int64_t max_keys = (int64_t)table_width * page_size;
   seq::Params p = {};

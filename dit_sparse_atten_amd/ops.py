@@ -1135,8 +1135,8 @@ def paged_write(k, v, k_cache, v_cache, slots):
     [pages, page_size, kv_heads, head_dim], row t at slot ``slots[t]`` (int64 on
     the device; page * page_size + row).  Rows whose slot lies outside the cache
     (-1) are skipped.  A call's slots are distinct, as ``paged_plan`` gives
-    them: of rows that share one, parts of either may be kept.  Any element type
-    of 2 or 4 bytes."""
+    them: of rows that share one, parts of either may be kept.  k and v do not
+    overlap the caches.  Any element type of 2 or 4 bytes."""
     lib = _lib.load()
     k, k_strides = _sequence_rows("k", k)
     v, v_strides = _sequence_rows("v", v, k.dtype)
@@ -1230,7 +1230,8 @@ def packed_attention(q, k, v, q_start, k_start=None, causal=True, scale=None, ou
 
     Returns O [rows, heads, head_dim] (0 for rows that see no key) and, with
     ``return_lse``, the natural-log LSE [heads, rows] fp32 (-inf for those).  Rows
-    outside every sequence are 0, or left as they were in a given ``out``.
+    outside every sequence are 0, or left as they were in a given ``out``, which
+    may be q itself but overlaps no other operand and no other part of q.
     Forward only, as every attention here.
     """
     lib = _lib.load()

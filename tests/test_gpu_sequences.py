@@ -183,7 +183,7 @@ def test_outlier_scores(cuda_device, keys):
 def test_hidden_values_do_not_reach_earlier_rows(cuda_device, value, group):
     """A later token's key and value that are not finite leave earlier rows as
     they are (packed and paged, wide and narrow tiles, whole and split keys)."""
-    for n, m in ((150, 150), (4, 900), (70, 3000)):
+    for n, m in ((150, 150), (4, 900), (3, 2500), (70, 3000)):
         q = _rows((n, 2 * group, 128), torch.bfloat16, 14, cuda_device)
         k = _rows((m, 2, 128), torch.bfloat16, 15, cuda_device)
         v = _rows((m, 2, 128), torch.bfloat16, 16, cuda_device)
@@ -213,16 +213,19 @@ def test_hidden_values_do_not_reach_earlier_rows(cuda_device, value, group):
         assert torch.isfinite(out[first:, :, 1::3].float()).all()
 
 
-def test_nan_query_row_stays_alone(cuda_device):
-    q = _rows((200, 4, 64), torch.float16, 17, cuda_device)
-    k = _rows((200, 4, 64), torch.float16, 18, cuda_device)
-    v = _rows((200, 4, 64), torch.float16, 19, cuda_device)
-    starts = _starts([200], cuda_device)
-    clean, stat = ops.packed_attention(q, k, v, starts, return_lse=True)
-    q[77, 2] = math.nan
-    out, lse = ops.packed_attention(q, k, v, starts, return_lse=True)
-    assert out[77, 2].isnan().all() and lse[2, 77].isnan()
-    out[77, 2], lse[2, 77] = clean[77, 2], stat[2, 77]
+@pytest.mark.parametrize("kv_heads,row", [(4, 177), (1, 1)])
+def test_nan_query_row_stays_alone(cuda_device, kv_heads, row):
+    """(200 rows, and 4 of them as four heads of one key head: both tile heights)"""
+    n = 200 if kv_heads == 4 else 4
+    q = _rows((n, 4, 64), torch.float16, 17, cuda_device)
+    k = _rows((200, kv_heads, 64), torch.float16, 18, cuda_device)
+    v = _rows((200, kv_heads, 64), torch.float16, 19, cuda_device)
+    starts = _starts([n], cuda_device), _starts([200], cuda_device)
+    clean, stat = ops.packed_attention(q, k, v, *starts, return_lse=True)
+    q[row, 2] = math.nan
+    out, lse = ops.packed_attention(q, k, v, *starts, return_lse=True)
+    assert out[row, 2].isnan().all() and lse[2, row].isnan()
+    out[row, 2], lse[2, row] = clean[row, 2], stat[2, row]
     assert torch.equal(out, clean) and torch.equal(lse, stat)
 
 
@@ -273,10 +276,12 @@ def test_starts_that_leave_the_tensors(cuda_device):
     assert (none == 0).all()
 
 
+@pytest.mark.parametrize("keys", [700, 2700])
 @pytest.mark.parametrize("q_lens", [[1, 1], [40, 90]], ids=str)
-def test_bad_pages_take_no_part(cuda_device, q_lens):
-    """Entries outside the cache: -1, the page count, the type's limits."""
-    kv_lens = [700, 333]
+def test_bad_pages_take_no_part(cuda_device, q_lens, keys):
+    """Entries outside the cache: -1, the page count, the type's limits (the longer
+    request's keys are cut into parts)."""
+    kv_lens = [keys, 333]
     k_cache, v_cache, table = _cache(kv_lens, 16, 2, 128, torch.bfloat16, 28, cuda_device)
     for r, bad in ((0, -1), (0, k_cache.shape[0]), (1, 2 ** 31 - 1), (1, -2 ** 31)):
         table[r][3 if bad < 0 else 9] = bad
@@ -285,11 +290,11 @@ def test_bad_pages_take_no_part(cuda_device, q_lens):
     out, lse = ops.paged_attention(q, k_cache, v_cache, _ints(table, cuda_device),
                                    _ints(kv_lens, cuda_device), _starts(q_lens, cuda_device),
                                    return_lse=True)
-    _check(out, lse, oracle.paged(q, k_cache, v_cache, table, kv_lens, q_lens), 128, 700,
+    _check(out, lse, oracle.paged(q, k_cache, v_cache, table, kv_lens, q_lens), 128, keys,
            v_cache[~v_cache.isnan()].abs().max().item())
     # A table of none but bad pages: rows without a key.
     out, lse = ops.paged_attention(q, k_cache, v_cache,
-                                   torch.full((2, 50), -1, dtype=torch.int32, device=cuda_device),
+                                   torch.full((2, 200), -1, dtype=torch.int32, device=cuda_device),
                                    _ints(kv_lens, cuda_device), _starts(q_lens, cuda_device),
                                    return_lse=True)
     assert (out == 0).all() and (lse == -math.inf).all()
@@ -312,6 +317,13 @@ def test_no_sequences_rows_or_keys(cuda_device):
                               torch.zeros((2, 3), dtype=torch.int32, device=cuda_device),
                               _ints([40, 1], cuda_device), _ints([0, 1, 2], cuda_device))
     assert (out == 0).all()
+    # No request at all, rows of padding only.
+    for pages in (0, 2):
+        cache = torch.zeros((pages, 16, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+        out, lse = ops.paged_attention(
+            rows(3, 4), cache, cache, torch.zeros((0, 3), dtype=torch.int32, device=cuda_device),
+            _ints([], cuda_device), _ints([0], cuda_device), return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
     cache = torch.zeros((2, 16, 2, 64), dtype=torch.bfloat16, device=cuda_device)
     out = ops.paged_attention(rows(2, 4), cache, cache,
                               torch.zeros((2, 0), dtype=torch.int32, device=cuda_device),

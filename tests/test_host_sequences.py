@@ -166,6 +166,18 @@ def test_attention_stride_refusals(lib):
         strides = [64] * (8 if call is _packed else 10)
         strides[at] = (1 << 25) + 8  # of K's tokens
         assert call(lib, strides=_lib.int64_array(strides)) == _lib.DSA_EUNSUPPORTED
+    for at in (2, 5):  # of K's and V's pages
+        strides = [64] * 10
+        strides[at] = 1 << 35
+        assert _paged(lib, strides=_lib.int64_array(strides)) == _lib.DSA_EUNSUPPORTED
+        assert "page stride" in _lib.last_error()
+
+
+def test_attention_refuses_too_many_tiles(lib):
+    # 2^23 rows of 300 heads of their own: 2^16 tiles each, 19,660,800 of them.
+    assert _packed(lib, q_rows=1 << 23, requests=1, heads=300, kv_heads=300,
+                   workspace_bytes=1 << 60) == _lib.DSA_EUNSUPPORTED
+    assert "tiles" in _lib.last_error()
 
 
 @pytest.mark.parametrize("name,value,text", [

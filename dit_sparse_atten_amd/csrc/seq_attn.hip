@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* lds, uint32
 // requests of 1,000 to 16,000 tokens: 582 us with parts listed longest first,
 // 554 us with chains.)
 //
-// Else (128-row tiles, bound by their products) the workgroups of the chip (p.slots
+// Else (128-row tiles, bound by their products) the workgroups of the chip (kWideSlots
 // at a time) take items in list order, longest first.  Which tiles are cut, in
 // key steps, with `work` the steps of all tiles and heads:
 //  * up to one round of tiles: every tile longer than `chunk` in near-equal parts
@@ -145,13 +145,13 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     // Units of a tile: its set-up, then its steps; chain c holds the units from c
     // quota on.  A tile starts in the chain of its first step.
     const int setup = (int)p.item_cost;
-    const int chains = max(1, p.slots / p.kv_heads);
+    const uint32_t chains = max(1, kNarrowSlots / p.kv_heads);
     const uint64_t all_units = work_lds + (uint64_t)tiles * setup;
     // More than 32 bits count (5e11 keys): whole tiles, as many to each chain.
     const bool vast = all_units >> 31 != 0;
-    const uint64_t units = vast ? (uint64_t)tiles : all_units;
+    const uint32_t units = vast ? (uint32_t)tiles : (uint32_t)all_units;
     const uint32_t quota =
-        (uint32_t)max((units + chains - 1) / (uint64_t)chains, (uint64_t)(vast ? 1 : setup + p.min_chunk));
+        max((units + chains - 1) / chains, (uint32_t)(vast ? 1 : setup + p.min_chunk));
     const int last_chain = (int)((units + quota - 1) / quota) - 1;
     for (int c = tid; c < kMaxChains; c += kThreads) starts[c] = 0x7fffffff;
     uint32_t items = 0, split_sums = 0, unit_sum = 0;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
   }
   const int longest = longest_lds;
   const int64_t work = (int64_t)work_lds * p.kv_heads, count = (int64_t)tiles * p.kv_heads;
-  const int slots = p.slots;
+  constexpr int slots = kWideSlots;
   const int whole = max(longest, 1);  // a chunk that cuts nothing
   // Bucket of a length, the longest first (by a multiplication: any monotone map
   // serves).
@@ -221,17 +221,24 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     // Up to a round of tiles: at most `slots` <= kLdsTiles of them.
     const int which = tid & 31;
     const int chunk = max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which]);
+    // (quotients of at most 512: the product is off by one at most)
+    const float per_chunk = 1.f / (float)chunk;
     uint32_t items = 0;
-    for (int i = tid >> 5; i < tiles; i += kThreads / 32)
-      items += max(1u, (uint32_t)(tile_steps[i] + chunk - 1) / (uint32_t)chunk);
+#pragma unroll 4
+    for (int i = tid >> 5; i < tiles; i += kThreads / 32) {
+      const int x = tile_steps[i] + chunk - 1;
+      int parts = (int)((float)x * per_chunk);
+      parts += (x >= (parts + 1) * chunk) - (x < parts * chunk);
+      items += max(1, parts);
+    }
     atomicAdd(&tried[which], items);
     __syncthreads();
     if (tid < 64) {
-      const int64_t n = (int64_t)tried[which] * p.kv_heads;
+      const uint32_t n = tried[which] * (uint32_t)p.kv_heads;  // (up to 512 parts of 512 tiles)
       const bool cuts = chunk < whole;
       const float cost = p.item_cost + (cuts ? p.part_cost : 0.f);
       const float mean = (float)work / (float)n + cost;
-      const float rounds = (float)((n + slots - 1) / slots);
+      const float rounds = (float)((n + slots - 1) / slots);  // (slots: a power of two)
       const float even = ((float)work + cost * (float)n) / (float)slots;
       float price = n <= slots ? (float)chunk + cost
                                : fmaxf(rounds * mean, even + 0.5f * ((float)chunk + cost));
@@ -274,8 +281,8 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
         float best = steps + p.item_cost;
         int parts = 1;
         for (int q = 2; q <= 8; ++q) {
-          const int64_t n = (int64_t)k * q * p.kv_heads;
-          if ((int64_t)k * q > p.max_slots || steps < (float)(q * p.min_chunk)) break;
+          const uint32_t n = (uint32_t)(k * q * p.kv_heads);  // (k heads: a round and less than one more)
+          if (k * q > p.max_slots || steps < (float)(q * p.min_chunk)) break;
           const float price =
               (float)((n + slots - 1) / slots) * (steps / (float)q + p.item_cost + p.part_cost) +
               p.merge_cost * (float)n;
@@ -435,7 +442,7 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   s.narrow = q_rows * group <= 16 * requests;
   s.tile_rows = s.narrow ? kNarrowRows : kWideRows;
   s.step_keys = s.narrow ? kNarrowKeys : kWideKeys;
-  s.slots = s.narrow ? 256 : 512;
+  s.slots = s.narrow ? kNarrowSlots : kWideSlots;
   s.min_chunk = s.narrow ? 1 : 2;
   s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);
   // Of one key head: no more than 2 `slots` partials over all of them.  Tiles cut
@@ -549,7 +556,7 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
     const dim3 lists((unsigned)(1 + outside)), threads(small ? 256 : 1024);
     auto schedule = [&](auto kernel) { hipLaunchKernelGGL(kernel, lists, threads, 0, stream, p); };
     if (s.narrow) {
-      groups = std::max(1, s.slots / p.kv_heads) * p.kv_heads;
+      groups = std::max(1, kNarrowSlots / p.kv_heads) * p.kv_heads;
       small ? schedule(seq_schedule_kernel<256, true>) : schedule(seq_schedule_kernel<1024, true>);
     } else {
       small ? schedule(seq_schedule_kernel<256, false>) : schedule(seq_schedule_kernel<1024, false>);

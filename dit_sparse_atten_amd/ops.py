@@ -989,7 +989,8 @@ class PagedPlan(typing.NamedTuple):
 # Short calls (a plan, a step's write, a decoding step of a few requests) are bound
 # by the host: the helpers below look at each tensor once.  Lean forms of the
 # checks and no device context where the device is current took a plan from 13.0
-# to 10.9 us, a step's write from 14.3 to 9.5 us.
+# to 10.9 us, and those and the checks kept per layout (below) a step's write from
+# 14.3 to 7.2 us.
 
 def _call(function, what, device, *args):
     """One libdsa call on the device's current stream (its last argument)."""
@@ -1034,15 +1035,14 @@ def _page_size(value):
         raise ValueError(f"page_size {value} unsupported (a power of two from 16)")
 
 
-def _row_strides(t):
-    """Element strides of all axes but the last, 0 for axes of one entry; None
-    where the kernels cannot address the tensor in place: its last axis is not
-    contiguous, or an address not a multiple of 16 bytes."""
-    *lead, last = t.stride()
-    shape = t.shape
-    if (last != 1 and shape[-1] != 1) or t.data_ptr() & 15:
+def _row_strides(shape, strides, size):
+    """Element strides of all axes but the last of a tensor of `size`-byte elements,
+    0 for axes of one entry; None where the kernels cannot address it in place: its
+    last axis is not contiguous, or a row not a multiple of 16 bytes from another."""
+    *lead, last = strides
+    if last != 1 and shape[-1] != 1:
         return None
-    mask = 16 // t.element_size() - 1
+    mask = 16 // size - 1
     for axis, stride in enumerate(lead):
         if shape[axis] == 1:
             lead[axis] = 0
@@ -1051,42 +1051,54 @@ def _row_strides(t):
     return lead
 
 
-def _cache_strides(name, t, dtype):
+def _layout(t):
+    return t.shape, t.stride(), t.dtype
+
+
+def _cache_strides(name, layout, dtype):
     """Strides of a [pages, page_size, kv_heads, head_dim] cache, used in place."""
-    _require_cuda(name, t)
-    if t.ndim != 4:
+    shape, strides, own = layout
+    if len(shape) != 4:
         raise ValueError(f"{name} must have shape [pages, page_size, kv_heads, head_dim]")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    strides = _row_strides(t)
+    if own != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {own}")
+    strides = _row_strides(shape, strides, dtype.itemsize)
     if strides is None:
-        if t.numel():
+        if 0 not in shape:
             raise ValueError(f"{name} must have a contiguous, 16-byte aligned head dimension")
         strides = [0, 0, 0]
     return strides
 
 
-def _apart(name, t):
+def _apart(name, layout):
     """Refuses a tensor to write into whose rows share memory (an expanded one)."""
-    if any(stride == 0 and size > 1 for stride, size in zip(t.stride(), t.shape)):
+    shape, strides, _ = layout
+    if any(stride == 0 and size > 1 for stride, size in zip(strides, shape)):
         raise ValueError(f"{name} is written in place and must not be an expanded view")
 
 
-def _sequence_rows(name, t, dtype=None):
-    """(tensor, strides) of a [rows, heads, head_dim] operand, copied if the
-    kernels cannot read it in place."""
-    _require_cuda(name, t)
-    if t.ndim != 3:
+def _sequence_strides(name, layout, dtype):
+    """Strides of a [rows, heads, head_dim] operand, None: to be copied."""
+    shape, strides, own = layout
+    if len(shape) != 3:
         raise ValueError(f"{name} must have shape [rows, heads, head_dim]")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} like q, got {t.dtype}")
-    if t.shape[0] >= 1 << 31:
+    if own != dtype:
+        raise ValueError(f"{name} must be {dtype} like q, got {own}")
+    if shape[0] >= 1 << 31:
         raise ValueError(f"{name} must have fewer than 2^31 rows")
-    strides = _row_strides(t)
-    if strides is None:
-        t = t.clone(memory_format=torch.contiguous_format)
-        strides = _row_strides(t) or [0, 0]  # (rows that are not whole 16 bytes are refused)
-    return t, strides
+    return _row_strides(shape, strides, dtype.itemsize)
+
+
+def _aligned(name, t):
+    if t.data_ptr() & 15 and t.numel():
+        raise ValueError(f"{name} must have a contiguous, 16-byte aligned head dimension")
+
+
+def _in_place(copies, *operands):
+    """The operands, copied where the kernels cannot read them in place: those of
+    `copies`, and those at an address that is no multiple of 16 bytes."""
+    return [t.clone(memory_format=torch.contiguous_format) if i in copies or t.data_ptr() & 15
+            else t for i, t in enumerate(operands)]
 
 
 def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
@@ -1126,8 +1138,34 @@ def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
           requests, table, table_stride, width, free_pages.data_ptr(), free_pages.shape[0],
           page_size, tokens, base, base + 4 * (requests + 1), slots.data_ptr(),
           base + 4 * (2 * requests + 1))
-    q_start, kv_lens, status = ints.split((requests + 1, requests, 2))
+    q_start, kv_lens, status = torch.split_with_sizes(ints, (requests + 1, requests, 2))
     return PagedPlan(q_start, kv_lens, slots, status)
+
+
+# What a call's shapes, strides and types decide is checked once per combination of
+# them (a step's write 11.4 -> 7.2 us); addresses and devices are looked at each time.
+@functools.lru_cache(maxsize=512)
+def _write_layout(k, v, k_cache, v_cache):
+    """(operands to copy first, strides in bytes, tokens, heads, row bytes, pages, page size)."""
+    dtype = k[2]
+    if dtype.itemsize not in (2, 4):
+        raise ValueError(f"paged_write moves elements of 2 or 4 bytes, not {dtype}")
+    rows = [_sequence_strides("k", k, dtype), _sequence_strides("v", v, dtype)]
+    caches = [_cache_strides("k_cache", k_cache, dtype), _cache_strides("v_cache", v_cache, dtype)]
+    tokens, heads, head_dim = k[0]
+    pages, page_size, cache_heads, cache_dim = k_cache[0]
+    if v[0] != k[0] or v_cache[0] != k_cache[0]:
+        raise ValueError("k and v, and their caches, must have the same shape")
+    if cache_heads != heads or cache_dim != head_dim:
+        raise ValueError("the caches and k must agree on heads and head dimension")
+    _page_size(page_size)
+    if head_dim * dtype.itemsize % 16:
+        raise ValueError("rows must be a multiple of 16 bytes")
+    _apart("k_cache", k_cache)
+    _apart("v_cache", v_cache)
+    copies = tuple(i for i, x in enumerate(rows) if x is None)
+    strides = None if copies else _I64x10(*[x * dtype.itemsize for t in rows + caches for x in t])
+    return copies, strides, tokens, heads, head_dim * dtype.itemsize, pages, page_size
 
 
 def paged_write(k, v, k_cache, v_cache, slots):
@@ -1138,37 +1176,26 @@ def paged_write(k, v, k_cache, v_cache, slots):
     them: of rows that share one, parts of either may be kept.  k and v do not
     overlap the caches.  Any element type of 2 or 4 bytes."""
     lib = _lib.load()
-    k, k_strides = _sequence_rows("k", k)
-    v, v_strides = _sequence_rows("v", v, k.dtype)
-    size = k.element_size()
-    if size not in (2, 4):
-        raise ValueError(f"paged_write moves elements of 2 or 4 bytes, not {k.dtype}")
-    kc_strides = _cache_strides("k_cache", k_cache, k.dtype)
-    vc_strides = _cache_strides("v_cache", v_cache, k.dtype)
-    tokens, heads, head_dim = k.shape
-    pages, page_size, cache_heads, cache_dim = k_cache.shape
-    if v.shape != k.shape or v_cache.shape != k_cache.shape:
-        raise ValueError("k and v, and their caches, must have the same shape")
-    if cache_heads != heads or cache_dim != head_dim:
-        raise ValueError("the caches and k must agree on heads and head dimension")
-    _page_size(page_size)
-    _require_cuda("slots", slots)
+    for name, t in (("k", k), ("v", v), ("k_cache", k_cache), ("v_cache", v_cache),
+                    ("slots", slots)):
+        _require_cuda(name, t)
+    copies, strides, tokens, heads, row_bytes, pages, page_size = _write_layout(
+        _layout(k), _layout(v), _layout(k_cache), _layout(v_cache))
     if slots.dtype != torch.int64 or slots.shape != (tokens,):
         raise ValueError(f"slots must be an int64 tensor of {tokens} values")
     device = k_cache.device
     if not (k.device == v.device == v_cache.device == slots.device == device):
         raise ValueError("k, v, the caches and slots must be on the same device")
-    if head_dim * size % 16:
-        raise ValueError("rows must be a multiple of 16 bytes")
-    _apart("k_cache", k_cache)
-    _apart("v_cache", v_cache)
-    if tokens == 0 or pages == 0 or heads == 0 or head_dim == 0:
+    _aligned("k_cache", k_cache)
+    _aligned("v_cache", v_cache)
+    if tokens == 0 or pages == 0 or heads == 0 or row_bytes == 0:
         return
+    if copies or (k.data_ptr() | v.data_ptr()) & 15:
+        return paged_write(*_in_place(copies, k, v), k_cache, v_cache, slots)
     if not slots.is_contiguous():
         slots = slots.contiguous()
-    strides = _I64x10(*[s * size for s in (*k_strides, *v_strides, *kc_strides, *vc_strides)])
     _call(lib.dsa_paged_write, "dsa_paged_write", device, k.data_ptr(), v.data_ptr(),
-          k_cache.data_ptr(), v_cache.data_ptr(), strides, tokens, heads, head_dim * size, pages,
+          k_cache.data_ptr(), v_cache.data_ptr(), strides, tokens, heads, row_bytes, pages,
           page_size, slots.data_ptr())
 
 
@@ -1178,41 +1205,64 @@ def _sequence_workspace_bytes(q_rows, requests, heads, kv_heads, head_dim, max_k
                                                          head_dim, max_keys)
 
 
-def _sequence_call(q, kv_heads, q_start, requests, scale, out, return_lse, max_keys):
-    """What both sequence attentions check and allocate beside their keys:
-    (q, its strides, q_start, scale, out, its strides, fill, lse, workspace)."""
-    q, q_strides = _sequence_rows("q", q)
-    rows, heads, head_dim = q.shape
+@functools.lru_cache(maxsize=512)
+def _attention_layout(paged, q, k, v, out):
+    """(operands to copy first, strides, rows, heads, kv_heads, head_dim, dtype code) of a call."""
+    code = dtype_code(q[2])
+    dtype = q[2]
+    if paged:
+        keys = [_cache_strides("k_cache", k, dtype), _cache_strides("v_cache", v, dtype)]
+        if k[0] != v[0] or len(q[0]) != 3 or k[0][3] != q[0][2]:
+            raise ValueError("the caches must share their shape, and q [rows, heads, head_dim] "
+                             "their head dimension")
+        _page_size(k[0][1])
+    else:
+        keys = [_sequence_strides("k", k, dtype), _sequence_strides("v", v, dtype)]
+        if k[0] != v[0] or len(q[0]) != 3 or k[0][2] != q[0][2]:
+            raise ValueError("k and v must share their shape, and q [rows, heads, head_dim] their "
+                             "head dimension")
+    q_strides = _sequence_strides("q", q, dtype)
+    rows, heads, head_dim = q[0]
+    kv_heads = k[0][-2]
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} query heads do not share {kv_heads} key/value heads")
     if head_dim % 8 or not 8 <= head_dim <= HEAD_DIM:
         raise ValueError(f"head_dim {head_dim} unsupported (a multiple of 8 up to {HEAD_DIM})")
-    device = q.device
-    q_start = _index_vector("q_start", q_start, device, requests)
-    if q_start.shape[0] == 0:
-        raise ValueError("q_start must hold one value more than there are sequences")
-    scale = head_dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    fill = out is None
-    if fill:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out is None:
         o_strides = [heads * head_dim, head_dim]
     else:
-        _require_cuda("out", out)
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+        if out[0] != q[0] or out[2] != dtype:
             raise ValueError("out must have q's shape, type and device")
         _apart("out", out)
-        o_strides = _row_strides(out)
+        o_strides = _row_strides(*out[:2], dtype.itemsize)
         if o_strides is None:
             if rows:
                 raise ValueError("out must have a contiguous, 16-byte aligned head dimension")
             o_strides = [0, 0]
+    every = [q_strides, *keys, o_strides]
+    copies = tuple(i for i, x in enumerate(every) if x is None)
+    strides = None if copies else (_I64x10 if paged else _I64x8)(*[x for t in every for x in t])
+    return copies, strides, rows, heads, kv_heads, head_dim, code
+
+
+def _sequence_buffers(q, layout, q_start, scale, out, return_lse, max_keys):
+    """(scale, out, lse, workspace) of an attention call."""
+    _, _, rows, heads, kv_heads, head_dim, _ = layout
+    device = q.device
+    scale = head_dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if out is None:
+        out = torch.empty((rows, heads, head_dim), dtype=q.dtype, device=device)
+    else:
+        if out.device != device:
+            raise ValueError("out must have q's shape, type and device")
+        _aligned("out", out)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
     workspace = torch.empty(
         _sequence_workspace_bytes(rows, q_start.shape[0] - 1, heads, kv_heads, head_dim, max_keys),
         dtype=torch.uint8, device=device)
-    return q, q_strides, q_start, scale, out, o_strides, fill, lse, workspace
+    return scale, out, lse, workspace
 
 
 def packed_attention(q, k, v, q_start, k_start=None, causal=True, scale=None, out=None,
@@ -1236,26 +1286,32 @@ def packed_attention(q, k, v, q_start, k_start=None, causal=True, scale=None, ou
     """
     lib = _lib.load()
     _require_cuda("q", q)
-    code = dtype_code(q.dtype)
-    k, k_strides = _sequence_rows("k", k, q.dtype)
-    v, v_strides = _sequence_rows("v", v, q.dtype)
-    if k.shape != v.shape or q.ndim != 3 or k.shape[2] != q.shape[2]:
-        raise ValueError("k and v must share their shape, and q [rows, heads, head_dim] their "
-                         "head dimension")
+    _require_cuda("k", k)
+    _require_cuda("v", v)
+    fill = out is None
+    if not fill:
+        _require_cuda("out", out)
+    layout = _attention_layout(False, _layout(q), _layout(k), _layout(v),
+                               None if fill else _layout(out))
+    copies, strides, rows, heads, kv_heads, head_dim, code = layout
     device = q.device
     if not (k.device == v.device == device):
         raise ValueError("q, k and v must be on the same device")
-    k_rows, kv_heads, _ = k.shape
-    q, q_strides, q_start, scale, out, o_strides, fill, lse, workspace = _sequence_call(
-        q, kv_heads, q_start, None, scale, out, return_lse, k_rows)
-    rows, heads, head_dim = q.shape
+    q_start = _index_vector("q_start", q_start, device)
+    if q_start.shape[0] == 0:
+        raise ValueError("q_start must hold one value more than there are sequences")
     requests = q_start.shape[0] - 1
     if k_start is not None:
         k_start = _index_vector("k_start", k_start, device, requests + 1)
+    if copies or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        return packed_attention(*_in_place(copies, q, k, v), q_start, k_start, causal, scale, out,
+                                return_lse)
+    k_rows = k.shape[0]
+    scale, out, lse, workspace = _sequence_buffers(q, layout, q_start, scale, out, return_lse,
+                                                   k_rows)
     if rows:
         _call(lib.dsa_packed_attention, "dsa_packed_attention", device, q.data_ptr(),
-              k.data_ptr(), v.data_ptr(), out.data_ptr(), code,
-              _I64x8(*q_strides, *k_strides, *v_strides, *o_strides), rows, k_rows, requests,
+              k.data_ptr(), v.data_ptr(), out.data_ptr(), code, strides, rows, k_rows, requests,
               heads, kv_heads, head_dim, q_start.data_ptr(),
               None if k_start is None else k_start.data_ptr(), scale, 1 if causal else 0,
               1 if fill else 0, None if lse is None else lse.data_ptr(), workspace.data_ptr(),
@@ -1278,28 +1334,33 @@ def paged_attention(q, k_cache, v_cache, block_table, kv_lens, q_start, causal=T
     """
     lib = _lib.load()
     _require_cuda("q", q)
-    code = dtype_code(q.dtype)
-    kc_strides = _cache_strides("k_cache", k_cache, q.dtype)
-    vc_strides = _cache_strides("v_cache", v_cache, q.dtype)
-    if k_cache.shape != v_cache.shape or q.ndim != 3 or k_cache.shape[3] != q.shape[2]:
-        raise ValueError("the caches must share their shape, and q [rows, heads, head_dim] "
-                         "their head dimension")
+    _require_cuda("k_cache", k_cache)
+    _require_cuda("v_cache", v_cache)
+    fill = out is None
+    if not fill:
+        _require_cuda("out", out)
+    layout = _attention_layout(True, _layout(q), _layout(k_cache), _layout(v_cache),
+                               None if fill else _layout(out))
+    copies, strides, rows, heads, kv_heads, head_dim, code = layout
     device = q.device
     if not (k_cache.device == v_cache.device == device):
         raise ValueError("q and the caches must be on the same device")
-    pages, page_size, kv_heads, _ = k_cache.shape
-    _page_size(page_size)
+    _aligned("k_cache", k_cache)
+    _aligned("v_cache", v_cache)
+    pages, page_size = k_cache.shape[:2]
     kv_lens = _index_vector("kv_lens", kv_lens, device)
     requests = kv_lens.shape[0]
     table, table_stride, width = _block_table(block_table, device, requests)
-    q, q_strides, q_start, scale, out, o_strides, fill, lse, workspace = _sequence_call(
-        q, kv_heads, q_start, requests + 1, scale, out, return_lse, width * page_size)
-    rows, heads, head_dim = q.shape
+    q_start = _index_vector("q_start", q_start, device, requests + 1)
+    if copies or q.data_ptr() & 15:
+        return paged_attention(*_in_place(copies, q), k_cache, v_cache, block_table, kv_lens, q_start, causal,
+                               scale, out, return_lse)
+    scale, out, lse, workspace = _sequence_buffers(q, layout, q_start, scale, out, return_lse,
+                                                   width * page_size)
     if rows:
         _call(lib.dsa_paged_attention, "dsa_paged_attention", device, q.data_ptr(),
-              k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), code,
-              _I64x10(*q_strides, *kc_strides, *vc_strides, *o_strides), rows, requests, heads,
-              kv_heads, head_dim, pages, page_size, table, table_stride, width,
+              k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), code, strides, rows, requests,
+              heads, kv_heads, head_dim, pages, page_size, table, table_stride, width,
               kv_lens.data_ptr(), q_start.data_ptr(), scale, 1 if causal else 0, 1 if fill else 0,
               None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.shape[0])
     return (out, lse) if return_lse else out

@@ -438,7 +438,11 @@ __device__ __forceinline__ void exact_row(LateParams p, const Item& it, int h, i
 // half-tile ahead; lane (g, qi) = (lane / 32, lane % 32) holds row qi's scores
 // of the keys 32 kt + 8 (r / 4) + 4 g + r % 4 and, of O, the dims 32 dt +
 // 8 (r / 4) + 4 g + r % 4.
-template <typename T, int kD, bool kPaged>
+//
+// Staged rows hold kD dims, of which the products take the first kUse: head dims of
+// 72 to 96 leave the last quarter of a 128-dim row out (8,192 x 8,192 x 32 heads: 96
+// dims 897 -> 804 us, 80 dims 985 -> 896).
+template <typename T, int kD, int kUse, bool kPaged>
 __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   typedef dsa::Elem<T> E;
   typedef typename E::x8 x8;
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   constexpr int kChunks = kD / 8;            // 16-byte chunks per row
   constexpr int kSlices = kD / 32;           // 1 KB loads per wave, K or V
   constexpr int kRowsPer = 64 / kChunks;     // rows of one load
-  constexpr int kDt = kD / 32;               // 32-dim output tiles
+  constexpr int kDt = kUse / 32;             // 32-dim output tiles
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v0[kStage];
@@ -477,12 +481,12 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   const int kend =
       p.causal ? max(0, min(it.m, it.m - it.n + last_row / p.group + 1)) : it.m;
 
-  x8 qf[kD / 16];
+  x8 qf[kUse / 16];
   {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
 #pragma unroll
-    for (int dc = 0; dc < kD / 16; ++dc) {
+    for (int dc = 0; dc < kUse / 16; ++dc) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) qf[dc][e] = (T)0.0f;
       if (dc * 16 + g * 8 < p.head_dim)
@@ -579,7 +583,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sacc[kt][r] = 0.f;
 #pragma unroll
-    for (int dc = 0; dc < kD / 16; ++dc)
+    for (int dc = 0; dc < kUse / 16; ++dc)
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         const int krow = kt * 32 + qi;
@@ -590,7 +594,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
     // Four K reads in flight ahead of the products.
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int i = 0; i < kD / 8 - 4; ++i) {
+    for (int i = 0; i < kUse / 8 - 4; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }

@@ -7,6 +7,12 @@
 
 namespace seq {
 
+template <typename T, int kD, int kUse>
+void launch_wide(const Params& p, bool paged, dim3 grid, hipStream_t stream) {
+  if (paged) hipLaunchKernelGGL((seq_wide_kernel<T, kD, kUse, true>), grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((seq_wide_kernel<T, kD, kUse, false>), grid, dim3(256), 0, stream, p);
+}
+
 template <typename T, int kD>
 int launch_dim(const Params& p, bool paged, bool narrow, int max_groups, bool merge,
                hipStream_t stream, const char* who) {
@@ -14,9 +20,10 @@ int launch_dim(const Params& p, bool paged, bool narrow, int max_groups, bool me
   if (narrow) {
     if (paged) hipLaunchKernelGGL((seq_narrow_kernel<T, kD, true>), grid, narrow_block, 0, stream, p);
     else hipLaunchKernelGGL((seq_narrow_kernel<T, kD, false>), grid, narrow_block, 0, stream, p);
+  } else if (kD == 128 && p.head_dim <= 96) {
+    launch_wide<T, kD, kD == 128 ? 96 : kD>(p, paged, grid, stream);
   } else {
-    if (paged) hipLaunchKernelGGL((seq_wide_kernel<T, kD, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((seq_wide_kernel<T, kD, false>), grid, block, 0, stream, p);
+    launch_wide<T, kD, kD>(p, paged, grid, stream);
   }
   if (merge) {
     const int units = (narrow ? kNarrowRows : kWideRows) / 16;

@@ -72,6 +72,7 @@ struct Params {
   int32_t unlisted;            // no schedule kernel: workgroups work their items out (own_item)
   int32_t tile_shift, step_shift, min_chunk;  // log2 of a tile's rows, of a step's keys
   int32_t slots;               // workgroups that run at a time
+  int32_t shared_lines;        // 16-row tiles: key heads lie in the same 128-byte lines
   int32_t max_tiles, max_items, max_splits, max_slots;  // room in the lists, per key head
   float item_cost, part_cost, merge_cost;    // of an item and a partial, in key steps
   int32_t* counts;             // items, split tiles, items that run by head groups
@@ -265,6 +266,17 @@ __device__ __forceinline__ void clear_outside(const Params& p, int share, int sh
   }
 }
 
+// Unit of workgroup `wg` of `used`, where an XCD takes a range of units instead of every
+// eighth: the key heads of an item are neighbours, and where they lie in the same
+// 128-byte lines (head dims that are no multiple of 64) the XCD's L2 then reads a line
+// once.  (64 requests of 12,000 tokens, 8 key heads: 80 dims 470 -> 350 us, 96 dims 471
+// -> 416; 5 key heads of 40 dims 225 -> 155.  Where no line is shared, every eighth
+// spreads the reads better: 582 against 628 us at 128 dims.)
+__device__ __forceinline__ int unit_of(int wg, int used) {
+  const int each = used >> 3, more = used & 7, xcd = wg & 7;
+  return xcd * each + min(xcd, more) + (wg >> 3);
+}
+
 // The item and key head of workgroup `wg` in a call without a schedule kernel:
 // at most 64 sequences and 64 tiles, all of them (times the key heads) at once on
 // the chip.  Every wave works it out for itself, a lane per sequence, then per
@@ -340,11 +352,13 @@ __device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int
     if (parts > 1) p.splits[(splits - split) & 0xffff] = it;
     if (lane == 63) p.counts[1] = (int)(splits & 0xffff);
   }
-  const int item = wg / p.kv_heads;
-  if (item >= items) {
-    clear_outside(p, wg - items * p.kv_heads, (int)gridDim.x - items * p.kv_heads);
+  const int used = items * p.kv_heads;
+  if (wg >= used) {
+    clear_outside(p, wg - used, (int)gridDim.x - used);
     return false;
   }
+  if (p.shared_lines) wg = unit_of(wg, used);
+  const int item = wg / p.kv_heads;
   const int i = (int)__popcll(__ballot(lane < count && first <= item)) - 1;
   const int part = item - __builtin_amdgcn_readlane(first, i);
   const int len = __builtin_amdgcn_readlane(steps, i);
@@ -856,8 +870,9 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
   // requests of 1,000 to 16,000 tokens, 8 key heads: 661 -> 601 us).  Keys that
   // still lie in the 256 MB cache from an earlier call take some 12% longer so,
   // but a model's layers each have their own.  (The same in seq_wide_kernel gained
-  // 14% on cold single tiles and cost the long calls 2 to 3%.)
-  const bool only_tile = rows <= kNarrowRows;
+  // 14% on cold single tiles and cost the long calls 2 to 3%.)  Lines that several
+  // heads share do not (unit_of).
+  const bool only_tile = rows <= kNarrowRows && !p.shared_lines;
 
   // Pages of a window of 32 steps: lane l holds granule l & 1 of step l / 2.
   auto window_ids = [&](int window) -> int {
@@ -1109,8 +1124,10 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
     if (own_item(p, (int)blockIdx.x, &it, &h)) run(it, h);
     return;
   }
-  const int chain = (int)blockIdx.x / p.kv_heads;
-  h = (int)blockIdx.x - chain * p.kv_heads;
+  const int wg = (int)blockIdx.x;
+  const int unit = p.shared_lines ? unit_of(wg, (int)gridDim.x) : wg;
+  const int chain = unit / p.kv_heads;
+  h = unit - chain * p.kv_heads;
   const int count = ((dsa::const_i32)p.counts)[0];
   int i = ((dsa::const_i32)p.chain_start)[chain];
   if (i >= count) return;

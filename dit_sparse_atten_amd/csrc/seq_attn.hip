@@ -528,6 +528,10 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   p.step_shift = __builtin_ctz(s.step_keys);
   p.min_chunk = s.min_chunk;
   p.slots = s.slots;
+  auto shares = [](const void* at, int64_t head_stride) {
+    return head_stride % 64 != 0 || (reinterpret_cast<uintptr_t>(at) & 127) != 0;
+  };
+  p.shared_lines = s.narrow && p.kv_heads > 1 && (shares(p.k, p.k_sh) || shares(p.v, p.v_sh));
   p.max_tiles = (int32_t)s.max_tiles;
   p.max_items = (int32_t)s.max_items;
   p.max_splits = (int32_t)s.max_splits;

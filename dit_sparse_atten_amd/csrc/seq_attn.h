@@ -244,6 +244,15 @@ struct Cut {
   __device__ __forceinline__ int from(int j) const { return j * each + min(j, more); }
 };
 
+// Parts of at most `chunk` steps, at least one; `per` = 1 / chunk.  (For up to 512
+// parts the product is off by one at most.)
+__device__ __forceinline__ int parts_in(int steps, int chunk, float per) {
+  const int x = steps + chunk - 1;
+  int parts = (int)((float)x * per);
+  parts += (x >= (parts + 1) * chunk) - (x < parts * chunk);
+  return max(1, parts);
+}
+
 // Rows that belong to no sequence, the `share`-th of `shares` workgroups' part of
 // them: O 0 with p.fill, LSE -inf.
 __device__ __forceinline__ void clear_outside(const Params& p, int share, int shares) {
@@ -313,11 +322,8 @@ __device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int
     const int mine = max(p.min_chunk, (longest + parts - 1) / parts);
     const float per = 1.f / (float)mine;
     int items = 0;
-    for (int i = 0; i < count; ++i) {
-      const int len = __builtin_amdgcn_readlane(steps, i);
-      // (rounded up generously; what is taken is counted below)
-      items += max(1, (int)((float)(len + mine - 1) * per + 0.01f));
-    }
+    for (int i = 0; i < count; ++i)
+      items += parts_in(__builtin_amdgcn_readlane(steps, i), mine, per);
     float price = (float)mine + (lane > 0 ? p.part_cost + p.merge_cost * (float)(items * p.kv_heads)
                                           : 0.f);
     if (lane > 0 && (items * p.kv_heads > p.slots || items > p.max_slots)) price = INFINITY;

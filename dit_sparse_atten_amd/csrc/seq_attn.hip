@@ -221,16 +221,11 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     // Up to a round of tiles: at most `slots` <= kLdsTiles of them.
     const int which = tid & 31;
     const int chunk = max(p.min_chunk, (longest + kTryParts[which] - 1) / kTryParts[which]);
-    // (quotients of at most 512: the product is off by one at most)
     const float per_chunk = 1.f / (float)chunk;
     uint32_t items = 0;
 #pragma unroll 4
-    for (int i = tid >> 5; i < tiles; i += kThreads / 32) {
-      const int x = tile_steps[i] + chunk - 1;
-      int parts = (int)((float)x * per_chunk);
-      parts += (x >= (parts + 1) * chunk) - (x < parts * chunk);
-      items += max(1, parts);
-    }
+    for (int i = tid >> 5; i < tiles; i += kThreads / 32)
+      items += parts_in(tile_steps[i], chunk, per_chunk);
     atomicAdd(&tried[which], items);
     __syncthreads();
     if (tid < 64) {

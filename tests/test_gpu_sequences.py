@@ -131,7 +131,7 @@ def test_packed_other_key_lengths(cuda_device, q_lens, k_lens, heads):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("page", [16, 64, 256])
-@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (8, 1, 96), (40, 40, 128)], ids=str)
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (8, 1, 96), (10, 5, 40), (40, 40, 128)], ids=str)
 @pytest.mark.parametrize("q_lens,kv_lens", [
     ([1, 1, 1, 1, 1], [1, 15, 16, 17, 700]),   # a decoding step
     ([1, 0, 1], [0, 300, 5000]),               # an empty cache, no new token, a long one
@@ -663,6 +663,29 @@ def test_many_requests(cuda_device, requests):
     q, k, v = (_rows((total, h, 64), torch.bfloat16, 94 + h, cuda_device) for h in (20, 1, 1))
     out = ops.packed_attention(q, k, v, _starts(lens, cuda_device))
     _check(out, None, oracle.packed(q, k, v, lens), 64, 3, v.abs().max().item())
+
+
+@pytest.mark.parametrize("requests", [7, 70])
+@pytest.mark.parametrize("heads", [(6, 3, 80), (12, 12, 96), (5, 5, 40), (4, 2, 128)], ids=str)
+def test_steps_of_heads_in_shared_lines(cuda_device, requests, heads):
+    """Decoding steps whose key heads share memory lines, with and without the list;
+    whole and cut keys.  (128 dims share lines when the cache starts inside one.)"""
+    h, kh, dim = heads
+    g = torch.Generator().manual_seed(requests)
+    kv_lens = torch.randint(0, 400, (requests,), generator=g).tolist()
+    kv_lens[1], kv_lens[5] = 4000, 2500
+    k_cache, v_cache, table = _cache(kv_lens, 16, kh, dim, torch.bfloat16, 101, cuda_device)
+    if dim == 128:
+        store = torch.empty(k_cache.numel() + 8, dtype=k_cache.dtype, device=cuda_device)
+        k_cache = store[8:].view(k_cache.shape).copy_(k_cache)
+        assert k_cache.data_ptr() % 128 == 16
+    q_lens = [1 + (i % 5 == 2) for i in range(requests)]
+    q = _rows((sum(q_lens), h, dim), torch.bfloat16, 102, cuda_device)
+    out, lse = ops.paged_attention(q, k_cache, v_cache, _ints(table, cuda_device),
+                                   _ints(kv_lens, cuda_device), _starts(q_lens, cuda_device),
+                                   return_lse=True)
+    _check(out, lse, oracle.paged(q, k_cache, v_cache, table, kv_lens, q_lens), dim, 4000,
+           v_cache[~v_cache.isnan()].abs().max().item())
 
 
 def test_tail_and_long_tiles_are_cut(cuda_device):

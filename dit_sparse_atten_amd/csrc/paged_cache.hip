@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool lead = blockIdx.x == 0;
   if (tid == 0) lost_lds = 0;
-  int tokens = 0, pages = 0;  // before this round of requests
+  int tokens = 0, pages = 0;  // before these requests
   for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
     const int r = r0 + tid;
     Need n = {0, 0, 0, 0};

@@ -162,10 +162,18 @@ struct WriteParams {
   const int64_t* slots;
   int64_t total;                   // slots of the cache
   int32_t tokens, row, chunks;     // 16-byte chunks per token of one tensor, per head
-  uint32_t row_magic, chunk_magic; // 2^32 / row and / chunks, rounded up
+  uint32_t row_magic, chunk_magic; // of quotient() by row and by chunks
   int32_t group_tokens;            // tokens of a workgroup
   int32_t page_shift;
 };
+
+// i / d by a multiplication, exact for 1 <= d < 2^15 and i < 2^15: the magic is
+// (2^31 + e) / d with e < d, so i magic / 2^31 exceeds i / d by i e / (d 2^31) < 1 / d,
+// which reaches no further quotient.  (2^32 in its place would leave 32 bits at d = 1.)
+uint32_t quotient_magic(uint32_t d) { return (uint32_t)(((1ull << 31) + d - 1) / d); }
+__device__ __forceinline__ uint32_t quotient(uint32_t i, uint32_t magic) {
+  return __umulhi(2 * i, magic);
+}
 
 // Moves 16 bytes per thread and turn, bound by memory on long calls.  A workgroup
 // takes `group_tokens` tokens of one tensor (y), their chunks to consecutive
@@ -175,8 +183,7 @@ struct WriteParams {
 // (non-temporal) but stored through the caches, where the attention that follows
 // finds them: with non-temporal stores the write alone took 130 us, but 131,072
 // tokens x 8 heads with a decoding step behind them 327 us against 299.
-// Indexes divide by a multiplication: below 2^16 / 2 chunks of a workgroup,
-// ceil(2^32 / d) leaves the quotient exact.
+// Indexes are divided by quotient(): a workgroup has fewer than 2^15 chunks.
 constexpr int kWriteTurns = 8;
 constexpr int kWriteChunks = 256 * kWriteTurns;  // at most, of a workgroup
 __global__ void __launch_bounds__(256) paged_write_kernel(WriteParams p) {
@@ -193,8 +200,8 @@ __global__ void __launch_bounds__(256) paged_write_kernel(WriteParams p) {
       const uint32_t i = i0 + u * 256;
       slot[u] = -1;
       if (i >= count) continue;
-      const uint32_t t = __umulhi(i, p.row_magic), c = i - t * p.row;
-      head[u] = __umulhi(c, p.chunk_magic);
+      const uint32_t t = quotient(i, p.row_magic), c = i - t * p.row;
+      head[u] = quotient(c, p.chunk_magic);
       at[u] = (c - head[u] * p.chunks) * 16;
       slot[u] = p.slots[first + t];
       x[u] = __builtin_nontemporal_load(reinterpret_cast<const dsa_u32x4*>(
@@ -288,8 +295,8 @@ extern "C" int dsa_paged_write(const void* k, const void* v, void* k_cache, void
   p.slots = slots;
   p.total = (int64_t)pages * page_size;
   p.tokens = tokens; p.row = (int32_t)row; p.chunks = chunks;
-  p.row_magic = (uint32_t)(((1ull << 32) + row - 1) / row);
-  p.chunk_magic = (uint32_t)(((1ull << 32) + chunks - 1) / chunks);
+  p.row_magic = quotient_magic((uint32_t)row);
+  p.chunk_magic = quotient_magic((uint32_t)chunks);
   p.group_tokens = (int32_t)std::max<int64_t>(1, kWriteChunks / row);
   p.page_shift = __builtin_ctz(page_size);
   dsa::clear_error();

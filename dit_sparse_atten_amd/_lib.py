@@ -174,6 +174,12 @@ SIGNATURES = {
         _c_ptr, _c_int, _c_int, _c_int,            # free_pages, free_count, page_size, tokens
         _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,    # q_start, kv_lens, slots, status, stream
     )),
+    "dsa_paged_plan_from": (_c_int, (
+        _c_ptr, _c_ptr, _c_int,                    # cached, fresh, requests
+        _c_ptr, _c_i64, _c_int,                    # table, table_stride, table_width
+        _c_ptr, _c_int, _c_ptr, _c_int, _c_int,    # free_pages, free_count, free_start, page_size, tokens
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,    # q_start, kv_lens, slots, status, stream
+    )),
     "dsa_paged_write": (_c_int, (
         _c_ptr, _c_ptr, _c_ptr, _c_ptr,            # k, v, k_cache, v_cache
         ctypes.POINTER(_c_i64),                    # strides[10], bytes

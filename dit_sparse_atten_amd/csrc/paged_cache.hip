@@ -14,6 +14,7 @@ struct PlanParams {
   const int32_t* fresh;
   int32_t* table;
   const int32_t* free_pages;
+  const int32_t* free_start;  // pages of the list given out before, or null
   int32_t* q_start;
   int32_t* kv_lens;
   int64_t* slots;
@@ -54,6 +55,13 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
   __shared__ int lost_lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool lead = blockIdx.x == 0;
+  // What is left of the free list (a count that leaves it, negative ones of a sum past
+  // 2^31 among them: nothing).
+  int given = p.free_start ? p.free_start[0] : 0;
+  if (given < 0) given = p.free_count;
+  given = min(given, p.free_count);
+  const int32_t* const free_pages = p.free_pages + given;
+  const int free_count = p.free_count - given;
   if (tid == 0) lost_lds = 0;
   int tokens = 0, pages = 0;  // before these requests
   for (int r0 = 0; r0 < p.requests; r0 += kThreads) {
@@ -95,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
         p.kv_lens[r] = n.cached + n.fresh;
         // Tokens past the last page the request got.
         const int from = upto_b - (n.want - n.held);
-        const int granted = max(0, min(p.free_count - from, n.want - n.held));
+        const int granted = max(0, min(free_count - from, n.want - n.held));
         const int64_t room = (int64_t)(n.held + granted) << p.page_shift;
         const int64_t past = (int64_t)n.cached + n.fresh - max(room, (int64_t)n.cached);
         const int64_t behind = upto_a - max((int64_t)p.tokens, (int64_t)upto_a - n.fresh);
@@ -139,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
         page = p.table[r * p.table_stride + index];
       } else if (index < n.want) {
         const int64_t from = first[r] + index - n.held;
-        if (from < p.free_count) page = p.free_pages[from];
+        if (from < free_count) page = free_pages[from];
       }
       if (page >= 0) slot = ((int64_t)page << p.page_shift) + (position & mask);
     }
@@ -150,7 +158,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
     const Need n = need_of(p, r);
     const int64_t index = n.held + (i - first[r]);
     if (index < n.want)
-      p.table[r * p.table_stride + index] = i < p.free_count ? p.free_pages[i] : -1;
+      p.table[r * p.table_stride + index] = i < free_count ? free_pages[i] : -1;
   }
 }
 
@@ -227,6 +235,17 @@ extern "C" int dsa_paged_plan(const int32_t* cached, const int32_t* fresh, int32
                               const int32_t* free_pages, int32_t free_count, int32_t page_size,
                               int32_t tokens, int32_t* q_start, int32_t* kv_lens, int64_t* slots,
                               int32_t* status, hipStream_t stream) {
+  return dsa_paged_plan_from(cached, fresh, requests, table, table_stride, table_width, free_pages,
+                             free_count, nullptr, page_size, tokens, q_start, kv_lens, slots,
+                             status, stream);
+}
+
+extern "C" int dsa_paged_plan_from(const int32_t* cached, const int32_t* fresh, int32_t requests,
+                                   int32_t* table, int64_t table_stride, int32_t table_width,
+                                   const int32_t* free_pages, int32_t free_count,
+                                   const int32_t* free_start, int32_t page_size, int32_t tokens,
+                                   int32_t* q_start, int32_t* kv_lens, int64_t* slots,
+                                   int32_t* status, hipStream_t stream) {
   const char* const who = "dsa_paged_plan";
   if (requests < 0 || tokens < 0 || free_count < 0 || table_width < 0 || table_stride < table_width)
     return dsa::set_error(DSA_EINVAL, "%s: negative size or table rows that overlap", who);
@@ -242,6 +261,7 @@ extern "C" int dsa_paged_plan(const int32_t* cached, const int32_t* fresh, int32
                           page_size);
   PlanParams p;
   p.cached = cached; p.fresh = fresh; p.table = table; p.free_pages = free_pages;
+  p.free_start = free_start;
   p.q_start = q_start; p.kv_lens = kv_lens; p.slots = slots; p.status = status;
   p.table_stride = table_stride;
   p.requests = requests; p.table_width = table_width; p.free_count = free_count;

@@ -1101,7 +1101,7 @@ def _in_place(copies, *operands):
             else t for i, t in enumerate(operands)]
 
 
-def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
+def paged_plan(cached, new, block_table, free_pages, page_size, tokens, free_start=None):
     """Places for a step's new tokens in a paged key/value cache.
 
     ``cached`` and ``new`` (int32 [requests], on the device): tokens of every
@@ -1112,6 +1112,13 @@ def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
     place.  ``tokens`` is the length of the slot map: at least the sum of
     ``new``, which the host need not know exactly.  Nothing is read back; at
     most 8,192 requests.
+
+    ``free_start`` (int32 [1] on the device): pages of ``free_pages`` given out
+    before; the plan takes those behind them.  The call leaves it as it is, so
+    that a repeated call gives the same plan; ``free_start += plan.status[:1]``
+    takes the pages off the list.  A step that is captured and replayed needs it
+    (and that addition in the capture): without it every replay starts at the
+    list's first page again, and gives pages out twice.
 
     Returns a ``PagedPlan``: ``q_start``, ``kv_lens`` for ``paged_attention``,
     ``slots`` for ``paged_write`` (-1 behind the last request's tokens, and for
@@ -1128,16 +1135,18 @@ def paged_plan(cached, new, block_table, free_pages, page_size, tokens):
     new = _index_vector("new", new, device, requests)
     table, table_stride, width = _block_table(block_table, device, requests)
     free_pages = _index_vector("free_pages", free_pages, device)
+    if free_start is not None:
+        free_start = _index_vector("free_start", free_start, device, 1)
     _page_size(page_size)
     if not 0 <= tokens < 1 << 31:
         raise ValueError(f"tokens must be in [0, 2^31), got {tokens}")
     ints = torch.empty(2 * requests + 3, dtype=torch.int32, device=device)
     slots = torch.empty(tokens, dtype=torch.int64, device=device)
     base = ints.data_ptr()
-    _call(lib.dsa_paged_plan, "dsa_paged_plan", device, cached.data_ptr(), new.data_ptr(),
+    _call(lib.dsa_paged_plan_from, "dsa_paged_plan", device, cached.data_ptr(), new.data_ptr(),
           requests, table, table_stride, width, free_pages.data_ptr(), free_pages.shape[0],
-          page_size, tokens, base, base + 4 * (requests + 1), slots.data_ptr(),
-          base + 4 * (2 * requests + 1))
+          None if free_start is None else free_start.data_ptr(), page_size, tokens, base,
+          base + 4 * (requests + 1), slots.data_ptr(), base + 4 * (2 * requests + 1))
     q_start, kv_lens, status = torch.split_with_sizes(ints, (requests + 1, requests, 2))
     return PagedPlan(q_start, kv_lens, slots, status)
 

@@ -506,6 +506,12 @@ int dsa_gated_residual(const void* x, int64_t x_stride, const void* y, int64_t y
  *   lengths count as 0.  Up to 8,192 requests.  Nothing but the new table entries
  *   changes, so a repeated call gives the same plan.
  *
+ * dsa_paged_plan_from: the same, with the pages from free_pages[*free_start] on
+ *   (a device int32, only read; NULL: 0).  Adding status[0] to it behind the call, on
+ *   the device, makes the next call go on where this one stopped, without the host:
+ *   a captured step that is replayed needs that.  A count outside [0, free_count]
+ *   leaves no page.
+ *
  * dsa_paged_write: row t of k and v [tokens, heads, row_bytes] into slot
  * slots[t] of the caches; a slot outside them is skipped.  strides[10] in BYTES,
  * multiples of 16: k (token, head), v (token, head), k_cache (page, token,
@@ -516,6 +522,11 @@ int dsa_paged_plan(const int32_t* cached, const int32_t* fresh, int32_t requests
                    int64_t table_stride, int32_t table_width, const int32_t* free_pages,
                    int32_t free_count, int32_t page_size, int32_t tokens, int32_t* q_start,
                    int32_t* kv_lens, int64_t* slots, int32_t* status, hipStream_t stream);
+int dsa_paged_plan_from(const int32_t* cached, const int32_t* fresh, int32_t requests,
+                        int32_t* table, int64_t table_stride, int32_t table_width,
+                        const int32_t* free_pages, int32_t free_count, const int32_t* free_start,
+                        int32_t page_size, int32_t tokens, int32_t* q_start, int32_t* kv_lens,
+                        int64_t* slots, int32_t* status, hipStream_t stream);
 int dsa_paged_write(const void* k, const void* v, void* k_cache, void* v_cache,
                     const int64_t* strides, int32_t tokens, int32_t heads, int32_t row_bytes,
                     int32_t pages, int32_t page_size, const int64_t* slots, hipStream_t stream);

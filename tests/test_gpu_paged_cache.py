@@ -1,10 +1,13 @@
 """The paged key/value cache on the GPU where it can go wrong: rows of one 16-byte
-chunk."""
+chunk, a free list that a captured step goes through."""
+
+import math
 
 import pytest
 import torch
 
 from dit_sparse_atten_amd import ops
+from oracle import sequences as oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +60,119 @@ def test_write_rows_of_one_chunk(cuda_device, dtype, dim, heads, head_major, fir
     ops.paged_write(-k.contiguous(), -v.contiguous(), *caches, slots.to(cuda_device))
     for got, expected in zip(stores, want):
         assert torch.equal(got, expected)
+
+
+def _ints(values, device):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("start", [0, 3, 11, 12, 13, 5000, -1, -2 ** 31])
+def test_plan_from_the_middle_of_the_free_list(cuda_device, start):
+    """The pages behind the first `start`; none where the count leaves the list."""
+    cached, new = [16, 20, 0, 5], [1, 4, 40, 100]
+    table = [[7] + [-1] * 9, [3, 4] + [-1] * 8, [-1] * 10, [9] + [-1] * 9]
+    free = list(range(50, 62))
+    expected = oracle.plan(cached, new, table, free[start:] if 0 <= start < 12 else [], 16, 150)
+    held, at = _ints(table, cuda_device), _ints([start], cuda_device)
+    args = (_ints(cached, cuda_device), _ints(new, cuda_device), held, _ints(free, cuda_device),
+            16, 150)
+    for _ in range(2):
+        got = ops.paged_plan(*args, free_start=at)
+        assert [x.tolist() for x in got] == [list(x) for x in expected[:4]]
+        assert held.tolist() == expected[4] and at.tolist() == [start]
+
+
+def test_plan_from_refusals(cuda_device):
+    def ints(*values):
+        return _ints(values, cuda_device)
+
+    table = torch.zeros((1, 2), dtype=torch.int32, device=cuda_device)
+    for bad in (ints(0).long(), ints(0, 1), ints(0)[0], ints()):
+        with pytest.raises(ValueError, match="free_start"):
+            ops.paged_plan(ints(0), ints(1), table, ints(1, 2), 16, 1, free_start=bad)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_plan(ints(0), ints(1), table, ints(1, 2), 16, 1, free_start=ints(0).cpu())
+
+
+def test_captured_step_takes_new_pages_on_every_replay(cuda_device):
+    """A decoding step captured once (plan, write, attention, the free list moved on)
+    and replayed 40 times: no page is held by two requests, and every output is
+    attention over the whole sequence.  (Tolerance: the probabilities' rounding and
+    the result's, half a step of bf16 each, of sums of at most max |v|, and half as
+    much again for everything in fp32.)"""
+    kh, h, dim, page, pages = 2, 8, 64, 16, 64
+    lens = [15, 0, 31, 47, 30]
+    requests = len(lens)
+    g = torch.Generator().manual_seed(5)
+
+    def rows(n, heads):
+        return torch.randn((n, heads, dim), generator=g).to(torch.bfloat16)
+
+    order = torch.randperm(pages, generator=g).tolist()
+    k_cache = torch.full((pages, page, kh, dim), math.nan, dtype=torch.bfloat16)
+    v_cache = k_cache.clone()
+    keys = [rows(n, kh) for n in lens]
+    values = [rows(n, kh) for n in lens]
+    table = [[-1] * 8 for _ in range(requests)]
+    for r, n in enumerate(lens):
+        for i in range(n):
+            if i % page == 0:
+                table[r][i // page] = order.pop()
+            k_cache[table[r][i // page], i % page] = keys[r][i]
+            v_cache[table[r][i // page], i % page] = values[r][i]
+    held = {"k": k_cache.to(cuda_device), "v": v_cache.to(cuda_device),
+            "table": _ints(table, cuda_device), "cached": _ints(lens, cuda_device),
+            "given": _ints([0], cuda_device)}
+    first = {name: t.clone() for name, t in held.items()}
+    free = _ints(order, cuda_device)
+    new = _ints([1] * requests, cuda_device)
+    q, k, v = (torch.zeros((requests, n, dim), dtype=torch.bfloat16, device=cuda_device)
+               for n in (h, kh, kh))
+
+    def step(s):
+        plan = ops.paged_plan(s["cached"], new, s["table"], free, page, requests, s["given"])
+        ops.paged_write(k, v, s["k"], s["v"], plan.slots)
+        out, lse = ops.paged_attention(q, s["k"], s["v"], s["table"], plan.kv_lens, plan.q_start,
+                                       return_lse=True)
+        s["given"] += plan.status[:1]
+        s["cached"].copy_(plan.kv_lens)
+        return out, lse, plan.status
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step({name: t.clone() for name, t in first.items()})
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        result = step(held)
+    for name, t in first.items():
+        held[name].copy_(t)
+    other = {name: t.clone() for name, t in first.items()}
+    crossed = set()
+    for i in range(40):
+        now = [rows(requests, n) for n in (h, kh, kh)]
+        for t, x in zip((q, k, v), now):
+            t.copy_(x)
+        graph.replay()
+        out, lse, status = (t.cpu() for t in result)
+        if i % 3 == 0:
+            step(other)  # eager work of another cache between the replays
+            torch.cuda.synchronize()
+        crossed |= {r for r in range(requests) if keys[r].shape[0] % page == 0}
+        assert status[1] == 0
+        for r in range(requests):
+            keys[r] = torch.cat((keys[r], now[1][r:r + 1]))
+            values[r] = torch.cat((values[r], now[2][r:r + 1]))
+        lengths = held["cached"].tolist()
+        assert lengths == [x.shape[0] for x in keys]
+        used = [p for row, n in zip(held["table"].tolist(), lengths)
+                for p in row[:-(-n // page)]]
+        assert len(set(used)) == len(used) and min(used) >= 0 and max(used) < pages, i
+        expected, stat, _, _ = oracle.packed(now[0], torch.cat(keys), torch.cat(values),
+                                             [1] * requests, lengths)
+        v_max = max(x.abs().max().item() for x in values)
+        assert (out.double() - expected).abs().max().item() <= 3 * 2 ** -8 * v_max, i
+        assert (lse.double() - stat).abs().max().item() <= 2 ** -12, i
+    assert crossed == set(range(requests))
+    assert held["given"].item() == sum(-(-(n + 40) // page) - -(-n // page) for n in lens)

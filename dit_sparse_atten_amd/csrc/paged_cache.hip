@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
   __shared__ int start[kMaxRequests + 1];  // tokens before each request
   __shared__ int first[kMaxRequests + 1];  // new pages before each request
   __shared__ int wave_sum[2][kThreads / 64];
-  __shared__ int lost_lds;
+  __shared__ unsigned long long lost_lds;  // tokens without a slot
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool lead = blockIdx.x == 0;
   // What is left of the free list (a count that leaves it, negative ones of a sum past
@@ -68,6 +68,13 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
     const int r = r0 + tid;
     Need n = {0, 0, 0, 0};
     if (r < p.requests) n = need_of(p, r);
+    // The page that the first new tokens share with cached ones, as the table has it
+    // (no page: a step that ran out of pages left it so).
+    const int partial = n.cached & ((1 << p.page_shift) - 1);
+    const bool shares = lead && n.fresh > 0 && partial != 0 &&
+                        (n.cached >> p.page_shift) < n.held;
+    const int shared =
+        shares ? p.table[r * p.table_stride + (n.cached >> p.page_shift)] : 0;
     int a = n.fresh, b = n.want - n.held;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -95,20 +102,25 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
     }
     const int64_t top = 0x7fffffff;
     const int upto_a = (int)min(before_a + a, top), upto_b = (int)min(before_b + b, top);
+    const int ahead = __shfl_up(a, 1);
+    const int64_t from_a = min(before_a + (lane > 0 ? ahead : 0), top);
     if (r < p.requests) {
       start[r + 1] = upto_a;
       first[r + 1] = upto_b;
       if (lead) {
         p.q_start[r + 1] = upto_a;
         p.kv_lens[r] = n.cached + n.fresh;
-        // Tokens past the last page the request got.
+        // Lost at the end: tokens past the last page the request got, or behind the
+        // slot map; at the start: those in a shared page that is none.
         const int from = upto_b - (n.want - n.held);
         const int granted = max(0, min(free_count - from, n.want - n.held));
+        const int64_t fresh = n.fresh, cached = n.cached;
         const int64_t room = (int64_t)(n.held + granted) << p.page_shift;
-        const int64_t past = (int64_t)n.cached + n.fresh - max(room, (int64_t)n.cached);
-        const int64_t behind = upto_a - max((int64_t)p.tokens, (int64_t)upto_a - n.fresh);
-        const int64_t lost = max(min(past, (int64_t)n.fresh), max(behind, (int64_t)0));
-        if (lost > 0) atomicAdd(&lost_lds, (int)lost);
+        const int64_t past = cached + fresh - max(room, cached);
+        const int64_t behind = fresh - min(max(p.tokens - from_a, (int64_t)0), fresh);
+        const int64_t head = shared < 0 ? (1 << p.page_shift) - partial : 0;
+        const int64_t lost = min(max(past, behind) + head, fresh);
+        if (lost > 0) atomicAdd(&lost_lds, (unsigned long long)lost);
       }
     }
     tokens = (int)min(all_a, top);
@@ -119,11 +131,6 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
     first[0] = 0;
   }
   dsa::lds_barrier();
-  if (lead && tid == 0) {
-    p.q_start[0] = 0;
-    p.status[0] = pages;
-    p.status[1] = lost_lds;
-  }
   auto find = [&](const int* before, int i) -> int {  // the last request with before <= i
     int lo = 0, hi = p.requests;
     while (hi - lo > 1) {
@@ -133,6 +140,26 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(PlanParams p) {
     }
     return lo;
   };
+  if (lead) {
+    // Tokens whose page would be an entry of the free list that is none.
+    const int granted = min(pages, free_count);
+    for (int i = tid; i < granted; i += kThreads) {
+      if (free_pages[i] >= 0) continue;
+      const int r = find(first, i);
+      const Need n = need_of(p, r);
+      const int64_t begin = (int64_t)(n.held + (i - first[r])) << p.page_shift;
+      const int64_t upto = n.cached + min((int64_t)n.fresh, max(p.tokens - (int64_t)start[r],
+                                                                (int64_t)0));
+      const int64_t lost = min(begin + (1 << p.page_shift), upto) - max(begin, (int64_t)n.cached);
+      if (lost > 0) atomicAdd(&lost_lds, (unsigned long long)lost);
+    }
+    dsa::lds_barrier();
+    if (tid == 0) {
+      p.q_start[0] = 0;
+      p.status[0] = pages;
+      p.status[1] = (int)min(lost_lds, 0x7fffffffull);
+    }
+  }
   const int at = blockIdx.x * kThreads + tid, all = gridDim.x * kThreads;
   const int mask = (1 << p.page_shift) - 1;
   for (int64_t t = at; t < p.tokens; t += all) {

@@ -983,7 +983,7 @@ class PagedPlan(typing.NamedTuple):
     q_start: torch.Tensor  # int32 [requests + 1]: new tokens before each request
     kv_lens: torch.Tensor  # int32 [requests]: cached and new tokens
     slots: torch.Tensor    # int64 [tokens]: page * page_size + row, -1: no place
-    status: torch.Tensor   # int32 [2]: pages needed, new tokens past their last page
+    status: torch.Tensor   # int32 [2]: pages needed, new tokens without a slot
 
 
 # Short calls (a plan, a step's write, a decoding step of a few requests) are bound
@@ -1122,10 +1122,13 @@ def paged_plan(cached, new, block_table, free_pages, page_size, tokens, free_sta
 
     Returns a ``PagedPlan``: ``q_start``, ``kv_lens`` for ``paged_attention``,
     ``slots`` for ``paged_write`` (-1 behind the last request's tokens, and for
-    tokens without a page because ``free_pages`` or the table's row is too
-    short), and ``status`` = (pages needed, new tokens past their request's last
-    page or behind ``tokens``): the caller's free list starts behind the first
-    ``status[0]`` pages next time.
+    tokens without a page: ``free_pages`` or the table's row is too short, or the
+    page's entry in either is negative), and ``status`` = (pages needed, new tokens
+    without a slot, those behind ``tokens`` among them): the caller's free list
+    starts behind the first ``status[0]`` pages next time.  A step that lost tokens
+    (``status[1]``) is not continued, for ``kv_lens`` counts tokens that are
+    nowhere: the same call, from the same ``cached`` and ``free_start``, is made
+    again once there are pages, and the step's keys are written again.
     """
     lib = _lib.load()
     _require_cuda("cached", cached)

@@ -500,11 +500,14 @@ int dsa_gated_residual(const void* x, int64_t x_stride, const void* y, int64_t y
  *   q_start[requests + 1]: new tokens before each request; kv_lens[r] = cached
  *   + fresh; slots[tokens]: the slot of every new token in request order, -1
  *   for a token without a page (the free list or the row is too short; its
- *   table entry becomes -1) and behind the last request's; status[2]: pages the
- *   step needs (more than free_count: the first free_count were given out), and
- *   new tokens past their request's last page or behind `tokens`.  Negative
- *   lengths count as 0.  Up to 8,192 requests.  Nothing but the new table entries
- *   changes, so a repeated call gives the same plan.
+ *   table entry becomes -1; or its page's entry, of the list or of a page held
+ *   before, is negative) and behind the last request's; status[2]: pages the step
+ *   needs (more than are left: those left were given out), and new tokens without
+ *   a slot, those behind `tokens` among them (at most 2^31 - 1).  Negative lengths
+ *   count as 0.  Up to 8,192 requests.  Nothing but the new table entries changes,
+ *   so a repeated call gives the same plan.  Where status[1] is not 0, kv_lens
+ *   counts tokens that are nowhere: the step is repeated from the same cached
+ *   (and free_start) once there are pages, not continued.
  *
  * dsa_paged_plan_from: the same, with the pages from free_pages[*free_start] on
  *   (a device int32, only read; NULL: 0).  Adding status[0] to it behind the call, on

@@ -1,5 +1,5 @@
 """The paged key/value cache on the GPU where it can go wrong: rows of one 16-byte
-chunk, a free list that a captured step goes through."""
+chunk, a free list that a captured step goes through, tokens that find no page."""
 
 import math
 
@@ -176,3 +176,62 @@ def test_captured_step_takes_new_pages_on_every_replay(cuda_device):
         assert (lse.double() - stat).abs().max().item() <= 2 ** -12, i
     assert crossed == set(range(requests))
     assert held["given"].item() == sum(-(-(n + 40) // page) - -(-n // page) for n in lens)
+
+
+def _plan(cached, new, table, free, page, tokens, device):
+    held = _ints(table, device)
+    got = ops.paged_plan(_ints(cached, device), _ints(new, device), held, _ints(free, device),
+                         page, tokens)
+    return [x.tolist() for x in got] + [held.tolist()]
+
+
+def test_plan_counts_tokens_of_a_held_page_that_is_none(cuda_device):
+    """A step finds no page for its tokens; the next one has no place in that page
+    either, and says so."""
+    table, page = [[7, -1, -1]], 16
+    *first, table = _plan([16], [4], table, [], page, 4, cuda_device)
+    assert first == [[0, 4], [20], [-1] * 4, [1, 4]] and table == [[7, -1, -1]]
+    # Continued all the same, with pages free again: the shared page is none.
+    got = _plan([20], [1], table, [3, 5], page, 1, cuda_device)
+    assert got == [[0, 1], [21], [-1], [0, 1], [[7, -1, -1]]]
+    got = _plan([20], [14], table, [3, 5], page, 14, cuda_device)
+    assert got == [[0, 14], [34], [-1] * 12 + [48, 49], [1, 12], [[7, -1, 3]]]
+    # Made again from the same lengths, the step has its page.
+    got = _plan([16], [4], table, [3, 5], page, 4, cuda_device)
+    assert got == [[0, 4], [20], [48, 49, 50, 51], [1, 0], [[7, 3, -1]]]
+
+
+@pytest.mark.parametrize("case", range(48))
+def test_plan_with_entries_that_are_no_page(cuda_device, case):
+    """Negative entries in held pages and in the free list, short lists, short rows and
+    short slot maps: the plan and its counts as the oracle has them."""
+    g = torch.Generator().manual_seed(1000 + case)
+
+    def rand(lo, hi):
+        return int(torch.randint(lo, hi + 1, (), generator=g))
+
+    page = (16, 32, 128)[case % 3]
+    requests = (1, 5, 64, 700)[case % 4]
+    cached = [rand(0, 6 * page) for _ in range(requests)]
+    new = [rand(0, (1, 3 * page)[case % 2]) for _ in range(requests)]
+    need = [-(-(c + n) // page) for c, n in zip(cached, new)]
+    width = max(1, max(need) - (0, 0, 2)[case % 3])
+    free = [rand(0, 999) if rand(0, 3) else -rand(1, 2 ** 31 - 1) for _ in range(sum(need) + 3)]
+    if case % 5 == 4:
+        free = free[:len(free) // 4]
+    table = [[rand(0, 10 ** 6) if rand(0, 2) else -1 for _ in range(width)]
+             for _ in range(requests)]
+    total = sum(new)
+    tokens = (total, total + 9, total * 2 // 3)[case % 7 % 3]
+    got = _plan(cached, new, table, free, page, tokens, cuda_device)
+    expected = oracle.plan(cached, new, table, free, page, tokens)
+    for name, a, b in zip(("q_start", "kv_lens", "slots", "status", "table"), got, expected):
+        assert a == b, name
+
+
+def test_plan_counts_past_31_bits(cuda_device):
+    """Sums of new tokens past 2^31 are cut there, the lost ones among them."""
+    most = 2 ** 31 - 1
+    got = _plan([0, 0, 0], [most, most, 5], [[-1], [-1], [-1]], [5], 16, 10, cuda_device)
+    assert got == [[0, most, most, most], [most, most, 5], list(range(80, 90)), [3, most],
+                   [[5], [-1], [-1]]]

@@ -406,49 +406,172 @@ __device__ __forceinline__ bool take_item(const Params& p, Item* it, int* h) {
   return true;
 }
 
-// One row's sum of p_j V_j over the keys it sees of `blocks` key blocks (`width`
-// <= 64 keys from key_lo, key_lo + stride, ..; below key_hi), element by element:
-// lane l ends with the dims l kD / 64 ...  In the matrix products a hidden key's
-// p is 0, and 0 times a value that is not finite is NaN, so a wave whose O is not
-// finite, and whose rows see different keys, takes this way instead.
-template <typename T, int kD, bool kPaged>
-__device__ __forceinline__ void exact_row(LateParams p, const Item& it, int h, int64_t q_at,
-                                          int key_lo, int blocks, int stride, int width,
-                                          int key_hi, float m_use, float acc[kD / 64]) {
+// 1 where a value is infinity times `sign`, or NaN, else 0.
+template <typename T>
+__device__ __forceinline__ T infinite_as(T v, float sign) {
+  const float x = sign * (float)v;
+  return x < INFINITY ? (T)0.0f : (T)1.0f;  // (NaN compares false)
+}
+
+// In the matrix products a hidden key's p is 0, and 0 times a value that is not finite
+// is NaN.  True where that may have reached a wave's O: a value of the keys [lo, hi),
+// which some of its rows see and others do not, or none, is not finite.
+template <typename T, bool kPaged>
+__device__ __forceinline__ bool hides_infinity(LateParams p, const Item& it, int h, int lo,
+                                               int hi) {
+  typedef typename dsa::Elem<T>::x8 x8;
+  const int chunks = p->head_dim / 8;
+  float sum = 0.f;  // NaN once an element is not finite
+  for (int i = threadIdx.x & 63; i < (hi - lo) * chunks; i += 64) {
+    const int key = lo + i / chunks, chunk = i % chunks;
+    int64_t at = (int64_t)(it.k0 + key) * p->v_st;
+    if (kPaged) {
+      const int page =
+          p->table[(int64_t)it.request * p->table_stride + (key >> p->page_shift)];
+      if ((unsigned)page >= (unsigned)p->pages) continue;
+      at = page * p->v_sp + (int64_t)(key & ((1 << p->page_shift) - 1)) * p->v_st;
+    }
+    const x8 v = *reinterpret_cast<const x8*>(static_cast<const T*>(p->v) + at + h * p->v_sh +
+                                              chunk * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf((float)v[e], 0.f, sum);
+  }
+  return __any(sum != 0.f);
+}
+
+// A wave's O over again, for a wave that hides_infinity: the same products (kRows = 32:
+// 32x32x16, 16: 16x16x32), 32 keys at a time from key0, key0 + stride, .. below `hi`,
+// with the final reference `m_use`, operands straight from memory.  Where keys from
+// lim_first on (hidden from some row) have values that are not finite, these count as
+// 0 in the product, and two products of "visible" with "+inf or NaN" and "-inf or NaN"
+// tell which elements they reach.  (4,096 causal tokens x 4 heads: 50 us, with such
+// values all over 150; element by element, a key to a lane, 14,000.  One infinity that
+// nearly every row sees is hidden from rows of its own wave alone: 55 us.)
+template <typename T, int kD, int kUse, bool kPaged, int kRows, typename Acc>
+__device__ __forceinline__ void walk_again(LateParams p, const Item& it, int h, int64_t q_at,
+                                           int lim, int lim_first, int key0, int stride, int hi,
+                                           float m_use, Acc* oacc) {
+  typedef dsa::Elem<T> E;
+  typedef typename E::x8 x8;
+  constexpr int kDims = 512 / kRows;          // of one product of scores
+  constexpr int kElems = kRows * kRows / 64;  // of one accumulator, per lane
+  constexpr int kSteps = kRows / 16;          // products of 32 keys with one tile of dims
   const int lane = threadIdx.x & 63;
-  const int d0 = lane * (kD / 64);
-  const T* const q = static_cast<const T*>(p->q) + q_at;
+  const int grp = lane / kRows, col = lane % kRows;
+  auto mfma = [](x8 a, x8 b, Acc c) -> Acc {
+    if constexpr (kRows == 32) return E::mfma32(a, b, c);
+    else return E::mfma16(a, b, c);
+  };
+  const Source ks = source_of<kPaged>(p->k, p->k_sp, p->k_st, p->k_sh, h, it.k0);
+  const Source vs = source_of<kPaged>(p->v, p->v_sp, p->v_st, p->v_sh, h, it.k0);
+  const T* q = static_cast<const T*>(p->q) + q_at;
 #pragma unroll
-  for (int e = 0; e < kD / 64; ++e) acc[e] = 0.f;
-#pragma unroll 1
-  for (int b = 0; b < blocks; ++b) {
-    const int key0 = key_lo + b * stride;
-    if (key0 >= key_hi) break;
-    const int key = key0 + lane;
-    int page = -1;
-    if (lane < width && key < key_hi) {
-      page = kPaged ? p->table[(int64_t)it.request * p->table_stride + (key >> p->page_shift)] : 0;
-      if (kPaged && (unsigned)page >= (unsigned)p->pages) page = -1;
-    }
-    const int in_page = kPaged ? key & ((1 << p->page_shift) - 1) : it.k0 + key;
-    float prob = 0.f;
-    if (page >= 0) {
-      const T* k = static_cast<const T*>(p->k) + page * p->k_sp + in_page * p->k_st + h * p->k_sh;
-      float s = 0.f;
-#pragma unroll 1
-      for (int d = 0; d < p->head_dim; ++d) s = fmaf((float)q[d], (float)k[d], s);
-      prob = __builtin_amdgcn_exp2f(fmaf(s, p->scale_log2, -m_use));
-    }
-#pragma unroll 1
-    for (int j = 0; j < width; ++j) {
-      const int page_j = __shfl(page, j);
-      if (page_j < 0) continue;
-      const float prob_j = __shfl(prob, j);
-      const T* v = static_cast<const T*>(p->v) + page_j * p->v_sp +
-                   (int64_t)__shfl(in_page, j) * p->v_st + h * p->v_sh;
+  for (int dt = 0; dt < kUse / kRows; ++dt)
 #pragma unroll
-      for (int e = 0; e < kD / 64; ++e)
-        if (d0 + e < p->head_dim) acc[e] = fmaf(prob_j, (float)v[d0 + e], acc[e]);
+    for (int r = 0; r < kElems; ++r) oacc[dt][r] = 0.f;
+#pragma unroll 1
+  for (; key0 < hi; key0 += stride) {
+    // The block's two 16-key granules; a row sees their keys below `bound`.
+    __amdgpu_buffer_rsrc_t kr[2], vr[2];
+    int bound[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int key = key0 + 16 * i;
+      int left = min(16, hi - key), row = key, page = 0;
+      if (kPaged) {
+        if (left > 0)
+          page = __builtin_amdgcn_readfirstlane(
+              p->table[(int64_t)it.request * p->table_stride + (key >> p->page_shift)]);
+        if ((unsigned)page >= (unsigned)p->pages) left = 0;
+        row &= (1 << p->page_shift) - 1;
+      }
+      kr[i] = rows_rsrc<kPaged>(ks, (uint32_t)page, row, left, p->head_dim);
+      vr[i] = rows_rsrc<kPaged>(vs, (uint32_t)page, row, left, p->head_dim);
+      bound[i] = left > 0 ? min(lim, hi) - key0 : 0;
+    }
+    // The block's key of slot t of product j, the same for scores and values, and
+    // whether the lane's row sees it.
+    auto granule_of = [&](int j, int t) { return kRows == 32 ? j : t >> 2; };
+    auto row_of = [&](int t) { return (kRows == 32 ? 8 * (t >> 2) : 0) + 4 * grp + (t & 3); };
+    auto visible = [&](int j, int t) {
+      const int i = granule_of(j, t);
+      return 16 * i + row_of(t) < bound[i];
+    };
+    x8 prob[kSteps];
+    {
+      asm volatile("" : "+v"(q));  // (Q is not held through the walk)
+      const uint32_t at = (uint32_t)((col & 15) * (int)p->k_st + grp * 8) * 2;
+      Acc s[32 / kRows];
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i)
+#pragma unroll
+        for (int r = 0; r < kElems; ++r) s[i][r] = 0.f;
+#pragma unroll
+      for (int dc = 0; dc < kUse / kDims; ++dc) {
+        const int d = dc * kDims + grp * 8;
+        x8 b;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = (T)0.0f;
+        if (d < p->head_dim) b = *reinterpret_cast<const x8*>(q + d);
+#pragma unroll
+        for (int i = 0; i < 32 / kRows; ++i) {
+          // (of 32 rows the upper 16 are the second granule's)
+          dsa_u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(kr[i], at + dc * kDims * 2, 0, 0);
+          if (kRows == 32) {
+            const dsa_u32x4 upper =
+                __builtin_amdgcn_raw_buffer_load_b128(kr[1], at + dc * kDims * 2, 0, 0);
+            if (col >= 16) a = upper;
+          }
+          if (d >= p->head_dim) a = dsa_u32x4{0u, 0u, 0u, 0u};
+          s[i] = mfma(__builtin_bit_cast(x8, a), b, s[i]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          const int f = j * 8 + t;
+          const float score = fmaf(s[f / kElems][f % kElems], p->scale_log2, -m_use);
+          prob[j][t] = (T)(visible(j, t) ? __builtin_amdgcn_exp2f(score) : 0.f);
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < kUse / kRows; ++dt) {
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        x8 a;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          // (dims past head_dim are between the rows' ends or 0, and go nowhere)
+          a[t] = __builtin_bit_cast(
+              T, __builtin_amdgcn_raw_buffer_load_b16(
+                     vr[granule_of(j, t)],
+                     (uint32_t)(row_of(t) * (int)p->v_st + col) * 2 + dt * kRows * 2, 0, 0));
+          sum = fmaf((float)a[t], 0.f, sum);
+        }
+        if (key0 + 32 > lim_first && __any(sum != 0.f)) {
+          x8 up, down, seen;
+          Acc ups, downs;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            up[t] = infinite_as(a[t], 1.f);
+            down[t] = infinite_as(a[t], -1.f);
+            seen[t] = (T)(visible(j, t) ? 1.f : 0.f);
+            if ((float)a[t] * 0.f != 0.f) a[t] = (T)0.0f;
+          }
+#pragma unroll
+          for (int r = 0; r < kElems; ++r) ups[r] = downs[r] = 0.f;
+          ups = mfma(up, seen, ups);
+          downs = mfma(down, seen, downs);
+#pragma unroll
+          for (int r = 0; r < kElems; ++r) {
+            if (ups[r] > 0.f) oacc[dt][r] += INFINITY;
+            if (downs[r] > 0.f) oacc[dt][r] -= INFINITY;
+          }
+        }
+        oacc[dt] = mfma(a, prob[j], oacc[dt]);
+      }
     }
   }
 }
@@ -463,7 +586,7 @@ __device__ __forceinline__ void exact_row(LateParams p, const Item& it, int h, i
 // 72 to 96 leave the last quarter of a 128-dim row out (8,192 x 8,192 x 32 heads: 96
 // dims 897 -> 804 us, 80 dims 985 -> 896).
 template <typename T, int kD, int kUse, bool kPaged>
-__global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
+__global__ void __launch_bounds__(256, kD == 64 ? 4 : 2) seq_wide_kernel(Params p) {
   typedef dsa::Elem<T> E;
   typedef typename E::x8 x8;
   constexpr int kRow = kD * 2;               // bytes of a staged row
@@ -732,49 +855,29 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) unfinite = fmaf(oacc[dt][r], 0.f, unfinite);
   // (a row whose scores are not finite stays as it is)
-  const bool redo = lim_first < kend && __any(unfinite != 0.f && l_tot * 0.f == 0.f);
-  if (redo) {
-#pragma unroll 1
-    for (int r = 0; r < 32; ++r) {
-      const int row_r = it.tile * kWideRows + wave * 32 + r;
-      if (row_r >= rows) break;
-      const int token_r = __builtin_amdgcn_readlane(token, r);
-      const int head_r = __builtin_amdgcn_readlane(head, r);
-      const float m_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), r));
-      const float l_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_tot), r));
-      const int lim_r = __builtin_amdgcn_readlane(lim, r);
-      float acc[kD / 64];
-      exact_row<T, kD, kPaged>(late, it, h, (it.q0 + token_r) * late->q_st + head_r * late->q_sh,
-                               it.s0 * kWideKeys, it.s1 - it.s0, kWideKeys, kWideKeys,
-                               min(lim_r, it.s1 * kWideKeys), m_r == -INFINITY ? 0.f : m_r, acc);
-      const float inv = l_r > 0.f ? 1.f / l_r : (l_r == 0.f ? 0.f : l_r);
-#pragma unroll
-      for (int e = 0; e < kD / 64; ++e) {
-        const int d = lane * (kD / 64) + e;
-        if (it.slot >= 0)
-          late->part[((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD) +
-                     part_at<kD, kWideRows>(wave * 32 + r, d)] = acc[e];
-        else if (d < late->head_dim)
-          static_cast<T*>(late->o)[(it.q0 + token_r) * late->o_st + head_r * late->o_sh + d] =
-              (T)(acc[e] * inv);
-      }
-    }
+  if (__builtin_expect(lim_first < kend && __any(unfinite != 0.f && l_tot * 0.f == 0.f), 0)) {
+    // Staged with the wave's last steps, but not seen by all of its rows.
+    const int last = min((lim_last + kWideKeys - 1) & -kWideKeys, it.s1 * kWideKeys);
+    if (hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kWideKeys),
+                                  min(last, kend)))
+      walk_again<T, kD, kUse, kPaged, 32>(
+          late, it, h, (int64_t)(it.q0 + token) * late->q_st + head * late->q_sh, lim, lim_first,
+          it.s0 * kWideKeys, 32, min(lim_last, it.s1 * kWideKeys),
+          m_run == -INFINITY ? 0.f : m_run, oacc);
   }
   if (it.slot >= 0) {
     // A partial keeps the accumulators' own order (part_at): whole lines per store.
     float* const po =
         late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD);
-    if (!redo) {
 #pragma unroll
-      for (int dt = 0; dt < kDt; ++dt)
+    for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-          const dsa_f32x4 v4 = {oacc[dt][rr * 4 + 0], oacc[dt][rr * 4 + 1],
-                                oacc[dt][rr * 4 + 2], oacc[dt][rr * 4 + 3]};
-          *reinterpret_cast<dsa_f32x4*>(po +
-                                        part_at<kD, kWideRows>(local, dt * 32 + rr * 8 + g * 4)) = v4;
-        }
-    }
+      for (int rr = 0; rr < 4; ++rr) {
+        const dsa_f32x4 v4 = {oacc[dt][rr * 4 + 0], oacc[dt][rr * 4 + 1],
+                              oacc[dt][rr * 4 + 2], oacc[dt][rr * 4 + 3]};
+        *reinterpret_cast<dsa_f32x4*>(po +
+                                      part_at<kD, kWideRows>(local, dt * 32 + rr * 8 + g * 4)) = v4;
+      }
     if (g == 0) {
       po[kWideRows * kD + local] = m_run;
       po[kWideRows * (kD + 1) + local] = l_tot;
@@ -784,7 +887,6 @@ __global__ void __launch_bounds__(256, 2) seq_wide_kernel(Params p) {
   if (late->lse && g == 0 && row_ok)
     late->lse[(int64_t)head * late->q_rows + it.q0 + token] =
         l_tot == 0.f ? -INFINITY : m_run * kLn2 + logf(l_tot);
-  if (redo) return;
   // O goes out through the wave's quarter of the stages that the last step left
   // alone (every wave is past its reads of them, and no load is on its way there):
   // written row by row as 16-byte chunks, whole rows to a store.
@@ -1043,29 +1145,19 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
   for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) unfinite = fmaf(oacc[dt][r], 0.f, unfinite);
+  // (a row whose scores are not finite stays as it is)
+  if (__builtin_expect(lim_first < kend && __any(unfinite != 0.f && l_wave * 0.f == 0.f), 0) &&
+      hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kNarrowKeys),
+                                min(kend, it.s1 * kNarrowKeys)))
+    walk_again<T, kD, kD, kPaged, 16>(
+        late, it, h, (int64_t)(it.q0 + token) * late->q_st + head * late->q_sh, lim, lim_first,
+        it.s0 * kNarrowKeys + wave * 32, kNarrowKeys, min(kend, it.s1 * kNarrowKeys),
+        m_run == -INFINITY ? 0.f : m_run, oacc);
   dsa::lds_barrier<true>();
   float* const mine = reinterpret_cast<float*>(lds_k0) + wave * kNarrowRows * kD;
-  // (a row whose scores are not finite stays as it is)
-  if (lim_first < kend && __any(unfinite != 0.f && l_wave * 0.f == 0.f)) {
-#pragma unroll 1
-    for (int r = 0; r < kNarrowRows; ++r) {
-      if (it.tile * kNarrowRows + r >= rows) break;
-      const int token_r = __builtin_amdgcn_readlane(token, r);
-      const int head_r = __builtin_amdgcn_readlane(head, r);
-      const float m_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), r));
-      float acc[kD / 64];
-      exact_row<T, kD, kPaged>(late, it, h, (it.q0 + token_r) * late->q_st + head_r * late->q_sh,
-                               it.s0 * kNarrowKeys + wave * 32, it.s1 - it.s0, kNarrowKeys, 32,
-                               __builtin_amdgcn_readlane(lim, r), m_r == -INFINITY ? 0.f : m_r,
-                               acc);
 #pragma unroll
-      for (int x = 0; x < kD / 64; ++x) mine[r * kD + lane * (kD / 64) + x] = acc[x];
-    }
-  } else {
-#pragma unroll
-    for (int dt = 0; dt < kDt; ++dt)
-      *reinterpret_cast<dsa_f32x4*>(mine + c16 * kD + 16 * dt + 4 * q4) = oacc[dt];
-  }
+  for (int dt = 0; dt < kDt; ++dt)
+    *reinterpret_cast<dsa_f32x4*>(mine + c16 * kD + 16 * dt + 4 * q4) = oacc[dt];
   if (q4 == 0) {
     join_ml[0][wave][c16] = m_run;
     join_ml[1][wave][c16] = l_wave;

@@ -439,6 +439,12 @@ __device__ __forceinline__ bool hides_infinity(LateParams p, const Item& it, int
   return __any(sum != 0.f);
 }
 
+// Rows that overlap (one key of stride 0, a V expanded along its tokens): a granule
+// that ends inside holds copies of them behind the last key, hidden from every row.
+__device__ __forceinline__ bool holds_copies(LateParams p, int kend) {
+  return p->v_st < p->head_dim && (kend & 15) != 0;
+}
+
 // A wave's O over again, for a wave that hides_infinity: the same products (kRows = 32:
 // 32x32x16, 16: 16x16x32), 32 keys at a time from key0, key0 + stride, .. below `hi`,
 // with the final reference `m_use`, operands straight from memory.  Where keys from
@@ -855,11 +861,13 @@ __global__ void __launch_bounds__(256, kD == 64 ? 4 : 2) seq_wide_kernel(Params 
 #pragma unroll
     for (int r = 0; r < 16; ++r) unfinite = fmaf(oacc[dt][r], 0.f, unfinite);
   // (a row whose scores are not finite stays as it is)
-  if (__builtin_expect(lim_first < kend && __any(unfinite != 0.f && l_tot * 0.f == 0.f), 0)) {
+  const bool copies = holds_copies(late, kend);
+  if (__builtin_expect(
+          (lim_first < kend || copies) && __any(unfinite != 0.f && l_tot * 0.f == 0.f), 0)) {
     // Staged with the wave's last steps, but not seen by all of its rows.
     const int last = min((lim_last + kWideKeys - 1) & -kWideKeys, it.s1 * kWideKeys);
-    if (hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kWideKeys),
-                                  min(last, kend)))
+    if (copies || hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kWideKeys),
+                                            min(last, kend)))
       walk_again<T, kD, kUse, kPaged, 32>(
           late, it, h, (int64_t)(it.q0 + token) * late->q_st + head * late->q_sh, lim, lim_first,
           it.s0 * kWideKeys, 32, min(lim_last, it.s1 * kWideKeys),
@@ -1146,9 +1154,11 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
 #pragma unroll
     for (int r = 0; r < 4; ++r) unfinite = fmaf(oacc[dt][r], 0.f, unfinite);
   // (a row whose scores are not finite stays as it is)
-  if (__builtin_expect(lim_first < kend && __any(unfinite != 0.f && l_wave * 0.f == 0.f), 0) &&
-      hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kNarrowKeys),
-                                min(kend, it.s1 * kNarrowKeys)))
+  const bool copies = holds_copies(late, kend);
+  if (__builtin_expect(
+          (lim_first < kend || copies) && __any(unfinite != 0.f && l_wave * 0.f == 0.f), 0) &&
+      (copies || hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kNarrowKeys),
+                                           min(kend, it.s1 * kNarrowKeys))))
     walk_again<T, kD, kD, kPaged, 16>(
         late, it, h, (int64_t)(it.q0 + token) * late->q_st + head * late->q_sh, lim, lim_first,
         it.s0 * kNarrowKeys + wave * 32, kNarrowKeys, min(kend, it.s1 * kNarrowKeys),

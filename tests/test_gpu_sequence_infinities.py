@@ -110,6 +110,36 @@ def test_values_that_are_not_finite(cuda_device, dtype, heads, q_lens, k_lens, w
     _compare(paged, oracle.packed(q, k, v, q_lens, k_lens, causal=False), v_max, max(k_lens))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [128, 96, 64])
+@pytest.mark.parametrize("stride", [0, 8])
+@pytest.mark.parametrize("n,m", [(1, 1), (40, 1), (1, 5), (3, 37), (60, 70), (16, 2000),
+                                 (150, 1500)], ids=str)
+def test_infinite_values_of_rows_that_overlap(cuda_device, n, m, stride, dim, causal):
+    """One key (an axis of one entry), and V whose tokens share memory: expanded, or 8
+    elements apart.  What the rows see is infinite, nothing turns to NaN."""
+    q = _rows((n, 4, dim), torch.bfloat16, 8, cuda_device)
+    k = _rows((m, 2, dim), torch.bfloat16, 9, cuda_device)
+    store = _rows((2 * dim + 8 * m,), torch.bfloat16, 10, cuda_device)
+    # (in rows 8 elements apart, the last ones alone reach the store's end)
+    store[3], store[-dim - 8] = math.inf, -math.inf
+    v = torch.as_strided(store, (m, 2, dim), (stride, dim, 1))
+    starts = _starts([n], cuda_device), _starts([m], cuda_device)
+    out = ops.packed_attention(q, k, v, *starts, causal=causal)
+    expected = oracle.packed(q, k, v.contiguous(), [n], [m], causal)
+    _compare(out, expected, 5.0, m)
+    # Packed in pages, every row of a page the same one.
+    pages = -(-m // 16)
+    kc = torch.full((pages * 16, 2, dim), math.nan, dtype=k.dtype, device=cuda_device)
+    kc[:m] = k
+    vc = torch.as_strided(store, (pages, 16, 2, dim), (0, 0, dim, 1))
+    table = torch.arange(pages, dtype=torch.int32, device=cuda_device)[None]
+    out = ops.paged_attention(q, kc.view(pages, 16, 2, dim), vc, table, starts[1][1:], starts[0],
+                              causal=causal)
+    expected = oracle.packed(q, k, vc.reshape(-1, 2, dim)[:m], [n], [m], causal)
+    _compare(out, expected, 5.0, m)
+
+
 def _time(call):
     best = math.inf
     for _ in range(5):

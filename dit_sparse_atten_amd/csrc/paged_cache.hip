@@ -346,8 +346,13 @@ extern "C" int dsa_paged_write(const void* k, const void* v, void* k_cache, void
   p.chunk_magic = quotient_magic((uint32_t)chunks);
   p.group_tokens = (int32_t)std::max<int64_t>(1, kWriteChunks / row);
   p.page_shift = __builtin_ctz(page_size);
+  const int64_t groups = ((int64_t)tokens + p.group_tokens - 1) / p.group_tokens;
+  // (a launch counts its threads, 256 for each, in 32 bits)
+  if (groups >= 1 << 24)
+    return dsa::set_error(DSA_EUNSUPPORTED,
+                          "%s: %d tokens of %d bytes (up to %d a workgroup, 2^24 - 1 workgroups)",
+                          who, tokens, (int)row * 16, p.group_tokens);
   dsa::clear_error();
-  const int groups = (tokens + p.group_tokens - 1) / p.group_tokens;
   hipLaunchKernelGGL(paged_write_kernel, dim3((unsigned)groups, 2), dim3(256), 0, stream, p);
   return dsa::check_launch(who);
 }

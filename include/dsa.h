@@ -518,7 +518,8 @@ int dsa_gated_residual(const void* x, int64_t x_stride, const void* y, int64_t y
  * dsa_paged_write: row t of k and v [tokens, heads, row_bytes] into slot
  * slots[t] of the caches; a slot outside them is skipped.  strides[10] in BYTES,
  * multiples of 16: k (token, head), v (token, head), k_cache (page, token,
- * head), v_cache (page, token, head).  Any element type; of tokens that share a
+ * head), v_cache (page, token, head).  Fewer than 2^24 workgroups of 2,048 16-byte
+ * chunks (of at least a token), at most 512 KB a token.  Any element type; of tokens that share a
  * slot one or parts of several are kept.  k and v do not overlap the caches.
  */
 int dsa_paged_plan(const int32_t* cached, const int32_t* fresh, int32_t requests, int32_t* table,

@@ -490,8 +490,10 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
     return dsa::set_error(DSA_EINVAL, "%s: negative size", who);
   if ((p.causal != 0 && p.causal != 1) || (p.fill != 0 && p.fill != 1))
     return dsa::set_error(DSA_EINVAL, "%s: causal and fill are 0 or 1", who);
-  if (!(scale > 0.f) || scale > 3e38f)
-    return dsa::set_error(DSA_EINVAL, "%s: scale must be positive and finite", who);
+  // (the softmax runs in base 2: a scale whose product with log2(e) is infinite would
+  // make NaN of a score of 0)
+  if (!(scale > 0.f) || scale > 2.3e38f)
+    return dsa::set_error(DSA_EINVAL, "%s: scale must be positive and finite, up to 2.3e38", who);
   const int64_t strides[] = {p.q_st, p.q_sh, p.o_st, p.o_sh, p.k_sp, p.k_st, p.k_sh,
                              p.v_sp, p.v_st, p.v_sh};
   for (int64_t s : strides)

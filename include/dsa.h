@@ -549,7 +549,7 @@ int dsa_paged_write(const void* k, const void* v, void* k_cache, void* v_cache,
  *     cache; strides[10]: q (token, head), k_cache, v_cache (page, token, head),
  *     o (token, head).  Keys of a table entry outside [0, pages) take no part.
  *   Strides multiples of 8, pointers 16-byte aligned, head_dim a multiple of 8 up
- *   to 128, scale > 0.  lse: [heads, q_rows] natural log or NULL.  fill = 1: rows
+ *   to 128, 0 < scale <= 2.3e38.  lse: [heads, q_rows] natural log or NULL.  fill = 1: rows
  *   of o outside every sequence become 0; 0: they are left as they were (lse
  *   has -inf there).  o may be q itself, and overlaps nothing else.  Starts and lengths are device arrays, never read on the host;
  *   ones that leave the tensors (or 2^30 keys) are cut to them.  workspace: at least

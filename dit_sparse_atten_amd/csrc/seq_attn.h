@@ -453,7 +453,7 @@ __device__ __forceinline__ bool holds_copies(LateParams p, int kend) {
 // tell which elements they reach.  (4,096 causal tokens x 4 heads: 50 us, with such
 // values all over 150; element by element, a key to a lane, 14,000.  One infinity that
 // nearly every row sees is hidden from rows of its own wave alone: 55 us.)
-template <typename T, int kD, int kUse, bool kPaged, int kRows, typename Acc>
+template <typename T, int kUse, bool kPaged, int kRows, typename Acc>
 __device__ __forceinline__ void walk_again(LateParams p, const Item& it, int h, int64_t q_at,
                                            int lim, int lim_first, int key0, int stride, int hi,
                                            float m_use, Acc* oacc) {
@@ -590,7 +590,8 @@ __device__ __forceinline__ void walk_again(LateParams p, const Item& it, int h, 
 //
 // Staged rows hold kD dims, of which the products take the first kUse: head dims of
 // 72 to 96 leave the last quarter of a 128-dim row out (8,192 x 8,192 x 32 heads: 96
-// dims 897 -> 804 us, 80 dims 985 -> 896).
+// dims 897 -> 804 us, 80 dims 985 -> 896).  64-dim rows take 32 KB of LDS and leave
+// room for four workgroups a compute unit, if their registers do (128 a lane).
 template <typename T, int kD, int kUse, bool kPaged>
 __global__ void __launch_bounds__(256, kD == 64 ? 4 : 2) seq_wide_kernel(Params p) {
   typedef dsa::Elem<T> E;
@@ -868,7 +869,7 @@ __global__ void __launch_bounds__(256, kD == 64 ? 4 : 2) seq_wide_kernel(Params 
     const int last = min((lim_last + kWideKeys - 1) & -kWideKeys, it.s1 * kWideKeys);
     if (copies || hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kWideKeys),
                                             min(last, kend)))
-      walk_again<T, kD, kUse, kPaged, 32>(
+      walk_again<T, kUse, kPaged, 32>(
           late, it, h, (int64_t)(it.q0 + token) * late->q_st + head * late->q_sh, lim, lim_first,
           it.s0 * kWideKeys, 32, min(lim_last, it.s1 * kWideKeys),
           m_run == -INFINITY ? 0.f : m_run, oacc);
@@ -1159,7 +1160,7 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
           (lim_first < kend || copies) && __any(unfinite != 0.f && l_wave * 0.f == 0.f), 0) &&
       (copies || hides_infinity<T, kPaged>(late, it, h, max(lim_first, it.s0 * kNarrowKeys),
                                            min(kend, it.s1 * kNarrowKeys))))
-    walk_again<T, kD, kD, kPaged, 16>(
+    walk_again<T, kD, kPaged, 16>(
         late, it, h, (int64_t)(it.q0 + token) * late->q_st + head * late->q_sh, lim, lim_first,
         it.s0 * kNarrowKeys + wave * 32, kNarrowKeys, min(kend, it.s1 * kNarrowKeys),
         m_run == -INFINITY ? 0.f : m_run, oacc);

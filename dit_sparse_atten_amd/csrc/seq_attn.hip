@@ -147,7 +147,9 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     const int setup = (int)p.item_cost;
     const uint32_t chains = max(1, kNarrowSlots / p.kv_heads);
     const uint64_t all_units = work_lds + (uint64_t)tiles * setup;
-    // More than 32 bits count (5e11 keys): whole tiles, as many to each chain.
+    // From 2^31 units on (2.7e11 keys of one head, set-ups among them): whole tiles, as
+    // many to each chain.  (Not 2^32: an item's range is an int, and the last chain's
+    // end, up to a quota past the units, still counts in 32 bits.)
     const bool vast = all_units >> 31 != 0;
     const uint32_t units = vast ? (uint32_t)tiles : (uint32_t)all_units;
     const uint32_t quota =

@@ -518,9 +518,10 @@ int dsa_gated_residual(const void* x, int64_t x_stride, const void* y, int64_t y
  * dsa_paged_write: row t of k and v [tokens, heads, row_bytes] into slot
  * slots[t] of the caches; a slot outside them is skipped.  strides[10] in BYTES,
  * multiples of 16: k (token, head), v (token, head), k_cache (page, token,
- * head), v_cache (page, token, head).  Fewer than 2^24 workgroups of 2,048 16-byte
- * chunks (of at least a token), at most 512 KB a token.  Any element type; of tokens that share a
- * slot one or parts of several are kept.  k and v do not overlap the caches.
+ * head), v_cache (page, token, head).  Any element type; of tokens that share a
+ * slot one or parts of several are kept.  k and v do not overlap the caches.  At
+ * most 512 KB a token, and fewer than 2^24 workgroups of 2,048 16-byte chunks (of
+ * whole tokens, at least one).
  */
 int dsa_paged_plan(const int32_t* cached, const int32_t* fresh, int32_t requests, int32_t* table,
                    int64_t table_stride, int32_t table_width, const int32_t* free_pages,
@@ -549,10 +550,11 @@ int dsa_paged_write(const void* k, const void* v, void* k_cache, void* v_cache,
  *     cache; strides[10]: q (token, head), k_cache, v_cache (page, token, head),
  *     o (token, head).  Keys of a table entry outside [0, pages) take no part.
  *   Strides multiples of 8, pointers 16-byte aligned, head_dim a multiple of 8 up
- *   to 128, 0 < scale <= 2.3e38.  lse: [heads, q_rows] natural log or NULL.  fill = 1: rows
- *   of o outside every sequence become 0; 0: they are left as they were (lse
- *   has -inf there).  o may be q itself, and overlaps nothing else.  Starts and lengths are device arrays, never read on the host;
- *   ones that leave the tensors (or 2^30 keys) are cut to them.  workspace: at least
+ *   to 128, 0 < scale <= 2.3e38.  lse: [heads, q_rows] natural log or NULL.  fill =
+ *   1: rows of o outside every sequence become 0; 0: they are left as they were
+ *   (lse has -inf there).  o may be q itself, and overlaps nothing else.  Starts and
+ *   lengths are device arrays, never read on the host; ones that leave the tensors
+ *   (or 2^30 keys) are cut to them.  workspace: at least
  *   dsa_seq_attention_workspace_bytes() with max_keys = k_rows, or table_width *
  *   page_size; calls that overlap in time need one each.
  */

@@ -235,3 +235,33 @@ def test_plan_counts_past_31_bits(cuda_device):
     got = _plan([0, 0, 0], [most, most, 5], [[-1], [-1], [-1]], [5], 16, 10, cuda_device)
     assert got == [[0, most, most, most], [most, most, 5], list(range(80, 90)), [3, most],
                    [[5], [-1], [-1]]]
+
+
+def test_step_that_lost_tokens_is_made_again(cuda_device):
+    """Steps that advance on the device only where every token has its place: the one
+    that runs out of pages leaves lengths and list as they were until a page returns."""
+    page = 16
+    table = _ints([[7, -1, -1], [8, -1, -1]], cuda_device)
+    cached, given = _ints([16, 30], cuda_device), _ints([1], cuda_device)
+    table[1, 1] = 9
+    free = _ints([3, 4, 5], cuda_device)  # (3 is in use elsewhere)
+    new = _ints([1, 3], cuda_device)
+
+    def step():
+        plan = ops.paged_plan(cached, new, table, free, page, 4, free_start=given)
+        whole = plan.status[1:] == 0
+        given.add_(plan.status[:1] * whole)
+        cached.copy_(torch.where(whole, plan.kv_lens, cached))
+        return plan.slots.tolist(), plan.status.tolist()
+
+    assert step() == ([4 * 16, 9 * 16 + 14, 9 * 16 + 15, 5 * 16], [2, 0])
+    assert cached.tolist() == [17, 33] and given.tolist() == [3]
+    cached[0] = 32
+    for _ in range(2):
+        assert step() == ([-1, 5 * 16 + 1, 5 * 16 + 2, 5 * 16 + 3], [1, 1])
+        assert cached.tolist() == [32, 33] and given.tolist() == [3]
+    given -= 1
+    free[2] = 3  # the page used elsewhere came back
+    assert step() == ([3 * 16, 5 * 16 + 1, 5 * 16 + 2, 5 * 16 + 3], [1, 0])
+    assert cached.tolist() == [33, 36] and given.tolist() == [3]
+    assert table.tolist() == [[7, 4, 3], [8, 9, 5]]

@@ -213,11 +213,12 @@ __device__ __forceinline__ uint32_t quotient(uint32_t i, uint32_t magic) {
 // Moves 16 bytes per thread and turn, bound by memory on long calls.  A workgroup
 // takes `group_tokens` tokens of one tensor (y), their chunks to consecutive
 // threads; every thread has all its loads on their way before its first store.
-// 57,600 tokens x 12 heads x 128 (708 MB): 138 us, 5.1 TB/s, against 198 us with
-// 64-bit indexes and four turns, and 148 us of a plain copy.  Rows are read once
-// (non-temporal) but stored through the caches, where the attention that follows
-// finds them: with non-temporal stores the write alone took 130 us, but 131,072
-// tokens x 8 heads with a decoding step behind them 327 us against 299.
+// 57,600 tokens x 12 heads x 128 (708 MB): 137 us, 5.2 TB/s, against 198 us with
+// 64-bit indexes and four turns; a plain copy of as much takes 126 us, one past the
+// caches 109.  Rows are read once (non-temporal) but stored through the caches, where
+// the attention that follows finds them: with non-temporal stores the write alone took
+// 130 us, but 131,072 tokens x 8 heads with a decoding step behind them 327 us against
+// 299.
 // Indexes are divided by quotient(): a workgroup has fewer than 2^15 chunks.
 constexpr int kWriteTurns = 8;
 constexpr int kWriteChunks = 256 * kWriteTurns;  // at most, of a workgroup

@@ -206,6 +206,26 @@ SIGNATURES = {
         _c_int, _c_int, _c_ptr,                    # causal, fill, lse
         _c_ptr, _c_size, _c_ptr,                   # workspace, workspace_bytes, stream
     )),
+    "dsa_paged_write_rotary": (_c_int, (
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,  # q, q_out, k, v, k_cache, v_cache
+        _c_int, ctypes.POINTER(_c_i64),            # dtype, strides[14]
+        _c_int, _c_int, _c_int, _c_int,            # tokens, heads, kv_heads, head_dim
+        _c_int, _c_int, _c_int, _c_int,            # rot_dim, halves, pages, page_size
+        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,    # slots, positions, cos_sin, max_positions, stream
+    )),
+    "dsa_paged_write_fp4": (_c_int, (
+        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,    # q, q_out, k, v, cache
+        _c_int, ctypes.POINTER(_c_i64),            # dtype, strides[10]
+        _c_int, _c_int, _c_int, _c_int,            # tokens, heads, kv_heads, head_dim
+        _c_int, _c_int, _c_int, _c_int,            # rot_dim, halves, pages, page_size
+        _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,    # slots, positions, cos_sin, max_positions, stream
+    )),
+    "dsa_paged_read_fp4": (_c_int, (
+        _c_ptr, ctypes.POINTER(_c_i64),            # cache, strides[2], bytes
+        _c_ptr, _c_ptr, _c_int,                    # k, v, dtype
+        _c_int, _c_int, _c_int, _c_int,            # pages, page_size, kv_heads, head_dim
+        _c_ptr, _c_int, _c_ptr,                    # list, count, stream
+    )),
     "dsa_seq_attention_workspace_bytes": (_c_size, (
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,  # q_rows, requests, heads, kv_heads, head_dim, max_keys
     )),

@@ -36,6 +36,7 @@ SOURCES = (
     "permute.hip",
     "dit_ops.hip",
     "paged_cache.hip",
+    "paged_rotary.hip",
     "seq_attn.hip",
     "seq_attn_f16.hip",
 )

@@ -974,7 +974,8 @@ def gated_residual(x, y, gate=None, out=None):
 # around it
 # ---------------------------------------------------------------------------
 
-_I64x8, _I64x10 = ctypes.c_int64 * 8, ctypes.c_int64 * 10
+_I64x2, _I64x6, _I64x8 = ctypes.c_int64 * 2, ctypes.c_int64 * 6, ctypes.c_int64 * 8
+_I64x10, _I64x14 = ctypes.c_int64 * 10, ctypes.c_int64 * 14
 
 
 class PagedPlan(typing.NamedTuple):
@@ -1376,3 +1377,251 @@ def paged_attention(q, k_cache, v_cache, block_table, kv_lens, q_start, causal=T
               kv_lens.data_ptr(), q_start.data_ptr(), scale, 1 if causal else 0, 1 if fill else 0,
               None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.shape[0])
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# Writes that turn keys and queries with their positions; caches of 4-bit elements
+# ---------------------------------------------------------------------------
+
+def _fp4_row(head_dim):
+    """Bytes of a token's keys and values in a 4-bit cache, for each key head."""
+    if head_dim % 8 or not 8 <= head_dim <= HEAD_DIM:
+        raise ValueError(f"head_dim {head_dim} unsupported (a multiple of 8 up to {HEAD_DIM})")
+    return 32 * -(-head_dim // 32) + 8
+
+
+def paged_cache_fp4(pages, page_size, kv_heads, head_dim, device="cuda"):
+    """An empty paged cache of 4-bit keys and values: uint8 [pages, kv_heads, page_size,
+    32 * G + 8] with G = ceil(head_dim / 32): 4.25 bits an element at 128 dims.
+
+    Groups of 32 neighbouring dims are E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+    their negatives) with a power of two between them.  The bytes of one page and head
+    are, one after the other, the keys' codes [page_size, 16 * G], the values' codes,
+    the keys' scale bytes [page_size, 4] and the values'; a scale byte b stands for
+    2^(b - 127), 255 for a group that held an infinity or a NaN (and reads as NaN).
+    Pages and heads may be any slices of a larger cache that are multiples of 16 bytes
+    apart."""
+    _page_size(page_size)
+    if pages < 0 or kv_heads < 1:
+        raise ValueError(f"a cache of {pages} pages of {kv_heads} key/value heads")
+    return torch.zeros((pages, kv_heads, page_size, _fp4_row(head_dim)), dtype=torch.uint8,
+                       device=device)
+
+
+def _fp4_strides(layout, kv_heads, head_dim):
+    """(page and head strides in bytes) of a 4-bit cache, used in place."""
+    shape, strides, dtype = layout
+    row = _fp4_row(head_dim)
+    if dtype != torch.uint8 or len(shape) != 4 or shape[3] != row:
+        raise ValueError(f"cache must be uint8 [pages, kv_heads, page_size, {row}] for "
+                         f"{head_dim}-dim heads")
+    if kv_heads is not None and shape[1] != kv_heads:
+        raise ValueError(f"cache holds {shape[1]} key/value heads, not {kv_heads}")
+    _page_size(shape[2])
+    if strides[3] != 1 or strides[2] != row:
+        raise ValueError("a page and head of the cache must be contiguous")
+    lead = [0 if size == 1 else stride for size, stride in zip(shape[:2], strides[:2])]
+    if any(stride % 16 for stride in lead):
+        raise ValueError("pages and heads of the cache must be multiples of 16 bytes apart")
+    return lead
+
+
+def _fp4_aligned(cache):
+    if cache.data_ptr() & 15 and cache.numel():
+        raise ValueError("cache must be 16-byte aligned")
+
+
+@functools.lru_cache(maxsize=512)
+def _turn_layout(q, q_out, k, v, caches, angles):
+    """(operands to copy first, strides, tokens, heads, kv_heads, head_dim, rot_dim, dtype
+    code, pages, page size) of a write that turns its rows."""
+    dtype = k[2]
+    code = dtype_code(dtype)
+    rows = [_sequence_strides("k", k, dtype), _sequence_strides("v", v, dtype)]
+    tokens, kv_heads, head_dim = k[0]
+    if v[0] != k[0]:
+        raise ValueError("k and v must have the same shape")
+    if kv_heads == 0:
+        raise ValueError("k must hold at least one head")
+    _fp4_row(head_dim)
+    rot = 0
+    if angles is not None:
+        shape, own = angles
+        if own != torch.float32 or len(shape) != 3 or shape[2] != 2:
+            raise ValueError("cos_sin must be a float32 tensor [positions, rot_dim / 2, 2]")
+        rot = 2 * shape[1]
+        if rot % 16 or rot > head_dim:
+            raise ValueError(f"{rot} turned dims unsupported (a multiple of 16 up to head_dim)")
+        if shape[0] >= 1 << 31:
+            raise ValueError("cos_sin must have fewer than 2^31 positions")
+    heads, q_strides, out_strides = 0, [0, 0], [0, 0]
+    if q is not None:
+        q_strides = _sequence_strides("q", q, dtype)
+        heads = q[0][1]
+        if q[0] != (tokens, heads, head_dim):
+            raise ValueError("q must have k's tokens and head dimension")
+        out_strides = [heads * head_dim, head_dim]
+        if q_out is not None:
+            if q_out[0] != q[0] or q_out[2] != dtype:
+                raise ValueError("q_out must have q's shape, type and device")
+            _apart("q_out", q_out)
+            out_strides = _row_strides(*q_out[:2], dtype.itemsize)
+            if out_strides is None:
+                if tokens and heads:
+                    raise ValueError("q_out must have a contiguous, 16-byte aligned head dimension")
+                out_strides = [0, 0]
+    if len(caches) == 1:
+        held = [_fp4_strides(caches[0], kv_heads, head_dim)]
+        pages, page_size = caches[0][0][0], caches[0][0][2]
+        _apart("cache", caches[0])
+    else:
+        held = [_cache_strides(name, c, dtype) for name, c in zip(("k_cache", "v_cache"), caches)]
+        pages, page_size = caches[0][0][:2]
+        if caches[0][0] != caches[1][0] or caches[0][0][2:] != (kv_heads, head_dim):
+            raise ValueError("the caches must share their shape, and k its heads and head "
+                             "dimension")
+        _page_size(page_size)
+        _apart("k_cache", caches[0])
+        _apart("v_cache", caches[1])
+    operands = [q_strides, out_strides, *rows, *held]
+    copies = tuple(i for i, x in enumerate((q_strides, *rows)) if x is None)
+    strides = None
+    if not copies:
+        strides = (_I64x10 if len(caches) == 1 else _I64x14)(*[x for t in operands for x in t])
+    return copies, strides, tokens, heads, kv_heads, head_dim, rot, code, pages, page_size
+
+
+def _angles(cos_sin, positions, tokens, device):
+    _require_cuda("cos_sin", cos_sin)
+    positions = _index_vector("positions", positions, device, tokens)
+    if cos_sin.device != device:
+        raise ValueError(f"cos_sin must live on {device}")
+    if not cos_sin.is_contiguous() or cos_sin.data_ptr() & 15:
+        cos_sin = cos_sin.clone(memory_format=torch.contiguous_format)
+    return cos_sin, positions
+
+
+def _write_turned(function, what, k, v, caches, slots, positions, cos_sin, q, q_out, halves):
+    """A write of both kinds; returns the turned queries, or None."""
+    device = caches[0].device
+    for name, t in (("k", k), ("v", v), ("slots", slots)):
+        _require_cuda(name, t)
+    if q is None and q_out is not None:
+        raise ValueError("q_out needs q")
+    for name, t in (("q", q), ("q_out", q_out)):
+        if t is not None:
+            _require_cuda(name, t)
+            if t.device != device:
+                raise ValueError(f"{name} must live on {device}")
+    copies, strides, tokens, heads, kv_heads, head_dim, rot, code, pages, page_size = _turn_layout(
+        None if q is None else _layout(q), None if q_out is None else _layout(q_out), _layout(k),
+        _layout(v), tuple(_layout(c) for c in caches),
+        None if cos_sin is None else (cos_sin.shape, cos_sin.dtype))
+    if slots.dtype != torch.int64 or slots.shape != (tokens,):
+        raise ValueError(f"slots must be an int64 tensor of {tokens} values")
+    if not (k.device == v.device == slots.device == device):
+        raise ValueError("k, v, the cache and slots must be on the same device")
+    if cos_sin is not None:
+        cos_sin, positions = _angles(cos_sin, positions, tokens, device)
+    elif positions is not None:
+        raise ValueError("positions need cos_sin")
+    if copies or (k.data_ptr() | v.data_ptr() | (0 if q is None else q.data_ptr())) & 15:
+        # (a copied q still goes to its own place where q_out is q)
+        operands = [torch.empty(0, device=device) if q is None else q, k, v]
+        new_q, k, v = _in_place(copies, *operands)
+        return _write_turned(function, what, k, v, caches, slots, positions, cos_sin,
+                             None if q is None else new_q, q_out, halves)
+    out = q_out
+    if q is not None:
+        if out is None:
+            out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
+        _aligned("q_out", out)
+    if tokens == 0:
+        return out
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    _call(function, what, device, q.data_ptr() if heads else None, out.data_ptr() if heads else None,
+          k.data_ptr(), v.data_ptr(), *[c.data_ptr() for c in caches], code, strides, tokens, heads,
+          kv_heads, head_dim, rot, 1 if halves else 0, pages, page_size, slots.data_ptr(),
+          positions.data_ptr() if rot else None, cos_sin.data_ptr() if rot else None,
+          cos_sin.shape[0] if rot else 0)
+    return out
+
+
+def paged_write_rotary(k, v, k_cache, v_cache, slots, positions, cos_sin, q=None, q_out=None,
+                       halves=False):
+    """``paged_write`` that turns the keys with their positions on the way, and the
+    queries beside them.
+
+    cos_sin: float32 [positions, rot_dim / 2, 2] on the device, (cos, sin) of every
+    position's angles (as ``rmsnorm_rope`` takes them); the first rot_dim dims of a
+    head, a multiple of 16, turn in neighbouring pairs (2 i, 2 i + 1) or, with
+    ``halves``, in pairs (i, i + rot_dim / 2).  positions: int32 [tokens] on the device,
+    the rows of cos_sin.  A step's, behind its plan and with nothing read back::
+
+        token = torch.arange(tokens, device=device)
+        r = torch.searchsorted(plan.q_start[1:], token, right=True).clamp_max(requests - 1)
+        positions = (cached[r] + token - plan.q_start[r]).int()
+
+    k, v, the caches and slots as in ``paged_write``, bf16 or fp16, head_dim a multiple
+    of 8 up to 128; a token whose position is outside cos_sin is skipped as one without
+    a slot.  q [tokens, heads, head_dim] (optional): returned turned, in a new tensor or
+    in ``q_out``, which may be q itself; a row whose position is outside cos_sin is
+    passed on as it is.  Elements are turned in float32 and rounded once.
+    """
+    lib = _lib.load()
+    _require_cuda("k_cache", k_cache)
+    _require_cuda("v_cache", v_cache)
+    if v_cache.device != k_cache.device:
+        raise ValueError("k, v, the cache and slots must be on the same device")
+    _aligned("k_cache", k_cache)
+    _aligned("v_cache", v_cache)
+    if cos_sin is None:
+        raise ValueError("cos_sin and positions are needed (paged_write turns nothing)")
+    return _write_turned(lib.dsa_paged_write_rotary, "dsa_paged_write_rotary", k, v,
+                         (k_cache, v_cache), slots, positions, cos_sin, q, q_out, halves)
+
+
+def paged_write_fp4(k, v, cache, slots, positions=None, cos_sin=None, q=None, q_out=None,
+                    halves=False):
+    """Writes keys and values [tokens, kv_heads, head_dim] (bf16 or fp16) into a cache of
+    4-bit elements (``paged_cache_fp4``), row t at slot ``slots[t]``.
+
+    With ``cos_sin`` and ``positions`` the keys (and q) turn first, as in
+    ``paged_write_rotary``; the rest of its conditions hold here too.  Each group of 32
+    neighbouring dims gets the smallest exponent e with max|x| <= 7 * 2^e, between -125
+    and 125 (fp16: -23 and 13, so that every element is a number of that type; larger
+    elements become the largest), and its elements the nearest codes, ties the even
+    ones, from the turned value in float32.  Normal values are off by 11% of their norm.
+    A group with an infinity or a NaN is kept as NaN.  Returns q turned (without
+    cos_sin: as it is), or None.
+    """
+    lib = _lib.load()
+    _require_cuda("cache", cache)
+    _fp4_aligned(cache)
+    return _write_turned(lib.dsa_paged_write_fp4, "dsa_paged_write_fp4", k, v, (cache,), slots,
+                         positions, cos_sin, q, q_out, halves)
+
+
+def paged_read_fp4(cache, head_dim, pages=None, dtype=torch.bfloat16):
+    """Keys and values that a 4-bit cache stands for, (k, v) [pages, page_size, kv_heads,
+    head_dim] in bf16 or fp16: of the listed ``pages`` (int32 on the device, zeros for
+    one outside the cache) or of all.  Exact, but for elements that fp16 cannot hold of a
+    cache written from bf16."""
+    lib = _lib.load()
+    _require_cuda("cache", cache)
+    code = dtype_code(dtype)
+    strides = _I64x2(*_fp4_strides(_layout(cache), None, head_dim))
+    _fp4_aligned(cache)
+    total, kv_heads, page_size, _ = cache.shape
+    device = cache.device
+    if pages is not None:
+        pages = _index_vector("pages", pages, device)
+    count = total if pages is None else pages.shape[0]
+    k = torch.empty((count, page_size, kv_heads, head_dim), dtype=dtype, device=device)
+    v = torch.empty_like(k)
+    if k.numel():
+        _call(lib.dsa_paged_read_fp4, "dsa_paged_read_fp4", device, cache.data_ptr(), strides,
+              k.data_ptr(), v.data_ptr(), code, total, page_size, kv_heads, head_dim,
+              None if pages is None else pages.data_ptr(), count)
+    return k, v

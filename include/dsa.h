@@ -574,6 +574,57 @@ int dsa_paged_attention(const void* q, const void* k_cache, const void* v_cache,
 size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32_t heads,
                                          int32_t kv_heads, int32_t head_dim, int64_t max_keys);
 
+/*
+ * Writes into a paged cache that turn keys and queries with their positions on the
+ * way, bf16 or fp16 (the reference turns whole tensors of one length before its
+ * attention).  With (c_i, s_i) = cos_sin[positions[t]][i] (fp32 [max_positions,
+ * rot_dim / 2, 2]), pair i = (a, b) of a row of token t becomes (a c_i - b s_i,
+ * b c_i + a s_i): pairs are the dims (2 i, 2 i + 1) or, with halves = 1, (i, i +
+ * rot_dim / 2); dims from rot_dim (a multiple of 16, 0: none turn) stay.
+ *   q [tokens, heads, head_dim] (heads = 0: none): its turned rows into q_out, which
+ *   may be q itself; a row whose position is outside [0, max_positions) is passed on
+ *   as it is.
+ *   k [tokens, kv_heads, head_dim], turned, and v into slot slots[t] of the cache; a
+ *   token whose slot lies outside it, or whose position has no angles, is skipped.
+ *   A call's slots are distinct.  head_dim a multiple of 8 up to 128; strides
+ *   multiples of 8 elements, pointers 16-byte aligned; up to 4,096 heads.  Nothing
+ *   but q_out and q overlaps.
+ * dsa_paged_write_rotary: strides[14], in elements: q, q_out, k, v (token, head),
+ *   k_cache, v_cache (page, token, head).  Turned in fp32, rounded once.
+ * dsa_paged_write_fp4: into a cache of 4-bit elements; strides[10]: q, q_out, k, v
+ *   (token, head) in elements, cache (page, head) in BYTES, multiples of 16.
+ *
+ * A 4-bit cache holds keys and values of one page and key head in page_size *
+ * (32 G + 8) bytes, G = ceil(head_dim / 32): the keys' codes [page_size, 16 G], the
+ * values' codes [page_size, 16 G], the keys' scales [page_size, 4] and the values'
+ * scales [page_size, 4].  32 neighbouring dims share a scale byte b, for 2^(b - 127);
+ * 255: the group held an infinity or a NaN, and each of its elements is NaN.  Element
+ * 2 i of a row is the low half of byte i: a sign bit over the magnitudes 0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6.  A group's exponent is the smallest e with max|x| <= 7 2^e, from
+ * -125 to 125 (fp16: -23 to 13, so that every element is a number of that type; larger
+ * elements become the largest); elements are rounded to the nearest code, ties to the
+ * even one, from the turned value in fp32.
+ *
+ * dsa_paged_read_fp4: the pages list[count] (list NULL: the first count) as 16-bit
+ *   values, k and v [count, page_size, kv_heads, head_dim]; zeros for a page outside
+ *   the cache.  strides[2]: cache (page, head) in bytes.
+ */
+int dsa_paged_write_rotary(const void* q, void* q_out, const void* k, const void* v, void* k_cache,
+                           void* v_cache, int32_t dtype, const int64_t* strides, int32_t tokens,
+                           int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t rot_dim,
+                           int32_t halves, int32_t pages, int32_t page_size, const int64_t* slots,
+                           const int32_t* positions, const float* cos_sin, int32_t max_positions,
+                           hipStream_t stream);
+int dsa_paged_write_fp4(const void* q, void* q_out, const void* k, const void* v, void* cache,
+                        int32_t dtype, const int64_t* strides, int32_t tokens, int32_t heads,
+                        int32_t kv_heads, int32_t head_dim, int32_t rot_dim, int32_t halves,
+                        int32_t pages, int32_t page_size, const int64_t* slots,
+                        const int32_t* positions, const float* cos_sin, int32_t max_positions,
+                        hipStream_t stream);
+int dsa_paged_read_fp4(const void* cache, const int64_t* strides, void* k, void* v, int32_t dtype,
+                       int32_t pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                       const int32_t* list, int32_t count, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

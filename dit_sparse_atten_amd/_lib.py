@@ -226,6 +226,17 @@ SIGNATURES = {
         _c_int, _c_int, _c_int, _c_int,            # pages, page_size, kv_heads, head_dim
         _c_ptr, _c_int, _c_ptr,                    # list, count, stream
     )),
+    "dsa_paged_attention_fp4": (_c_int, (
+        _c_ptr, _c_ptr, _c_ptr, _c_int,            # q, cache, o, dtype
+        ctypes.POINTER(_c_i64),                    # strides[6]
+        _c_int, _c_int,                            # q_rows, requests
+        _c_int, _c_int, _c_int,                    # heads, kv_heads, head_dim
+        _c_int, _c_int,                            # pages, page_size
+        _c_ptr, _c_i64, _c_int,                    # table, table_stride, table_width
+        _c_ptr, _c_ptr, _c_float,                  # kv_lens, q_start, scale
+        _c_int, _c_int, _c_ptr,                    # causal, fill, lse
+        _c_ptr, _c_size, _c_ptr,                   # workspace, workspace_bytes, stream
+    )),
     "dsa_seq_attention_workspace_bytes": (_c_size, (
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,  # q_rows, requests, heads, kv_heads, head_dim, max_keys
     )),

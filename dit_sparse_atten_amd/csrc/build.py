@@ -39,6 +39,7 @@ SOURCES = (
     "paged_rotary.hip",
     "seq_attn.hip",
     "seq_attn_f16.hip",
+    "seq_attn_fp4.hip",
 )
 
 # Packed FP32 VALU forms are disabled: the device code relies on scalar and

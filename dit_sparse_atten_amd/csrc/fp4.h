@@ -24,6 +24,12 @@ constexpr int kGroup = 32;  // dims to a scale byte
 __host__ __device__ constexpr int groups_of(int head_dim) { return (head_dim + 31) / 32; }
 __host__ __device__ constexpr int row_bytes(int groups) { return 32 * groups + 8; }
 
+// Pages of up to 2^20 tokens, so that a page and head's bytes count in 32 bits.
+constexpr int kMaxPage = 1 << 20;
+inline bool bad_page_size(int32_t size) {
+  return size < 16 || size > kMaxPage || (size & (size - 1)) != 0;
+}
+
 // Offsets within a page and head.
 struct Layout {
   int32_t code_row, v_codes, k_scales, v_scales;

@@ -418,7 +418,11 @@ extern "C" int dsa_paged_write_rotary(const void* q, void* q_out, const void* k,
 
 namespace {
 
-int check_cache(const void* cache, int64_t sp, int64_t sh, int32_t pages, const char* who) {
+int check_cache(const void* cache, int64_t sp, int64_t sh, int32_t pages, int32_t page_size,
+                const char* who) {
+  if (fp4::bad_page_size(page_size))
+    return dsa::set_error(DSA_EUNSUPPORTED, "%s: page_size %d (a power of two, 16 to %d)", who,
+                          page_size, fp4::kMaxPage);
   if (sp % 16 != 0 || sh % 16 != 0 || sp < 0 || sh < 0)
     return dsa::set_error(DSA_EINVAL, "%s: cache strides must be multiples of 16 bytes", who);
   if (pages > 0 && !cache) return dsa::set_error(DSA_EINVAL, "%s: null pointer", who);
@@ -441,9 +445,9 @@ extern "C" int dsa_paged_write_fp4(const void* q, void* q_out, const void* k, co
   int status = prepare(&p, who, q, q_out, k, v, dtype, strides, 0, tokens, heads, kv_heads,
                        head_dim, rot_dim, halves, pages, page_size, slots, positions, cos_sin,
                        max_positions);
-  if (status != DSA_OK || tokens == 0) return status;
-  status = check_cache(cache, strides[8], strides[9], pages, who);
   if (status != DSA_OK) return status;
+  status = check_cache(cache, strides[8], strides[9], pages, page_size, who);
+  if (status != DSA_OK || tokens == 0) return status;
   p.cache = static_cast<unsigned char*>(cache);
   p.cache_sp = strides[8];
   p.cache_sh = strides[9];
@@ -469,17 +473,14 @@ extern "C" int dsa_paged_read_fp4(const void* cache, const int64_t* strides, voi
   if (head_dim <= 0 || head_dim > 128 || head_dim % 8 != 0)
     return dsa::set_error(DSA_EUNSUPPORTED, "%s: head_dim %d (a multiple of 8 up to 128)", who,
                           head_dim);
-  if (bad_page_size(page_size))
-    return dsa::set_error(DSA_EUNSUPPORTED, "%s: page_size %d (a power of two from 16)", who,
-                          page_size);
   if (!list && count > pages)
     return dsa::set_error(DSA_EINVAL, "%s: %d of %d pages", who, count, pages);
+  const int status = check_cache(cache, strides[0], strides[1], pages, page_size, who);
+  if (status != DSA_OK) return status;
   if (count == 0) return DSA_OK;
   if (!k || !v) return dsa::set_error(DSA_EINVAL, "%s: null pointer", who);
   if (!aligned(k, 16) || !aligned(v, 16))
     return dsa::set_error(DSA_EINVAL, "%s: pointers must be 16-byte aligned", who);
-  const int status = check_cache(cache, strides[0], strides[1], pages, who);
-  if (status != DSA_OK) return status;
   ReadParams p;
   p.cache = static_cast<const unsigned char*>(cache);
   p.cache_sp = strides[0];

@@ -1369,3 +1369,9 @@ __global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
 // fp16 instances (seq_attn_f16.hip).
 int seq_launch_f16(const seq::Params& p, bool paged, bool narrow, int max_groups, bool merge,
                    hipStream_t stream, const char* who);
+// Over a cache of 4-bit elements (seq_attn_fp4.hip), with the joins of the 16-bit
+// instances (seq_attn.hip, seq_attn_f16.hip).
+int seq_launch_fp4(const seq::Params& p, int32_t dtype, bool narrow, int max_groups, bool merge,
+                   hipStream_t stream, const char* who);
+void seq_merge_bf16(const seq::Params& p, bool narrow, hipStream_t stream);
+void seq_merge_f16(const seq::Params& p, bool narrow, hipStream_t stream);

@@ -1,6 +1,7 @@
 // Attention of packed sequences and of new tokens over a paged cache: the
 // schedule kernel, the bf16 instances and the C-ABI entry points (seq_attn.h
 // has the kernels).
+#include "fp4.h"
 #include "seq_launch.h"
 
 namespace seq {
@@ -474,9 +475,12 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
 
 constexpr int64_t kMaxItems = (1 << 21) - 1;
 
-// Checks what both entry points share, lays out the workspace and launches.
-int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void* workspace,
+enum Keys { kPacked, kPages, kFp4Pages };
+
+// Checks what the entry points share, lays out the workspace and launches.
+int run(Params p, int32_t dtype, Keys kind, int64_t max_keys, float scale, void* workspace,
         size_t workspace_bytes, hipStream_t stream, const char* who) {
+  const bool paged = kind != kPacked;
   const bool keys = paged ? p.pages > 0 && p.table_width > 0 : p.k_rows > 0;
   if (!p.q || !p.o || !p.q_start || (keys && (!p.k || !p.v)))
     return dsa::set_error(DSA_EINVAL, "%s: null pointer", who);
@@ -530,7 +534,8 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
   auto shares = [](const void* at, int64_t head_stride) {
     return head_stride % 64 != 0 || (reinterpret_cast<uintptr_t>(at) & 127) != 0;
   };
-  p.shared_lines = s.narrow && p.kv_heads > 1 && (shares(p.k, p.k_sh) || shares(p.v, p.v_sh));
+  p.shared_lines = s.narrow && kind != kFp4Pages && p.kv_heads > 1 &&
+                   (shares(p.k, p.k_sh) || shares(p.v, p.v_sh));
   p.max_tiles = (int32_t)s.max_tiles;
   p.max_items = (int32_t)s.max_items;
   p.max_splits = (int32_t)s.max_splits;
@@ -565,6 +570,8 @@ int run(Params p, int32_t dtype, bool paged, int64_t max_keys, float scale, void
       small ? schedule(seq_schedule_kernel<256, false>) : schedule(seq_schedule_kernel<1024, false>);
     }
   }
+  if (kind == kFp4Pages)
+    return seq_launch_fp4(p, dtype, s.narrow, groups, s.merge, stream, who);
   return dtype == DSA_BF16
              ? launch_typed<__bf16>(p, paged, s.narrow, groups, s.merge, stream, who)
              : seq_launch_f16(p, paged, s.narrow, groups, s.merge, stream, who);
@@ -601,7 +608,7 @@ extern "C" int dsa_packed_attention(const void* q, const void* k, const void* v,
   p.q_rows = q_rows; p.k_rows = k_rows; p.requests = requests;
   p.heads = heads; p.kv_heads = kv_heads; p.head_dim = head_dim;
   p.causal = causal; p.fill = fill;
-  return seq::run(p, dtype, false, k_rows, scale, workspace, workspace_bytes, stream,
+  return seq::run(p, dtype, seq::kPacked, k_rows, scale, workspace, workspace_bytes, stream,
                   "dsa_packed_attention");
 }
 
@@ -635,5 +642,45 @@ extern "C" int dsa_paged_attention(const void* q, const void* k_cache, const voi
   p.q_rows = q_rows; p.requests = requests;
   p.heads = heads; p.kv_heads = kv_heads; p.head_dim = head_dim;
   p.causal = causal; p.fill = fill;
-  return seq::run(p, dtype, true, max_keys, scale, workspace, workspace_bytes, stream, who);
+  return seq::run(p, dtype, seq::kPages, max_keys, scale, workspace, workspace_bytes, stream, who);
+}
+
+void seq_merge_bf16(const seq::Params& p, bool narrow, hipStream_t stream) {
+  if (p.head_dim <= 64) seq::launch_merge<__bf16, 64>(p, narrow, stream);
+  else seq::launch_merge<__bf16, 128>(p, narrow, stream);
+}
+
+extern "C" int dsa_paged_attention_fp4(const void* q, const void* cache, void* o, int32_t dtype,
+                                       const int64_t* strides, int32_t q_rows, int32_t requests,
+                                       int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                       int32_t pages, int32_t page_size, const int32_t* table,
+                                       int64_t table_stride, int32_t table_width,
+                                       const int32_t* kv_lens, const int32_t* q_start, float scale,
+                                       int32_t causal, int32_t fill, float* lse, void* workspace,
+                                       size_t workspace_bytes, hipStream_t stream) {
+  const char* const who = "dsa_paged_attention_fp4";
+  if (!strides) return dsa::set_error(DSA_EINVAL, "%s: null strides", who);
+  if (fp4::bad_page_size(page_size))
+    return dsa::set_error(DSA_EUNSUPPORTED, "%s: page_size %d (a power of two, 16 to %d)", who,
+                          page_size, fp4::kMaxPage);
+  if (pages < 0 || table_width < 0 || table_stride < table_width)
+    return dsa::set_error(DSA_EINVAL, "%s: bad table or page count", who);
+  if (requests > 0 && (!kv_lens || (!table && table_width > 0)))
+    return dsa::set_error(DSA_EINVAL, "%s: null block table or lengths", who);
+  if (strides[2] % 16 != 0 || strides[3] % 16 != 0)
+    return dsa::set_error(DSA_EINVAL, "%s: cache strides must be multiples of 16 bytes", who);
+  const int64_t max_keys = (int64_t)table_width * page_size;
+  seq::Params p = {};
+  p.q = q; p.k = cache; p.v = cache; p.o = o; p.lse = lse;
+  p.q_st = strides[0]; p.q_sh = strides[1];
+  p.k_sp = strides[2]; p.k_sh = strides[3];  // bytes
+  p.o_st = strides[4]; p.o_sh = strides[5];
+  p.q_start = q_start; p.kv_lens = kv_lens;
+  p.table = table; p.table_stride = table_stride; p.table_width = table_width;
+  p.pages = pages; p.page_shift = __builtin_ctz(page_size);
+  p.q_rows = q_rows; p.requests = requests;
+  p.heads = heads; p.kv_heads = kv_heads; p.head_dim = head_dim;
+  p.causal = causal; p.fill = fill;
+  return seq::run(p, dtype, seq::kFp4Pages, max_keys, scale, workspace, workspace_bytes, stream,
+                  who);
 }

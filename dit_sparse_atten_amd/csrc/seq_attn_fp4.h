@@ -1,0 +1,810 @@
+// Attention of new tokens over a paged cache of 4-bit elements (fp4.h has its layout),
+// bf16 or fp16 in and out, fp32 softmax: the walks of seq_attn.h, whose schedule, items
+// and joins these kernels share, over keys and values of 32-dim groups with a scale.
+//
+// Scores.  The matrix instructions take a 4-bit key as it lies in memory, with its
+// groups' scales, against 8-bit operands at twice the 16-bit rate.  A query is the exact
+// sum of two (bf16) or three (fp16) E4M3 terms of 4 bits each, 2^4 apart in scale, so
+// that keys are never expanded: S = K (Q_0 + 2^-4 Q_1 + 2^-8 Q_2).  (The queries of a row
+// share one exponent, its largest element's: elements 2^13 below it lose bits that are
+// 2^-21 of it.)
+//
+// Values.  Their scales vary along the keys, which the product with P sums over, so
+// they are expanded to 16 bits (exactly: the conversion takes the scale) on the way into
+// LDS, and O^T = V^T P^T is that of the 16-bit cache.  A group that is not a number
+// enters as zeros, for 0 times it would reach rows that do not see its key, and the rows
+// that do are set to NaN at the end (unfinite_groups).
+#pragma once
+
+#include "fp4.h"
+#include "seq_attn.h"
+
+namespace seq {
+
+typedef int32_t fp4_x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+constexpr int kTerms = sizeof(T) == 2 && __is_same(T, __bf16) ? 2 : 3;
+
+// The larger exponents of a cache written from bf16 would be infinite in fp16, and 0
+// times that NaN in rows that do not see the key.
+template <typename T>
+__device__ __forceinline__ uint32_t value_scale(uint32_t b, bool take) {
+  if (__is_same(T, _Float16)) b = min(b, (uint32_t)(13 + 127));
+  return take ? b : 0u;
+}
+
+// Terms of 16 query elements x, already divided by 2^exponent: E4M3 bytes in order.
+template <typename T, int kCount>
+__device__ __forceinline__ void query_terms(float (&x)[16], int32_t (&term)[kCount][4]) {
+#pragma unroll
+  for (int n = 0; n < kCount; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int32_t w = 0;
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], w, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
+      term[n][i] = w;
+      if (n + 1 < kCount) {
+        x[4 * i + 0] = (x[4 * i + 0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * 16.f;
+        x[4 * i + 1] = (x[4 * i + 1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * 16.f;
+        x[4 * i + 2] = (x[4 * i + 2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * 16.f;
+        x[4 * i + 3] = (x[4 * i + 3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * 16.f;
+      }
+    }
+}
+
+// 16 dims from `d` of a query row, zeros past head_dim.
+template <typename T>
+__device__ __forceinline__ void query_dims(const T* row, int d, int head_dim, float (&x)[16]) {
+  typedef typename dsa::Elem<T>::x8 x8;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (T)0.f;
+    if (d + 8 * c < head_dim) y = *reinterpret_cast<const x8*>(row + d + 8 * c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[8 * c + e] = (float)y[e];
+  }
+}
+
+__device__ __forceinline__ uint32_t top_bits(const float (&x)[16], uint32_t top) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+  return top;
+}
+
+// The exponent that brings a row's largest element (its bits) to [2^7, 2^8): E4M3 ends
+// at 448.  (Rows below 2^-103 keep less.)
+__device__ __forceinline__ int query_exponent(uint32_t top) {
+  return max((int)(top >> 23) - 134, -110);
+}
+// The scale byte of term n; 255 (NaN) for a row that is not finite.
+__device__ __forceinline__ int term_scale(uint32_t top, int exponent, int n) {
+  return top >= 0x7f800000u ? 255 : exponent + 127 - 4 * n;
+}
+
+// A wave's groups of values that are not numbers: bit g of the result where a key of [lo,
+// hi) that the lane's row sees (those below `lim`) has such a group g.
+__device__ __forceinline__ uint32_t unfinite_groups(LateParams p, const Item& it, int h, int lo,
+                                                    int hi, int lim) {
+  const int groups = fp4::groups_of(p->head_dim);
+  const fp4::Layout at(groups, p->page_shift);
+  uint32_t found = 0;
+  for (int key0 = lo; key0 < hi; key0 += 64) {
+    const int key = key0 + (int)(threadIdx.x & 63);
+    uint32_t mine = 0;
+    if (key < hi) {
+      const int page = p->table[(int64_t)it.request * p->table_stride + (key >> p->page_shift)];
+      if ((unsigned)page < (unsigned)p->pages) {
+        const uint32_t four = *reinterpret_cast<const uint32_t*>(
+            static_cast<const unsigned char*>(p->k) + page * p->k_sp + h * p->k_sh + at.v_scales +
+            4 * (key & ((1 << p->page_shift) - 1)));
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (g < groups && (four >> (8 * g) & 255) == 255) mine |= 1u << g;
+      }
+    }
+    uint64_t left = __ballot(mine != 0);
+    while (left != 0) {
+      const int l = (int)__builtin_ctzll(left);
+      left &= left - 1;
+      const uint32_t theirs = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
+      if (key0 + l < lim) found |= theirs;
+    }
+  }
+  return found;
+}
+
+// LDS serves a wave's operations in order; this keeps the compiler from reordering the
+// writes of some lanes and the reads of others.
+__device__ __forceinline__ void own_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// One page and key head of the cache; no bytes, and so zeros, where `any` is false.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const Params& p, uint32_t page, int h,
+                                                           int bytes, bool any) {
+  return make_rsrc(static_cast<const unsigned char*>(p.k) + (uint64_t)page * (uint64_t)p.k_sp +
+                       (uint64_t)h * (uint64_t)p.k_sh,
+                   any ? (uint32_t)bytes : 0u);
+}
+
+// 16 rows x the item's keys: eight waves, 64 keys at a time each (wave w those from 64 w,
+// 64 w + 512, ..), joined at the end.  Bound by the reads of the cache: codes and scales
+// go to registers a turn ahead, 70 KB on their way on a compute unit.  Lane (q4, c16) =
+// (lane / 16, lane % 16) holds group q4 of the keys 16 i + c16, row c16's scores of the
+// keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
+constexpr int kFp4Waves = 8;
+constexpr int kFp4Keys = 64;                          // of a wave's turn
+constexpr int kFp4Turn = kFp4Waves * kFp4Keys;        // of the workgroup's
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Params p) {
+  typedef dsa::Elem<T> E;
+  typedef typename E::x8 x8;
+  constexpr int kRow = kD * 2;
+  constexpr int kStage = 32 * kRow;  // a wave's 32 keys' values, expanded
+  constexpr int kDt = kD / 16;
+  constexpr int kChunks = kD / 8;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v[kFp4Waves * kStage];
+  __shared__ float join_ml[2][kFp4Waves][16];
+  static_assert(kNarrowRows * kD * 4 <= kStage, "a wave joins through its own stage");
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q4 = lane >> 4, c16 = lane & 15;
+  const int groups = fp4::groups_of(p.head_dim);
+  const fp4::Layout at(groups, p.page_shift);
+  const int block_bytes = fp4::row_bytes(groups) << p.page_shift;
+  const uint32_t dead = q4 < groups ? 0u : dsa::kDeadChunk;
+  const uint32_t code_at = (uint32_t)(c16 * at.code_row + q4 * 16) | dead;
+  const uint32_t scale_at = (uint32_t)(c16 * 4 + q4) | dead;
+
+  auto run = [&](const Item& it, const int h) __attribute__((always_inline)) {
+  const int rows = it.n * p.group;
+  const int row_c = min(it.tile * kNarrowRows + c16, rows - 1);
+  const int token = row_c / p.group;
+  const int head = h * p.group + row_c - token * p.group;
+  const int lim = p.causal ? max(0, min(it.m, it.m - it.n + token + 1)) : it.m;
+  const int lim_first = __builtin_amdgcn_readlane(lim, 0);
+  const int kend = min(__builtin_amdgcn_readlane(lim, 15), it.s1 * kNarrowKeys);
+  const int key_first = it.s0 * kNarrowKeys + wave * kFp4Keys;
+
+  // The row's query in its terms: bytes 0..15 of the lane are the dims 16 q4 .., 16..31
+  // the dims 64 + 16 q4 ...
+  fp4_x8 qf[kTerms<T>];
+  int q_scale[kTerms<T>];
+  {
+    const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
+                    head * p.q_sh;
+    float x[2][16];
+    query_dims<T>(qrow, 16 * q4, p.head_dim, x[0]);
+    query_dims<T>(qrow, 64 + 16 * q4, p.head_dim, x[1]);
+    uint32_t top = top_bits(x[1], top_bits(x[0], 0));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const int exponent = query_exponent(top);
+    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[i][e] *= down;
+      int32_t term[kTerms<T>][4];
+      query_terms<T>(x[i], term);
+#pragma unroll
+      for (int n = 0; n < kTerms<T>; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[n][4 * i + j] = term[n][j];
+    }
+#pragma unroll
+    for (int n = 0; n < kTerms<T>; ++n) q_scale[n] = term_scale(top, exponent, n);
+  }
+
+  // Pages of a window of 16 turns: lane l holds granule l & 3 of turn l / 4.
+  auto window_ids = [&](int window) -> int {
+    const int key = key_first + (window * 16 + (lane >> 2)) * kFp4Turn + (lane & 3) * 16;
+    return key < kend ? page_at(p, it.request, key) : -1;
+  };
+  int ids = window_ids(0), ids_next = window_ids(1);
+  uint64_t bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
+
+  struct Turn {
+    dsa_u32x4 k[4], v[4];
+    uint32_t ks[4], vs[4];
+    int bad;  // granules (bits 0..3) that take no part
+  };
+  auto load = [&](int turn, Turn& t) __attribute__((always_inline)) {
+    if ((turn & 15) == 0 && turn > 0) {
+      ids = ids_next;
+      bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
+      ids_next = window_ids((turn >> 4) + 1);
+    }
+    t.bad = (int)(bad_ids >> ((turn & 15) * 4)) & 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = key_first + turn * kFp4Turn + 16 * i;
+      const int row = key & ((1 << p.page_shift) - 1);
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, (turn & 15) * 4 + i);
+      const __amdgpu_buffer_rsrc_t rsrc =
+          fp4_rsrc(p, page, h, block_bytes, page < (uint32_t)p.pages);
+      t.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at, row * at.code_row, 0);
+      t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.k_scales + 4 * row, 0);
+      t.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at,
+                                                     at.v_codes + row * at.code_row, 0);
+      t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.v_scales + 4 * row, 0);
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  dsa_f32x4 oacc[kDt];
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt) oacc[dt] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
+  bool unfinite = false;  // a group of values that is not a number
+  // V chunk c of row r sits at c ^ 2 (r & 7) (256-byte rows) or c ^ 2 ((r / 2) & 3).
+  auto v_swz = [](int r, int c) { return kD == 128 ? c ^ (2 * (r & 7)) : c ^ (2 * ((r >> 1) & 3)); };
+  const int vr_row = 4 * q4 + (c16 >> 2);
+  unsigned char* const stage = lds_v + wave * kStage;
+
+  auto compute = [&](const Turn& t, int key0) __attribute__((always_inline)) {
+    dsa_f32x4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const fp4_x8 a = {(int)t.k[i][0], (int)t.k[i][1], (int)t.k[i][2], (int)t.k[i][3], 0, 0, 0, 0};
+      s[i] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = kTerms<T> - 1; n >= 0; --n)
+        s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[n], s[i], 4, 0, 0,
+                                                                (int)t.ks[i], 0, q_scale[n]);
+    }
+    if (key0 + kFp4Keys > lim_first) {
+      const int bound = min(lim, kend) - key0 - 4 * q4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + r >= bound) s[i][r] = -INFINITY;
+    }
+    if (t.bad != 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t.bad & (1 << i)) s[i][r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[i][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
+    const bool up = mx2 > m_run + kRescaleLog2;
+    if (__any(up)) {
+      const float m_new = up ? mx2 : m_run;
+      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) oacc[dt] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    x8 pf[2];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][r], p.scale_log2, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], p.scale_log2, -m_use));
+        const dsa_f32x2 two = {p0, p1};
+        const typename E::x2 pb = __builtin_convertvector(two, typename E::x2);
+        sum += p0 + p1;
+        pf[i >> 1][4 * (i & 1) + r] = pb[0];
+        pf[i >> 1][4 * (i & 1) + r + 1] = pb[1];
+      }
+    l_run += sum;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int g = 2 * half + i;
+        const bool held = key0 + 16 * g + c16 < kend;
+        const bool number = t.vs[g] != 255u;
+        unfinite |= held && !number;
+        const float scale = fp4::scale_of(value_scale<T>(t.vs[g], held && number));
+        if (kD == 128 || q4 < 2) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<x8*>(stage + (16 * i + c16) * kRow +
+                                   v_swz(c16, 4 * q4 + j) * 16) =
+                fp4::expand(t.v[g][j], scale, T());
+        }
+      }
+      own_lds_order();
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) {
+        const int pos = v_swz(vr_row, 2 * dt + ((c16 & 3) >> 1));
+        const unsigned char* from = stage + vr_row * kRow + pos * 16 + (c16 & 1) * 8;
+        const typename E::x4 lo = read_tr<T>(from);
+        const typename E::x4 hi = read_tr<T>(from + 16 * kRow);
+        const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        oacc[dt] = E::mfma16(a, pf[half], oacc[dt]);
+      }
+      own_lds_order();
+    }
+  };
+  // Two turns' registers in turn: one on its way, one at work.
+  Turn even, odd;
+  if (key_first < kend) {
+    load(0, even);
+#pragma unroll 1
+    for (int turn = 0;; turn += 2) {
+      const int key0 = key_first + turn * kFp4Turn;
+      const bool more = key0 + kFp4Turn < kend;
+      if (more) load(turn + 1, odd);
+      compute(even, key0);
+      if (!more) break;
+      const bool again = key0 + 2 * kFp4Turn < kend;
+      if (again) load(turn + 2, even);
+      compute(odd, key0 + kFp4Turn);
+      if (!again) break;
+    }
+  }
+
+  const LateParams late = late_params();
+  if (__builtin_expect(__any(unfinite), 0)) {
+    // (the wave's own keys alone would do; this is all of the item's)
+    const uint32_t found = unfinite_groups(late, it, h, it.s0 * kNarrowKeys, kend, lim);
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+      if (found >> (dt / 2) & 1) oacc[dt] = dsa_f32x4{NAN, NAN, NAN, NAN};
+  }
+  // Join the waves: their O, m and l through the stages (row-major fp32).
+  l_run += __shfl_xor(l_run, 16);
+  const float l_wave = dsa::pair32_sum(l_run);
+  dsa::lds_barrier();
+  float* const mine = reinterpret_cast<float*>(stage);
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+    *reinterpret_cast<dsa_f32x4*>(mine + c16 * kD + 16 * dt + 4 * q4) = oacc[dt];
+  if (q4 == 0) {
+    join_ml[0][wave][c16] = m_run;
+    join_ml[1][wave][c16] = l_wave;
+  }
+  dsa::lds_barrier();
+  // Thread (r, c): row r, dims 8 c .. 8 c + 7.
+  const int r = tid / kChunks, d0 = tid % kChunks * 8;
+  const int out_row = it.tile * kNarrowRows + r;
+  if (r < kNarrowRows && out_row < rows) {
+    float m_all = -INFINITY, l_all = 0.f, w[kFp4Waves];
+#pragma unroll
+    for (int i = 0; i < kFp4Waves; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
+#pragma unroll
+    for (int i = 0; i < kFp4Waves; ++i) {
+      const float mi = join_ml[0][i][r];
+      // (no finite score: l is 0, or NaN from NaN scores)
+      w[i] = mi == -INFINITY ? join_ml[1][i][r] : __builtin_amdgcn_exp2f(mi - m_all);
+      l_all = fmaf(w[i], join_ml[1][i][r], l_all);
+    }
+    float acc[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFp4Waves; ++i) {
+      if (w[i] == 0.f) continue;
+      const float* src = reinterpret_cast<const float*>(lds_v + i * kStage) + r * kD + d0;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc[x] = fmaf(w[i], src[x], acc[x]);
+    }
+    if (it.slot >= 0) {
+      float* po =
+          late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kNarrowRows, kD);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<dsa_f32x4*>(po + r * kD + d0 + 4 * c) =
+            dsa_f32x4{acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]};
+      if (d0 == 0) {
+        po[kNarrowRows * kD + r] = m_all;
+        po[kNarrowRows * (kD + 1) + r] = l_all;
+      }
+    } else {
+      const int out_token = it.q0 + out_row / late->group;
+      const int out_head = h * late->group + out_row % late->group;
+      const float inv = l_all > 0.f ? 1.f / l_all : (l_all == 0.f ? 0.f : l_all);
+      if (d0 < late->head_dim) {
+        x8 y;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) y[x] = (T)(acc[x] * inv);
+        *reinterpret_cast<x8*>(static_cast<T*>(late->o) + (int64_t)out_token * late->o_st +
+                               out_head * late->o_sh + d0) = y;
+      }
+      if (late->lse && d0 == 0)
+        late->lse[(int64_t)out_head * late->q_rows + out_token] =
+            l_all == 0.f ? -INFINITY : m_all * kLn2 + logf(l_all);
+    }
+  }
+  };
+
+  // An unlisted call gives the workgroup one item, a listed one its chain.
+  Item it;
+  int h;
+  if (p.unlisted) {
+    if (own_item(p, (int)blockIdx.x, &it, &h)) run(it, h);
+    return;
+  }
+  const int chain = (int)blockIdx.x / p.kv_heads;
+  h = (int)blockIdx.x - chain * p.kv_heads;
+  const int count = ((dsa::const_i32)p.counts)[0];
+  int i = ((dsa::const_i32)p.chain_start)[chain];
+  if (i >= count) return;
+  it = load_item(p.items + i);
+#pragma unroll 1
+  for (;;) {
+    run(it, h);
+    if (++i >= count) break;
+    it = load_item(p.items + i);
+    if (it.chain != chain) break;
+    dsa::lds_barrier();  // the join's reads are done
+  }
+}
+
+// 128 rows x the item's keys, bound by the matrix instructions: four waves of 32 rows,
+// 64 keys a step, as seq_wide_kernel walks a 16-bit cache.  Keys' codes go to LDS as they
+// are (a quarter of the bytes, and of the reads by every wave); values are expanded there
+// by the thread that loaded them, a step ahead.  Lane (g, qi) = (lane / 32, lane % 32)
+// holds row qi's scores of the keys 32 kt + 8 (r / 4) + 4 g + r % 4 and, of O, the dims
+// 32 dt + 8 (r / 4) + 4 g + r % 4.
+template <typename T, int kD, int kUse>
+__global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
+  typedef dsa::Elem<T> E;
+  typedef typename E::x8 x8;
+  constexpr int kRow = kD * 2;               // bytes of an expanded row
+  constexpr int kStage = kWideKeys * kRow;
+  constexpr int kCodeRow = kD / 2;           // of a row of codes
+  constexpr int kSteps = kD / 64;            // products of 64 dims
+  constexpr int kDt = kUse / 32;
+  constexpr int kChunks = kD / 8;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k[2][4096];  // 1 KB a wave
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_s[2][1024];  // scales, by wave
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v[2][kStage];
+
+  Item it;
+  int h;
+  if (!take_item(p, &it, &h)) return;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 5, qi = lane & 31;
+  const int rows = it.n * p.group;
+  const int local = wave * 32 + qi;
+  const int row = it.tile * kWideRows + local;
+  const bool row_ok = row < rows;
+  const int row_c = min(row, rows - 1);
+  const int token = row_c / p.group;
+  const int head = h * p.group + row_c - token * p.group;
+  // Keys [0, lim) are visible to the lane's row.
+  const int lim = p.causal ? max(0, min(it.m, it.m - it.n + token + 1)) : it.m;
+  const bool wave_active = it.tile * kWideRows + wave * 32 < rows;
+  const int lim_first = __builtin_amdgcn_readlane(lim, 0);
+  const int lim_last = __builtin_amdgcn_readlane(lim, 31);
+  // Keys the tile's last row sees.
+  const int last_row = min(it.tile * kWideRows + kWideRows, rows) - 1;
+  const int kend =
+      p.causal ? max(0, min(it.m, it.m - it.n + last_row / p.group + 1)) : it.m;
+  const int groups = fp4::groups_of(p.head_dim);
+  const fp4::Layout at(groups, p.page_shift);
+  const int block_bytes = fp4::row_bytes(groups) << p.page_shift;
+
+  // The row's query in its terms, for products of 64 dims: bytes 0..15 of the lane are
+  // the dims 64 j + 16 g .., 16..31 the dims 64 j + 32 + 16 g ...
+  fp4_x8 qf[kSteps][kTerms<T>];
+  int q_scale[kTerms<T>];
+  {
+    const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
+                    head * p.q_sh;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 2 * kSteps; ++j) {
+      float x[16];
+      query_dims<T>(qrow, 32 * j + 16 * g, p.head_dim, x);
+      top = top_bits(x, top);
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const int exponent = query_exponent(top);
+    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+#pragma unroll
+    for (int j = 0; j < 2 * kSteps; ++j) {
+      float x[16];
+      query_dims<T>(qrow, 32 * j + 16 * g, p.head_dim, x);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] *= down;
+      int32_t term[kTerms<T>][4];
+      query_terms<T>(x, term);
+#pragma unroll
+      for (int n = 0; n < kTerms<T>; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[j >> 1][n][4 * (j & 1) + i] = term[n][i];
+    }
+#pragma unroll
+    for (int n = 0; n < kTerms<T>; ++n) q_scale[n] = term_scale(top, exponent, n);
+  }
+
+  // Wave w stages the keys 16 w .. 16 w + 15 of a step, one page: lane (r, c) = (lane / 4,
+  // lane % 4) row r's chunk c, 16 bytes of codes (of 32-byte rows of keys: the lower 32
+  // lanes, (lane / 2, lane % 2)).  K chunk c of row r sits at c ^ (r / 4 & 3) or c ^ (r / 8
+  // & 1).
+  auto k_swz = [](int r, int c) { return kD == 128 ? c ^ (r >> 2 & 3) : c ^ (r >> 3 & 1); };
+  constexpr int kLanes = kD / 32;  // chunks of a row
+  const int k_row = lane / kLanes, k_chunk = k_swz(k_row, lane % kLanes);
+  const uint32_t code_at = k_row < 16 && k_chunk < groups
+                               ? (uint32_t)(k_row * at.code_row + k_chunk * 16) : dsa::kDeadChunk;
+  const int v_row = lane >> 2, v_group = lane & 3;
+  const uint32_t value_at =
+      v_group < groups ? (uint32_t)(v_row * at.code_row + v_group * 16) : dsa::kDeadChunk;
+  const uint32_t value_scale_at = v_group < groups ? (uint32_t)(v_row * 4 + v_group)
+                                                   : dsa::kDeadChunk;
+  const uint32_t scale_at = lane < 16 ? (uint32_t)(lane * 4) : dsa::kDeadChunk;
+  auto v_swz = [](int r, int c) {
+    return kD == 128 ? c ^ ((0xCA60 >> (4 * (r & 3))) & 15) : c ^ (4 * ((r >> 1) & 1));
+  };
+  int vfrag[kDt];
+  {
+    const int lam = lane & 15, r = lam >> 2, c = lam & 3;
+    const int vrow = 4 * g + r;
+    const int sub = 2 * ((lane >> 4) & 1) + (c >> 1);
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+      vfrag[dt] = vrow * kRow + v_swz(vrow, 4 * dt + sub) * 16 + (c & 1) * 8;
+  }
+
+  // Pages of a 1,024-key window, one 16-key granule per lane; the next window's are
+  // loaded a window ahead.
+  auto window_ids = [&](int window) -> int {
+    const int key = window * 1024 + lane * 16;
+    return key < kend ? page_at(p, it.request, key) : -1;
+  };
+  int ids = window_ids(it.s0 >> 4), ids_next = window_ids((it.s0 >> 4) + 1);
+  uint64_t bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
+  if ((it.s0 & 15) == 0) ids_next = ids;  // locate() takes it up
+  // Where step s of this wave's keys lies: its page, its first row in there.
+  __amdgpu_buffer_rsrc_t rsrc;
+  int at_row = 0, bad_next = 0;
+  auto locate = [&](int s) __attribute__((always_inline)) {
+    if ((s & 15) == 0) {  // the next window (step s0's is there already)
+      ids = ids_next;
+      bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
+      ids_next = window_ids((s >> 4) + 1);
+    }
+    const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, (s & 15) * 4 + wave);
+    bad_next = (int)(bad_ids >> ((s & 15) * 4)) & 15;
+    at_row = (s * kWideKeys + wave * 16) & ((1 << p.page_shift) - 1);
+    rsrc = fp4_rsrc(p, page, h, block_bytes, page < (uint32_t)p.pages);
+  };
+  dsa_u32x4 v_codes;
+  uint32_t v_scale = 0;
+  auto issue = [&](int to) __attribute__((always_inline)) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rsrc, (DSA_LDS void*)(lds_k[to] + wave * 1024), 16, code_at, at_row * at.code_row, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (DSA_LDS void*)(lds_s[to] + wave * 256), 4,
+                                             scale_at, at.k_scales + 4 * at_row, 0, 0);
+    v_codes = __builtin_amdgcn_raw_buffer_load_b128(rsrc, value_at,
+                                                    at.v_codes + at_row * at.code_row, 0);
+    v_scale = __builtin_amdgcn_raw_buffer_load_b8(rsrc, value_scale_at,
+                                                  at.v_scales + 4 * at_row, 0);
+  };
+  bool unfinite = false;  // a group of values that is not a number
+  // The values of step s, on their way since issue(), into their stage.
+  auto expand = [&](int s, int to) __attribute__((always_inline)) {
+    const bool held = s * kWideKeys + wave * 16 + v_row < kend;
+    const bool number = v_scale != 255u;
+    unfinite |= held && !number;
+    const float scale = fp4::scale_of(value_scale<T>(v_scale, held && number));
+    const int r = wave * 16 + v_row;
+    if (kD == 128 || v_group < 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<x8*>(lds_v[to] + r * kRow + v_swz(r, 4 * v_group + j) * 16) =
+            fp4::expand(v_codes[j], scale, T());
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  dsa_f32x16 oacc[kDt];
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
+
+  auto compute = [&](int from, int key0, int bad) __attribute__((always_inline)) {
+    const unsigned char* const k_lds = lds_k[from];
+    const unsigned char* const v_lds = lds_v[from];
+    __builtin_amdgcn_s_setprio(0);
+    dsa_f32x16 sacc[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sacc[kt][r] = 0.f;
+      const int krow = kt * 32 + qi;
+      // Group g of a product's two, at the dword's bytes 0 and 2.
+      const uint32_t four = *reinterpret_cast<const uint32_t*>(
+          lds_s[from] + (krow >> 4) * 256 + (krow & 15) * 4) >> (8 * g);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const dsa_u32x4 c = *reinterpret_cast<const dsa_u32x4*>(
+            k_lds + (krow >> 4) * 1024 + (krow & 15) * kCodeRow + k_swz(krow & 15, 2 * j + g) * 16);
+        const fp4_x8 a = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+        // (bytes of groups that a row has not: codes of zeros, scales of no NaN)
+        const int ks = 2 * j + g < groups ? (int)four : 0;
+#pragma unroll
+        for (int n = kTerms<T> - 1; n >= 0; --n) {
+          if (j == 0)
+            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, qf[j][n], sacc[kt], 4, 0,
+                                                                       0, ks, 0, q_scale[n]);
+          else
+            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, qf[j][n], sacc[kt], 4, 0,
+                                                                       2, ks, 0, q_scale[n]);
+        }
+      }
+    }
+    if (key0 + kWideKeys > lim_first) {
+      const int bound = lim - key0 - 4 * g;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (kt * 32 + 8 * (r >> 2) + (r & 3) >= bound) sacc[kt][r] = -INFINITY;
+    }
+    if (bad != 0) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (bad & (1 << (2 * kt + (r >> 3)))) sacc[kt][r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kt][r]);
+    const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
+    const bool up = mx2 > m_run + kRescaleLog2;
+    if (__any(up)) {
+      const float m_new = up ? mx2 : m_run;
+      const float alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    x8 pf[4];
+    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int t = 0; t < 8; t += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(
+            fmaf(sacc[j >> 1][(j & 1) * 8 + t], p.scale_log2, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(
+            fmaf(sacc[j >> 1][(j & 1) * 8 + t + 1], p.scale_log2, -m_use));
+        const dsa_f32x2 two = {p0, p1};
+        const typename E::x2 pb = __builtin_convertvector(two, typename E::x2);
+        sum0 += p0;
+        sum1 += p1;
+        pf[j][t] = pb[0];
+        pf[j][t + 1] = pb[1];
+      }
+    l_run += sum0 + sum1;
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) {
+        // Key rows 16 j + 4 g + r (slots 0..3) and 16 j + 8 + 4 g + r (4..7).
+        const unsigned char* from_v = v_lds + vfrag[dt] + j * 16 * kRow;
+        const typename E::x4 lo = read_tr<T>(from_v);
+        const typename E::x4 hi = read_tr<T>(from_v + 8 * kRow);
+        const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        oacc[dt] = E::mfma32(a, pf[j], oacc[dt]);
+      }
+    // Four products' V reads (two each) ahead.
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+    for (int i = 0; i < 4 * kDt - 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
+  };
+  // A step: its keys' codes are in their stage once the loads are done, its values once
+  // they are expanded; then the next step's loads go out and its products run.
+  int bad_cur = 0;
+  auto step = [&](int s, int stage) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(vmcnt(0));
+    expand(s, stage);
+    bad_cur = bad_next;
+    dsa::lds_barrier();
+    if (s + 1 < it.s1) {
+      locate(s + 1);
+      issue(stage ^ 1);
+    }
+    // (a wave whose rows see none of the step's keys only stages)
+    if (wave_active && s * kWideKeys < lim_last) compute(stage, s * kWideKeys, bad_cur);
+  };
+  if (it.s0 < it.s1) {
+    locate(it.s0);
+    issue(0);
+    for (int s = it.s0; s < it.s1; s += 2) {
+      step(s, 0);
+      if (s + 1 >= it.s1) break;
+      step(s + 1, 1);
+    }
+  }
+
+  const LateParams late = late_params();
+  const float l_tot = dsa::pair32_sum(l_run);
+  if (__syncthreads_or(unfinite)) {
+    const uint32_t found = unfinite_groups(late, it, h, it.s0 * kWideKeys,
+                                           min(it.s1 * kWideKeys, kend), lim);
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (found >> dt & 1) oacc[dt][r] = NAN;
+  }
+  if (it.slot >= 0) {
+    // A partial keeps the accumulators' own order (part_at): whole lines per store.
+    float* const po =
+        late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kWideRows, kD);
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) {
+        const dsa_f32x4 v4 = {oacc[dt][rr * 4 + 0], oacc[dt][rr * 4 + 1],
+                              oacc[dt][rr * 4 + 2], oacc[dt][rr * 4 + 3]};
+        *reinterpret_cast<dsa_f32x4*>(po +
+                                      part_at<kD, kWideRows>(local, dt * 32 + rr * 8 + g * 4)) = v4;
+      }
+    if (g == 0) {
+      po[kWideRows * kD + local] = m_run;
+      po[kWideRows * (kD + 1) + local] = l_tot;
+    }
+    return;
+  }
+  if (late->lse && g == 0 && row_ok)
+    late->lse[(int64_t)head * late->q_rows + it.q0 + token] =
+        l_tot == 0.f ? -INFINITY : m_run * kLn2 + logf(l_tot);
+  // O goes out through the value stages (every wave is past its reads of them: the
+  // barrier of __syncthreads_or), row by row as 16-byte chunks, whole rows to a store.
+  const float inv = l_tot > 0.f ? 1.f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
+  unsigned char* const mine = lds_v[0] + wave * 32 * kRow;
+  auto o_swz = [](int r, int c) { return kD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7); };
+#pragma unroll
+  for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+      typename E::x4 v4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v4[e] = (T)(oacc[dt][rr * 4 + e] * inv);
+      *reinterpret_cast<typename E::x4*>(mine + qi * kRow + o_swz(qi, dt * 4 + rr) * 16 + g * 8) =
+          v4;
+    }
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_wave_barrier();
+  const int64_t o_at = row_ok ? (int64_t)(it.q0 + token) * late->o_st + head * late->o_sh : -1;
+  constexpr int kRowsPer = 64 / kChunks;
+#pragma unroll
+  for (int i = 0; i < kD / 16; ++i) {
+    const int r = i * kRowsPer + lane / kChunks, c = lane % kChunks;
+    const x8 y = *reinterpret_cast<const x8*>(mine + r * kRow + o_swz(r, c) * 16);
+    const int64_t o_row = __shfl(o_at, r);
+    if (o_row >= 0 && c * 8 < late->head_dim)
+      *reinterpret_cast<x8*>(static_cast<T*>(late->o) + o_row + c * 8) = y;
+  }
+}
+
+}  // namespace seq

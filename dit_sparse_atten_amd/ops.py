@@ -1218,6 +1218,22 @@ def _sequence_workspace_bytes(q_rows, requests, heads, kv_heads, head_dim, max_k
                                                          head_dim, max_keys)
 
 
+def _out_strides(q, out):
+    """Strides of an attention's output, new (None) or given."""
+    (rows, heads, head_dim), dtype = q[0], q[2]
+    if out is None:
+        return [heads * head_dim, head_dim]
+    if out[0] != q[0] or out[2] != dtype:
+        raise ValueError("out must have q's shape, type and device")
+    _apart("out", out)
+    strides = _row_strides(*out[:2], dtype.itemsize)
+    if strides is None:
+        if rows:
+            raise ValueError("out must have a contiguous, 16-byte aligned head dimension")
+        strides = [0, 0]
+    return strides
+
+
 @functools.lru_cache(maxsize=512)
 def _attention_layout(paged, q, k, v, out):
     """(operands to copy first, strides, rows, heads, kv_heads, head_dim, dtype code) of a call."""
@@ -1241,17 +1257,7 @@ def _attention_layout(paged, q, k, v, out):
         raise ValueError(f"{heads} query heads do not share {kv_heads} key/value heads")
     if head_dim % 8 or not 8 <= head_dim <= HEAD_DIM:
         raise ValueError(f"head_dim {head_dim} unsupported (a multiple of 8 up to {HEAD_DIM})")
-    if out is None:
-        o_strides = [heads * head_dim, head_dim]
-    else:
-        if out[0] != q[0] or out[2] != dtype:
-            raise ValueError("out must have q's shape, type and device")
-        _apart("out", out)
-        o_strides = _row_strides(*out[:2], dtype.itemsize)
-        if o_strides is None:
-            if rows:
-                raise ValueError("out must have a contiguous, 16-byte aligned head dimension")
-            o_strides = [0, 0]
+    o_strides = _out_strides(q, out)
     every = [q_strides, *keys, o_strides]
     copies = tuple(i for i, x in enumerate(every) if x is None)
     strides = None if copies else (_I64x10 if paged else _I64x8)(*[x for t in every for x in t])
@@ -1390,6 +1396,12 @@ def _fp4_row(head_dim):
     return 32 * -(-head_dim // 32) + 8
 
 
+def _fp4_page_size(value):
+    _page_size(value)
+    if value > 1 << 20:
+        raise ValueError(f"page_size {value} unsupported for a 4-bit cache (up to 2^20)")
+
+
 def paged_cache_fp4(pages, page_size, kv_heads, head_dim, device="cuda"):
     """An empty paged cache of 4-bit keys and values: uint8 [pages, kv_heads, page_size,
     32 * G + 8] with G = ceil(head_dim / 32): 4.25 bits an element at 128 dims.
@@ -1401,7 +1413,7 @@ def paged_cache_fp4(pages, page_size, kv_heads, head_dim, device="cuda"):
     2^(b - 127), 255 for a group that held an infinity or a NaN (and reads as NaN).
     Pages and heads may be any slices of a larger cache that are multiples of 16 bytes
     apart."""
-    _page_size(page_size)
+    _fp4_page_size(page_size)
     if pages < 0 or kv_heads < 1:
         raise ValueError(f"a cache of {pages} pages of {kv_heads} key/value heads")
     return torch.zeros((pages, kv_heads, page_size, _fp4_row(head_dim)), dtype=torch.uint8,
@@ -1417,7 +1429,7 @@ def _fp4_strides(layout, kv_heads, head_dim):
                          f"{head_dim}-dim heads")
     if kv_heads is not None and shape[1] != kv_heads:
         raise ValueError(f"cache holds {shape[1]} key/value heads, not {kv_heads}")
-    _page_size(shape[2])
+    _fp4_page_size(shape[2])
     if strides[3] != 1 or strides[2] != row:
         raise ValueError("a page and head of the cache must be contiguous")
     lead = [0 if size == 1 else stride for size, stride in zip(shape[:2], strides[:2])]
@@ -1625,3 +1637,61 @@ def paged_read_fp4(cache, head_dim, pages=None, dtype=torch.bfloat16):
               k.data_ptr(), v.data_ptr(), code, total, page_size, kv_heads, head_dim,
               None if pages is None else pages.data_ptr(), count)
     return k, v
+
+
+@functools.lru_cache(maxsize=512)
+def _fp4_attention_layout(q, cache, out):
+    """As ``_attention_layout`` over a 4-bit cache."""
+    dtype = q[2]
+    code = dtype_code(dtype)
+    q_strides = _sequence_strides("q", q, dtype)
+    rows, heads, head_dim = q[0]
+    held = _fp4_strides(cache, None, head_dim)
+    kv_heads = cache[0][1]
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key/value heads")
+    o_strides = _out_strides(q, out)
+    copies = () if q_strides is not None else (0,)
+    strides = None if copies else _I64x6(*q_strides, *held, *o_strides)
+    return copies, strides, rows, heads, kv_heads, head_dim, code
+
+
+def paged_attention_fp4(q, cache, block_table, kv_lens, q_start, causal=True, scale=None, out=None,
+                        return_lse=False):
+    """``paged_attention`` over a cache of 4-bit elements (``paged_cache_fp4``).
+
+    The keys and values are those that the cache stands for (``paged_read_fp4``), read
+    in place: a decoding step reads 27% of a 16-bit cache's bytes.  q's type is the one
+    that the cache was written from.  Everything else, and what is returned, as in
+    ``paged_attention``.  A group of 32 dims that is not a number (``paged_write_fp4``)
+    makes the rows that see its key NaN, one of values those dims of them.
+    """
+    lib = _lib.load()
+    _require_cuda("q", q)
+    _require_cuda("cache", cache)
+    fill = out is None
+    if not fill:
+        _require_cuda("out", out)
+    layout = _fp4_attention_layout(_layout(q), _layout(cache), None if fill else _layout(out))
+    copies, strides, rows, heads, kv_heads, head_dim, code = layout
+    device = q.device
+    if cache.device != device:
+        raise ValueError("q and the cache must be on the same device")
+    _fp4_aligned(cache)
+    pages, _, page_size, _ = cache.shape
+    kv_lens = _index_vector("kv_lens", kv_lens, device)
+    requests = kv_lens.shape[0]
+    table, table_stride, width = _block_table(block_table, device, requests)
+    q_start = _index_vector("q_start", q_start, device, requests + 1)
+    if copies or q.data_ptr() & 15:
+        return paged_attention_fp4(*_in_place(copies, q), cache, block_table, kv_lens, q_start,
+                                   causal, scale, out, return_lse)
+    scale, out, lse, workspace = _sequence_buffers(q, layout, q_start, scale, out, return_lse,
+                                                   width * page_size)
+    if rows:
+        _call(lib.dsa_paged_attention_fp4, "dsa_paged_attention_fp4", device, q.data_ptr(),
+              cache.data_ptr(), out.data_ptr(), code, strides, rows, requests, heads, kv_heads,
+              head_dim, pages, page_size, table, table_stride, width, kv_lens.data_ptr(),
+              q_start.data_ptr(), scale, 1 if causal else 0, 1 if fill else 0,
+              None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.shape[0])
+    return (out, lse) if return_lse else out

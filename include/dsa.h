@@ -575,6 +575,22 @@ size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32
                                          int32_t kv_heads, int32_t head_dim, int64_t max_keys);
 
 /*
+ * dsa_paged_attention over a cache of 4-bit elements (below): keys and values are what
+ * its codes and scales stand for, q's type the one that the cache was written from (in
+ * fp16 values of exponents above 13 count as of 13).  strides[6]: q (token, head) in
+ * elements, cache (page, head) in BYTES, o (token, head) in elements; page_size up to
+ * 2^20.  A key group that is not a number makes the rows that see it NaN, a value
+ * group its dims of them.  All else, the workspace among it, as there.
+ */
+int dsa_paged_attention_fp4(const void* q, const void* cache, void* o, int32_t dtype,
+                            const int64_t* strides, int32_t q_rows, int32_t requests,
+                            int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t pages,
+                            int32_t page_size, const int32_t* table, int64_t table_stride,
+                            int32_t table_width, const int32_t* kv_lens, const int32_t* q_start,
+                            float scale, int32_t causal, int32_t fill, float* lse,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Writes into a paged cache that turn keys and queries with their positions on the
  * way, bf16 or fp16 (the reference turns whole tensors of one length before its
  * attention).  With (c_i, s_i) = cos_sin[positions[t]][i] (fp32 [max_positions,
@@ -594,8 +610,8 @@ size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32
  * dsa_paged_write_fp4: into a cache of 4-bit elements; strides[10]: q, q_out, k, v
  *   (token, head) in elements, cache (page, head) in BYTES, multiples of 16.
  *
- * A 4-bit cache holds keys and values of one page and key head in page_size *
- * (32 G + 8) bytes, G = ceil(head_dim / 32): the keys' codes [page_size, 16 G], the
+ * A 4-bit cache (page_size up to 2^20) holds keys and values of one page and key head
+ * in page_size * (32 G + 8) bytes, G = ceil(head_dim / 32): the keys' codes [page_size, 16 G], the
  * values' codes [page_size, 16 G], the keys' scales [page_size, 4] and the values'
  * scales [page_size, 4].  32 neighbouring dims share a scale byte b, for 2^(b - 127);
  * 255: the group held an infinity or a NaN, and each of its elements is NaN.  Element

@@ -197,6 +197,18 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   return v;
 }
 
+// Largest of the 64 lanes' values, for every lane (the same steps).  Every lane of the
+// wave must be active.
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 struct Sequence {
   int32_t q0, n, k0, m;
 };
@@ -301,21 +313,23 @@ __device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int
   const int base = (int)wave_scan((uint32_t)tiles) - tiles;
   // (starts that overlap list more tiles than fit)
   const int count = min(__builtin_amdgcn_readlane(base + tiles, 63), p.max_tiles);
-  // Lane i: tile i of sequence r, the last that starts at or before it.
-  // (at most 64 sequences: six bisection steps)
-  int r = 0;
+  // Lane i: tile i of sequence r, the last that starts at or before it: its own where
+  // every sequence has one tile (a decoding step), else by bisection (at most 64
+  // sequences: six steps).
+  int r = lane, tile = 0;
+  Sequence t = s;
+  if (!__all(lane >= p.requests || tiles == 1)) {
+    r = 0;
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const int at = __shfl(base, r + d);
-    if (r + d < p.requests && at <= lane) r += d;
+    for (int d = 32; d > 0; d >>= 1) {
+      const int at = __shfl(base, r + d);
+      if (r + d < p.requests && at <= lane) r += d;
+    }
+    t.q0 = __shfl(s.q0, r); t.n = __shfl(s.n, r); t.k0 = __shfl(s.k0, r); t.m = __shfl(s.m, r);
+    tile = lane - __shfl(base, r);
   }
-  Sequence t;
-  t.q0 = __shfl(s.q0, r); t.n = __shfl(s.n, r); t.k0 = __shfl(s.k0, r); t.m = __shfl(s.m, r);
-  const int tile = lane - __shfl(base, r);
   const int steps = lane < count ? steps_of(p, t, tile) : 0;
-  int longest = steps;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) longest = max(longest, __shfl_xor(longest, d));
+  const int longest = wave_max(steps);
   int chunk = max(longest, 1);
   if (p.max_slots > 0 && longest >= 2 * p.min_chunk) {
     const int parts = lane < 32 ? lane + 1 : 32 + (lane - 31) * 8;
@@ -327,17 +341,10 @@ __device__ __forceinline__ bool own_item(const Params& p, int wg, Item* out, int
     float price = (float)mine + (lane > 0 ? p.part_cost + p.merge_cost * (float)(items * p.kv_heads)
                                           : 0.f);
     if (lane > 0 && (items * p.kv_heads > p.slots || items > p.max_slots)) price = INFINITY;
-    int best = lane;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const float other = __shfl_xor(price, d);
-      const int its = __shfl_xor(best, d);
-      if (other < price || (other == price && its < best)) {
-        price = other;
-        best = its;
-      }
-    }
-    chunk = __shfl(mine, best);
+    // (the first of the cheapest; prices are positive floats, whose bits order as they do)
+    const int least = -wave_max(-__float_as_int(price));
+    const int best = (int)__builtin_ctzll(__ballot(__float_as_int(price) == least));
+    chunk = __builtin_amdgcn_readlane(mine, best);
   }
   int parts = lane < count ? max(1, (steps + chunk - 1) / chunk) : 0;
   uint32_t split = parts > 1 ? (uint32_t)parts << 16 | 1u : 0u;

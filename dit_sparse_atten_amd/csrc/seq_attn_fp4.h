@@ -56,18 +56,22 @@ __device__ __forceinline__ void query_terms(float (&x)[16], int32_t (&term)[kCou
 
 // 16 dims from `d` of a query row, zeros past head_dim.
 template <typename T>
-__device__ __forceinline__ void query_dims(const T* row, int d, int head_dim, float (&x)[16]) {
-  typedef typename dsa::Elem<T>::x8 x8;
+struct QueryDims {
+  typename dsa::Elem<T>::x8 y[2];
+  __device__ __forceinline__ void load(const T* row, int d, int head_dim) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    x8 y;
+    for (int c = 0; c < 2; ++c) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (T)0.f;
-    if (d + 8 * c < head_dim) y = *reinterpret_cast<const x8*>(row + d + 8 * c);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[8 * c + e] = (float)y[e];
+      for (int e = 0; e < 8; ++e) y[c][e] = (T)0.f;
+      if (d + 8 * c < head_dim)
+        y[c] = *reinterpret_cast<const typename dsa::Elem<T>::x8*>(row + d + 8 * c);
+    }
   }
-}
+  __device__ __forceinline__ void widen(float (&x)[16]) const {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = (float)y[e / 8][e % 8];
+  }
+};
 
 __device__ __forceinline__ uint32_t top_bits(const float (&x)[16], uint32_t top) {
 #pragma unroll
@@ -145,12 +149,12 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
   typedef dsa::Elem<T> E;
   typedef typename E::x8 x8;
   constexpr int kRow = kD * 2;
-  constexpr int kStage = 32 * kRow;  // a wave's 32 keys' values, expanded
+  constexpr int kStage = kFp4Keys * kRow;  // a wave's values of a turn, expanded
   constexpr int kDt = kD / 16;
-  constexpr int kChunks = kD / 8;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v[kFp4Waves * kStage];
   __shared__ float join_ml[2][kFp4Waves][16];
-  static_assert(kNarrowRows * kD * 4 <= kStage, "a wave joins through its own stage");
+  constexpr int kJoinRow = kD + 4;  // floats
+  static_assert(kNarrowRows * kJoinRow * 4 <= kStage, "a wave joins through its own stage");
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -172,34 +176,12 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
   const int kend = min(__builtin_amdgcn_readlane(lim, 15), it.s1 * kNarrowKeys);
   const int key_first = it.s0 * kNarrowKeys + wave * kFp4Keys;
 
-  // The row's query in its terms: bytes 0..15 of the lane are the dims 16 q4 .., 16..31
-  // the dims 64 + 16 q4 ...
-  fp4_x8 qf[kTerms<T>];
-  int q_scale[kTerms<T>];
+  QueryDims<T> raw[2];
   {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
-    float x[2][16];
-    query_dims<T>(qrow, 16 * q4, p.head_dim, x[0]);
-    query_dims<T>(qrow, 64 + 16 * q4, p.head_dim, x[1]);
-    uint32_t top = top_bits(x[1], top_bits(x[0], 0));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    const int exponent = query_exponent(top);
-    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[i][e] *= down;
-      int32_t term[kTerms<T>][4];
-      query_terms<T>(x[i], term);
-#pragma unroll
-      for (int n = 0; n < kTerms<T>; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) qf[n][4 * i + j] = term[n][j];
-    }
-#pragma unroll
-    for (int n = 0; n < kTerms<T>; ++n) q_scale[n] = term_scale(top, exponent, n);
+    raw[0].load(qrow, 16 * q4, p.head_dim);
+    raw[1].load(qrow, 64 + 16 * q4, p.head_dim);
   }
 
   // Pages of a window of 16 turns: lane l holds granule l & 3 of turn l / 4.
@@ -229,21 +211,57 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
       const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, (turn & 15) * 4 + i);
       const __amdgpu_buffer_rsrc_t rsrc =
           fp4_rsrc(p, page, h, block_bytes, page < (uint32_t)p.pages);
-      t.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at, row * at.code_row, 0);
-      t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.k_scales + 4 * row, 0);
+      t.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at, row * at.code_row, 2);
+      t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.k_scales + 4 * row, 2);
       t.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at,
-                                                     at.v_codes + row * at.code_row, 0);
-      t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.v_scales + 4 * row, 0);
+                                                     at.v_codes + row * at.code_row, 2);
+      t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.v_scales + 4 * row, 2);
     }
   };
+
+  // Two turns' registers in turn: one on its way, one at work.  (Loads past the last key
+  // have no bytes.  They go out all the same: the wait for a turn counts those behind it,
+  // and where some paths have none it would wait for them too.)
+  Turn even, odd;
+  load(0, even);
+  __builtin_amdgcn_sched_barrier(0);
+  // The row's query in its terms: bytes 0..15 of the lane are the dims 16 q4 .., 16..31
+  // the dims 64 + 16 q4 ...
+  fp4_x8 qf[kTerms<T>];
+  int q_scale[kTerms<T>];
+  {
+    float x[2][16];
+    raw[0].widen(x[0]);
+    raw[1].widen(x[1]);
+    uint32_t top = top_bits(x[1], top_bits(x[0], 0));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    const int exponent = query_exponent(top);
+    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[i][e] *= down;
+      int32_t term[kTerms<T>][4];
+      query_terms<T>(x[i], term);
+#pragma unroll
+      for (int n = 0; n < kTerms<T>; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[n][4 * i + j] = term[n][j];
+    }
+#pragma unroll
+    for (int n = 0; n < kTerms<T>; ++n) q_scale[n] = term_scale(top, exponent, n);
+  }
 
   float m_run = -INFINITY, l_run = 0.f;
   dsa_f32x4 oacc[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) oacc[dt] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
   bool unfinite = false;  // a group of values that is not a number
-  // V chunk c of row r sits at c ^ 2 (r & 7) (256-byte rows) or c ^ 2 ((r / 2) & 3).
-  auto v_swz = [](int r, int c) { return kD == 128 ? c ^ (2 * (r & 7)) : c ^ (2 * ((r >> 1) & 3)); };
+  // V chunk c of row r sits at c ^ (2 (r & 3) + (r / 4 & 1)): eight rows of a chunk, as
+  // eight lanes write them, and four rows of two chunks, as 16 lanes read them, lie in
+  // distinct banks.
+  auto v_swz = [](int r, int c) { return c ^ (2 * (r & 3) + (r >> 2 & 1)); };
   const int vr_row = 4 * q4 + (c16 >> 2);
   unsigned char* const stage = lds_v + wave * kStage;
 
@@ -258,6 +276,21 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
         s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[n], s[i], 4, 0, 0,
                                                                 (int)t.ks[i], 0, q_scale[n]);
     }
+    // (the values' way into LDS covers the products' latency)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool held = key0 + 16 * i + c16 < kend;
+      const bool number = t.vs[i] != 255u;
+      unfinite |= held && !number;
+      const float scale = fp4::scale_of(value_scale<T>(t.vs[i], held && number));
+      if (kD == 128 || q4 < 2) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<x8*>(stage + (16 * i + c16) * kRow + v_swz(c16, 4 * q4 + j) * 16) =
+              fp4::expand(t.v[i][j], scale, T());
+      }
+    }
+    own_lds_order();
     if (key0 + kFp4Keys > lim_first) {
       const int bound = min(lim, kend) - key0 - 4 * q4;
 #pragma unroll
@@ -278,10 +311,12 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[i][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
-    const bool up = mx2 > m_run + kRescaleLog2;
-    if (__any(up)) {
+    // The reference moves only where a lane's own scores call for it: the row's largest is
+    // not needed before.
+    if (__any(mx * p.scale_log2 > m_run + kRescaleLog2)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
+      const bool up = mx2 > m_run + kRescaleLog2;
       const float m_new = up ? mx2 : m_run;
       const float alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
       m_run = m_new;
@@ -306,50 +341,31 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
       }
     l_run += sum;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int g = 2 * half + i;
-        const bool held = key0 + 16 * g + c16 < kend;
-        const bool number = t.vs[g] != 255u;
-        unfinite |= held && !number;
-        const float scale = fp4::scale_of(value_scale<T>(t.vs[g], held && number));
-        if (kD == 128 || q4 < 2) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<x8*>(stage + (16 * i + c16) * kRow +
-                                   v_swz(c16, 4 * q4 + j) * 16) =
-                fp4::expand(t.v[g][j], scale, T());
-        }
-      }
-      own_lds_order();
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int dt = 0; dt < kDt; ++dt) {
         const int pos = v_swz(vr_row, 2 * dt + ((c16 & 3) >> 1));
-        const unsigned char* from = stage + vr_row * kRow + pos * 16 + (c16 & 1) * 8;
+        const unsigned char* from =
+            stage + (32 * half + vr_row) * kRow + pos * 16 + (c16 & 1) * 8;
         const typename E::x4 lo = read_tr<T>(from);
         const typename E::x4 hi = read_tr<T>(from + 16 * kRow);
         const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         oacc[dt] = E::mfma16(a, pf[half], oacc[dt]);
       }
-      own_lds_order();
-    }
+    own_lds_order();
   };
-  // Two turns' registers in turn: one on its way, one at work.
-  Turn even, odd;
   if (key_first < kend) {
-    load(0, even);
 #pragma unroll 1
     for (int turn = 0;; turn += 2) {
       const int key0 = key_first + turn * kFp4Turn;
-      const bool more = key0 + kFp4Turn < kend;
-      if (more) load(turn + 1, odd);
+      load(turn + 1, odd);
+      __builtin_amdgcn_sched_barrier(0);
       compute(even, key0);
-      if (!more) break;
-      const bool again = key0 + 2 * kFp4Turn < kend;
-      if (again) load(turn + 2, even);
+      if (key0 + kFp4Turn >= kend) break;
+      load(turn + 2, even);
+      __builtin_amdgcn_sched_barrier(0);
       compute(odd, key0 + kFp4Turn);
-      if (!again) break;
+      if (key0 + 2 * kFp4Turn >= kend) break;
     }
   }
 
@@ -361,21 +377,21 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
     for (int dt = 0; dt < kDt; ++dt)
       if (found >> (dt / 2) & 1) oacc[dt] = dsa_f32x4{NAN, NAN, NAN, NAN};
   }
-  // Join the waves: their O, m and l through the stages (row-major fp32).
+  // Join the waves: their O, m and l through the stages, rows of kD + 4 floats (16 bytes
+  // from bank to bank between them).
   l_run += __shfl_xor(l_run, 16);
   const float l_wave = dsa::pair32_sum(l_run);
-  dsa::lds_barrier();
   float* const mine = reinterpret_cast<float*>(stage);
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt)
-    *reinterpret_cast<dsa_f32x4*>(mine + c16 * kD + 16 * dt + 4 * q4) = oacc[dt];
+    *reinterpret_cast<dsa_f32x4*>(mine + c16 * kJoinRow + 16 * dt + 4 * q4) = oacc[dt];
   if (q4 == 0) {
     join_ml[0][wave][c16] = m_run;
     join_ml[1][wave][c16] = l_wave;
   }
   dsa::lds_barrier();
-  // Thread (r, c): row r, dims 8 c .. 8 c + 7.
-  const int r = tid / kChunks, d0 = tid % kChunks * 8;
+  // Thread (r, c): row r, dims 4 c .. 4 c + 3.
+  const int r = tid / (kD / 4), d0 = tid % (kD / 4) * 4;
   const int out_row = it.tile * kNarrowRows + r;
   if (r < kNarrowRows && out_row < rows) {
     float m_all = -INFINITY, l_all = 0.f, w[kFp4Waves];
@@ -388,23 +404,18 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
       w[i] = mi == -INFINITY ? join_ml[1][i][r] : __builtin_amdgcn_exp2f(mi - m_all);
       l_all = fmaf(w[i], join_ml[1][i][r], l_all);
     }
-    float acc[8];
-#pragma unroll
-    for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+    dsa_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kFp4Waves; ++i) {
-      if (w[i] == 0.f) continue;
-      const float* src = reinterpret_cast<const float*>(lds_v + i * kStage) + r * kD + d0;
+      const dsa_f32x4 x = *reinterpret_cast<const dsa_f32x4*>(
+          reinterpret_cast<const float*>(lds_v + i * kStage) + r * kJoinRow + d0);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) acc[x] = fmaf(w[i], src[x], acc[x]);
+      for (int e = 0; e < 4; ++e) acc[e] = w[i] == 0.f ? acc[e] : fmaf(w[i], x[e], acc[e]);
     }
     if (it.slot >= 0) {
       float* po =
           late->part + ((int64_t)it.slot * late->kv_heads + h) * part_floats(kNarrowRows, kD);
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<dsa_f32x4*>(po + r * kD + d0 + 4 * c) =
-            dsa_f32x4{acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]};
+      *reinterpret_cast<dsa_f32x4*>(po + r * kD + d0) = acc;
       if (d0 == 0) {
         po[kNarrowRows * kD + r] = m_all;
         po[kNarrowRows * (kD + 1) + r] = l_all;
@@ -414,11 +425,12 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
       const int out_head = h * late->group + out_row % late->group;
       const float inv = l_all > 0.f ? 1.f / l_all : (l_all == 0.f ? 0.f : l_all);
       if (d0 < late->head_dim) {
-        x8 y;
+        typename E::x4 y;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) y[x] = (T)(acc[x] * inv);
-        *reinterpret_cast<x8*>(static_cast<T*>(late->o) + (int64_t)out_token * late->o_st +
-                               out_head * late->o_sh + d0) = y;
+        for (int e = 0; e < 4; ++e) y[e] = (T)(acc[e] * inv);
+        *reinterpret_cast<typename E::x4*>(static_cast<T*>(late->o) +
+                                           (int64_t)out_token * late->o_st +
+                                           out_head * late->o_sh + d0) = y;
       }
       if (late->lse && d0 == 0)
         late->lse[(int64_t)out_head * late->q_rows + out_token] =
@@ -505,10 +517,15 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
     uint32_t top = 0;
+    QueryDims<T> raw[2 * kSteps];
+#pragma unroll
+    for (int j = 0; j < 2 * kSteps; ++j) {
+      raw[j].load(qrow, 32 * j + 16 * g, p.head_dim);
+    }
 #pragma unroll
     for (int j = 0; j < 2 * kSteps; ++j) {
       float x[16];
-      query_dims<T>(qrow, 32 * j + 16 * g, p.head_dim, x);
+      raw[j].widen(x);
       top = top_bits(x, top);
     }
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
@@ -517,7 +534,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
     for (int j = 0; j < 2 * kSteps; ++j) {
       float x[16];
-      query_dims<T>(qrow, 32 * j + 16 * g, p.head_dim, x);
+      raw[j].widen(x);
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] *= down;
       int32_t term[kTerms<T>][4];
@@ -546,9 +563,10 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const uint32_t value_scale_at = v_group < groups ? (uint32_t)(v_row * 4 + v_group)
                                                    : dsa::kDeadChunk;
   const uint32_t scale_at = lane < 16 ? (uint32_t)(lane * 4) : dsa::kDeadChunk;
-  auto v_swz = [](int r, int c) {
-    return kD == 128 ? c ^ ((0xCA60 >> (4 * (r & 3))) & 15) : c ^ (4 * ((r >> 1) & 1));
-  };
+  // V chunk c of row r sits at c ^ (c / 8) ^ 2 (r & 3): two rows of four chunks 4 apart,
+  // as eight lanes write them, and four rows of two chunks, as 16 lanes read them, lie in
+  // distinct banks.
+  auto v_swz = [](int r, int c) { return c ^ (c >> 3) ^ (2 * (r & 3)); };
   int vfrag[kDt];
   {
     const int lam = lane & 15, r = lam >> 2, c = lam & 3;

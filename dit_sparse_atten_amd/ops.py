@@ -1444,9 +1444,9 @@ def _fp4_aligned(cache):
 
 
 @functools.lru_cache(maxsize=512)
-def _turn_layout(q, q_out, k, v, caches, angles):
+def _turn_layout(q, q_out, k, v, cache, v_cache, angles):
     """(operands to copy first, strides, tokens, heads, kv_heads, head_dim, rot_dim, dtype
-    code, pages, page size) of a write that turns its rows."""
+    code, pages, page size) of a write that turns its rows; v_cache None: to 4 bits."""
     dtype = k[2]
     code = dtype_code(dtype)
     rows = [_sequence_strides("k", k, dtype), _sequence_strides("v", v, dtype)]
@@ -1482,81 +1482,83 @@ def _turn_layout(q, q_out, k, v, caches, angles):
                 if tokens and heads:
                     raise ValueError("q_out must have a contiguous, 16-byte aligned head dimension")
                 out_strides = [0, 0]
-    if len(caches) == 1:
-        held = [_fp4_strides(caches[0], kv_heads, head_dim)]
-        pages, page_size = caches[0][0][0], caches[0][0][2]
-        _apart("cache", caches[0])
+    if v_cache is None:
+        held = [_fp4_strides(cache, kv_heads, head_dim)]
+        pages, _, page_size, _ = cache[0]
+        _apart("cache", cache)
     else:
-        held = [_cache_strides(name, c, dtype) for name, c in zip(("k_cache", "v_cache"), caches)]
-        pages, page_size = caches[0][0][:2]
-        if caches[0][0] != caches[1][0] or caches[0][0][2:] != (kv_heads, head_dim):
+        held = [_cache_strides("k_cache", cache, dtype), _cache_strides("v_cache", v_cache, dtype)]
+        pages, page_size = cache[0][:2]
+        if cache[0] != v_cache[0] or cache[0][2:] != (kv_heads, head_dim):
             raise ValueError("the caches must share their shape, and k its heads and head "
                              "dimension")
         _page_size(page_size)
-        _apart("k_cache", caches[0])
-        _apart("v_cache", caches[1])
+        _apart("k_cache", cache)
+        _apart("v_cache", v_cache)
     operands = [q_strides, out_strides, *rows, *held]
     copies = tuple(i for i, x in enumerate((q_strides, *rows)) if x is None)
     strides = None
     if not copies:
-        strides = (_I64x10 if len(caches) == 1 else _I64x14)(*[x for t in operands for x in t])
+        strides = (_I64x10 if v_cache is None else _I64x14)(*[x for t in operands for x in t])
     return copies, strides, tokens, heads, kv_heads, head_dim, rot, code, pages, page_size
 
 
-def _angles(cos_sin, positions, tokens, device):
-    _require_cuda("cos_sin", cos_sin)
-    positions = _index_vector("positions", positions, device, tokens)
-    if cos_sin.device != device:
-        raise ValueError(f"cos_sin must live on {device}")
-    if not cos_sin.is_contiguous() or cos_sin.data_ptr() & 15:
-        cos_sin = cos_sin.clone(memory_format=torch.contiguous_format)
-    return cos_sin, positions
+def _on_device(name, t, device):
+    """Refuses what is not a tensor on the call's (HIP) device."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        _require_cuda(name, t)
+        raise ValueError(f"{name} must live on {device}")
 
 
 def _write_turned(function, what, k, v, caches, slots, positions, cos_sin, q, q_out, halves):
     """A write of both kinds; returns the turned queries, or None."""
     device = caches[0].device
-    for name, t in (("k", k), ("v", v), ("slots", slots)):
-        _require_cuda(name, t)
-    if q is None and q_out is not None:
-        raise ValueError("q_out needs q")
-    for name, t in (("q", q), ("q_out", q_out)):
-        if t is not None:
-            _require_cuda(name, t)
-            if t.device != device:
-                raise ValueError(f"{name} must live on {device}")
+    _on_device("k", k, device)
+    _on_device("v", v, device)
+    _on_device("slots", slots, device)
+    if q is not None:
+        _on_device("q", q, device)
+    if q_out is not None:
+        _on_device("q_out", q_out, device)
+        if q is None:
+            raise ValueError("q_out needs q")
     copies, strides, tokens, heads, kv_heads, head_dim, rot, code, pages, page_size = _turn_layout(
         None if q is None else _layout(q), None if q_out is None else _layout(q_out), _layout(k),
-        _layout(v), tuple(_layout(c) for c in caches),
+        _layout(v), _layout(caches[0]), _layout(caches[1]) if len(caches) > 1 else None,
         None if cos_sin is None else (cos_sin.shape, cos_sin.dtype))
     if slots.dtype != torch.int64 or slots.shape != (tokens,):
         raise ValueError(f"slots must be an int64 tensor of {tokens} values")
-    if not (k.device == v.device == slots.device == device):
-        raise ValueError("k, v, the cache and slots must be on the same device")
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    angles = turns = None
     if cos_sin is not None:
-        cos_sin, positions = _angles(cos_sin, positions, tokens, device)
+        _on_device("cos_sin", cos_sin, device)
+        positions = _index_vector("positions", positions, device, tokens)
+        if not cos_sin.is_contiguous() or cos_sin.data_ptr() & 15:
+            cos_sin = cos_sin.clone(memory_format=torch.contiguous_format)
+        if rot:
+            turns, angles = positions.data_ptr(), cos_sin.data_ptr()
     elif positions is not None:
         raise ValueError("positions need cos_sin")
-    if copies or (k.data_ptr() | v.data_ptr() | (0 if q is None else q.data_ptr())) & 15:
+    at_q, at_k, at_v = 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if copies or (at_q | at_k | at_v) & 15:
         # (a copied q still goes to its own place where q_out is q)
-        operands = [torch.empty(0, device=device) if q is None else q, k, v]
-        new_q, k, v = _in_place(copies, *operands)
+        new_q, k, v = _in_place(copies, k if q is None else q, k, v)
         return _write_turned(function, what, k, v, caches, slots, positions, cos_sin,
                              None if q is None else new_q, q_out, halves)
-    out = q_out
+    out, at_out = q_out, 0
     if q is not None:
         if out is None:
             out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
-        _aligned("q_out", out)
-    if tokens == 0:
-        return out
-    if not slots.is_contiguous():
-        slots = slots.contiguous()
-    _call(function, what, device, q.data_ptr() if heads else None, out.data_ptr() if heads else None,
-          k.data_ptr(), v.data_ptr(), *[c.data_ptr() for c in caches], code, strides, tokens, heads,
-          kv_heads, head_dim, rot, 1 if halves else 0, pages, page_size, slots.data_ptr(),
-          positions.data_ptr() if rot else None, cos_sin.data_ptr() if rot else None,
-          cos_sin.shape[0] if rot else 0)
+        else:
+            _aligned("q_out", out)
+        at_out = out.data_ptr()
+    if tokens:
+        first = caches[0].data_ptr()
+        held = (first,) if len(caches) == 1 else (first, caches[1].data_ptr())
+        _call(function, what, device, at_q, at_out, at_k, at_v, *held, code, strides, tokens, heads,
+              kv_heads, head_dim, rot, 1 if halves else 0, pages, page_size, slots.data_ptr(), turns,
+              angles, cos_sin.shape[0] if rot else 0)
     return out
 
 
@@ -1583,9 +1585,7 @@ def paged_write_rotary(k, v, k_cache, v_cache, slots, positions, cos_sin, q=None
     """
     lib = _lib.load()
     _require_cuda("k_cache", k_cache)
-    _require_cuda("v_cache", v_cache)
-    if v_cache.device != k_cache.device:
-        raise ValueError("k, v, the cache and slots must be on the same device")
+    _on_device("v_cache", v_cache, k_cache.device)
     _aligned("k_cache", k_cache)
     _aligned("v_cache", v_cache)
     if cos_sin is None:
@@ -1615,6 +1615,15 @@ def paged_write_fp4(k, v, cache, slots, positions=None, cos_sin=None, q=None, q_
                          positions, cos_sin, q, q_out, halves)
 
 
+@functools.lru_cache(maxsize=512)
+def _read_layout(cache, head_dim, dtype):
+    """(dtype code, strides, pages, key heads, page size) of a read."""
+    code = dtype_code(dtype)
+    strides = _I64x2(*_fp4_strides(cache, None, head_dim))
+    pages, kv_heads, page_size, _ = cache[0]
+    return code, strides, pages, kv_heads, page_size
+
+
 def paged_read_fp4(cache, head_dim, pages=None, dtype=torch.bfloat16):
     """Keys and values that a 4-bit cache stands for, (k, v) [pages, page_size, kv_heads,
     head_dim] in bf16 or fp16: of the listed ``pages`` (int32 on the device, zeros for
@@ -1622,17 +1631,16 @@ def paged_read_fp4(cache, head_dim, pages=None, dtype=torch.bfloat16):
     cache written from bf16."""
     lib = _lib.load()
     _require_cuda("cache", cache)
-    code = dtype_code(dtype)
-    strides = _I64x2(*_fp4_strides(_layout(cache), None, head_dim))
+    code, strides, total, kv_heads, page_size = _read_layout(_layout(cache), head_dim, dtype)
     _fp4_aligned(cache)
-    total, kv_heads, page_size, _ = cache.shape
     device = cache.device
     if pages is not None:
         pages = _index_vector("pages", pages, device)
     count = total if pages is None else pages.shape[0]
-    k = torch.empty((count, page_size, kv_heads, head_dim), dtype=dtype, device=device)
-    v = torch.empty_like(k)
-    if k.numel():
+    shape = (count, page_size, kv_heads, head_dim)
+    k = torch.empty(shape, dtype=dtype, device=device)
+    v = torch.empty(shape, dtype=dtype, device=device)
+    if count and kv_heads:
         _call(lib.dsa_paged_read_fp4, "dsa_paged_read_fp4", device, cache.data_ptr(), strides,
               k.data_ptr(), v.data_ptr(), code, total, page_size, kv_heads, head_dim,
               None if pages is None else pages.data_ptr(), count)

@@ -18,7 +18,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxBatch = 8;   // heads that a workgroup walks
-constexpr int kHeadTurns = 4;  // heads whose loads are on their way at a time
+// Heads whose loads are on their way at a time: of 16-bit rows, and of rows to 4 bits,
+// whose loads (non-temporal) are followed by more work.  (57,600 tokens x 12 heads to 4
+// bits: two 94 us, 4.9 TB/s, four 95, six and eight 102 and 104; kept loads 97.)
+constexpr int kHeadTurns = 4;
+constexpr int kPackTurns = 2;
 
 enum Rows { kQ = 0, kK = 1, kV = 2 };
 
@@ -55,7 +59,9 @@ __device__ __forceinline__ int64_t slot_of(const TurnParams& p, int t, int posit
   return slot >= 0 && slot < p.total && angles ? slot : -1;
 }
 
-// 16-bit rows to 16-bit rows.  A thread takes 16-byte chunks of a row in pairs (c, c +
+// 16-bit rows to 16-bit rows, bound by memory: 57,600 tokens x 12 query and key heads x
+// 128 (1.09 GB) 218 us, 5.0 TB/s, the rate of a large copy (with non-temporal loads 225,
+// stores 240).  A thread takes 16-byte chunks of a row in pairs (c, c +
 // rot / 16): with halves a pair's elements turn with each other, so that a row may be
 // turned in place.  Chunks behind the turned ones go in neighbouring pairs.  The thread
 // keeps its angles and walks the heads of the workgroup's batch.
@@ -98,8 +104,8 @@ __device__ __forceinline__ void turn_rows(const TurnParams& p, int which, int he
     for (int i = 0; i < kHeadTurns; ++i) {
       if (h0 + i >= heads) continue;
       const uint16_t* const at = src + (h0 + i) * p.src_sh[which];
-      x[i][0] = __builtin_nontemporal_load(reinterpret_cast<const x8*>(at + c0 * 8));
-      if (second) x[i][1] = __builtin_nontemporal_load(reinterpret_cast<const x8*>(at + c1 * 8));
+      x[i][0] = *reinterpret_cast<const x8*>(at + c0 * 8);
+      if (second) x[i][1] = *reinterpret_cast<const x8*>(at + c1 * 8);
     }
 #pragma unroll
     for (int i = 0; i < kHeadTurns; ++i) {
@@ -178,19 +184,19 @@ __device__ __forceinline__ void pack_rows(const TurnParams& p, int which, int he
   unsigned char* const codes = dst + (which == kV ? at.v_codes : 0) + row * at.code_row + 4 * c;
   unsigned char* const scales = dst + (which == kV ? at.v_scales : at.k_scales) + 4 * row + c / 4;
 #pragma unroll 1
-  for (int h0 = 0; h0 < heads; h0 += kHeadTurns) {
-    x8 x[kHeadTurns], y[kHeadTurns];
+  for (int h0 = 0; h0 < heads; h0 += kPackTurns) {
+    x8 x[kPackTurns], y[kPackTurns];
 #pragma unroll
-    for (int i = 0; i < kHeadTurns; ++i) {
+    for (int i = 0; i < kPackTurns; ++i) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[i][e] = (T)0.f;
       if (h0 + i >= heads || !real) continue;
       const uint16_t* const from = src + (h0 + i) * p.src_sh[which];
-      x[i] = *reinterpret_cast<const x8*>(from + 8 * c);
+      x[i] = __builtin_nontemporal_load(reinterpret_cast<const x8*>(from + 8 * c));
       if (kHalves && turn) y[i] = *reinterpret_cast<const x8*>(from + 8 * pair);
     }
 #pragma unroll
-    for (int i = 0; i < kHeadTurns; ++i) {
+    for (int i = 0; i < kPackTurns; ++i) {
       if (h0 + i >= heads) continue;
       float f[8];
 #pragma unroll
@@ -244,33 +250,47 @@ struct ReadParams {
   int64_t cache_sp, cache_sh;
   void* dst[2];            // [count, page_size, kv_heads, head_dim]
   const int32_t* list;     // pages, or null: all of them
-  int64_t rows;            // count * kv_heads * page_size
+  int64_t units;           // of 16 tokens and a head
   int32_t pages, kv_heads, head_dim, page_shift;
 };
 
-// Rows of a 4-bit cache, keys or values (y), in the cache's order: a lane to 8 dims, four
-// bytes in and 16 out.
+// Rows of a 4-bit cache, keys or values (y): a lane to 8 dims, four bytes in and 16 out.
+// 16 tokens of a head (1 KB of codes in a row) at a time, the heads of the same tokens
+// one after the other, which together fill the memory that they go to.
+//
+// kOnce: the values go past the caches, in reads of 192 MB and more of them, which the
+// 256 MB cache would not keep for whoever takes them up.  (Read alone, and with a
+// paged_write of all of them behind it, kept / past: 101 MB 22.7 / 20.6 and 54.0 / 55.3
+// us, 201 MB 40.6 / 39.8 and 110.6 / 100.4, 403 MB 96.9 / 75.5 and 239.6 / 241.4, 805 MB
+// 190 / 148 and 478 / 494.)
+constexpr int64_t kOnceBytes = (int64_t)192 << 20;
 constexpr int kReadTurns = 8;
-template <typename T>
+constexpr int kReadRows = 16;
+__host__ __device__ constexpr int read_units(int groups) {  // that a workgroup reads at a time
+  return kThreads / (kReadRows * 4 * groups);
+}
+template <typename T, bool kOnce>
 __global__ void __launch_bounds__(kThreads) paged_read_fp4_kernel(ReadParams p) {
   const int which = blockIdx.y;
   const int groups = fp4::groups_of(p.head_dim);
-  const int lanes = 4 * groups, per_group = kThreads / lanes;
+  const int lanes = 4 * groups, each = read_units(groups);
   const int local = threadIdx.x / lanes, c = threadIdx.x - local * lanes;
-  if (local >= per_group || c >= p.head_dim / 8) return;
+  const int unit0 = local / kReadRows, in_unit = local % kReadRows;
+  if (unit0 >= each || c >= p.head_dim / 8) return;
   const fp4::Layout at(groups, p.page_shift);
+  const int per_page = p.page_shift - 4;  // log2 of the 16-token units of a page
   uint32_t code[kReadTurns], scale[kReadTurns];
   int64_t to[kReadTurns];
 #pragma unroll
   for (int i = 0; i < kReadTurns; ++i) {
-    const int64_t r = ((int64_t)blockIdx.x * kReadTurns + i) * per_group + local;
+    const int64_t unit = ((int64_t)blockIdx.x * kReadTurns + i) * each + unit0;
     code[i] = scale[i] = 0;
     to[i] = -1;
-    if (r >= p.rows) continue;
-    const int row = (int)(r & ((1 << p.page_shift) - 1));
-    const int64_t unit = r >> p.page_shift;  // listed page and head
-    const int64_t index = unit / p.kv_heads;
-    const int head = (int)(unit - index * p.kv_heads);
+    if (unit >= p.units) continue;
+    const int64_t tokens = unit / p.kv_heads;  // 16 of a listed page's
+    const int head = (int)(unit - tokens * p.kv_heads);
+    const int64_t index = tokens >> per_page;
+    const int row = (int)(tokens & ((1 << per_page) - 1)) * kReadRows + in_unit;
     to[i] = (((index << p.page_shift) + row) * p.kv_heads + head) * p.head_dim + 8 * c;
     const int64_t page = p.list ? p.list[index] : index;
     if (page < 0 || page >= p.pages) continue;  // (zeros)
@@ -282,8 +302,11 @@ __global__ void __launch_bounds__(kThreads) paged_read_fp4_kernel(ReadParams p) 
 #pragma unroll
   for (int i = 0; i < kReadTurns; ++i) {
     if (to[i] < 0) continue;
-    *reinterpret_cast<typename dsa::Elem<T>::x8*>(static_cast<T*>(p.dst[which]) + to[i]) =
-        fp4::expand(code[i], fp4::scale_of(scale[i]), T());
+    typedef typename dsa::Elem<T>::x8 x8;
+    const x8 y = fp4::expand(code[i], fp4::scale_of(scale[i]), T());
+    x8* const at_y = reinterpret_cast<x8*>(static_cast<T*>(p.dst[which]) + to[i]);
+    if (kOnce) __builtin_nontemporal_store(y, at_y);
+    else *at_y = y;
   }
 }
 
@@ -488,17 +511,22 @@ extern "C" int dsa_paged_read_fp4(const void* cache, const int64_t* strides, voi
   p.dst[0] = k;
   p.dst[1] = v;
   p.list = list;
-  p.rows = (int64_t)count * kv_heads * page_size;
+  p.units = (int64_t)count * kv_heads * (page_size / kReadRows);
   p.pages = pages; p.kv_heads = kv_heads; p.head_dim = head_dim;
   p.page_shift = __builtin_ctz(page_size);
-  const int64_t each = kReadTurns * (kThreads / (4 * fp4::groups_of(head_dim)));
-  const int64_t groups = (p.rows + each - 1) / each;
+  const int64_t each = kReadTurns * read_units(fp4::groups_of(head_dim));
+  const int64_t groups = (p.units + each - 1) / each;
   if (groups >= 1 << 24) return dsa::set_error(DSA_EUNSUPPORTED, "%s: too many rows", who);
   dsa::clear_error();
   const dim3 grid((unsigned)groups, 2);
+  const bool once = p.units * kReadRows * head_dim * 4 >= kOnceBytes;  // keys and values
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, p);
+  };
   if (dtype == DSA_BF16)
-    hipLaunchKernelGGL(paged_read_fp4_kernel<__bf16>, grid, dim3(kThreads), 0, stream, p);
+    once ? launch(paged_read_fp4_kernel<__bf16, true>) : launch(paged_read_fp4_kernel<__bf16, false>);
   else
-    hipLaunchKernelGGL(paged_read_fp4_kernel<_Float16>, grid, dim3(kThreads), 0, stream, p);
+    once ? launch(paged_read_fp4_kernel<_Float16, true>)
+         : launch(paged_read_fp4_kernel<_Float16, false>);
   return dsa::check_launch(who);
 }

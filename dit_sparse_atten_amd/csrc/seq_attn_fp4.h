@@ -478,9 +478,12 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   constexpr int kSteps = kD / 64;            // products of 64 dims
   constexpr int kDt = kUse / 32;
   constexpr int kChunks = kD / 8;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_k[2][4096];  // 1 KB a wave
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_s[2][1024];  // scales, by wave
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_v[2][kStage];
+  // (an array to a stage: a read of one that loads go to waits for them)
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[4096];  // codes, 1 KB a wave
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[4096];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_s0[1024];  // scales, by wave
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_s1[1024];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v[2 * kStage];
 
   Item it;
   int h;
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   // Wave w stages the keys 16 w .. 16 w + 15 of a step, one page: lane (r, c) = (lane / 4,
   // lane % 4) row r's chunk c, 16 bytes of codes (of 32-byte rows of keys: the lower 32
   // lanes, (lane / 2, lane % 2)).  K chunk c of row r sits at c ^ (r / 4 & 3) or c ^ (r / 8
-  // & 1).
+  // & 1) (by r / 2 and r / 4 the reads met 20% more conflicts).
   auto k_swz = [](int r, int c) { return kD == 128 ? c ^ (r >> 2 & 3) : c ^ (r >> 3 & 1); };
   constexpr int kLanes = kD / 32;  // chunks of a row
   const int k_row = lane / kLanes, k_chunk = k_swz(k_row, lane % kLanes);
@@ -600,30 +603,32 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     at_row = (s * kWideKeys + wave * 16) & ((1 << p.page_shift) - 1);
     rsrc = fp4_rsrc(p, page, h, block_bytes, page < (uint32_t)p.pages);
   };
+  auto issue_keys = [&](unsigned char* k_to, unsigned char* s_to) __attribute__((always_inline)) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (DSA_LDS void*)(k_to + wave * 1024), 16,
+                                             code_at, at_row * at.code_row, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (DSA_LDS void*)(s_to + wave * 256), 4,
+                                             scale_at, at.k_scales + 4 * at_row, 0, 0);
+  };
   dsa_u32x4 v_codes;
   uint32_t v_scale = 0;
-  auto issue = [&](int to) __attribute__((always_inline)) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rsrc, (DSA_LDS void*)(lds_k[to] + wave * 1024), 16, code_at, at_row * at.code_row, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (DSA_LDS void*)(lds_s[to] + wave * 256), 4,
-                                             scale_at, at.k_scales + 4 * at_row, 0, 0);
+  auto issue_values = [&]() __attribute__((always_inline)) {
     v_codes = __builtin_amdgcn_raw_buffer_load_b128(rsrc, value_at,
                                                     at.v_codes + at_row * at.code_row, 0);
     v_scale = __builtin_amdgcn_raw_buffer_load_b8(rsrc, value_scale_at,
                                                   at.v_scales + 4 * at_row, 0);
   };
-  bool unfinite = false;  // a group of values that is not a number
-  // The values of step s, on their way since issue(), into their stage.
+  uint32_t unfinite = 0;  // 1 where a group of values is not a number
+  // The values of step s, on their way since issue_values(), into their stage.
   auto expand = [&](int s, int to) __attribute__((always_inline)) {
     const bool held = s * kWideKeys + wave * 16 + v_row < kend;
     const bool number = v_scale != 255u;
-    unfinite |= held && !number;
+    unfinite |= held && !number ? 1u : 0u;
     const float scale = fp4::scale_of(value_scale<T>(v_scale, held && number));
     const int r = wave * 16 + v_row;
     if (kD == 128 || v_group < 2) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<x8*>(lds_v[to] + r * kRow + v_swz(r, 4 * v_group + j) * 16) =
+        *reinterpret_cast<x8*>(lds_v + to * kStage + r * kRow + v_swz(r, 4 * v_group + j) * 16) =
             fp4::expand(v_codes[j], scale, T());
     }
   };
@@ -635,37 +640,65 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
 
-  auto compute = [&](int from, int key0, int bad) __attribute__((always_inline)) {
-    const unsigned char* const k_lds = lds_k[from];
-    const unsigned char* const v_lds = lds_v[from];
+  // Step s from stage `from`; the values of step s + 1 go to the other stage meanwhile.
+  auto compute = [&](int from, const unsigned char* k_lds, const unsigned char* s_lds, int s,
+                     int bad) __attribute__((always_inline)) {
+    const int key0 = s * kWideKeys;
+    const unsigned char* const v_lds = lds_v + from * kStage;
     __builtin_amdgcn_s_setprio(0);
     dsa_f32x16 sacc[2];
+    dsa_u32x4 codes[2][kSteps];
+    int ks[2][kSteps];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int krow = kt * 32 + qi;
+      // Group g of a product's two, at the dword's bytes 0 and 2.
+      const uint32_t four = *reinterpret_cast<const uint32_t*>(
+          s_lds + (krow >> 4) * 256 + (krow & 15) * 4) >> (8 * g);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        codes[kt][j] = *reinterpret_cast<const dsa_u32x4*>(
+            k_lds + (krow >> 4) * 1024 + (krow & 15) * kCodeRow +
+            k_swz(krow & 15, 2 * j + g) * 16);
+        // (bytes of groups that a row has not: codes of zeros, scales of no NaN)
+        ks[kt][j] = 2 * j + g < groups ? (int)four : 0;
+      }
+    }
+    // The values' fragments of 16 keys (two reads each), read 16 keys ahead.
+    typename E::x4 vf[2][kDt][2];
+    auto read_values = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) {
+        // Key rows 16 j + 4 g + r (slots 0..3) and 16 j + 8 + 4 g + r (4..7).
+        const unsigned char* const at_v = v_lds + vfrag[dt] + j * 16 * kRow;
+        vf[j & 1][dt][0] = read_tr<T>(at_v);
+        vf[j & 1][dt][1] = read_tr<T>(at_v + 8 * kRow);
+      }
+    };
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sacc[kt][r] = 0.f;
-      const int krow = kt * 32 + qi;
-      // Group g of a product's two, at the dword's bytes 0 and 2.
-      const uint32_t four = *reinterpret_cast<const uint32_t*>(
-          lds_s[from] + (krow >> 4) * 256 + (krow & 15) * 4) >> (8 * g);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        const dsa_u32x4 c = *reinterpret_cast<const dsa_u32x4*>(
-            k_lds + (krow >> 4) * 1024 + (krow & 15) * kCodeRow + k_swz(krow & 15, 2 * j + g) * 16);
+        const dsa_u32x4 c = codes[kt][j];
         const fp4_x8 a = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-        // (bytes of groups that a row has not: codes of zeros, scales of no NaN)
-        const int ks = 2 * j + g < groups ? (int)four : 0;
 #pragma unroll
         for (int n = kTerms<T> - 1; n >= 0; --n) {
           if (j == 0)
-            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, qf[j][n], sacc[kt], 4, 0,
-                                                                       0, ks, 0, q_scale[n]);
+            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                a, qf[j][n], sacc[kt], 4, 0, 0, ks[kt][j], 0, q_scale[n]);
           else
-            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, qf[j][n], sacc[kt], 4, 0,
-                                                                       2, ks, 0, q_scale[n]);
+            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                a, qf[j][n], sacc[kt], 4, 0, 2, ks[kt][j], 0, q_scale[n]);
         }
       }
     }
+    expand(s + 1, from ^ 1);
+    asm volatile("" : "+v"(unfinite));  // (here, so that the scales' register is free)
+    __builtin_amdgcn_sched_barrier(0);
+    issue_values();
+    read_values(0);
     if (key0 + kWideKeys > lim_first) {
       const int bound = lim - key0 - 4 * g;
 #pragma unroll
@@ -686,9 +719,11 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kt][r]);
-    const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
-    const bool up = mx2 > m_run + kRescaleLog2;
-    if (__any(up)) {
+    // The reference moves only where a lane's own scores call for it: the row's largest is
+    // not needed before.
+    if (__any(mx * p.scale_log2 > m_run + kRescaleLog2)) {
+      const float mx2 = dsa::pair32_max(mx) * p.scale_log2;
+      const bool up = mx2 > m_run + kRescaleLog2;
       const float m_new = up ? mx2 : m_run;
       const float alpha = up ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
       m_run = m_new;
@@ -699,10 +734,9 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
         for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
     }
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
-    x8 pf[4];
+    x8 pf[2];
     float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
+    auto weigh = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < 8; t += 2) {
         const float p0 = __builtin_amdgcn_exp2f(
@@ -713,59 +747,78 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
         const typename E::x2 pb = __builtin_convertvector(two, typename E::x2);
         sum0 += p0;
         sum1 += p1;
-        pf[j][t] = pb[0];
-        pf[j][t + 1] = pb[1];
+        pf[j & 1][t] = pb[0];
+        pf[j & 1][t + 1] = pb[1];
       }
-    l_run += sum0 + sum1;
+    };
+    // 16 keys' products with the next 16 keys' exponentials and reads between them.
+    weigh(0);
+    __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
+      if (j < 3) {
+        read_values(j + 1);
+        weigh(j + 1);
+      }
 #pragma unroll
       for (int dt = 0; dt < kDt; ++dt) {
-        // Key rows 16 j + 4 g + r (slots 0..3) and 16 j + 8 + 4 g + r (4..7).
-        const unsigned char* from_v = v_lds + vfrag[dt] + j * 16 * kRow;
-        const typename E::x4 lo = read_tr<T>(from_v);
-        const typename E::x4 hi = read_tr<T>(from_v + 8 * kRow);
+        const typename E::x4 lo = vf[j & 1][dt][0], hi = vf[j & 1][dt][1];
         const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        oacc[dt] = E::mfma32(a, pf[j], oacc[dt]);
+        oacc[dt] = E::mfma32(a, pf[j & 1], oacc[dt]);
       }
-    // Four products' V reads (two each) ahead.
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+      if (j < 3) {
 #pragma unroll
-    for (int i = 0; i < 4 * kDt - 4; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        for (int dt = 0; dt < kDt; ++dt) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, 7, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
+    l_run += sum0 + sum1;
   };
-  // A step: its keys' codes are in their stage once the loads are done, its values once
-  // they are expanded; then the next step's loads go out and its products run.
+  // Step s, of stage i: behind the barrier its keys and values are there; the values of
+  // step s + 1, in registers by then, go to the other stage, and the loads of the keys of
+  // step s + 1 and the values of step s + 2 go out.
   int bad_cur = 0;
-  auto step = [&](int s, int stage) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(vmcnt(0));
-    expand(s, stage);
-    bad_cur = bad_next;
+  auto step = [&](int s, int i, const unsigned char* k_lds, const unsigned char* s_lds,
+                  unsigned char* k_to, unsigned char* s_to) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(vmcnt(2));  // (the keys; the values behind them may be on their way)
     dsa::lds_barrier();
-    if (s + 1 < it.s1) {
-      locate(s + 1);
-      issue(stage ^ 1);
-    }
+    issue_keys(k_to, s_to);
+    const int bad_then = bad_next;
+    locate(s + 2);  // (past the last key: no bytes)
     // (a wave whose rows see none of the step's keys only stages)
-    if (wave_active && s * kWideKeys < lim_last) compute(stage, s * kWideKeys, bad_cur);
+    if (wave_active && s * kWideKeys < lim_last) {
+      compute(i, k_lds, s_lds, s, bad_cur);
+    } else {
+      expand(s + 1, i ^ 1);
+      issue_values();
+    }
+    bad_cur = bad_then;
   };
   if (it.s0 < it.s1) {
     locate(it.s0);
-    issue(0);
+    bad_cur = bad_next;
+    issue_keys(lds_k0, lds_s0);
+    issue_values();
+    __builtin_amdgcn_s_waitcnt(vmcnt(0));
+    expand(it.s0, 0);
+    locate(it.s0 + 1);
+    issue_values();
     for (int s = it.s0; s < it.s1; s += 2) {
-      step(s, 0);
+      step(s, 0, lds_k0, lds_s0, lds_k1, lds_s1);
       if (s + 1 >= it.s1) break;
-      step(s + 1, 1);
+      step(s + 1, 1, lds_k1, lds_s1, lds_k0, lds_s0);
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt(0));  // (loads behind the last step, into the stages)
   }
 
   const LateParams late = late_params();
   const float l_tot = dsa::pair32_sum(l_run);
-  if (__syncthreads_or(unfinite)) {
+  if (__syncthreads_or((int)unfinite)) {
     const uint32_t found = unfinite_groups(late, it, h, it.s0 * kWideKeys,
                                            min(it.s1 * kWideKeys, kend), lim);
 #pragma unroll
@@ -799,7 +852,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   // O goes out through the value stages (every wave is past its reads of them: the
   // barrier of __syncthreads_or), row by row as 16-byte chunks, whole rows to a store.
   const float inv = l_tot > 0.f ? 1.f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
-  unsigned char* const mine = lds_v[0] + wave * 32 * kRow;
+  unsigned char* const mine = lds_v + wave * 32 * kRow;
   auto o_swz = [](int r, int c) { return kD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7); };
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt)

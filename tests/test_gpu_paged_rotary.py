@@ -225,3 +225,116 @@ def test_read_fp4(cuda_device, dim, page):
                 assert torch.equal(torch.isnan(x.cpu()), torch.isnan(values))
                 finite = ~torch.isnan(values)
                 assert torch.equal(x.cpu()[finite], values[finite].to(dtype))
+
+
+def test_refusals(cuda_device):
+    def rows(n, h, d=64, t=torch.bfloat16):
+        return torch.zeros((n, h, d), dtype=t, device=cuda_device)
+
+    q, k = rows(4, 4), rows(4, 2)
+    slots = torch.zeros(4, dtype=torch.int64, device=cuda_device)
+    turns = torch.zeros(4, dtype=torch.int32, device=cuda_device)
+    angles = _angles(5, 32).to(cuda_device)
+    held = torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+    cache = ops.paged_cache_fp4(3, 16, 2, 64, cuda_device)
+
+    def rotary(match, k=k, v=k, k_cache=held, v_cache=held, slots=slots, positions=turns,
+               cos_sin=angles, **more):
+        with pytest.raises(ValueError, match=match):
+            ops.paged_write_rotary(k, v, k_cache, v_cache, slots, positions, cos_sin, **more)
+
+    def fp4(match, k=k, v=k, cache=cache, slots=slots, positions=turns, cos_sin=angles, **more):
+        with pytest.raises(ValueError, match=match):
+            ops.paged_write_fp4(k, v, cache, slots, positions, cos_sin, **more)
+
+    for refuse in (rotary, fp4):
+        refuse("float32", k=rows(4, 2, t=torch.float32), v=rows(4, 2, t=torch.float32))
+        refuse("like q", v=k.half())
+        refuse("same shape", v=rows(4, 1))
+        refuse("rows, heads", k=k[0], v=k[0])
+        refuse("head", k=rows(4, 2, 136), v=rows(4, 2, 136))
+        refuse("slots", slots=slots.int())
+        refuse("slots", slots=slots[:3])
+        refuse("CUDA", slots=slots.cpu())
+        refuse("CUDA", k=k.cpu())
+        refuse("positions", positions=turns.long())
+        refuse("positions", positions=turns[:3])
+        refuse("cos_sin", cos_sin=angles.double())
+        refuse("cos_sin", cos_sin=angles[..., 0])
+        refuse("CUDA", cos_sin=angles.cpu())
+        refuse("turned dims", cos_sin=angles[:, :12])
+        refuse("turned dims", cos_sin=_angles(5, 80).to(cuda_device))
+        refuse("q must", q=rows(3, 4))
+        refuse("like q", q=q.half())
+        refuse("q_out needs q", q_out=q)
+        refuse("q_out", q=q, q_out=k)
+        refuse("expanded", q=q, q_out=q[:1].expand(4, -1, -1))
+        refuse("aligned", q=q, q_out=rows(4, 4, 66)[..., :64])
+        refuse("CUDA", q=q, q_out=q.cpu())
+    rotary("needed", positions=None, cos_sin=None)
+    rotary("k_cache", k_cache=held.half())
+    rotary("heads", k_cache=held[:, :, :1], v_cache=held[:, :, :1])
+    rotary("share", v_cache=held[:2])
+    rotary("expanded", k_cache=held[:1].expand(3, -1, -1, -1))
+    rotary("page_size", k_cache=held[:, :8], v_cache=held[:, :8])
+    fp4("positions need", cos_sin=None)
+    fp4("uint8", cache=held)
+    fp4("uint8", cache=cache[..., :71])
+    fp4("heads", cache=cache[:, :1])
+    fp4("page_size", cache=cache[:, :, ::2])
+    fp4("contiguous", cache=ops.paged_cache_fp4(3, 32, 2, 64, cuda_device)[:, :, ::2])
+    fp4("expanded", cache=cache[:1].expand(3, -1, -1, -1))
+    store = torch.zeros(3 * 2 * 16 * 72 + 8, dtype=torch.uint8, device=cuda_device)
+    fp4("aligned", cache=store[8:].view(3, 2, 16, 72))
+    wide = torch.zeros((3, 2 * 16 * 72 + 8), dtype=torch.uint8, device=cuda_device)
+    fp4("16 bytes apart", cache=wide[:, :-8].view(3, 2, 16, 72))
+    with pytest.raises(ValueError, match="float32"):
+        ops.paged_read_fp4(cache, 64, dtype=torch.float32)
+    with pytest.raises(ValueError, match="uint8"):
+        ops.paged_read_fp4(cache, 128)
+    with pytest.raises(ValueError, match="pages"):
+        ops.paged_read_fp4(cache, 64, slots)
+    starts, table = torch.tensor([0, 4], dtype=torch.int32, device=cuda_device), turns[:2][None]
+
+    def attend(match, q=q, cache=cache, table=table, lens=starts[1:], starts=starts, **more):
+        with pytest.raises(ValueError, match=match):
+            ops.paged_attention_fp4(q, cache, table, lens, starts, **more)
+
+    attend("uint8", cache=held)
+    attend("uint8", q=rows(4, 4, 128))
+    attend("share", q=rows(4, 5))
+    attend("float32", q=q.float())
+    attend("block_table", table=table.long())
+    attend("block_table", table=table.expand(2, -1))
+    attend("kv_lens", lens=starts[1:].long())
+    attend("q_start", starts=starts[:1])
+    attend("scale", scale=0.0)
+    attend("out", out=torch.zeros_like(k))
+    attend("expanded", out=q[:1].expand(4, -1, -1))
+    attend("CUDA", cache=cache.cpu())
+    # Nothing was written.
+    torch.cuda.synchronize()
+    assert (held == 0).all() and (cache == 0).all() and (q == 0).all()
+
+
+def test_nothing_to_write(cuda_device):
+    """No tokens, no pages, no head of queries: nothing happens but the queries' turn."""
+    k = torch.ones((4, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+    slots = torch.arange(4, device=cuda_device)
+    turns, angles = slots.int(), _angles(5, 32).to(cuda_device)
+    held = torch.zeros((3, 16, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+    cache = ops.paged_cache_fp4(3, 16, 2, 64, cuda_device)
+    none = ops.paged_write_rotary(k[:0], k[:0], held, held.clone(), slots[:0], turns[:0], angles,
+                                  q=k[:0])
+    assert none.shape == (0, 2, 64)
+    ops.paged_write_fp4(k[:0], k[:0], cache, slots[:0])
+    turned = ops.paged_write_rotary(k, k, held[:0], held[:0], slots, turns, angles, q=k)
+    assert torch.equal(turned, ops.paged_write_fp4(k, k, cache[:0], slots, turns, angles, q=k))
+    assert ops.paged_write_fp4(k, k, cache[:0], slots, turns, angles, q=k[:, :0]).shape == (4, 0, 64)
+    assert (held == 0).all() and (cache == 0).all()
+    got = ops.paged_read_fp4(cache[:0], 64)
+    assert got[0].shape == got[1].shape == (0, 16, 2, 64)
+    # One page and one head, whatever their strides.
+    one = torch.as_strided(cache, (1, 1, 16, 72), (8, 24, 72, 1))
+    ops.paged_write_fp4(k[:, :1], k[:, :1], one, slots)
+    assert (ops.paged_read_fp4(one, 64)[0][0, :4] == 1).all()

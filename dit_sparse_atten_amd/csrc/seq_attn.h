@@ -104,7 +104,8 @@ constexpr int kWideRows = 128, kWideKeys = 64;
 // Workgroups of the chip that run at a time: two of 128-row tiles on a compute unit;
 // one of 16-row tiles, whose four waves keep the memory busy (two: 2 to 5% slower).
 constexpr int kWideSlots = 512, kNarrowSlots = 256;
-constexpr int kMaxChains = kNarrowSlots;
+constexpr int kFp4Slots = 512;  // 16-row tiles of a 4-bit cache where they are many: two
+constexpr int kMaxChains = kFp4Slots;
 constexpr int kNarrowWaves = 4;
 constexpr int kNarrowRows = 16, kNarrowKeys = 32 * kNarrowWaves;  // 32 keys for each wave
 

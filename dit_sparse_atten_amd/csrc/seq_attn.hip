@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     // Units of a tile: its set-up, then its steps; chain c holds the units from c
     // quota on.  A tile starts in the chain of its first step.
     const int setup = (int)p.item_cost;
-    const uint32_t chains = max(1, kNarrowSlots / p.kv_heads);
+    const uint32_t chains = max(1, p.slots / p.kv_heads);
     const uint64_t all_units = work_lds + (uint64_t)tiles * setup;
     // From 2^31 units on (2.7e11 keys of one head, set-ups among them): whole tiles, as
     // many to each chain.  (Not 2^32: an item's range is an int, and the last chain's
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
     const uint32_t quota =
         max((units + chains - 1) / chains, (uint32_t)(vast ? 1 : setup + p.min_chunk));
     const int last_chain = (int)((units + quota - 1) / quota) - 1;
-    for (int c = tid; c < kMaxChains; c += kThreads) starts[c] = 0x7fffffff;
+    for (int c = tid; c < (int)chains; c += kThreads) starts[c] = 0x7fffffff;
     uint32_t items = 0, split_sums = 0, unit_sum = 0;
     for (int i0 = 0; i0 < tiles; i0 += kThreads) {
       const int i = i0 + tid;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) seq_schedule_kernel(Params p) {
       }
     }
     __syncthreads();
-    for (int c = tid; c < kMaxChains; c += kThreads) p.chain_start[c] = starts[c];
+    for (int c = tid; c < (int)chains; c += kThreads) p.chain_start[c] = starts[c];
     if (tid == 0) {
       p.counts[0] = (int)min(items, (uint32_t)p.max_items);
       p.counts[1] = (int)min(split_sums & 0xffff, (uint32_t)p.max_splits);
@@ -435,12 +435,18 @@ struct Plan {
 // and 16 rows 172 us on 16-row tiles and 212 on 128-row ones, 24 and 32 rows (two
 // 16-row tiles) 365 and 212 us, 64 rows 716 and 213.
 Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int head_dim,
-               int64_t max_keys) {
+               int64_t max_keys, bool fp4) {
   Plan s;
   s.narrow = q_rows * group <= 16 * requests;
   s.tile_rows = s.narrow ? kNarrowRows : kWideRows;
   s.step_keys = s.narrow ? kNarrowKeys : kWideKeys;
-  s.slots = s.narrow ? kNarrowSlots : kWideSlots;
+  // 16-row tiles of a 4-bit cache: one workgroup of eight waves on a compute unit, or two
+  // of four where there are more tiles than units, whose starts and joins then lie under
+  // each other's walks.  (One against two, 8 key heads, D = 128: 512 requests of 750 tokens
+  // 138 / 106 us, 128 of 3,000 90 / 77, 64 of 6,000 80 / 76, 64 of up to 32,768 162 / 164;
+  // fewer tiles, 16 requests 30.4 / 31.6.)
+  const bool pairs = fp4 && requests * kv_heads > kNarrowSlots;
+  s.slots = !s.narrow ? kWideSlots : pairs ? kFp4Slots : kNarrowSlots;
   s.min_chunk = s.narrow ? 1 : 2;
   s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);
   // Of one key head: no more than 2 `slots` partials over all of them.  Tiles cut
@@ -459,7 +465,8 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // list may cut them into more than one round of parts.  (16 tiles x 8 key heads,
   // listed against not: 4,096 keys 59 / 54 us, 16,384 keys 146 / 143, 32,768 keys
   // 272 / 294.)
-  s.unlisted = requests <= 64 && s.max_tiles <= 64 && s.max_tiles * kv_heads <= s.slots &&
+  s.unlisted = requests <= 64 && s.max_tiles <= 64 &&
+               s.max_tiles * kv_heads <= (s.narrow ? kNarrowSlots : kWideSlots) &&
                (s.narrow || s.max_tiles * kv_heads * std::min<int64_t>(max_keys, kMaxKeys) <=
                                 80 * (int64_t)s.slots * s.step_keys);
   const int dim = head_dim <= 64 ? 64 : 128;
@@ -517,7 +524,8 @@ int run(Params p, int32_t dtype, Keys kind, int64_t max_keys, float scale, void*
   if ((int64_t)p.q_rows * p.group > 0x7fffff00)
     return dsa::set_error(DSA_EUNSUPPORTED, "%s: more than 2^31 query rows per key head", who);
   if (p.q_rows == 0) return DSA_OK;
-  const Plan s = make_plan(p.q_rows, p.requests, p.group, p.kv_heads, p.head_dim, max_keys);
+  const Plan s = make_plan(p.q_rows, p.requests, p.group, p.kv_heads, p.head_dim, max_keys,
+                           kind == kFp4Pages);
   // (a launch counts its threads, 256 for each item and key head, in 32 bits)
   if (s.max_items > kMaxItems || (!s.narrow && s.max_items * p.kv_heads >= 1 << 24))
     return dsa::set_error(DSA_EUNSUPPORTED, "%s: too many query tiles (%lld)", who,
@@ -564,7 +572,7 @@ int run(Params p, int32_t dtype, Keys kind, int64_t max_keys, float scale, void*
     const dim3 lists((unsigned)(1 + outside)), threads(small ? 256 : 1024);
     auto schedule = [&](auto kernel) { hipLaunchKernelGGL(kernel, lists, threads, 0, stream, p); };
     if (s.narrow) {
-      groups = std::max(1, kNarrowSlots / p.kv_heads) * p.kv_heads;
+      groups = std::max(1, s.slots / p.kv_heads) * p.kv_heads;
       small ? schedule(seq_schedule_kernel<256, true>) : schedule(seq_schedule_kernel<1024, true>);
     } else {
       small ? schedule(seq_schedule_kernel<256, false>) : schedule(seq_schedule_kernel<1024, false>);
@@ -586,7 +594,9 @@ extern "C" size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requ
   if (q_rows <= 0 || requests < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 ||
       head_dim <= 0 || max_keys < 0)
     return 0;
-  return seq::make_plan(q_rows, requests, heads / kv_heads, kv_heads, head_dim, max_keys).bytes;
+  // (a 4-bit cache needs as much room as a 16-bit one, or more)
+  return seq::make_plan(q_rows, requests, heads / kv_heads, kv_heads, head_dim, max_keys, true)
+      .bytes;
 }
 
 extern "C" int dsa_packed_attention(const void* q, const void* k, const void* v, void* o,

@@ -135,24 +135,24 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const Params& p, uint
                    any ? (uint32_t)bytes : 0u);
 }
 
-// 16 rows x the item's keys: eight waves, 64 keys at a time each (wave w those from 64 w,
-// 64 w + 512, ..), joined at the end.  Bound by the reads of the cache: codes and scales
-// go to registers a turn ahead, 70 KB on their way on a compute unit.  Lane (q4, c16) =
+// 16 rows x the item's keys: kWaves waves, 64 keys at a time each (wave w those from 64 w,
+// 64 (w + kWaves), ..), joined at the end.  Bound by the reads of the cache: codes and
+// scales go to registers a turn ahead, 70 KB on their way on a compute unit, by eight waves
+// of one workgroup or four each of two.  Lane (q4, c16) =
 // (lane / 16, lane % 16) holds group q4 of the keys 16 i + c16, row c16's scores of the
 // keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
-constexpr int kFp4Waves = 8;
-constexpr int kFp4Keys = 64;                          // of a wave's turn
-constexpr int kFp4Turn = kFp4Waves * kFp4Keys;        // of the workgroup's
+constexpr int kFp4Keys = 64;  // of a wave's turn
 
-template <typename T, int kD>
-__global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Params p) {
+template <typename T, int kD, int kWaves>
+__global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p) {
   typedef dsa::Elem<T> E;
   typedef typename E::x8 x8;
   constexpr int kRow = kD * 2;
+  constexpr int kTurn = kWaves * kFp4Keys;  // keys of the workgroup's turn
   constexpr int kStage = kFp4Keys * kRow;  // a wave's values of a turn, expanded
   constexpr int kDt = kD / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_v[kFp4Waves * kStage];
-  __shared__ float join_ml[2][kFp4Waves][16];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_v[kWaves * kStage];
+  __shared__ float join_ml[2][kWaves][16];
   constexpr int kJoinRow = kD + 4;  // floats
   static_assert(kNarrowRows * kJoinRow * 4 <= kStage, "a wave joins through its own stage");
   const int tid = threadIdx.x;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
 
   // Pages of a window of 16 turns: lane l holds granule l & 3 of turn l / 4.
   auto window_ids = [&](int window) -> int {
-    const int key = key_first + (window * 16 + (lane >> 2)) * kFp4Turn + (lane & 3) * 16;
+    const int key = key_first + (window * 16 + (lane >> 2)) * kTurn + (lane & 3) * 16;
     return key < kend ? page_at(p, it.request, key) : -1;
   };
   int ids = window_ids(0), ids_next = window_ids(1);
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
     t.bad = (int)(bad_ids >> ((turn & 15) * 4)) & 15;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int key = key_first + turn * kFp4Turn + 16 * i;
+      const int key = key_first + turn * kTurn + 16 * i;
       const int row = key & ((1 << p.page_shift) - 1);
       const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, (turn & 15) * 4 + i);
       const __amdgpu_buffer_rsrc_t rsrc =
@@ -357,15 +357,15 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
   if (key_first < kend) {
 #pragma unroll 1
     for (int turn = 0;; turn += 2) {
-      const int key0 = key_first + turn * kFp4Turn;
+      const int key0 = key_first + turn * kTurn;
       load(turn + 1, odd);
       __builtin_amdgcn_sched_barrier(0);
       compute(even, key0);
-      if (key0 + kFp4Turn >= kend) break;
+      if (key0 + kTurn >= kend) break;
       load(turn + 2, even);
       __builtin_amdgcn_sched_barrier(0);
-      compute(odd, key0 + kFp4Turn);
-      if (key0 + 2 * kFp4Turn >= kend) break;
+      compute(odd, key0 + kTurn);
+      if (key0 + 2 * kTurn >= kend) break;
     }
   }
 
@@ -390,15 +390,17 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
     join_ml[1][wave][c16] = l_wave;
   }
   dsa::lds_barrier();
-  // Thread (r, c): row r, dims 4 c .. 4 c + 3.
-  const int r = tid / (kD / 4), d0 = tid % (kD / 4) * 4;
-  const int out_row = it.tile * kNarrowRows + r;
-  if (r < kNarrowRows && out_row < rows) {
-    float m_all = -INFINITY, l_all = 0.f, w[kFp4Waves];
+  // Thread (r, c): row r and those kWaves * 256 / kD further on, dims 4 c .. 4 c + 3.
+  const int d0 = tid % (kD / 4) * 4;
 #pragma unroll
-    for (int i = 0; i < kFp4Waves; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
+  for (int r = tid / (kD / 4); r < kNarrowRows; r += kWaves * 64 / (kD / 4)) {
+    const int out_row = it.tile * kNarrowRows + r;
+    if (out_row >= rows) break;
+    float m_all = -INFINITY, l_all = 0.f, w[kWaves];
 #pragma unroll
-    for (int i = 0; i < kFp4Waves; ++i) {
+    for (int i = 0; i < kWaves; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
       const float mi = join_ml[0][i][r];
       // (no finite score: l is 0, or NaN from NaN scores)
       w[i] = mi == -INFINITY ? join_ml[1][i][r] : __builtin_amdgcn_exp2f(mi - m_all);
@@ -406,7 +408,7 @@ __global__ void __launch_bounds__(kFp4Waves * 64, 1) seq_narrow_fp4_kernel(Param
     }
     dsa_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kFp4Waves; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
       const dsa_f32x4 x = *reinterpret_cast<const dsa_f32x4*>(
           reinterpret_cast<const float*>(lds_v + i * kStage) + r * kJoinRow + d0);
 #pragma unroll

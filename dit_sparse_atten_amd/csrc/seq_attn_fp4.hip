@@ -7,8 +7,10 @@ namespace seq {
 
 template <typename T, int kD>
 void launch_fp4(const Params& p, bool narrow, dim3 grid, hipStream_t stream) {
-  if (narrow)
-    hipLaunchKernelGGL((seq_narrow_fp4_kernel<T, kD>), grid, dim3(kFp4Waves * 64), 0, stream, p);
+  if (narrow && p.slots == kFp4Slots)
+    hipLaunchKernelGGL((seq_narrow_fp4_kernel<T, kD, 4>), grid, dim3(256), 0, stream, p);
+  else if (narrow)
+    hipLaunchKernelGGL((seq_narrow_fp4_kernel<T, kD, 8>), grid, dim3(512), 0, stream, p);
   else if (kD == 128 && p.head_dim <= 96)
     hipLaunchKernelGGL((seq_wide_fp4_kernel<T, kD, kD == 128 ? 96 : kD>), grid, dim3(256), 0,
                        stream, p);

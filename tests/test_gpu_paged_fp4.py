@@ -378,6 +378,27 @@ def test_many_requests(cuda_device, requests):
     _check(out, lse, cache.expected(q, q_lens), 64, 60, cache.v_max())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("requests,heads", [(300, (8, 1, 128)), (43, (12, 6, 40)),
+                                            (33, (8, 8, 64)), (7, (64, 64, 96))], ids=str)
+def test_more_tiles_than_compute_units(cuda_device, dtype, requests, heads):
+    """Chains of short and long tiles, one cut over many chains, requests without keys or
+    new tokens, pages outside the cache."""
+    h, kh, dim = heads
+    g = torch.Generator().manual_seed(requests)
+    kv_lens = torch.randint(0, 400, (requests,), generator=g).tolist()
+    kv_lens[2], kv_lens[5] = 6000, 1700
+    q_lens = [int(i % 7 != 3) for i in range(requests)]
+    cache = _Cache(kv_lens, 16, kh, dim, 32, cuda_device)
+    cache.table[2][200] = cache.table[5][0] = -1
+    q = _rows((sum(q_lens), h, dim), DTYPES[dtype], 33, cuda_device)
+    args = (q, *cache.args(cuda_device), _starts(q_lens, cuda_device))
+    out, lse = ops.paged_attention_fp4(*args, return_lse=True)
+    _check(out, lse, cache.expected(q, q_lens), dim, 6000, cache.v_max())
+    again = ops.paged_attention_fp4(*args, return_lse=True)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
 def _angles(positions, rot):
     rate = 100.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
     angle = torch.arange(positions, dtype=torch.float64)[:, None] * rate

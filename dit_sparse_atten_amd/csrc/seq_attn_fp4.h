@@ -139,9 +139,35 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const Params& p, uint
 // 64 (w + kWaves), ..), joined at the end.  Bound by the reads of the cache: codes and
 // scales go to registers a turn ahead, 70 KB on their way on a compute unit, by eight waves
 // of one workgroup or four each of two.  Lane (q4, c16) =
-// (lane / 16, lane % 16) holds group q4 of the keys 16 i + c16, row c16's scores of the
-// keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
+// (lane / 16, lane % 16) holds the dims kD / 4 q4 .. of the keys 16 i + c16, row c16's scores
+// of the keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
 constexpr int kFp4Keys = 64;  // of a wave's turn
+
+// A lane's codes of a key: 32, or 16 where kD = 64, so that no lane is without.  (64 requests
+// of 12,000 tokens, 8 key heads, D = 64: 99 us with 32 codes in half the lanes, 96 so; 128
+// of 3,000 59 and 56, 512 of 750 87 and 79.)
+template <int kBytes>
+struct Codes;
+template <>
+struct Codes<16> {
+  typedef dsa_u32x4 type;
+  static __device__ __forceinline__ type load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at, int from) {
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, from, 2);
+  }
+  static __device__ __forceinline__ fp4_x8 operand(type k) {
+    return fp4_x8{(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  }
+};
+template <>
+struct Codes<8> {
+  typedef dsa_u32x2 type;
+  static __device__ __forceinline__ type load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at, int from) {
+    return __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, from, 2);
+  }
+  static __device__ __forceinline__ fp4_x8 operand(type k) {
+    return fp4_x8{(int)k[0], (int)k[1], 0, 0, 0, 0, 0, 0};
+  }
+};
 
 template <typename T, int kD, int kWaves>
 __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p) {
@@ -151,6 +177,8 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   constexpr int kTurn = kWaves * kFp4Keys;  // keys of the workgroup's turn
   constexpr int kStage = kFp4Keys * kRow;  // a wave's values of a turn, expanded
   constexpr int kDt = kD / 16;
+  constexpr int kLaneDims = kD / 4;
+  typedef Codes<kLaneDims / 2> C;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v[kWaves * kStage];
   __shared__ float join_ml[2][kWaves][16];
   constexpr int kJoinRow = kD + 4;  // floats
@@ -162,9 +190,10 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   const int groups = fp4::groups_of(p.head_dim);
   const fp4::Layout at(groups, p.page_shift);
   const int block_bytes = fp4::row_bytes(groups) << p.page_shift;
-  const uint32_t dead = q4 < groups ? 0u : dsa::kDeadChunk;
-  const uint32_t code_at = (uint32_t)(c16 * at.code_row + q4 * 16) | dead;
-  const uint32_t scale_at = (uint32_t)(c16 * 4 + q4) | dead;
+  const int group_of = q4 * kLaneDims / 32;
+  const uint32_t dead = group_of < groups ? 0u : dsa::kDeadChunk;
+  const uint32_t code_at = (uint32_t)(c16 * at.code_row + q4 * kLaneDims / 2) | dead;
+  const uint32_t scale_at = (uint32_t)(c16 * 4 + group_of) | dead;
 
   auto run = [&](const Item& it, const int h) __attribute__((always_inline)) {
   const int rows = it.n * p.group;
@@ -180,8 +209,12 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
-    raw[0].load(qrow, 16 * q4, p.head_dim);
-    raw[1].load(qrow, 64 + 16 * q4, p.head_dim);
+    // The products' elements 32 q4 .. 32 q4 + 31 are those that the keys' lane q4 holds; the
+    // queries' lane q4 has 16 q4 .. and 64 + 16 q4 ...  (kD = 64: the keys' lanes hold the
+    // dims 16 q4 .. and 16 zeros, so that every other query lane meets zeros only.)
+    const int d0 = kD == 128 ? 16 * q4 : q4 & 1 ? kD : 8 * q4;
+    raw[0].load(qrow, d0, p.head_dim);
+    raw[1].load(qrow, kD / 2 + d0, p.head_dim);
   }
 
   // Pages of a window of 16 turns: lane l holds granule l & 3 of turn l / 4.
@@ -193,7 +226,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   uint64_t bad_ids = __ballot((unsigned)ids >= (unsigned)p.pages);
 
   struct Turn {
-    dsa_u32x4 k[4], v[4];
+    typename C::type k[4], v[4];
     uint32_t ks[4], vs[4];
     int bad;  // granules (bits 0..3) that take no part
   };
@@ -211,10 +244,9 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
       const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(ids, (turn & 15) * 4 + i);
       const __amdgpu_buffer_rsrc_t rsrc =
           fp4_rsrc(p, page, h, block_bytes, page < (uint32_t)p.pages);
-      t.k[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at, row * at.code_row, 2);
+      t.k[i] = C::load(rsrc, code_at, row * at.code_row);
       t.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.k_scales + 4 * row, 2);
-      t.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at,
-                                                     at.v_codes + row * at.code_row, 2);
+      t.v[i] = C::load(rsrc, code_at, at.v_codes + row * at.code_row);
       t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.v_scales + 4 * row, 2);
     }
   };
@@ -225,8 +257,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   Turn even, odd;
   load(0, even);
   __builtin_amdgcn_sched_barrier(0);
-  // The row's query in its terms: bytes 0..15 of the lane are the dims 16 q4 .., 16..31
-  // the dims 64 + 16 q4 ...
+  // The row's query in its terms: bytes 0..15 of the lane are raw[0]'s dims, 16..31 raw[1]'s.
   fp4_x8 qf[kTerms<T>];
   int q_scale[kTerms<T>];
   {
@@ -269,7 +300,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
     dsa_f32x4 s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const fp4_x8 a = {(int)t.k[i][0], (int)t.k[i][1], (int)t.k[i][2], (int)t.k[i][3], 0, 0, 0, 0};
+      const fp4_x8 a = C::operand(t.k[i]);
       s[i] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = kTerms<T> - 1; n >= 0; --n)
@@ -283,12 +314,11 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
       const bool number = t.vs[i] != 255u;
       unfinite |= held && !number;
       const float scale = fp4::scale_of(value_scale<T>(t.vs[i], held && number));
-      if (kD == 128 || q4 < 2) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<x8*>(stage + (16 * i + c16) * kRow + v_swz(c16, 4 * q4 + j) * 16) =
-              fp4::expand(t.v[i][j], scale, T());
-      }
+      for (int j = 0; j < kLaneDims / 8; ++j)
+        *reinterpret_cast<x8*>(stage + (16 * i + c16) * kRow +
+                               v_swz(c16, kLaneDims / 8 * q4 + j) * 16) =
+            fp4::expand(t.v[i][j], scale, T());
     }
     own_lds_order();
     if (key0 + kFp4Keys > lim_first) {

@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(kThreads) paged_write_rotary_kernel(TurnParams
   turn_rows<T, kHalves>(p, which, head0, heads);
 }
 
-// 16-bit rows to 4-bit rows.  A thread takes a chunk of 8 dims, four neighbours a group;
+// 16-bit rows to 4-bit rows, bound by memory (57,600 tokens x 12 heads x 128, 447 MB: 86
+// to 94 us).  A thread takes a chunk of 8 dims, four neighbours a group;
 // with halves it reads the chunk that its own turns with too.  A code may hang on the
 // last bit of what it rounds, so the turned element is the exact one rounded to float32:
 // in 64 bits the products of a 16-bit and a 32-bit float are exact, and their sum is
@@ -250,13 +251,14 @@ struct ReadParams {
   int64_t cache_sp, cache_sh;
   void* dst[2];            // [count, page_size, kv_heads, head_dim]
   const int32_t* list;     // pages, or null: all of them
-  int64_t units;           // of 16 tokens and a head
+  uint32_t units;          // of 16 tokens and a head (up to 2^29, by the launch's bound)
   int32_t pages, kv_heads, head_dim, page_shift;
 };
 
 // Rows of a 4-bit cache, keys or values (y): a lane to 8 dims, four bytes in and 16 out.
 // 16 tokens of a head (1 KB of codes in a row) at a time, the heads of the same tokens
-// one after the other, which together fill the memory that they go to.
+// one after the other, which together fill the memory that they go to.  Bound by memory:
+// 57,600 tokens x 12 heads x 128 (447 MB) 100 us, 4.5 TB/s, a large copy 5.0.
 //
 // kOnce: the values go past the caches, in reads of 192 MB and more of them, which the
 // 256 MB cache would not keep for whoever takes them up.  (Read alone, and with a
@@ -283,14 +285,14 @@ __global__ void __launch_bounds__(kThreads) paged_read_fp4_kernel(ReadParams p) 
   int64_t to[kReadTurns];
 #pragma unroll
   for (int i = 0; i < kReadTurns; ++i) {
-    const int64_t unit = ((int64_t)blockIdx.x * kReadTurns + i) * each + unit0;
+    const uint32_t unit = (blockIdx.x * kReadTurns + i) * each + unit0;
     code[i] = scale[i] = 0;
     to[i] = -1;
     if (unit >= p.units) continue;
-    const int64_t tokens = unit / p.kv_heads;  // 16 of a listed page's
-    const int head = (int)(unit - tokens * p.kv_heads);
+    const uint32_t tokens = unit / (uint32_t)p.kv_heads;  // 16 of a listed page's
+    const int head = (int)(unit - tokens * (uint32_t)p.kv_heads);
     const int64_t index = tokens >> per_page;
-    const int row = (int)(tokens & ((1 << per_page) - 1)) * kReadRows + in_unit;
+    const int row = (int)(tokens & ((1u << per_page) - 1)) * kReadRows + in_unit;
     to[i] = (((index << p.page_shift) + row) * p.kv_heads + head) * p.head_dim + 8 * c;
     const int64_t page = p.list ? p.list[index] : index;
     if (page < 0 || page >= p.pages) continue;  // (zeros)
@@ -511,15 +513,16 @@ extern "C" int dsa_paged_read_fp4(const void* cache, const int64_t* strides, voi
   p.dst[0] = k;
   p.dst[1] = v;
   p.list = list;
-  p.units = (int64_t)count * kv_heads * (page_size / kReadRows);
+  const int64_t units = (int64_t)count * kv_heads * (page_size / kReadRows);
   p.pages = pages; p.kv_heads = kv_heads; p.head_dim = head_dim;
   p.page_shift = __builtin_ctz(page_size);
   const int64_t each = kReadTurns * read_units(fp4::groups_of(head_dim));
-  const int64_t groups = (p.units + each - 1) / each;
+  const int64_t groups = (units + each - 1) / each;
   if (groups >= 1 << 24) return dsa::set_error(DSA_EUNSUPPORTED, "%s: too many rows", who);
+  p.units = (uint32_t)units;
   dsa::clear_error();
   const dim3 grid((unsigned)groups, 2);
-  const bool once = p.units * kReadRows * head_dim * 4 >= kOnceBytes;  // keys and values
+  const bool once = units * kReadRows * head_dim * 4 >= kOnceBytes;  // keys and values
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, p);
   };

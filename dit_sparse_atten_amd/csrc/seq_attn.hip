@@ -443,7 +443,7 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // 16-row tiles of a 4-bit cache: one workgroup of eight waves on a compute unit, or two
   // of four where there are more tiles than units, whose starts and joins then lie under
   // each other's walks.  (One against two, 8 key heads, D = 128: 512 requests of 750 tokens
-  // 138 / 106 us, 128 of 3,000 90 / 77, 64 of 6,000 80 / 76, 64 of up to 32,768 162 / 164;
+  // 138 / 106 us, 128 of 3,000 90 / 77, 64 of 6,000 80 / 76, 64 of 1,000 to 16,000 162 / 164;
   // fewer tiles, 16 requests 30.4 / 31.6.)
   const bool pairs = fp4 && requests * kv_heads > kNarrowSlots;
   s.slots = !s.narrow ? kWideSlots : pairs ? kFp4Slots : kNarrowSlots;

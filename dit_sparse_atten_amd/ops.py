@@ -1272,7 +1272,7 @@ def _sequence_buffers(q, layout, q_start, scale, out, return_lse, max_keys):
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if out is None:
-        out = torch.empty((rows, heads, head_dim), dtype=q.dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         if out.device != device:
             raise ValueError("out must have q's shape, type and device")
@@ -1549,7 +1549,7 @@ def _write_turned(function, what, k, v, caches, slots, positions, cos_sin, q, q_
     out, at_out = q_out, 0
     if q is not None:
         if out is None:
-            out = torch.empty((tokens, heads, head_dim), dtype=q.dtype, device=device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             _aligned("q_out", out)
         at_out = out.data_ptr()
@@ -1639,7 +1639,7 @@ def paged_read_fp4(cache, head_dim, pages=None, dtype=torch.bfloat16):
     count = total if pages is None else pages.shape[0]
     shape = (count, page_size, kv_heads, head_dim)
     k = torch.empty(shape, dtype=dtype, device=device)
-    v = torch.empty(shape, dtype=dtype, device=device)
+    v = torch.empty_like(k)
     if count and kv_heads:
         _call(lib.dsa_paged_read_fp4, "dsa_paged_read_fp4", device, cache.data_ptr(), strides,
               k.data_ptr(), v.data_ptr(), code, total, page_size, kv_heads, head_dim,

@@ -399,6 +399,15 @@ def test_more_tiles_than_compute_units(cuda_device, dtype, requests, heads):
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
 
 
+def test_more_key_heads_than_chains(cuda_device):
+    kv_lens = [1500, 0, 40]
+    cache = _Cache(kv_lens, 16, 600, 8, 34, cuda_device)
+    q = _rows((3, 600, 8), torch.bfloat16, 35, cuda_device)
+    out, lse = ops.paged_attention_fp4(q, *cache.args(cuda_device), _starts([1] * 3, cuda_device),
+                                       return_lse=True)
+    _check(out, lse, cache.expected(q, [1, 1, 1]), 8, 1500, cache.v_max())
+
+
 def _angles(positions, rot):
     rate = 100.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
     angle = torch.arange(positions, dtype=torch.float64)[:, None] * rate

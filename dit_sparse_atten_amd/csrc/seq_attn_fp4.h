@@ -142,9 +142,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const Params& p, uint
 // 64 (w + kWaves), ..), joined at the end.  Bound by the reads of the cache: codes and
 // scales go to registers a turn ahead, 70 KB on their way on a compute unit, by eight waves
 // of one workgroup or four each of two.  (64 requests of 1,000 to 16,000 tokens, 8 key
-// heads: D = 128 164 us, 6.0 TB/s, of 7.0 for a plain streaming read.  D = 64, 64 requests
-// of 12,000: 96 us, 4.4 TB/s; a key costs 4 instructions a wave whatever its dims, and
-// waves wait for each other's and their own, a fifth of the time for data.)  Lane (q4, c16) =
+// heads: D = 128 164 us, 6.0 TB/s, of 7.0 for a plain streaming read.  64 of 12,000, D = 64:
+// 96 us, 4.4 TB/s; 10 us of each are the schedule, the join and their launches, and with
+// half the bytes a turn waits a fifth of its time for data and twice that to be issued.)
+// Lane (q4, c16) =
 // (lane / 16, lane % 16) holds the dims kD / 4 q4 .. of the keys 16 i + c16, row c16's scores
 // of the keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
 constexpr int kFp4Keys = 64;  // of a wave's turn

@@ -237,6 +237,9 @@ SIGNATURES = {
         _c_int, _c_int, _c_ptr,                    # causal, fill, lse
         _c_ptr, _c_size, _c_ptr,                   # workspace, workspace_bytes, stream
     )),
+    "dsa_paged_attention_fp4_workspace_bytes": (_c_size, (
+        _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,  # q_rows, requests, heads, kv_heads, head_dim, max_keys
+    )),
     "dsa_seq_attention_workspace_bytes": (_c_size, (
         _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,  # q_rows, requests, heads, kv_heads, head_dim, max_keys
     )),

@@ -76,7 +76,7 @@ struct Params {
   int32_t max_tiles, max_items, max_splits, max_slots;  // room in the lists, per key head
   float item_cost, part_cost, merge_cost;    // of an item and a partial, in key steps
   int32_t* counts;             // items, split tiles, items that run by head groups
-  int32_t* chain_start;        // [kMaxChains] first item of each chain (16-row tiles)
+  int32_t* chain_start;        // first item of each chain (16-row tiles)
   int32_t* tile_base;          // [requests + 1] tiles before each sequence
   Item* items;
   Item* splits;                // split tiles: slot = the first of `parts` slots

@@ -445,7 +445,7 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // each other's walks.  (One against two, 8 key heads, D = 128: 512 requests of 750 tokens
   // 138 / 106 us, 128 of 3,000 90 / 77, 64 of 6,000 80 / 76, 64 of 1,000 to 16,000 162 / 164;
   // fewer tiles, 16 requests 30.4 / 31.6.)
-  const bool pairs = fp4 && requests * kv_heads > kNarrowSlots;
+  const bool pairs = fp4 && s.narrow && requests * kv_heads > kNarrowSlots;
   s.slots = !s.narrow ? kWideSlots : pairs ? kFp4Slots : kNarrowSlots;
   s.min_chunk = s.narrow ? 1 : 2;
   s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);
@@ -472,7 +472,7 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   const int dim = head_dim <= 64 ? 64 : 128;
   s.counts = 0;
   s.chains = 256;
-  s.base = s.chains + kMaxChains * sizeof(int32_t);
+  s.base = s.chains + (pairs ? kFp4Slots : kNarrowSlots) * sizeof(int32_t);
   s.items = s.base + round256((size_t)(requests + 1) * sizeof(int32_t));
   s.splits = s.items + (size_t)s.max_items * sizeof(Item);
   s.parts = s.splits + round256((size_t)s.max_splits * sizeof(Item));
@@ -588,15 +588,29 @@ int run(Params p, int32_t dtype, Keys kind, int64_t max_keys, float scale, void*
 }  // namespace
 }  // namespace seq
 
-extern "C" size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32_t heads,
-                                                    int32_t kv_heads, int32_t head_dim,
-                                                    int64_t max_keys) {
+namespace {
+
+size_t workspace_bytes(int32_t q_rows, int32_t requests, int32_t heads, int32_t kv_heads,
+                       int32_t head_dim, int64_t max_keys, bool fp4) {
   if (q_rows <= 0 || requests < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0 ||
       head_dim <= 0 || max_keys < 0)
     return 0;
-  // (a 4-bit cache needs as much room as a 16-bit one, or more)
-  return seq::make_plan(q_rows, requests, heads / kv_heads, kv_heads, head_dim, max_keys, true)
+  return seq::make_plan(q_rows, requests, heads / kv_heads, kv_heads, head_dim, max_keys, fp4)
       .bytes;
+}
+
+}  // namespace
+
+extern "C" size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32_t heads,
+                                                    int32_t kv_heads, int32_t head_dim,
+                                                    int64_t max_keys) {
+  return workspace_bytes(q_rows, requests, heads, kv_heads, head_dim, max_keys, false);
+}
+
+extern "C" size_t dsa_paged_attention_fp4_workspace_bytes(int32_t q_rows, int32_t requests,
+                                                          int32_t heads, int32_t kv_heads,
+                                                          int32_t head_dim, int64_t max_keys) {
+  return workspace_bytes(q_rows, requests, heads, kv_heads, head_dim, max_keys, true);
 }
 
 extern "C" int dsa_packed_attention(const void* q, const void* k, const void* v, void* o,

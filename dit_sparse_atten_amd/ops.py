@@ -1213,9 +1213,11 @@ def paged_write(k, v, k_cache, v_cache, slots):
 
 
 @functools.lru_cache(maxsize=256)
-def _sequence_workspace_bytes(q_rows, requests, heads, kv_heads, head_dim, max_keys):
-    return _lib.load().dsa_seq_attention_workspace_bytes(q_rows, requests, heads, kv_heads,
-                                                         head_dim, max_keys)
+def _sequence_workspace_bytes(fp4, q_rows, requests, heads, kv_heads, head_dim, max_keys):
+    lib = _lib.load()
+    size = (lib.dsa_paged_attention_fp4_workspace_bytes if fp4
+            else lib.dsa_seq_attention_workspace_bytes)
+    return size(q_rows, requests, heads, kv_heads, head_dim, max_keys)
 
 
 def _out_strides(q, out):
@@ -1264,7 +1266,7 @@ def _attention_layout(paged, q, k, v, out):
     return copies, strides, rows, heads, kv_heads, head_dim, code
 
 
-def _sequence_buffers(q, layout, q_start, scale, out, return_lse, max_keys):
+def _sequence_buffers(q, layout, q_start, scale, out, return_lse, max_keys, fp4=False):
     """(scale, out, lse, workspace) of an attention call."""
     _, _, rows, heads, kv_heads, head_dim, _ = layout
     device = q.device
@@ -1279,7 +1281,8 @@ def _sequence_buffers(q, layout, q_start, scale, out, return_lse, max_keys):
         _aligned("out", out)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=device) if return_lse else None
     workspace = torch.empty(
-        _sequence_workspace_bytes(rows, q_start.shape[0] - 1, heads, kv_heads, head_dim, max_keys),
+        _sequence_workspace_bytes(fp4, rows, q_start.shape[0] - 1, heads, kv_heads, head_dim,
+                                  max_keys),
         dtype=torch.uint8, device=device)
     return scale, out, lse, workspace
 
@@ -1695,7 +1698,7 @@ def paged_attention_fp4(q, cache, block_table, kv_lens, q_start, causal=True, sc
         return paged_attention_fp4(*_in_place(copies, q), cache, block_table, kv_lens, q_start,
                                    causal, scale, out, return_lse)
     scale, out, lse, workspace = _sequence_buffers(q, layout, q_start, scale, out, return_lse,
-                                                   width * page_size)
+                                                   width * page_size, fp4=True)
     if rows:
         _call(lib.dsa_paged_attention_fp4, "dsa_paged_attention_fp4", device, q.data_ptr(),
               cache.data_ptr(), out.data_ptr(), code, strides, rows, requests, heads, kv_heads,

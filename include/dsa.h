@@ -580,7 +580,8 @@ size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32
  * fp16 values of exponents above 13 count as of 13).  strides[6]: q (token, head) in
  * elements, cache (page, head) in BYTES, o (token, head) in elements; page_size up to
  * 2^20.  A key group that is not a number makes the rows that see it NaN, a value
- * group its dims of them.  All else, the workspace among it, as there.
+ * group its dims of them.  All else as there, but for the workspace's size
+ * (dsa_paged_attention_fp4_workspace_bytes, of the same arguments).
  */
 int dsa_paged_attention_fp4(const void* q, const void* cache, void* o, int32_t dtype,
                             const int64_t* strides, int32_t q_rows, int32_t requests,
@@ -589,6 +590,9 @@ int dsa_paged_attention_fp4(const void* q, const void* cache, void* o, int32_t d
                             int32_t table_width, const int32_t* kv_lens, const int32_t* q_start,
                             float scale, int32_t causal, int32_t fill, float* lse,
                             void* workspace, size_t workspace_bytes, hipStream_t stream);
+size_t dsa_paged_attention_fp4_workspace_bytes(int32_t q_rows, int32_t requests, int32_t heads,
+                                               int32_t kv_heads, int32_t head_dim,
+                                               int64_t max_keys);
 
 /*
  * Writes into a paged cache that turn keys and queries with their positions on the

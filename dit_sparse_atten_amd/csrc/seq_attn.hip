@@ -456,7 +456,9 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // 8 key heads: 16-row tiles of 4 requests, 1,024 keys 15.9 / 13.1 us (the host's
   // time), 1,536 keys 16.0 / 18.2; 128-row tiles of 2 requests, 512 keys 17.5 / 16.9,
   // 768 keys 19.3 / 21.7, 1,536 keys 22.7 / 36.1.
-  s.merge = max_keys > (s.narrow ? 1024 : 640) && s.slots >= kv_heads;
+  // A 4-bit cache's 16-row tiles take 512 keys a turn: 1,500 keys 15.9 / 13.9, 2,000 15.4 /
+  // 15.4, 3,000 17.0 / 18.9; 16 requests, 1,500 keys 18.0 / 14.2, 4,000 24.1 / 23.6.
+  s.merge = max_keys > (!s.narrow ? 640 : fp4 ? 2048 : 1024) && s.slots >= kv_heads;
   s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
   s.max_splits = std::min(s.max_tiles, s.max_slots / 2);
   s.max_items = s.max_tiles + s.max_slots;

@@ -535,6 +535,39 @@ def test_captured_step_replays_with_new_lengths(cuda_device):
             assert torch.equal(eager[name], captured[name]), (i, name)
 
 
+def test_captured_step_of_many_tiles(cuda_device):
+    """Chains and joins of a captured call follow the lengths of each replay."""
+    requests, kh, h, dim = 40, 8, 16, 128
+    cache = _Cache([2500] + [200] * (requests - 1), 16, kh, dim, 36, cuda_device)
+    data, table, lens = cache.args(cuda_device)
+    q = _rows((requests, h, dim), torch.bfloat16, 37, cuda_device)
+    start = _starts([1] * requests, cuda_device)
+
+    def call():
+        return ops.paged_attention_fp4(q, data, table, lens, start, return_lse=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for i in range(6):
+        kv_lens = [(0, 2500, 3, 1111, 2499, 700)[i]] + [(37 * r + 91 * i) % 201
+                                                        for r in range(1, requests)]
+        lens.copy_(_ints(kv_lens, cuda_device))
+        q.copy_(_rows(q.shape, q.dtype, 38 + i, cuda_device))
+        graph.replay()
+        got = [t.clone() for t in held]
+        torch.cuda.synchronize()
+        expected = call()
+        assert torch.equal(got[0], expected[0]) and torch.equal(got[1], expected[1]), i
+        cache.kv_lens = kv_lens
+        _check(got[0], got[1], cache.expected(q, [1] * requests), dim, 2500, cache.v_max())
+
+
 def test_calls_on_two_streams_and_two_graphs(cuda_device):
     """Calls that overlap, and graphs replayed in turn, keep their workspaces apart."""
     kv_lens = [9000, 500]

@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   typedef Codes<kLaneDims / 2> C;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v[kWaves * kStage];
   __shared__ float join_ml[2][kWaves][16];
+  __shared__ int join_row[2][16];  // token and head
   constexpr int kJoinRow = kD + 4;  // floats
   static_assert(kNarrowRows * kJoinRow * 4 <= kStage, "a wave joins through its own stage");
   const int tid = threadIdx.x;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   auto run = [&](const Item& it, const int h) __attribute__((always_inline)) {
   const int rows = it.n * p.group;
   const int row_c = min(it.tile * kNarrowRows + c16, rows - 1);
-  const int token = row_c / p.group;
+  const int token = (int)((uint32_t)row_c / (uint32_t)p.group);
   const int head = h * p.group + row_c - token * p.group;
   const int lim = p.causal ? max(0, min(it.m, it.m - it.n + token + 1)) : it.m;
   const int lim_first = __builtin_amdgcn_readlane(lim, 0);
@@ -425,6 +426,10 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   if (q4 == 0) {
     join_ml[0][wave][c16] = m_run;
     join_ml[1][wave][c16] = l_wave;
+    if (wave == 0) {
+      join_row[0][c16] = it.q0 + token;
+      join_row[1][c16] = head;
+    }
   }
   dsa::lds_barrier();
   // Thread (r, c): row r and those kWaves * 256 / kD further on, dims 4 c .. 4 c + 3.
@@ -433,15 +438,18 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   for (int r = tid / (kD / 4); r < kNarrowRows; r += kWaves * 64 / (kD / 4)) {
     const int out_row = it.tile * kNarrowRows + r;
     if (out_row >= rows) break;
-    float m_all = -INFINITY, l_all = 0.f, w[kWaves];
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) m_all = fmaxf(m_all, join_ml[0][i][r]);
+    float m_all = -INFINITY, l_all = 0.f, w[kWaves], m[kWaves], l[kWaves];
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-      const float mi = join_ml[0][i][r];
+      m[i] = join_ml[0][i][r];
+      l[i] = join_ml[1][i][r];
+      m_all = fmaxf(m_all, m[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
       // (no finite score: l is 0, or NaN from NaN scores)
-      w[i] = mi == -INFINITY ? join_ml[1][i][r] : __builtin_amdgcn_exp2f(mi - m_all);
-      l_all = fmaf(w[i], join_ml[1][i][r], l_all);
+      w[i] = m[i] == -INFINITY ? l[i] : __builtin_amdgcn_exp2f(m[i] - m_all);
+      l_all = fmaf(w[i], l[i], l_all);
     }
     dsa_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -460,8 +468,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
         po[kNarrowRows * (kD + 1) + r] = l_all;
       }
     } else {
-      const int out_token = it.q0 + out_row / late->group;
-      const int out_head = h * late->group + out_row % late->group;
+      const int out_token = join_row[0][r], out_head = join_row[1][r];
       const float inv = l_all > 0.f ? 1.f / l_all : (l_all == 0.f ? 0.f : l_all);
       if (d0 < late->head_dim) {
         typename E::x4 y;

@@ -1516,11 +1516,15 @@ def _on_device(name, t, device):
 def _write_turned(function, what, k, v, caches, slots, positions, cos_sin, q, q_out, halves):
     """A write of both kinds; returns the turned queries, or None."""
     device = caches[0].device
-    _on_device("k", k, device)
-    _on_device("v", v, device)
-    _on_device("slots", slots, device)
-    if q is not None:
-        _on_device("q", q, device)
+    try:
+        here = (k.device == device and v.device == device and slots.device == device
+                and (q is None or q.device == device))
+    except AttributeError:
+        here = False
+    if not here:
+        for name, t in (("k", k), ("v", v), ("slots", slots), ("q", q)):
+            if t is not None or name != "q":
+                _on_device(name, t, device)
     if q_out is not None:
         _on_device("q_out", q_out, device)
         if q is None:

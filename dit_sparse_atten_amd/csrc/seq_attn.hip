@@ -433,11 +433,16 @@ struct Plan {
 // Calls of at most 16 rows (tokens x heads of a group) per sequence on average,
 // decoding steps, run 16-row tiles.  32 requests of 8,000 tokens, 8 key heads: 8
 // and 16 rows 172 us on 16-row tiles and 212 on 128-row ones, 24 and 32 rows (two
-// 16-row tiles) 365 and 212 us, 64 rows 716 and 213.
+// 16-row tiles) 365 and 212 us, 64 rows 716 and 213.  A 4-bit cache streams faster: 24
+// and 32 rows 80 and 111 us, 40 and 48 rows 152 and 127 (D = 64: 63 and 94, 103 and 104),
+// and up to 64 rows in calls that leave compute units idle (4 requests of 2,000 tokens, 64
+// rows 16 and 25 us; 2 of 60,000 70 and 77).
 Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int head_dim,
                int64_t max_keys, bool fp4) {
   Plan s;
-  s.narrow = q_rows * group <= 16 * requests;
+  const int64_t rows = q_rows * group;
+  s.narrow = rows <= (fp4 ? 32 : 16) * requests ||
+             (fp4 && rows <= 64 * requests && rows * kv_heads <= 16 * kNarrowSlots);
   s.tile_rows = s.narrow ? kNarrowRows : kWideRows;
   s.step_keys = s.narrow ? kNarrowKeys : kWideKeys;
   // 16-row tiles of a 4-bit cache: one workgroup of eight waves on a compute unit, or two
@@ -445,7 +450,8 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // each other's walks.  (One against two, 8 key heads, D = 128: 512 requests of 750 tokens
   // 138 / 106 us, 128 of 3,000 90 / 77, 64 of 6,000 80 / 76, 64 of 1,000 to 16,000 162 / 164;
   // fewer tiles, 16 requests 30.4 / 31.6.)
-  const bool pairs = fp4 && s.narrow && requests * kv_heads > kNarrowSlots;
+  const bool pairs =
+      fp4 && s.narrow && std::max(requests, rows / 16) * kv_heads > kNarrowSlots;
   s.slots = !s.narrow ? kWideSlots : pairs ? kFp4Slots : kNarrowSlots;
   s.min_chunk = s.narrow ? 1 : 2;
   s.max_tiles = std::max<int64_t>(1, q_rows * group / s.tile_rows + requests);

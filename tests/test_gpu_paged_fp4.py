@@ -184,6 +184,26 @@ def test_every_bit_of_the_queries(cuda_device, dtype, n, m):
     _check(out, lse, expected, dim, m, 1.0, 0.0)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("requests,new,heads", [(37, 4, (64, 8, 128)), (34, 3, (16, 2, 64)),
+                                                (4, 16, (8, 2, 128)), (2, 13, (10, 2, 40)),
+                                                (5, 20, (16, 8, 96))], ids=str)
+def test_a_few_tokens_each(cuda_device, requests, new, heads, causal, dtype):
+    """Requests of up to 64 rows for each key head: several 16-row tiles of one, the last
+    of them part of a tile, more rows than keys."""
+    h, kh, dim = heads
+    g = torch.Generator().manual_seed(requests)
+    q_lens = torch.randint(0, new + 1, (requests,), generator=g).tolist()
+    kv_lens = torch.randint(0, 300, (requests,), generator=g).tolist()
+    kv_lens[1], q_lens[1] = 3500, new
+    cache = _Cache(kv_lens, 32, kh, dim, 50, cuda_device)
+    q = _rows((sum(q_lens), h, dim), DTYPES[dtype], 51, cuda_device)
+    out, lse = ops.paged_attention_fp4(q, *cache.args(cuda_device), _starts(q_lens, cuda_device),
+                                       causal=causal, return_lse=True)
+    _check(out, lse, cache.expected(q, q_lens, causal), dim, 3500, cache.v_max())
+
+
 @pytest.mark.parametrize("rows", [1, 2, 5, 9, 33])
 @pytest.mark.parametrize("keys", [20000, 33333])
 def test_long_split(cuda_device, rows, keys):

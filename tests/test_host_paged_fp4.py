@@ -207,14 +207,16 @@ def test_attention_refusals(lib, name, value, text):
 
 
 def test_workspace_sizes(lib):
-    """As over 16-bit pages; 512 workgroups of 16 rows instead of 256 where requests x key
-    heads are more than 256, and whole tiles up to 2,048 keys."""
+    """As over 16-bit pages; 16-row tiles up to 32 rows a request, or 64 where they leave
+    compute units idle, 512 workgroups for them instead of 256 where they are more, whole
+    tiles up to 2,048 keys."""
     size = lib.dsa_paged_attention_fp4_workspace_bytes
 
     def expected(rows, requests, heads, kv, dim, keys):
         group = heads // kv
-        narrow = rows * group <= 16 * requests
-        many = narrow and requests * kv > 256
+        narrow = rows * group <= 32 * requests or (
+            rows * group <= 64 * requests and rows * heads <= 4096)
+        many = narrow and max(requests, rows * group // 16) * kv > 256
         tile, slots, uncut = (16, 512 if many else 256, 2048) if narrow else (128, 512, 640)
         tiles = max(1, rows * group // tile + requests)
         cut = keys > uncut and slots >= kv
@@ -227,6 +229,8 @@ def test_workspace_sizes(lib):
     for case in ((8, 2, 4, 2, 64, 100), (32, 32, 64, 8, 128, 16384), (33, 33, 64, 8, 128, 16384),
                  (512, 512, 64, 8, 64, 1000), (300, 300, 4, 1, 40, 5000), (2, 2, 600, 600, 64, 2000),
                  (2, 2, 300, 300, 64, 2100), (4, 4, 32, 8, 128, 2048), (4, 4, 32, 8, 128, 2049),
+                 (128, 32, 64, 8, 128, 9000), (129, 32, 64, 8, 128, 9000), (64, 4, 32, 8, 128, 9000),
+                 (65, 4, 32, 8, 128, 9000), (128, 16, 64, 8, 128, 9000), (32, 2, 32, 2, 64, 9000),
                  (2500, 40, 32, 8, 128, 30000), (5, 0, 1, 1, 8, 0)):
         assert size(*case) == expected(*case), case
     for bad in ((0, 1, 1, 1, 64, 9), (1, -1, 1, 1, 64, 9), (1, 1, 3, 2, 64, 9), (1, 1, 1, 0, 64, 9),

@@ -14,9 +14,10 @@
 //
 // Values.  Their scales vary along the keys, which the product with P sums over, so
 // they are expanded to 16 bits (exactly: the conversion takes the scale) on the way into
-// LDS, and O^T = V^T P^T is that of the 16-bit cache.  A group that is not a number
-// enters as zeros, for 0 times it would reach rows that do not see its key, and the rows
-// that do are set to NaN at the end (unfinite_groups).
+// LDS, and O^T = V^T P^T is that of the 16-bit cache, P rounded to the input type (the
+// matrix operand's; by at most 2^-8 of a weight in bf16, below the cache's own error).  A
+// group that is not a number enters as zeros, for 0 times it would reach rows that do not
+// see its key, and the rows that do are set to NaN at the end (unfinite_groups).
 #pragma once
 
 #include "fp4.h"

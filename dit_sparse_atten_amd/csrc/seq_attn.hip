@@ -434,7 +434,7 @@ struct Plan {
 // decoding steps, run 16-row tiles.  32 requests of 8,000 tokens, 8 key heads: 8
 // and 16 rows 172 us on 16-row tiles and 212 on 128-row ones, 24 and 32 rows (two
 // 16-row tiles) 365 and 212 us, 64 rows 716 and 213.  A 4-bit cache streams faster: 24
-// and 32 rows 80 and 111 us, 40 and 48 rows 152 and 127 (D = 64: 63 and 94, 103 and 104),
+// and 32 rows 80 and 111 us, 40 and 48 rows 152 and 111 (D = 64: 63 and 94, 103 and 92),
 // and up to 64 rows in calls that leave compute units idle (4 requests of 2,000 tokens, 64
 // rows 16 and 25 us; 2 of 60,000 70 and 77).
 Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int head_dim,

@@ -544,7 +544,12 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5, qi = lane & 31;
   const int rows = it.n * p.group;
-  const int local = wave * 32 + qi;
+  // Of a tile of up to 64 rows two waves take each 32 rows, 32 of a step's keys each, and
+  // join at the end.  (32 requests of 8,000 tokens, 8 key heads, 64 rows each: 124 us with
+  // two of the waves idle, 111 so; 16 of 4,000, 40 key heads, 150 rows: 301 and 281.)
+  const bool half = rows - it.tile * kWideRows <= kWideRows / 2;
+  const int wave_row = (half ? wave & 1 : wave) * 32;
+  const int local = wave_row + qi;
   const int row = it.tile * kWideRows + local;
   const bool row_ok = row < rows;
   const int row_c = min(row, rows - 1);
@@ -552,7 +557,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const int head = h * p.group + row_c - token * p.group;
   // Keys [0, lim) are visible to the lane's row.
   const int lim = p.causal ? max(0, min(it.m, it.m - it.n + token + 1)) : it.m;
-  const bool wave_active = it.tile * kWideRows + wave * 32 < rows;
+  const bool wave_active = it.tile * kWideRows + wave_row < rows;
   const int lim_first = __builtin_amdgcn_readlane(lim, 0);
   const int lim_last = __builtin_amdgcn_readlane(lim, 31);
   // Keys the tile's last row sees.
@@ -691,18 +696,21 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
 
-  // Step s from stage `from`; the values of step s + 1 go to the other stage meanwhile.
-  auto compute = [&](int from, const unsigned char* k_lds, const unsigned char* s_lds, int s,
+  // Step s from stage `from`, the wave's 32 or 64 keys of it; the values of step s + 1 go to
+  // the other stage meanwhile.
+  auto compute = [&](auto tiles, int from, const unsigned char* k_lds, const unsigned char* s_lds, int s,
                      int bad) __attribute__((always_inline)) {
-    const int key0 = s * kWideKeys;
-    const unsigned char* const v_lds = lds_v + from * kStage;
+    constexpr int kKt = decltype(tiles)::value;  // tiles of 32 keys
+    const int row0 = kKt == 2 ? 0 : (wave >> 1) * 32;
+    const int key0 = s * kWideKeys + row0;
+    const unsigned char* const v_lds = lds_v + from * kStage + row0 * kRow;
     __builtin_amdgcn_s_setprio(0);
-    dsa_f32x16 sacc[2];
-    dsa_u32x4 codes[2][kSteps];
-    int ks[2][kSteps];
+    dsa_f32x16 sacc[kKt];
+    dsa_u32x4 codes[kKt][kSteps];
+    int ks[kKt][kSteps];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const int krow = kt * 32 + qi;
+    for (int kt = 0; kt < kKt; ++kt) {
+      const int krow = row0 + kt * 32 + qi;
       // Group g of a product's two, at the dword's bytes 0 and 2.
       const uint32_t four = *reinterpret_cast<const uint32_t*>(
           s_lds + (krow >> 4) * 256 + (krow & 15) * 4) >> (8 * g);
@@ -727,7 +735,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
       }
     };
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < kKt; ++kt) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sacc[kt][r] = 0.f;
 #pragma unroll
@@ -750,24 +758,25 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     __builtin_amdgcn_sched_barrier(0);
     issue_values();
     read_values(0);
-    if (key0 + kWideKeys > lim_first) {
+    if (key0 + 32 * kKt > lim_first) {
       const int bound = lim - key0 - 4 * g;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < kKt; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (kt * 32 + 8 * (r >> 2) + (r & 3) >= bound) sacc[kt][r] = -INFINITY;
     }
+    bad >>= row0 / 16;
     if (bad != 0) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < kKt; ++kt)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (bad & (1 << (2 * kt + (r >> 3)))) sacc[kt][r] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < kKt; ++kt)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kt][r]);
     // The reference moves only where a lane's own scores call for it: the row's largest is
@@ -807,8 +816,8 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j < 3) {
+    for (int j = 0; j < 2 * kKt; ++j) {
+      if (j < 2 * kKt - 1) {
         read_values(j + 1);
         weigh(j + 1);
       }
@@ -818,7 +827,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
         const x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         oacc[dt] = E::mfma32(a, pf[j & 1], oacc[dt]);
       }
-      if (j < 3) {
+      if (j < 2 * kKt - 1) {
 #pragma unroll
         for (int dt = 0; dt < kDt; ++dt) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -834,7 +843,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   // step s + 1, in registers by then, go to the other stage, and the loads of the keys of
   // step s + 1 and the values of step s + 2 go out.
   int bad_cur = 0;
-  auto step = [&](int s, int i, const unsigned char* k_lds, const unsigned char* s_lds,
+  auto step = [&](auto tiles, int s, int i, const unsigned char* k_lds, const unsigned char* s_lds,
                   unsigned char* k_to, unsigned char* s_to) __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(vmcnt(2));  // (the keys; the values behind them may be on their way)
     dsa::lds_barrier();
@@ -843,7 +852,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     locate(s + 2);  // (past the last key: no bytes)
     // (a wave whose rows see none of the step's keys only stages)
     if (wave_active && s * kWideKeys < lim_last) {
-      compute(i, k_lds, s_lds, s, bad_cur);
+      compute(tiles, i, k_lds, s_lds, s, bad_cur);
     } else {
       expand(s + 1, i ^ 1);
       issue_values();
@@ -859,16 +868,20 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     expand(it.s0, 0);
     locate(it.s0 + 1);
     issue_values();
-    for (int s = it.s0; s < it.s1; s += 2) {
-      step(s, 0, lds_k0, lds_s0, lds_k1, lds_s1);
-      if (s + 1 >= it.s1) break;
-      step(s + 1, 1, lds_k1, lds_s1, lds_k0, lds_s0);
-    }
+    auto walk = [&](auto tiles) __attribute__((always_inline)) {
+      for (int s = it.s0; s < it.s1; s += 2) {
+        step(tiles, s, 0, lds_k0, lds_s0, lds_k1, lds_s1);
+        if (s + 1 >= it.s1) break;
+        step(tiles, s + 1, 1, lds_k1, lds_s1, lds_k0, lds_s0);
+      }
+    };
+    if (half) walk(std::integral_constant<int, 1>());
+    else walk(std::integral_constant<int, 2>());
     __builtin_amdgcn_s_waitcnt(vmcnt(0));  // (loads behind the last step, into the stages)
   }
 
   const LateParams late = late_params();
-  const float l_tot = dsa::pair32_sum(l_run);
+  float l_tot = dsa::pair32_sum(l_run);
   if (__syncthreads_or((int)unfinite)) {
     const uint32_t found = unfinite_groups(late, it, h, it.s0 * kWideKeys,
                                            min(it.s1 * kWideKeys, kend), lim);
@@ -877,6 +890,36 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (found >> dt & 1) oacc[dt][r] = NAN;
+  }
+  if (half) {
+    // Waves 2 and 3 hand theirs to waves 0 and 1 (every wave is past its reads of the
+    // stages), which go on with the rows.
+    float* const theirs = reinterpret_cast<float*>(lds_v + (wave & 1) * 64 * kRow) + lane;
+    float* const stats = reinterpret_cast<float*>(lds_k0) + (wave & 1) * 128 + lane;
+    if (wave >= 2) {
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) theirs[(dt * 16 + r) * 64] = oacc[dt][r];
+      stats[0] = m_run;
+      stats[64] = l_tot;
+    }
+    dsa::lds_barrier();
+    if (wave >= 2) return;
+    const float m_they = stats[0], l_they = stats[64], m_all = fmaxf(m_run, m_they);
+    // (no finite score: l is 0, or NaN from NaN scores)
+    const float w = m_run == -INFINITY ? l_tot : __builtin_amdgcn_exp2f(m_run - m_all);
+    const float w_they = m_they == -INFINITY ? l_they : __builtin_amdgcn_exp2f(m_they - m_all);
+    l_tot = fmaf(w, l_tot, w_they * l_they);
+    m_run = m_all;
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = theirs[(dt * 16 + r) * 64];
+        const float own = w == 0.f ? 0.f : w * oacc[dt][r];
+        oacc[dt][r] = w_they == 0.f ? own : fmaf(w_they, x, own);
+      }
   }
   if (it.slot >= 0) {
     // A partial keeps the accumulators' own order (part_at): whole lines per store.
@@ -903,7 +946,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   // O goes out through the value stages (every wave is past its reads of them: the
   // barrier of __syncthreads_or), row by row as 16-byte chunks, whole rows to a store.
   const float inv = l_tot > 0.f ? 1.f / l_tot : (l_tot == 0.f ? 0.f : l_tot);
-  unsigned char* const mine = lds_v + wave * 32 * kRow;
+  unsigned char* const mine = lds_v + wave * (half ? 64 : 32) * kRow;
   auto o_swz = [](int r, int c) { return kD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7); };
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt)

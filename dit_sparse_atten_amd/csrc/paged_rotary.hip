@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "fp4.h"
+#include "paged_rows.h"
 
 namespace {
 
@@ -72,8 +73,8 @@ __device__ __forceinline__ void turn_rows(const TurnParams& p, int which, int he
   const int chunks = p.head_dim / 8;
   const int units = (chunks + 1) / 2, per_group = kThreads / units;
   const int local = threadIdx.x / units, u = threadIdx.x - local * units;
-  const int t = blockIdx.x * per_group + local;
-  if (local >= per_group || t >= p.tokens) return;
+  const int t = paged::token_of(blockIdx.x, per_group, local, p.tokens);
+  if (t < 0) return;
   bool turn = u < turned;
   const int c0 = turn ? u : 2 * u;  // 2 turned + 2 (u - turned)
   const int c1 = turn ? u + turned : c0 + 1;
@@ -158,8 +159,8 @@ __device__ __forceinline__ void pack_rows(const TurnParams& p, int which, int he
   const int lanes = 4 * groups;  // of a row
   const int per_group = kThreads / lanes;
   const int local = threadIdx.x / lanes, c = threadIdx.x - local * lanes;
-  const int t = blockIdx.x * per_group + local;
-  if (local >= per_group || t >= p.tokens) return;  // (whole quads)
+  const int t = paged::token_of(blockIdx.x, per_group, local, p.tokens);
+  if (t < 0) return;  // (whole quads)
   const bool real = c < p.head_dim / 8;
   const bool turn = which == kK && c < p.rot / 8;
   const int position = p.rot > 0 ? p.positions[t] : 0;

@@ -1200,9 +1200,9 @@ __global__ void __launch_bounds__(kNarrowWaves * 64, 1) seq_narrow_kernel(Params
   float acc[8];
 #pragma unroll
   for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+  // (a weight that has gone to 0 does not drop its wave: 0 times what is not finite is NaN)
 #pragma unroll
   for (int i = 0; i < kNarrowWaves; ++i) {
-    if (w[i] == 0.f) continue;
     const float* src = reinterpret_cast<const float*>(lds_k0) + (i * kNarrowRows + r) * kD + d0;
 #pragma unroll
     for (int x = 0; x < 8; ++x) acc[x] = fmaf(w[i], src[x], acc[x]);
@@ -1311,11 +1311,11 @@ __global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        // (a part no key of which is visible has l 0)
-        if (i0 + u * step >= it.parts || li[u] == 0.f) continue;
+        if (i0 + u * step >= it.parts) continue;
         const float m_new = fmaxf(m, mi[u]);
         const float a = m == m_new ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-        // (no finite score: l is NaN)
+        // (no finite score: l is 0, or NaN from NaN scores; a weight of 0 does not drop its
+        // part, for 0 times what is not finite is NaN)
         const float b = mi[u] == -INFINITY ? li[u] : __builtin_amdgcn_exp2f(mi[u] - m_new);
         l = fmaf(l, a, b * li[u]);
 #pragma unroll
@@ -1356,7 +1356,6 @@ __global__ void __launch_bounds__(256) seq_merge_kernel(Params p) {
       for (int i = 0; i < 16; ++i) {
         const float w =
             ml[0][i] == -INFINITY ? ml[1][i] : __builtin_amdgcn_exp2f(ml[0][i] - m_all);
-        if (w == 0.f) continue;
         l_all = fmaf(w, ml[1][i], l_all);
         o = fmaf(w, acc_lds[i][tid], o);
       }

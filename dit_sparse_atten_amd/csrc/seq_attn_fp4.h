@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
       const dsa_f32x4 x = *reinterpret_cast<const dsa_f32x4*>(
           reinterpret_cast<const float*>(lds_v + i * kStage) + r * kJoinRow + d0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = w[i] == 0.f ? acc[e] : fmaf(w[i], x[e], acc[e]);
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w[i], x[e], acc[e]);
     }
     if (it.slot >= 0) {
       float* po =
@@ -917,8 +917,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float x = theirs[(dt * 16 + r) * 64];
-        const float own = w == 0.f ? 0.f : w * oacc[dt][r];
-        oacc[dt][r] = w_they == 0.f ? own : fmaf(w_they, x, own);
+        oacc[dt][r] = fmaf(w_they, x, w * oacc[dt][r]);
       }
   }
   if (it.slot >= 0) {

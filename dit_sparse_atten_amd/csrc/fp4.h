@@ -3,8 +3,8 @@
 //
 // Groups of 32 neighbouring dims are E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
 // negatives) with a scale byte b for 2^(b - 127), 255 for a group that holds an infinity
-// or a NaN: the operand format of the scaled matrix instructions, which multiply the
-// codes as they lie in memory.
+// or a NaN: a format that the conversions expand to 16 bits, scale and all, two elements at
+// a time.
 //
 // The bytes of one page and key head, one after the other, with G = ceil(head_dim / 32)
 // and S = page_size:

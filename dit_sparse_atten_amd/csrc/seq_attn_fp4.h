@@ -2,33 +2,25 @@
 // bf16 or fp16 in and out, fp32 softmax: the walks of seq_attn.h, whose schedule, items
 // and joins these kernels share, over keys and values of 32-dim groups with a scale.
 //
-// Scores.  The matrix instructions take a 4-bit key as it lies in memory, with its
-// groups' scales, against 8-bit operands at twice the 16-bit rate.  A query is the exact
-// sum of two (bf16) or three (fp16) E4M3 terms of 4 bits each, 2^4 apart in scale, so
-// that keys are never expanded: S = K (Q_0 + 2^-4 Q_1 + 2^-8 Q_2).  (The queries of a row
-// share one exponent, its largest element's: elements 2^13 below it lose bits that are
-// 2^-21 of it.)  The instruction adds the products of eight neighbouring dims aligned to
-// the largest of them and cuts what lies below 2^-13 of it; all else is summed in fp32.
-// Against 64 bits the outputs of normal values are off by 0.0023 of their norm in bf16 and
-// 0.00029 in fp16 (0.0017 and 0.00021 with fp32 throughout, the output rounded).
+// Keys and values are expanded to 16 bits (exactly: the conversion takes the scale), keys in
+// registers or on the way into LDS, values on the way into LDS, and the products are those
+// of a 16-bit cache: S = K Q^T, exact products summed in fp32, and O^T = V^T P^T, P rounded
+// to the input type (the matrix operand's; by at most 2^-8 of a weight in bf16, below the
+// cache's own error).  Against 64 bits the outputs of normal values are off by 0.0023 of
+// their norm in bf16 and 0.00029 in fp16 (0.0017 and 0.00021 with fp32 throughout, the
+// output rounded).  The scaled matrix instructions would take the codes as they lie in
+// memory, against 8-bit terms of the queries, in 10 to 12% less time for chunks and 1 to
+// 3% less for single tokens, but they cut a product that lies 2^-13 below the largest of
+// eight neighbours: with one outlier dim a score was off by up to 100 times its fp32 bound.
 //
-// Values.  Their scales vary along the keys, which the product with P sums over, so
-// they are expanded to 16 bits (exactly: the conversion takes the scale) on the way into
-// LDS, and O^T = V^T P^T is that of the 16-bit cache, P rounded to the input type (the
-// matrix operand's; by at most 2^-8 of a weight in bf16, below the cache's own error).  A
-// group that is not a number enters as zeros, for 0 times it would reach rows that do not
-// see its key, and the rows that do are set to NaN at the end (unfinite_groups).
+// A value group that is not a number enters as zeros, for 0 times it would reach rows that
+// do not see its key, and the rows that do are set to NaN at the end (unfinite_groups).
 #pragma once
 
 #include "fp4.h"
 #include "seq_attn.h"
 
 namespace seq {
-
-typedef int32_t fp4_x8 __attribute__((ext_vector_type(8)));
-
-template <typename T>
-constexpr int kTerms = sizeof(T) == 2 && __is_same(T, __bf16) ? 2 : 3;
 
 // The larger exponents of a cache written from bf16 would be infinite in fp16, and 0
 // times that NaN in rows that do not see the key.
@@ -38,59 +30,14 @@ __device__ __forceinline__ uint32_t value_scale(uint32_t b, bool take) {
   return take ? b : 0u;
 }
 
-// Terms of 16 query elements x, already divided by 2^exponent: E4M3 bytes in order.
-template <typename T, int kCount>
-__device__ __forceinline__ void query_terms(float (&x)[16], int32_t (&term)[kCount][4]) {
-#pragma unroll
-  for (int n = 0; n < kCount; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      int32_t w = 0;
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], w, false);
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
-      term[n][i] = w;
-      if (n + 1 < kCount) {
-        x[4 * i + 0] = (x[4 * i + 0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * 16.f;
-        x[4 * i + 1] = (x[4 * i + 1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * 16.f;
-        x[4 * i + 2] = (x[4 * i + 2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * 16.f;
-        x[4 * i + 3] = (x[4 * i + 3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * 16.f;
-      }
-    }
-}
-
-// 16 dims from `d` of a query row, zeros past head_dim.
+// 8 dims from `d` of a query row, zeros past head_dim.
 template <typename T>
-struct QueryDims {
-  typename dsa::Elem<T>::x8 y[2];
-  __device__ __forceinline__ void load(const T* row, int d, int head_dim) {
+__device__ __forceinline__ typename dsa::Elem<T>::x8 query_dims(const T* row, int d, int head_dim) {
+  typename dsa::Elem<T>::x8 y;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[c][e] = (T)0.f;
-      if (d + 8 * c < head_dim)
-        y[c] = *reinterpret_cast<const typename dsa::Elem<T>::x8*>(row + d + 8 * c);
-    }
-  }
-  __device__ __forceinline__ void widen(float (&x)[16]) const {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = (float)y[e / 8][e % 8];
-  }
-};
-
-__device__ __forceinline__ uint32_t top_bits(const float (&x)[16], uint32_t top) {
-#pragma unroll
-  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-  return top;
-}
-
-// The exponent that brings a row's largest element (its bits) to [2^7, 2^8): E4M3 ends
-// at 448.  (Rows below 2^-103 keep less.)
-__device__ __forceinline__ int query_exponent(uint32_t top) {
-  return max((int)(top >> 23) - 134, -110);
-}
-// The scale byte of term n; 255 (NaN) for a row that is not finite.
-__device__ __forceinline__ int term_scale(uint32_t top, int exponent, int n) {
-  return top >= 0x7f800000u ? 255 : exponent + 127 - 4 * n;
+  for (int e = 0; e < 8; ++e) y[e] = (T)0.f;
+  if (d < head_dim) y = *reinterpret_cast<const typename dsa::Elem<T>::x8*>(row + d);
+  return y;
 }
 
 // A wave's groups of values that are not numbers: bit g of the result where a key of [lo,
@@ -143,17 +90,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const Params& p, uint
 // 64 (w + kWaves), ..), joined at the end.  Bound by the reads of the cache: codes and
 // scales go to registers a turn ahead, 70 KB on their way on a compute unit, by eight waves
 // of one workgroup or four each of two.  (64 requests of 1,000 to 16,000 tokens, 8 key
-// heads: D = 128 164 us, 6.0 TB/s, of 7.0 for a plain streaming read.  64 of 12,000, D = 64:
-// 96 us, 4.4 TB/s; 10 us of each are the schedule, the join and their launches, and with
+// heads: D = 128 167 us, 5.9 TB/s, of 7.0 for a plain streaming read.  64 of 12,000, D = 64:
+// 93 us, 4.5 TB/s; 10 us of each are the schedule, the join and their launches, and with
 // half the bytes a turn waits a fifth of its time for data and twice that to be issued.)
 // Lane (q4, c16) =
 // (lane / 16, lane % 16) holds the dims kD / 4 q4 .. of the keys 16 i + c16, row c16's scores
 // of the keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
 constexpr int kFp4Keys = 64;  // of a wave's turn
 
-// A lane's codes of a key: 32, or 16 where kD = 64, so that no lane is without.  (64 requests
-// of 12,000 tokens, 8 key heads, D = 64: 99 us with 32 codes in half the lanes, 96 so; 128
-// of 3,000 59 and 56, 512 of 750 87 and 79.)
+// A lane's codes of a key: 32, or 16 where kD = 64.
 template <int kBytes>
 struct Codes;
 template <>
@@ -162,18 +107,12 @@ struct Codes<16> {
   static __device__ __forceinline__ type load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at, int from) {
     return __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, from, 2);
   }
-  static __device__ __forceinline__ fp4_x8 operand(type k) {
-    return fp4_x8{(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
-  }
 };
 template <>
 struct Codes<8> {
   typedef dsa_u32x2 type;
   static __device__ __forceinline__ type load(__amdgpu_buffer_rsrc_t rsrc, uint32_t at, int from) {
     return __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, from, 2);
-  }
-  static __device__ __forceinline__ fp4_x8 operand(type k) {
-    return fp4_x8{(int)k[0], (int)k[1], 0, 0, 0, 0, 0, 0};
   }
 };
 
@@ -214,16 +153,14 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   const int kend = min(__builtin_amdgcn_readlane(lim, 15), it.s1 * kNarrowKeys);
   const int key_first = it.s0 * kNarrowKeys + wave * kFp4Keys;
 
-  QueryDims<T> raw[2];
+  // The row's query, of the dims whose codes the lane holds.
+  x8 qf[kLaneDims / 8];
   {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
-    // The products' elements 32 q4 .. 32 q4 + 31 are those that the keys' lane q4 holds; the
-    // queries' lane q4 has 16 q4 .. and 64 + 16 q4 ...  (kD = 64: the keys' lanes hold the
-    // dims 16 q4 .. and 16 zeros, so that every other query lane meets zeros only.)
-    const int d0 = kD == 128 ? 16 * q4 : q4 & 1 ? kD : 8 * q4;
-    raw[0].load(qrow, d0, p.head_dim);
-    raw[1].load(qrow, kD / 2 + d0, p.head_dim);
+#pragma unroll
+    for (int j = 0; j < kLaneDims / 8; ++j)
+      qf[j] = query_dims<T>(qrow, kLaneDims * q4 + 8 * j, p.head_dim);
   }
 
   // Pages of a window of 16 turns: lane l holds granule l & 3 of turn l / 4.
@@ -266,33 +203,6 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   Turn even, odd;
   load(0, even);
   __builtin_amdgcn_sched_barrier(0);
-  // The row's query in its terms: bytes 0..15 of the lane are raw[0]'s dims, 16..31 raw[1]'s.
-  fp4_x8 qf[kTerms<T>];
-  int q_scale[kTerms<T>];
-  {
-    float x[2][16];
-    raw[0].widen(x[0]);
-    raw[1].widen(x[1]);
-    uint32_t top = top_bits(x[1], top_bits(x[0], 0));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    const int exponent = query_exponent(top);
-    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[i][e] *= down;
-      int32_t term[kTerms<T>][4];
-      query_terms<T>(x[i], term);
-#pragma unroll
-      for (int n = 0; n < kTerms<T>; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) qf[n][4 * i + j] = term[n][j];
-    }
-#pragma unroll
-    for (int n = 0; n < kTerms<T>; ++n) q_scale[n] = term_scale(top, exponent, n);
-  }
-
   float m_run = -INFINITY, l_run = 0.f;
   dsa_f32x4 oacc[kDt];
 #pragma unroll
@@ -309,12 +219,11 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
     dsa_f32x4 s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const fp4_x8 a = C::operand(t.k[i]);
       s[i] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
+      const float scale = fp4::scale_of(t.ks[i]);
 #pragma unroll
-      for (int n = kTerms<T> - 1; n >= 0; --n)
-        s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, qf[n], s[i], 4, 0, 0,
-                                                                (int)t.ks[i], 0, q_scale[n]);
+      for (int j = 0; j < kLaneDims / 8; ++j)
+        s[i] = E::mfma16(fp4::expand(t.k[i][j], scale, T()), qf[j], s[i]);
     }
     // (the values' way into LDS covers the products' latency)
 #pragma unroll
@@ -510,13 +419,12 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
 }
 
 // 128 rows x the item's keys, bound by the matrix instructions: four waves of 32 rows,
-// 64 keys a step, as seq_wide_kernel walks a 16-bit cache.  Keys' codes go to LDS as they
-// are (a quarter of the bytes, and of the reads by every wave); values are expanded there
-// by the thread that loaded them, a step ahead.  (3,600 rows over 57,600 keys, 40 heads,
-// D = 128: 3,430 us, 1.24 PFLOP/s counted as 16-bit products, of 1.36 to 1.39 in a library
-// product; a 16-bit cache 3,930.  The chip is at its power limit, 70% of the time in
-// matrix instructions at 1.6 GHz.  With fewer dims the exponentials weigh more: D = 96
-// 1.07, D = 64 0.89 PFLOP/s.)  Lane (g, qi) = (lane / 32, lane % 32)
+// 64 keys a step, as seq_wide_kernel walks a 16-bit cache.  Keys and values are expanded into
+// LDS by the thread that loaded their codes, a step ahead.  (3,600 rows over 57,600 keys, 40
+// heads, D = 128: 3,840 to 3,890 us, 1.09 to 1.11 PFLOP/s, of 1.36 to 1.39 in a library
+// product; a 16-bit cache 3,930.  Keys expanded by every wave for itself, from codes in
+// LDS: 4,000 to 4,200.  The chip is at its power limit.  With fewer dims the exponentials
+// weigh more: D = 96 1.04, D = 64 0.84 PFLOP/s.)  Lane (g, qi) = (lane / 32, lane % 32)
 // holds row qi's scores of the keys 32 kt + 8 (r / 4) + 4 g + r % 4 and, of O, the dims
 // 32 dt + 8 (r / 4) + 4 g + r % 4.
 template <typename T, int kD, int kUse>
@@ -525,15 +433,9 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   typedef typename E::x8 x8;
   constexpr int kRow = kD * 2;               // bytes of an expanded row
   constexpr int kStage = kWideKeys * kRow;
-  constexpr int kCodeRow = kD / 2;           // of a row of codes
-  constexpr int kSteps = kD / 64;            // products of 64 dims
   constexpr int kDt = kUse / 32;
   constexpr int kChunks = kD / 8;
-  // (an array to a stage: a read of one that loads go to waits for them)
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_k0[4096];  // codes, 1 KB a wave
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_k1[4096];
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_s0[1024];  // scales, by wave
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_s1[1024];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_k[2 * kStage];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_v[2 * kStage];
 
   Item it;
@@ -568,60 +470,25 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const fp4::Layout at(groups, p.page_shift);
   const int block_bytes = fp4::row_bytes(groups) << p.page_shift;
 
-  // The row's query in its terms, for products of 64 dims: bytes 0..15 of the lane are
-  // the dims 64 j + 16 g .., 16..31 the dims 64 j + 32 + 16 g ...
-  fp4_x8 qf[kSteps][kTerms<T>];
-  int q_scale[kTerms<T>];
+  x8 qf[kUse / 16];
   {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
-    uint32_t top = 0;
-    QueryDims<T> raw[2 * kSteps];
 #pragma unroll
-    for (int j = 0; j < 2 * kSteps; ++j) {
-      raw[j].load(qrow, 32 * j + 16 * g, p.head_dim);
-    }
-#pragma unroll
-    for (int j = 0; j < 2 * kSteps; ++j) {
-      float x[16];
-      raw[j].widen(x);
-      top = top_bits(x, top);
-    }
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
-    const int exponent = query_exponent(top);
-    const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-#pragma unroll
-    for (int j = 0; j < 2 * kSteps; ++j) {
-      float x[16];
-      raw[j].widen(x);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] *= down;
-      int32_t term[kTerms<T>][4];
-      query_terms<T>(x, term);
-#pragma unroll
-      for (int n = 0; n < kTerms<T>; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qf[j >> 1][n][4 * (j & 1) + i] = term[n][i];
-    }
-#pragma unroll
-    for (int n = 0; n < kTerms<T>; ++n) q_scale[n] = term_scale(top, exponent, n);
+    for (int i = 0; i < kUse / 16; ++i) qf[i] = query_dims<T>(qrow, 16 * i + 8 * g, p.head_dim);
   }
 
   // Wave w stages the keys 16 w .. 16 w + 15 of a step, one page: lane (r, c) = (lane / 4,
-  // lane % 4) row r's chunk c, 16 bytes of codes (of 32-byte rows of keys: the lower 32
-  // lanes, (lane / 2, lane % 2)).  K chunk c of row r sits at c ^ (r / 4 & 3) or c ^ (r / 8
-  // & 1) (by r / 2 and r / 4 the reads met 20% more conflicts).
-  auto k_swz = [](int r, int c) { return kD == 128 ? c ^ (r >> 2 & 3) : c ^ (r >> 3 & 1); };
-  constexpr int kLanes = kD / 32;  // chunks of a row
-  const int k_row = lane / kLanes, k_chunk = k_swz(k_row, lane % kLanes);
-  const uint32_t code_at = k_row < 16 && k_chunk < groups
-                               ? (uint32_t)(k_row * at.code_row + k_chunk * 16) : dsa::kDeadChunk;
-  const int v_row = lane >> 2, v_group = lane & 3;
-  const uint32_t value_at =
-      v_group < groups ? (uint32_t)(v_row * at.code_row + v_group * 16) : dsa::kDeadChunk;
-  const uint32_t value_scale_at = v_group < groups ? (uint32_t)(v_row * 4 + v_group)
-                                                   : dsa::kDeadChunk;
-  const uint32_t scale_at = lane < 16 ? (uint32_t)(lane * 4) : dsa::kDeadChunk;
+  // lane % 4) row r's group c, 16 bytes of codes and a scale byte, of keys and of values.
+  const int own_row = lane >> 2, own_group = lane & 3;
+  const uint32_t code_at = own_group < groups ? (uint32_t)(own_row * at.code_row + own_group * 16)
+                                              : dsa::kDeadChunk;
+  const uint32_t scale_at = own_group < groups ? (uint32_t)(own_row * 4 + own_group)
+                                               : dsa::kDeadChunk;
+  // K chunk c of row r sits at c ^ (c / 8) ^ (2 (r & 3) + (r / 4 & 1)): two rows of four chunks
+  // 4 apart, as eight lanes write them, and eight rows of a chunk, as eight lanes read
+  // them, lie in distinct banks.
+  auto k_swz = [](int r, int c) { return c ^ (c >> 3) ^ (2 * (r & 3) + (r >> 2 & 1)); };
   // V chunk c of row r sits at c ^ (c / 8) ^ 2 (r & 3): two rows of four chunks 4 apart,
   // as eight lanes write them, and four rows of two chunks, as 16 lanes read them, lie in
   // distinct banks.
@@ -659,33 +526,33 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     at_row = (s * kWideKeys + wave * 16) & ((1 << p.page_shift) - 1);
     rsrc = fp4_rsrc(p, page, h, block_bytes, page < (uint32_t)p.pages);
   };
-  auto issue_keys = [&](unsigned char* k_to, unsigned char* s_to) __attribute__((always_inline)) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (DSA_LDS void*)(k_to + wave * 1024), 16,
-                                             code_at, at_row * at.code_row, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (DSA_LDS void*)(s_to + wave * 256), 4,
-                                             scale_at, at.k_scales + 4 * at_row, 0, 0);
-  };
-  dsa_u32x4 v_codes;
-  uint32_t v_scale = 0;
-  auto issue_values = [&]() __attribute__((always_inline)) {
-    v_codes = __builtin_amdgcn_raw_buffer_load_b128(rsrc, value_at,
+  dsa_u32x4 k_codes, v_codes;
+  uint32_t k_scale = 0, v_scale = 0;
+  auto issue = [&]() __attribute__((always_inline)) {
+    k_codes = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at, at_row * at.code_row, 0);
+    k_scale = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.k_scales + 4 * at_row, 0);
+    v_codes = __builtin_amdgcn_raw_buffer_load_b128(rsrc, code_at,
                                                     at.v_codes + at_row * at.code_row, 0);
-    v_scale = __builtin_amdgcn_raw_buffer_load_b8(rsrc, value_scale_at,
-                                                  at.v_scales + 4 * at_row, 0);
+    v_scale = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.v_scales + 4 * at_row, 0);
   };
   uint32_t unfinite = 0;  // 1 where a group of values is not a number
-  // The values of step s, on their way since issue_values(), into their stage.
+  // The keys and values of step s, on their way since issue(), into their stage.
   auto expand = [&](int s, int to) __attribute__((always_inline)) {
-    const bool held = s * kWideKeys + wave * 16 + v_row < kend;
+    const bool held = s * kWideKeys + wave * 16 + own_row < kend;
     const bool number = v_scale != 255u;
     unfinite |= held && !number ? 1u : 0u;
-    const float scale = fp4::scale_of(value_scale<T>(v_scale, held && number));
-    const int r = wave * 16 + v_row;
-    if (kD == 128 || v_group < 2) {
+    const float k_by = fp4::scale_of(k_scale);
+    const float v_by = fp4::scale_of(value_scale<T>(v_scale, held && number));
+    const int r = wave * 16 + own_row;
+    if (kD == 128 || own_group < 2) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<x8*>(lds_v + to * kStage + r * kRow + v_swz(r, 4 * v_group + j) * 16) =
-            fp4::expand(v_codes[j], scale, T());
+        *reinterpret_cast<x8*>(lds_k + to * kStage + r * kRow + k_swz(r, 4 * own_group + j) * 16) =
+            fp4::expand(k_codes[j], k_by, T());
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<x8*>(lds_v + to * kStage + r * kRow + v_swz(r, 4 * own_group + j) * 16) =
+            fp4::expand(v_codes[j], v_by, T());
     }
   };
 
@@ -698,31 +565,14 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 
   // Step s from stage `from`, the wave's 32 or 64 keys of it; the values of step s + 1 go to
   // the other stage meanwhile.
-  auto compute = [&](auto tiles, int from, const unsigned char* k_lds, const unsigned char* s_lds, int s,
-                     int bad) __attribute__((always_inline)) {
+  auto compute = [&](auto tiles, int from, int s, int bad) __attribute__((always_inline)) {
     constexpr int kKt = decltype(tiles)::value;  // tiles of 32 keys
     const int row0 = kKt == 2 ? 0 : (wave >> 1) * 32;
     const int key0 = s * kWideKeys + row0;
+    const unsigned char* const k_lds = lds_k + from * kStage + row0 * kRow;
     const unsigned char* const v_lds = lds_v + from * kStage + row0 * kRow;
     __builtin_amdgcn_s_setprio(0);
     dsa_f32x16 sacc[kKt];
-    dsa_u32x4 codes[kKt][kSteps];
-    int ks[kKt][kSteps];
-#pragma unroll
-    for (int kt = 0; kt < kKt; ++kt) {
-      const int krow = row0 + kt * 32 + qi;
-      // Group g of a product's two, at the dword's bytes 0 and 2.
-      const uint32_t four = *reinterpret_cast<const uint32_t*>(
-          s_lds + (krow >> 4) * 256 + (krow & 15) * 4) >> (8 * g);
-#pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
-        codes[kt][j] = *reinterpret_cast<const dsa_u32x4*>(
-            k_lds + (krow >> 4) * 1024 + (krow & 15) * kCodeRow +
-            k_swz(krow & 15, 2 * j + g) * 16);
-        // (bytes of groups that a row has not: codes of zeros, scales of no NaN)
-        ks[kt][j] = 2 * j + g < groups ? (int)four : 0;
-      }
-    }
     // The values' fragments of 16 keys (two reads each), read 16 keys ahead.
     typename E::x4 vf[2][kDt][2];
     auto read_values = [&](int j) __attribute__((always_inline)) {
@@ -739,24 +589,15 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sacc[kt][r] = 0.f;
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
-        const dsa_u32x4 c = codes[kt][j];
-        const fp4_x8 a = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
-#pragma unroll
-        for (int n = kTerms<T> - 1; n >= 0; --n) {
-          if (j == 0)
-            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                a, qf[j][n], sacc[kt], 4, 0, 0, ks[kt][j], 0, q_scale[n]);
-          else
-            sacc[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                a, qf[j][n], sacc[kt], 4, 0, 2, ks[kt][j], 0, q_scale[n]);
-        }
-      }
+      for (int i = 0; i < kUse / 16; ++i)
+        sacc[kt] = E::mfma32(*reinterpret_cast<const x8*>(k_lds + (kt * 32 + qi) * kRow +
+                                                          k_swz(qi, 2 * i + g) * 16),
+                             qf[i], sacc[kt]);
     }
     expand(s + 1, from ^ 1);
     asm volatile("" : "+v"(unfinite));  // (here, so that the scales' register is free)
     __builtin_amdgcn_sched_barrier(0);
-    issue_values();
+    issue();
     read_values(0);
     if (key0 + 32 * kKt > lim_first) {
       const int bound = lim - key0 - 4 * g;
@@ -839,45 +680,38 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     }
     l_run += sum0 + sum1;
   };
-  // Step s, of stage i: behind the barrier its keys and values are there; the values of
-  // step s + 1, in registers by then, go to the other stage, and the loads of the keys of
-  // step s + 1 and the values of step s + 2 go out.
+  // Step s, of stage i: behind the barrier its keys and values are there; those of step
+  // s + 1, in registers by then, go to the other stage, and the loads of step s + 2 go out.
   int bad_cur = 0;
-  auto step = [&](auto tiles, int s, int i, const unsigned char* k_lds, const unsigned char* s_lds,
-                  unsigned char* k_to, unsigned char* s_to) __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(vmcnt(2));  // (the keys; the values behind them may be on their way)
+  auto step = [&](auto tiles, int s, int i) __attribute__((always_inline)) {
     dsa::lds_barrier();
-    issue_keys(k_to, s_to);
     const int bad_then = bad_next;
     locate(s + 2);  // (past the last key: no bytes)
     // (a wave whose rows see none of the step's keys only stages)
     if (wave_active && s * kWideKeys < lim_last) {
-      compute(tiles, i, k_lds, s_lds, s, bad_cur);
+      compute(tiles, i, s, bad_cur);
     } else {
       expand(s + 1, i ^ 1);
-      issue_values();
+      issue();
     }
     bad_cur = bad_then;
   };
   if (it.s0 < it.s1) {
     locate(it.s0);
     bad_cur = bad_next;
-    issue_keys(lds_k0, lds_s0);
-    issue_values();
-    __builtin_amdgcn_s_waitcnt(vmcnt(0));
+    issue();
     expand(it.s0, 0);
     locate(it.s0 + 1);
-    issue_values();
+    issue();
     auto walk = [&](auto tiles) __attribute__((always_inline)) {
       for (int s = it.s0; s < it.s1; s += 2) {
-        step(tiles, s, 0, lds_k0, lds_s0, lds_k1, lds_s1);
+        step(tiles, s, 0);
         if (s + 1 >= it.s1) break;
-        step(tiles, s + 1, 1, lds_k1, lds_s1, lds_k0, lds_s0);
+        step(tiles, s + 1, 1);
       }
     };
     if (half) walk(std::integral_constant<int, 1>());
     else walk(std::integral_constant<int, 2>());
-    __builtin_amdgcn_s_waitcnt(vmcnt(0));  // (loads behind the last step, into the stages)
   }
 
   const LateParams late = late_params();
@@ -895,7 +729,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
     // Waves 2 and 3 hand theirs to waves 0 and 1 (every wave is past its reads of the
     // stages), which go on with the rows.
     float* const theirs = reinterpret_cast<float*>(lds_v + (wave & 1) * 64 * kRow) + lane;
-    float* const stats = reinterpret_cast<float*>(lds_k0) + (wave & 1) * 128 + lane;
+    float* const stats = reinterpret_cast<float*>(lds_k) + (wave & 1) * 128 + lane;
     if (wave >= 2) {
 #pragma unroll
       for (int dt = 0; dt < kDt; ++dt)

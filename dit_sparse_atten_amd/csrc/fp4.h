@@ -21,6 +21,9 @@ namespace fp4 {
 
 constexpr int kGroup = 32;  // dims to a scale byte
 
+// Exponents of the groups that a write makes: every element is a number of its type.
+constexpr int kLowBf16 = -125, kHighBf16 = 125, kLowF16 = -23, kHighF16 = 13;
+
 __host__ __device__ constexpr int groups_of(int head_dim) { return (head_dim + 31) / 32; }
 __host__ __device__ constexpr int row_bytes(int groups) { return 32 * groups + 8; }
 

@@ -371,8 +371,8 @@ int prepare(TurnParams* p, const char* who, const void* q, void* q_out, const vo
   p->tokens = tokens; p->heads = heads; p->kv_heads = kv_heads; p->head_dim = head_dim;
   p->rot = rot_dim; p->max_positions = max_positions;
   p->page_shift = __builtin_ctz(page_size);
-  p->low = dtype == DSA_BF16 ? -125 : -23;
-  p->high = dtype == DSA_BF16 ? 125 : 13;
+  p->low = dtype == DSA_BF16 ? fp4::kLowBf16 : fp4::kLowF16;
+  p->high = dtype == DSA_BF16 ? fp4::kHighBf16 : fp4::kHighF16;
   return DSA_OK;
 }
 

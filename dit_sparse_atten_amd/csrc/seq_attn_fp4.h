@@ -13,8 +13,9 @@
 // 3% less for single tokens, but they cut a product that lies 2^-13 below the largest of
 // eight neighbours: with one outlier dim a score was off by up to 100 times its fp32 bound.
 //
-// A value group that is not a number enters as zeros, for 0 times it would reach rows that
-// do not see its key, and the rows that do are set to NaN at the end (unfinite_groups).
+// A value group that is not of the type's numbers (kLargestScale) enters as zeros, for 0 times
+// it would reach rows that do not see its key, and the rows that do are set to NaN at the
+// end (unfinite_groups).
 #pragma once
 
 #include "fp4.h"
@@ -22,13 +23,10 @@
 
 namespace seq {
 
-// The larger exponents of a cache written from bf16 would be infinite in fp16, and 0
-// times that NaN in rows that do not see the key.
+// The largest scale byte of a group of numbers: every group past it (255, or in fp16 one of a
+// cache written from bf16) holds elements that the type has not.
 template <typename T>
-__device__ __forceinline__ uint32_t value_scale(uint32_t b, bool take) {
-  if (__is_same(T, _Float16)) b = min(b, (uint32_t)(13 + 127));
-  return take ? b : 0u;
-}
+constexpr uint32_t kLargestScale = (__is_same(T, _Float16) ? fp4::kHighF16 : fp4::kHighBf16) + 127;
 
 // 8 dims from `d` of a query row, zeros past head_dim.
 template <typename T>
@@ -40,8 +38,9 @@ __device__ __forceinline__ typename dsa::Elem<T>::x8 query_dims(const T* row, in
   return y;
 }
 
-// A wave's groups of values that are not numbers: bit g of the result where a key of [lo,
+// A wave's groups of values that are not numbers of type T: bit g of the result where a key of [lo,
 // hi) that the lane's row sees (those below `lim`) has such a group g.
+template <typename T>
 __device__ __forceinline__ uint32_t unfinite_groups(LateParams p, const Item& it, int h, int lo,
                                                     int hi, int lim) {
   const int groups = fp4::groups_of(p->head_dim);
@@ -58,7 +57,7 @@ __device__ __forceinline__ uint32_t unfinite_groups(LateParams p, const Item& it
             4 * (key & ((1 << p->page_shift) - 1)));
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          if (g < groups && (four >> (8 * g) & 255) == 255) mine |= 1u << g;
+          if (g < groups && (four >> (8 * g) & 255) > kLargestScale<T>) mine |= 1u << g;
       }
     }
     uint64_t left = __ballot(mine != 0);
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   dsa_f32x4 oacc[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) oacc[dt] = dsa_f32x4{0.f, 0.f, 0.f, 0.f};
-  bool unfinite = false;  // a group of values that is not a number
+  bool unfinite = false;  // a group of values that is not of the type's numbers
   // V chunk c of row r sits at c ^ (2 (r & 3) + (r / 4 & 1)): eight rows of a chunk, as
   // eight lanes write them, and four rows of two chunks, as 16 lanes read them, lie in
   // distinct banks.
@@ -229,9 +228,9 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool held = key0 + 16 * i + c16 < kend;
-      const bool number = t.vs[i] != 255u;
+      const bool number = t.vs[i] <= kLargestScale<T>;
       unfinite |= held && !number;
-      const float scale = fp4::scale_of(value_scale<T>(t.vs[i], held && number));
+      const float scale = fp4::scale_of(held && number ? t.vs[i] : 0u);
 #pragma unroll
       for (int j = 0; j < kLaneDims / 8; ++j)
         *reinterpret_cast<x8*>(stage + (16 * i + c16) * kRow +
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
   const LateParams late = late_params();
   if (__builtin_expect(__any(unfinite), 0)) {
     // (the wave's own keys alone would do; this is all of the item's)
-    const uint32_t found = unfinite_groups(late, it, h, it.s0 * kNarrowKeys, kend, lim);
+    const uint32_t found = unfinite_groups<T>(late, it, h, it.s0 * kNarrowKeys, kend, lim);
 #pragma unroll
     for (int dt = 0; dt < kDt; ++dt)
       if (found >> (dt / 2) & 1) oacc[dt] = dsa_f32x4{NAN, NAN, NAN, NAN};
@@ -535,14 +534,14 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
                                                     at.v_codes + at_row * at.code_row, 0);
     v_scale = __builtin_amdgcn_raw_buffer_load_b8(rsrc, scale_at, at.v_scales + 4 * at_row, 0);
   };
-  uint32_t unfinite = 0;  // 1 where a group of values is not a number
+  uint32_t unfinite = 0;  // 1 where a group of values is not of the type's numbers
   // The keys and values of step s, on their way since issue(), into their stage.
   auto expand = [&](int s, int to) __attribute__((always_inline)) {
     const bool held = s * kWideKeys + wave * 16 + own_row < kend;
-    const bool number = v_scale != 255u;
+    const bool number = v_scale <= kLargestScale<T>;
     unfinite |= held && !number ? 1u : 0u;
     const float k_by = fp4::scale_of(k_scale);
-    const float v_by = fp4::scale_of(value_scale<T>(v_scale, held && number));
+    const float v_by = fp4::scale_of(held && number ? v_scale : 0u);
     const int r = wave * 16 + own_row;
     if (kD == 128 || own_group < 2) {
 #pragma unroll
@@ -717,8 +716,8 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const LateParams late = late_params();
   float l_tot = dsa::pair32_sum(l_run);
   if (__syncthreads_or((int)unfinite)) {
-    const uint32_t found = unfinite_groups(late, it, h, it.s0 * kWideKeys,
-                                           min(it.s1 * kWideKeys, kend), lim);
+    const uint32_t found = unfinite_groups<T>(late, it, h, it.s0 * kWideKeys,
+                                              min(it.s1 * kWideKeys, kend), lim);
 #pragma unroll
     for (int dt = 0; dt < kDt; ++dt)
 #pragma unroll

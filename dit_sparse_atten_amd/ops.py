@@ -1675,11 +1675,13 @@ def paged_attention_fp4(q, cache, block_table, kv_lens, q_start, causal=True, sc
                         return_lse=False):
     """``paged_attention`` over a cache of 4-bit elements (``paged_cache_fp4``).
 
-    The keys and values are those that the cache stands for (``paged_read_fp4``), read
-    in place: a decoding step reads 27% of a 16-bit cache's bytes.  q's type is the one
+    The keys and values are those that ``paged_read_fp4`` gives in q's type, read in
+    place: a decoding step reads 27% of a 16-bit cache's bytes.  q's type is the one
     that the cache was written from.  Everything else, and what is returned, as in
     ``paged_attention``.  A group of 32 dims that is not a number (``paged_write_fp4``)
-    makes the rows that see its key NaN, one of values those dims of them.
+    makes the rows that see its key NaN, one of values those dims of them; so does, with
+    fp16 queries over a cache written from bf16, a group of values past 57,344, which has
+    elements that fp16 cannot hold.
     """
     lib = _lib.load()
     _require_cuda("q", q)

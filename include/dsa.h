@@ -576,12 +576,13 @@ size_t dsa_seq_attention_workspace_bytes(int32_t q_rows, int32_t requests, int32
 
 /*
  * dsa_paged_attention over a cache of 4-bit elements (below): keys and values are what
- * its codes and scales stand for, q's type the one that the cache was written from (in
- * fp16 values of exponents above 13 count as of 13).  strides[6]: q (token, head) in
- * elements, cache (page, head) in BYTES, o (token, head) in elements; page_size up to
- * 2^20.  A key group that is not a number makes the rows that see it NaN, a value
- * group its dims of them.  All else as there, but for the workspace's size
- * (dsa_paged_attention_fp4_workspace_bytes, of the same arguments).
+ * dsa_paged_read_fp4 gives in q's type, the one that the cache was written from.
+ * strides[6]: q (token, head) in elements, cache (page, head) in BYTES, o (token, head) in
+ * elements; page_size up to 2^20.  A key group that is not a number makes the rows that
+ * see it NaN, a value group its dims of them; so does a value group with an exponent that
+ * no write of q's type makes (above 125, in fp16 above 13: of a cache written from bf16),
+ * which has elements past the type's largest.  All else as there, but for the workspace's
+ * size (dsa_paged_attention_fp4_workspace_bytes, of the same arguments).
  */
 int dsa_paged_attention_fp4(const void* q, const void* cache, void* o, int32_t dtype,
                             const int64_t* strides, int32_t q_rows, int32_t requests,

@@ -119,8 +119,13 @@ __device__ __forceinline__ void turn_rows(const TurnParams& p, int which, int he
           const int ca = across ? 0 : e / 4, cb = across ? 1 : e / 4;
           const int ea = across ? e : e % 4 * 2, eb = across ? e : e % 4 * 2 + 1;
           const float a = (float)x[i][ca][ea], b = (float)x[i][cb][eb];
-          x[i][ca][ea] = (T)(a * cs[2 * e] - b * cs[2 * e + 1]);
-          x[i][cb][eb] = (T)(b * cs[2 * e] + a * cs[2 * e + 1]);
+          // To float32 and from there to 16 bits, in every turn of the loops alike: left to
+          // itself the compiler fuses the last step in some of them.
+          float ya = fmaf(a, cs[2 * e], -(b * cs[2 * e + 1]));
+          float yb = fmaf(b, cs[2 * e], a * cs[2 * e + 1]);
+          asm("" : "+v"(ya), "+v"(yb));
+          x[i][ca][ea] = (T)ya;
+          x[i][cb][eb] = (T)yb;
         }
       }
       uint16_t* const at = dst + (h0 + i) * p.dst_sh[which];
@@ -149,9 +154,9 @@ __global__ void __launch_bounds__(kThreads) paged_write_rotary_kernel(TurnParams
 // 16-bit rows to 4-bit rows, bound by memory (57,600 tokens x 12 heads x 128, 447 MB: 86
 // to 94 us).  A thread takes a chunk of 8 dims, four neighbours a group;
 // with halves it reads the chunk that its own turns with too.  A code may hang on the
-// last bit of what it rounds, so the turned element is the exact one rounded to float32:
-// in 64 bits the products of a 16-bit and a 32-bit float are exact, and their sum is
-// rounded once whether or not the compiler fuses it.
+// last bit of what it rounds, so the turned element does not depend on what the compiler
+// fuses: in 64 bits the products of a 16-bit and a 32-bit float are exact, and so their
+// sum in 64 bits, which is then rounded to float32, is the same either way.
 template <typename T, bool kHalves>
 __device__ __forceinline__ void pack_rows(const TurnParams& p, int which, int head0, int heads) {
   typedef typename dsa::Elem<T>::x8 x8;

@@ -434,9 +434,10 @@ struct Plan {
 // decoding steps, run 16-row tiles.  32 requests of 8,000 tokens, 8 key heads: 8
 // and 16 rows 172 us on 16-row tiles and 212 on 128-row ones, 24 and 32 rows (two
 // 16-row tiles) 365 and 212 us, 64 rows 716 and 213.  A 4-bit cache streams faster: 24
-// and 32 rows 80 and 111 us, 40 and 48 rows 152 and 111 (D = 64: 63 and 94, 103 and 92),
+// and 32 rows 82 and 85 us, 40 and 48 rows 150 and 106 (D = 64: 60 and 70, 98 and 82),
 // and up to 64 rows in calls that leave compute units idle (4 requests of 2,000 tokens, 64
-// rows 16 and 25 us; 2 of 60,000 70 and 77).
+// rows 15 and 22 us; where their walks are long as well 128-row tiles are ahead: 4 of 9,000
+// 31 and 28, 2 of 60,000 70 and 62).
 Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int head_dim,
                int64_t max_keys, bool fp4) {
   Plan s;
@@ -448,8 +449,8 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // 16-row tiles of a 4-bit cache: one workgroup of eight waves on a compute unit, or two
   // of four where there are more tiles than units, whose starts and joins then lie under
   // each other's walks.  (One against two, 8 key heads, D = 128: 512 requests of 750 tokens
-  // 138 / 106 us, 128 of 3,000 90 / 77, 64 of 6,000 80 / 76, 64 of 1,000 to 16,000 162 / 164;
-  // fewer tiles, 16 requests 30.4 / 31.6.)
+  // 131 / 100 us, 128 of 3,000 87 / 77, 64 of 6,000 79 / 75, 64 of 1,000 to 16,000 164 / 166;
+  // fewer tiles, 4 requests of 1,500 11.7 / 12.8, 32 of 8,000 53 / 56.)
   const bool pairs =
       fp4 && s.narrow && std::max(requests, rows / 16) * kv_heads > kNarrowSlots;
   s.slots = !s.narrow ? kWideSlots : pairs ? kFp4Slots : kNarrowSlots;
@@ -462,8 +463,8 @@ Plan make_plan(int64_t q_rows, int64_t requests, int group, int kv_heads, int he
   // 8 key heads: 16-row tiles of 4 requests, 1,024 keys 15.9 / 13.1 us (the host's
   // time), 1,536 keys 16.0 / 18.2; 128-row tiles of 2 requests, 512 keys 17.5 / 16.9,
   // 768 keys 19.3 / 21.7, 1,536 keys 22.7 / 36.1.
-  // A 4-bit cache's 16-row tiles take 512 keys a turn: 1,500 keys 15.9 / 13.9, 2,000 15.4 /
-  // 15.4, 3,000 17.0 / 18.9; 16 requests, 1,500 keys 18.0 / 14.2, 4,000 24.1 / 23.6.
+  // A 4-bit cache's 16-row tiles take 512 keys a turn: 1,500 keys 12.4 / 11.7, 2,000 13.4 /
+  // 14.1, 3,000 14.4 / 17.9; 16 requests, 1,500 keys 15.9 / 12.3, 4,000 21.9 / 22.8.
   s.merge = max_keys > (!s.narrow ? 640 : fp4 ? 2048 : 1024) && s.slots >= kv_heads;
   s.max_slots = s.merge ? 2 * s.slots / kv_heads : 0;
   s.max_splits = std::min(s.max_tiles, s.max_slots / 2);

@@ -91,7 +91,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t fp4_rsrc(const Params& p, uint
 // of one workgroup or four each of two.  (64 requests of 1,000 to 16,000 tokens, 8 key
 // heads: D = 128 167 us, 5.9 TB/s, of 7.0 for a plain streaming read.  64 of 12,000, D = 64:
 // 93 us, 4.5 TB/s; 10 us of each are the schedule, the join and their launches, and with
-// half the bytes a turn waits a fifth of its time for data and twice that to be issued.)
+// half the bytes a turn waits a quarter of its time for data and a third to be issued.)
 // Lane (q4, c16) =
 // (lane / 16, lane % 16) holds the dims kD / 4 q4 .. of the keys 16 i + c16, row c16's scores
 // of the keys 16 i + 4 q4 + r and, of O, the dims 16 dt + 4 q4 + r.
@@ -420,10 +420,10 @@ __global__ void __launch_bounds__(kWaves * 64, 1) seq_narrow_fp4_kernel(Params p
 // 128 rows x the item's keys, bound by the matrix instructions: four waves of 32 rows,
 // 64 keys a step, as seq_wide_kernel walks a 16-bit cache.  Keys and values are expanded into
 // LDS by the thread that loaded their codes, a step ahead.  (3,600 rows over 57,600 keys, 40
-// heads, D = 128: 3,840 to 3,890 us, 1.09 to 1.11 PFLOP/s, of 1.36 to 1.39 in a library
+// heads, D = 128: 3,840 to 3,960 us, 1.07 to 1.11 PFLOP/s, of 1.36 to 1.39 in a library
 // product; a 16-bit cache 3,930.  Keys expanded by every wave for itself, from codes in
 // LDS: 4,000 to 4,200.  The chip is at its power limit.  With fewer dims the exponentials
-// weigh more: D = 96 1.04, D = 64 0.84 PFLOP/s.)  Lane (g, qi) = (lane / 32, lane % 32)
+// weigh more: D = 96 1.00, D = 64 0.80 PFLOP/s.)  Lane (g, qi) = (lane / 32, lane % 32)
 // holds row qi's scores of the keys 32 kt + 8 (r / 4) + 4 g + r % 4 and, of O, the dims
 // 32 dt + 8 (r / 4) + 4 g + r % 4.
 template <typename T, int kD, int kUse>
@@ -446,8 +446,8 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const int g = lane >> 5, qi = lane & 31;
   const int rows = it.n * p.group;
   // Of a tile of up to 64 rows two waves take each 32 rows, 32 of a step's keys each, and
-  // join at the end.  (32 requests of 8,000 tokens, 8 key heads, 64 rows each: 124 us with
-  // two of the waves idle, 111 so; 16 of 4,000, 40 key heads, 150 rows: 301 and 281.)
+  // join at the end.  (32 requests of 8,000 tokens, 8 key heads, 64 rows each: 126 us with
+  // two of the waves idle, 108 so; 16 of 4,000, 40 key heads, 150 rows: 308 and 289.)
   const bool half = rows - it.tile * kWideRows <= kWideRows / 2;
   const int wave_row = (half ? wave & 1 : wave) * 32;
   const int local = wave_row + qi;

@@ -1407,7 +1407,9 @@ def _fp4_page_size(value):
 
 def paged_cache_fp4(pages, page_size, kv_heads, head_dim, device="cuda"):
     """An empty paged cache of 4-bit keys and values: uint8 [pages, kv_heads, page_size,
-    32 * G + 8] with G = ceil(head_dim / 32): 4.25 bits an element at 128 dims.
+    32 * G + 8] with G = ceil(head_dim / 32): 4.25 bits an element at 128 dims, 4.5 at 64,
+    and more where the last group is not full (5.2 at 80, 7.2 at 40, 20 at 8: more than 16
+    bits).
 
     Groups of 32 neighbouring dims are E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
     their negatives) with a power of two between them.  The bytes of one page and head
@@ -1678,7 +1680,8 @@ def paged_attention_fp4(q, cache, block_table, kv_lens, q_start, causal=True, sc
     The keys and values are those that ``paged_read_fp4`` gives in q's type, read in
     place: a decoding step reads 27% of a 16-bit cache's bytes.  q's type is the one
     that the cache was written from.  Everything else, and what is returned, as in
-    ``paged_attention``.  A group of 32 dims that is not a number (``paged_write_fp4``)
+    ``paged_attention``, its precision too: scores and sums in float32, the probabilities
+    rounded to q's type before they meet V.  A group of 32 dims that is not a number (``paged_write_fp4``)
     makes the rows that see its key NaN, one of values those dims of them; so does, with
     fp16 queries over a cache written from bf16, a group of values past 57,344, which has
     elements that fp16 cannot hold.

@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
   const fp4::Layout at(groups, p.page_shift);
   const int block_bytes = fp4::row_bytes(groups) << p.page_shift;
 
-  x8 qf[kUse / 16];
+  x8 qf[kUse / 16];  // the row's query: dims 16 i + 8 g ..
   {
     const T* qrow = static_cast<const T*>(p.q) + (int64_t)(it.q0 + token) * p.q_st +
                     head * p.q_sh;
@@ -562,8 +562,8 @@ __global__ void __launch_bounds__(256, 2) seq_wide_fp4_kernel(Params p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) oacc[dt][r] = 0.f;
 
-  // Step s from stage `from`, the wave's 32 or 64 keys of it; the values of step s + 1 go to
-  // the other stage meanwhile.
+  // Step s from stage `from`, the wave's 32 or 64 keys of it; the keys and values of step
+  // s + 1 go to the other stage meanwhile.
   auto compute = [&](auto tiles, int from, int s, int bad) __attribute__((always_inline)) {
     constexpr int kKt = decltype(tiles)::value;  // tiles of 32 keys
     const int row0 = kKt == 2 ? 0 : (wave >> 1) * 32;

@@ -9,8 +9,8 @@
 // cache's own error).  Against 64 bits the outputs of normal values are off by 0.0023 of
 // their norm in bf16 and 0.00029 in fp16 (0.0017 and 0.00021 with fp32 throughout, the
 // output rounded).  The scaled matrix instructions would take the codes as they lie in
-// memory, against 8-bit terms of the queries, in 10 to 12% less time for chunks and 1 to
-// 3% less for single tokens, but they cut a product that lies 2^-13 below the largest of
+// memory, against 8-bit terms of the queries, in 4 to 12% less time for bf16 chunks and 1 to
+// 5% less for single tokens, but they cut a product that lies 2^-13 below the largest of
 // eight neighbours: with one outlier dim a score was off by up to 100 times its fp32 bound.
 //
 // A value group that is not of the type's numbers (kLargestScale) enters as zeros, for 0 times
